@@ -131,7 +131,7 @@ __device__ __forceinline__ lpx8_t pack8(const float* lo, const float* hi) {
 
 // The backward kernels are VALU-issue-bound (a wave64 VALU instruction holds its SIMD's issue port for 4 cycles: 930 VALU against
 // 164 MFMAs per 16-query strip of dQ, profiles/r03_sweeps.md): the per-score arithmetic  ds = exp2(s c - lse) (dp - delta)  is
-// written on pairs so that hipcc emits v_pk_fma_f32 / v_pk_add_f32 / v_pk_mul_f32 (same IEEE operations, half the instructions)
+// written on pairs (the build switches packed fp32 instructions off, simvg_amd/build.py: a pair compiles to two scalar operations)
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void ds_pair(float s0, float s1, f32x2_t c, f32x2_t nl, float dp0, float dp1, f32x2_t dl, float& p0,
                                         float& p1, float& ds0, float& ds1) {

@@ -103,8 +103,9 @@ __device__ __forceinline__ void gelu_parts(float x, float& cdf, float& pdf) {
   cdf = 0.5f + copysignf(h, x);
   pdf = 0.39894228040143267794f * e;
 }
-// the same on two values at once: every multiply / fma is a packed v_pk_*_f32 (one issue slot for both values); the reciprocal,
+// the same on two values at once: written on pairs; the reciprocal,
 // the exponential, |x| and the sign transfer stay per value.  Same operations in the same order as gelu_parts: identical results.
+// (The build switches packed fp32 instructions off, simvg_amd/build.py: a pair compiles to two scalar operations.)
 __device__ __forceinline__ void gelu_parts2(hw_f32x2_t x, hw_f32x2_t& cdf, hw_f32x2_t& pdf) {
   hw_f32x2_t t, e;
   t[0] = __builtin_amdgcn_rcpf(fmaf(0.3275911f, fabsf(x[0]) * 0.70710678118654752440f, 1.0f));

@@ -198,7 +198,7 @@ __global__ __launch_bounds__(256, NIT8 <= 6 ? 4 : 3) void ln_fwd_wide_kernel(con
     const int row = row0 + r;
     if (row >= M) break;
     const int g = row >= split;
-    // two values per register pair: the arithmetic below is packed fp32 (v_pk_fma / v_pk_mul / v_pk_add: one issue slot for two values)
+    // two values per register pair: the build switches packed fp32 instructions off (simvg_amd/build.py), so each operation below is two
     hw_f32x2_t v[NIT8][4];
     hw_f32x2_t s2 = {0.f, 0.f};
 #pragma unroll
@@ -796,7 +796,7 @@ __global__ __launch_bounds__(256) void ln_bwd_ffn_kernel(const lp_t* __restrict_
                                                          lp_t* __restrict__ out, int ldo, int M, int D, int split,
                                                          int rows_per_block, int blocks0, float* __restrict__ partial,
                                                          float pscale) {
-  // D == NITW * 1024 (launcher).  The arithmetic is packed fp32, two values per instruction: the kernel is bound by VALU issue
+  // D == NITW * 1024 (launcher).  The arithmetic is written on pairs of values (two instructions each): the kernel is bound by VALU issue
   // (GELU, GELU' and the LayerNorm backward are ~33 operations per element, two of them transcendental)
   __shared__ float part[2][4][2];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
