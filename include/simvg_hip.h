@@ -439,6 +439,86 @@ int simvg_dropout_mult(float* out, long n, float keep, const float* keep_seg, lo
 /* the same generator evaluated on the host: out[4] = Philox4x32-10(ctr[4], key[2]) (known-answer tests) */
 int simvg_philox4x32(const unsigned* ctr, const unsigned* key, unsigned* out);
 
+/* ---- sequence operators: what a language model over this path's image and text tokens needs (csrc/rope.hip, packed_attn.hip,
+ * vocab_ce.hip).  Unlike the encoder's entry points they take the element type per call, round to nearest without saturation (an
+ * overflow is an inf), and read q / k / v rows through a token stride and a head stride (in elements; the innermost dimension is
+ * contiguous), so that slices of one fused projection need no copy.  16-bit attention and loss operands start at multiples of 16
+ * bytes in every row.  Nothing is kept between calls; every result is the same bits at every run. */
+#define SIMVG_F32 0
+#define SIMVG_F16 1
+#define SIMVG_BF16 2
+
+/* Norm of every head of q and k, then the rotation by up to four position axes, one pass:
+ *   z = g x / sqrt(mean(x^2) + eps);   y[a_j] = z[a_j] cos t_j - z[b_j] sin t_j,   y[b_j] = z[a_j] sin t_j + z[b_j] cos t_j
+ *   t_j = pos[row][axis(j)] * inv_freq[j] (in 64 bits),  j < P = sum(sections), axis(j) = the section that j falls into,
+ *   (a_j, b_j) = (j, j + P) or, interleaved, (2j, 2j + 1); values from 2P on are normalised and not rotated.
+ * x: [T][H][D], D even and <= 256, fp32 / fp16 / bf16; pos: [T][n_axes] int32 or (pos_is_64) int64; gq, gk: fp32 [D], both or
+ * neither (rotation alone).  Forward writes q_out / k_out (which may be q / k themselves).  Backward reads q, k and the gradients
+ * dq, dk of the outputs, writes the inputs' gradients to q_out / k_out and the weights' to dgq / dgk (sums over rows and heads,
+ * written, not added); ws: simvg_qk_norm_rope_ws_floats(T, D) floats. */
+typedef struct simvg_qk_norm_rope_args {
+  int dtype, T, Hq, Hkv, D, n_axes, sections[4], interleaved, pos_is_64;
+  float eps;
+  const void* pos; long pos_ld;
+  const double* inv_freq;
+  const float *gq, *gk;
+  const void* q; long q_ts, q_hs; const void* k; long k_ts, k_hs;
+  void* q_out; long qo_ts, qo_hs; void* k_out; long ko_ts, ko_hs;
+  const void* dq; long dq_ts, dq_hs; const void* dk; long dk_ts, dk_hs;
+  float *dgq, *dgk, *ws;
+} simvg_qk_norm_rope_args;
+long simvg_qk_norm_rope_ws_floats(int T, int D);
+int simvg_qk_norm_rope_fwd(const simvg_qk_norm_rope_args* args, simvg_stream_t stream);
+int simvg_qk_norm_rope_bwd(const simvg_qk_norm_rope_args* args, simvg_stream_t stream);
+
+/* Attention over sequences packed one after the other: rows [cu[s], cu[s + 1]) are sequence s (any length, 0 too), a row sees the keys
+ * of its own sequence, under `causal` up to itself.  Hq heads of q share Hkv heads of k and v (Hq a multiple of Hkv); D a multiple
+ * of 8, <= 128; fp16 / bf16.
+ * simvg_packed_plan lays a batch's lengths out for the kernels once (cu: device int32 [nseq + 1], cu[0] = 0, rising, at most T); every
+ * layer's forward and backward of that batch read it.  A list that is none makes a plan without entries: nothing is computed, and
+ * with fill_tail the outputs are NaN.
+ * Forward writes o and lse [Hq][T] (natural logarithm of the softmax's denominator, scale included).  Backward reads q, k, v, o, lse and
+ * d_o, writes dq, dk, dv; ws: simvg_packed_attn_ws_floats() floats.  Rows behind the last sequence are left as they were, or, with
+ * fill_tail, become zeros. */
+typedef struct simvg_packed_attn_args {
+  int dtype, T, nseq, Hq, Hkv, D, causal, fill_tail;
+  float scale;
+  const int* plan;
+  const void* q; long q_ts, q_hs; const void* k; long k_ts, k_hs; const void* v; long v_ts, v_hs;
+  void* o; long o_ts, o_hs;
+  float* lse; long lse_hs;
+  const void* d_o; long do_ts, do_hs;
+  void* dq; long dq_ts, dq_hs; void* dk; long dk_ts, dk_hs; void* dv; long dv_ts, dv_hs;
+  float* ws;
+} simvg_packed_attn_args;
+long simvg_packed_plan_ints(int T, int nseq);
+int simvg_packed_plan(const int* cu_seqlens, int nseq, int T, int* plan, simvg_stream_t stream);
+long simvg_packed_attn_ws_floats(int T, int nseq, int Hq, int Hkv);
+int simvg_packed_attn_fwd(const simvg_packed_attn_args* args, simvg_stream_t stream);
+int simvg_packed_attn_bwd(const simvg_packed_attn_args* args, simvg_stream_t stream);
+
+/* Softmax cross entropy of z = x w^T + bias over a vocabulary, the logits never stored:
+ *   lse[i] = log sum_v exp(z[i][v]);   loss[i] = lse[i] - z[i][target[i]], 0 where target[i] == ignore_index, NaN where the target is
+ *   neither a word in [0, V) nor ignore_index.
+ * x: [M][K], w: [V][K], fp16 / bf16, K a multiple of 8; bias: fp32 [V] or NULL; target: int64 [M].
+ * Backward, for the gradients dloss [M] of the rows' losses: dx [M][K], dw [V][K] in the operands' type, dbias fp32 [V] (NULL: not
+ * wanted); all are written, not added.  Ignored rows, and rows whose target is no word, have no part in any of them.
+ * ws: simvg_vocab_ce_ws_bytes(M, V, K, bias wanted, backward) bytes, aligned to 256. */
+typedef struct simvg_vocab_ce_args {
+  int dtype, M, V, K;
+  const void* x; long ldx;
+  const void* w; long ldw;
+  const float* bias;
+  const long* target; long ignore_index;
+  float *loss, *lse;
+  const float* dloss;
+  void* dx; long lddx; void* dw; long lddw; float* dbias;
+  void* ws; long ws_bytes;
+} simvg_vocab_ce_args;
+long simvg_vocab_ce_ws_bytes(int M, int V, int K, int with_bias, int backward);
+int simvg_vocab_ce_fwd(const simvg_vocab_ce_args* args, simvg_stream_t stream);
+int simvg_vocab_ce_bwd(const simvg_vocab_ce_args* args, simvg_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

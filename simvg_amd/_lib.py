@@ -79,7 +79,46 @@ class DecFfnBwdArgs(C.Structure):       # simvg_dec_ffn_bwd_args
                                          "db2n", "dgP", "dbP")])
 
 
+class QkNormRopeArgs(C.Structure):      # simvg_qk_norm_rope_args
+    _fields_ = ([(n, c_int) for n in ("dtype", "T", "Hq", "Hkv", "D", "n_axes")] + [("sections", c_int * 4)] +
+                [("interleaved", c_int), ("pos_is_64", c_int), ("eps", c_float), ("pos", c_void_p), ("pos_ld", c_long),
+                 ("inv_freq", c_void_p), ("gq", c_void_p), ("gk", c_void_p)] +
+                [f for n, s in (("q", "q"), ("k", "k"), ("q_out", "qo"), ("k_out", "ko"), ("dq", "dq"), ("dk", "dk"))
+                 for f in ((n, c_void_p), (s + "_ts", c_long), (s + "_hs", c_long))] +
+                [("dgq", c_void_p), ("dgk", c_void_p), ("ws", c_void_p)])
+
+
+class PackedAttnArgs(C.Structure):      # simvg_packed_attn_args
+    _fields_ = ([(n, c_int) for n in ("dtype", "T", "nseq", "Hq", "Hkv", "D", "causal", "fill_tail")] + [("scale", c_float), ("plan", c_void_p)] +
+                [f for n in ("q", "k", "v", "o") for f in ((n, c_void_p), (n + "_ts", c_long), (n + "_hs", c_long))] +
+                [("lse", c_void_p), ("lse_hs", c_long)] +
+                [f for n, s in (("d_o", "do"), ("dq", "dq"), ("dk", "dk"), ("dv", "dv"))
+                 for f in ((n, c_void_p), (s + "_ts", c_long), (s + "_hs", c_long))] + [("ws", c_void_p)])
+
+
+class VocabCeArgs(C.Structure):         # simvg_vocab_ce_args
+    _fields_ = ([(n, c_int) for n in ("dtype", "M", "V", "K")] +
+                [("x", c_void_p), ("ldx", c_long), ("w", c_void_p), ("ldw", c_long), ("bias", c_void_p), ("target", c_void_p),
+                 ("ignore_index", c_long), ("loss", c_void_p), ("lse", c_void_p), ("dloss", c_void_p), ("dx", c_void_p), ("lddx", c_long),
+                 ("dw", c_void_p), ("lddw", c_long), ("dbias", c_void_p), ("ws", c_void_p), ("ws_bytes", c_long)])
+
+
+# entry points that return a size: {name: arguments}
+_SIZES = {
+    "simvg_qk_norm_rope_ws_floats": [c_int, c_int],
+    "simvg_packed_plan_ints": [c_int, c_int],
+    "simvg_packed_attn_ws_floats": [c_int, c_int, c_int, c_int],
+    "simvg_vocab_ce_ws_bytes": [c_int, c_int, c_int, c_int, c_int],
+}
+
 _SIGS = {
+    "simvg_qk_norm_rope_fwd": [c_void_p, c_void_p],
+    "simvg_qk_norm_rope_bwd": [c_void_p, c_void_p],
+    "simvg_packed_plan": [c_void_p, c_int, c_int, c_void_p, c_void_p],
+    "simvg_packed_attn_fwd": [c_void_p, c_void_p],
+    "simvg_packed_attn_bwd": [c_void_p, c_void_p],
+    "simvg_vocab_ce_fwd": [c_void_p, c_void_p],
+    "simvg_vocab_ce_bwd": [c_void_p, c_void_p],
     "simvg_text_filt_fwd": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p],
     "simvg_text_filt_bwd": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p],
     "simvg_query_mix_fwd": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p],
@@ -209,6 +248,9 @@ def load():
     lib.simvg_ln_bwd_ws_floats.argtypes = [c_int, c_int, c_int]
     lib.simvg_gemm_tn_ws_floats.restype = c_long
     lib.simvg_gemm_tn_ws_floats.argtypes = [c_int, c_int, c_int]
+    for name, args in _SIZES.items():
+        fn = getattr(lib, name)
+        fn.restype, fn.argtypes = c_long, args
     lib.simvg_dec_attn_max_keys.restype = c_int
     lib.simvg_dec_attn_max_keys.argtypes = []
     _lib = lib
@@ -222,7 +264,7 @@ def lowp_format():
 
 def exported_symbols():
     return sorted(_SIGS) + ["simvg_last_error", "simvg_version", "simvg_source_hash", "simvg_lowp_format", "simvg_ln_bwd_ws_floats", "simvg_gemm_tn_ws_floats",
-                            "simvg_dec_attn_max_keys"]
+                            "simvg_dec_attn_max_keys"] + list(_SIZES)
 
 
 def check(rc, what):

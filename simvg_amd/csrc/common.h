@@ -179,7 +179,7 @@ __device__ __forceinline__ lpx8_t frag8(u32x2_t lo, u32x2_t hi) {
 }
 __device__ __forceinline__ unsigned lds_addr(const void* p) { return (unsigned)(uintptr_t)LDS_PTR(p); }
 
-static inline int cdiv(int a, int b) { return (a + b - 1) / b; }
+static __host__ __device__ inline int cdiv(int a, int b) { return (a + b - 1) / b; }
 // wgrad.hip: XCD-partitioned weight gradient for the ViT-B encoder shapes; false = not handled (generic kernels run)
 // include/simvg_hip.h: the second stage of one slab-flushed wgrad (sum of the row partitions' slabs into dW)
 struct simvg_wgrad_reduce_desc {

@@ -1,0 +1,704 @@
+// Attention over packed sequences, forward and backward: rows [cu[s], cu[s + 1]) of q, k, v are sequence s.  A row sees the keys of its
+// own sequence, under `causal` those up to itself; Hq heads of q share Hkv heads of k and v, G = Hq / Hkv neighbours each.
+//
+//   S = scale q k^T,  lse_i = log sum_j exp(S_ij),  P = exp(S - lse),  O = P V
+//   backward: D_i = sum_d dO_id O_id;  dV = P^T dO;  dP = dO V^T;  dS = P (dP - D);  dQ = scale dS K;  dK = scale dS^T Q
+//
+// Bound by the matrix pipes (4 D products per visible pair forward, 10 D backward).  One workgroup takes 128 rows of one sequence and
+// head, a wave 32 of them, in tiles of 64 keys (queries, for dK and dV) that pass through LDS once for the workgroup.  All scores are
+// computed transposed, S^T = K Q^T by 32x32x16 MFMAs: a lane then holds ONE query's scores (keys in its registers), so that the
+// softmax needs a single exchange, between the two halves of the wave, and what the next product takes as its B operand is what the
+// lane already has -- the order of the contraction's keys is free, and the transposed reads (ds_read_b64_tr_b16) that fetch V^T use
+// the order in which the accumulator holds them.  P and dS never leave registers.
+//
+// Which rows a workgroup takes stands in a plan that the caller has built once for a batch (packed_plan_kernel): one entry for each
+// tile of 128 rows of each sequence, tiles far down a sequence first, because under `causal` they cost most and the last workgroups to
+// start should be the short ones.
+//
+// Masks: rows and keys past a sequence are zeros in LDS and are never stored, so nothing of a neighbour is read.  In a tile that the
+// diagonal crosses, P is an exact 0 above it, and 0 x inf in the matrix product would still carry a later row's inf or NaN to an
+// earlier one: such a tile is looked through for values that are not finite, and if there are any they are taken out of the operand and
+// added, as themselves, to the rows that do see them (see `add_nonfinite`).
+#include "seq.h"
+
+struct simvg_packed_attn_args {
+  int dtype, T, nseq, Hq, Hkv, D, causal, fill_tail;        // fill_tail: rows past the last sequence become zeros (else: as they were)
+  float scale;
+  const int* plan;
+  const void* q; long q_ts, q_hs; const void* k; long k_ts, k_hs; const void* v; long v_ts, v_hs;
+  void* o; long o_ts, o_hs;                                  // forward: output; backward: the forward's output
+  float* lse; long lse_hs;                                   // [Hq][T]: head stride, rows are neighbours
+  const void* d_o; long do_ts, do_hs;                        // backward
+  void* dq; long dq_ts, dq_hs; void* dk; long dk_ts, dk_hs; void* dv; long dv_ts, dv_hs;
+  float* ws;                                                 // backward: simvg_packed_attn_ws_floats() floats
+};
+
+namespace {
+using namespace seq;
+
+constexpr int QT = 128;                                      // rows of a plan entry
+constexpr int KT = 64;                                       // rows of a tile in LDS
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+constexpr float NEG_INF = -__builtin_huge_valf();
+
+// ---------------------------------------------------------------------------------------------------------------- the plan
+// ints: [0] entries, [1] the row after the last sequence (-1: `cu` is no such list, there are no entries), [2..3] unused, then int4
+// {first row, rows, tile of the sequence, tiles of all sequences before} per entry, then nseq + 1 prefix sums of tiles (used while
+// building).  A list that does not start at 0, falls, or passes T is found here, so the kernels below stay inside their tensors
+// whatever it holds.
+constexpr int PLAN_HEAD = 4, PLAN_BINS = 1024;
+// one more than the tiles of any valid list: what a launch has left over is enough for the tiles behind the last sequence
+__host__ __device__ __forceinline__ int plan_capacity(int T, int nseq) { return T / QT + nseq + 1; }
+
+// in place: scan[i] = sum of scan[0 .. i], 1024 threads
+__device__ __forceinline__ void scan1024(long* scan, int tid) {
+  __syncthreads();
+  for (int o = 1; o < 1024; o <<= 1) {
+    const long v = tid >= o ? scan[tid - o] : 0;
+    __syncthreads();
+    scan[tid] += v;
+    __syncthreads();
+  }
+}
+__global__ __launch_bounds__(1024) void packed_plan_kernel(const int* cu, int nseq, int T, int* plan) {
+  __shared__ long scan[1024];
+  __shared__ int bins[PLAN_BINS];
+  const int tid = threadIdx.x, cap = plan_capacity(T, nseq);
+  int* base = plan + PLAN_HEAD + 4 * cap;
+  int bad = cu[0] != 0;
+  for (int s = tid; s < nseq; s += 1024) bad |= cu[s + 1] < cu[s] || cu[s + 1] > T;
+  if (__syncthreads_or(bad)) {
+    if (tid == 0) { plan[0] = 0; plan[1] = -1; }
+    return;
+  }
+  long carry = 0;
+  for (int s0 = 0; s0 < nseq; s0 += 1024) {                  // prefix sums of the sequences' tiles
+    const int s = s0 + tid;
+    const long mine = s < nseq ? (cu[s + 1] - cu[s] + QT - 1) / QT : 0;
+    scan[tid] = mine;
+    scan1024(scan, tid);
+    if (s < nseq) base[s] = (int)(carry + scan[tid] - mine);
+    carry += scan[1023];
+    __syncthreads();
+  }
+  const int total = (int)carry;
+  if (tid == 0) { base[nseq] = total; plan[0] = total; plan[1] = cu[nseq]; }
+  bins[tid] = 0;
+  __threadfence_block();
+  __syncthreads();
+  // tiles far down their sequence first: count them by their place, then hand out the places from the back
+  for (int pass = 0; pass < 2; ++pass) {
+    for (int i = tid; i < total; i += 1024) {
+      int lo = 0, hi = nseq;                                 // the sequence with base[s] <= i < base[s + 1]
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (base[mid] <= i) lo = mid; else hi = mid;
+      }
+      const int t = i - base[lo], bin = PLAN_BINS - 1 - min(t, PLAN_BINS - 1);
+      const int at = atomicAdd(&bins[bin], 1);               // the order within a bin changes which workgroup does a tile, not what it does
+      if (pass) {
+        int* e = plan + PLAN_HEAD + 4 * at;
+        e[0] = cu[lo]; e[1] = cu[lo + 1] - cu[lo]; e[2] = t; e[3] = base[lo];
+      }
+    }
+    __syncthreads();
+    if (!pass) {                                             // counts to starting places
+      const int mine = bins[tid];
+      scan[tid] = mine;
+      scan1024(scan, tid);
+      bins[tid] = (int)scan[tid] - mine;
+      __syncthreads();
+    }
+  }
+}
+
+// --------------------------------------------------------------------------------------------------- tiles and fragments
+// A tile in LDS: rows of DP 16-bit values, in slots of 16 bytes.  Slot s of row r lies at s ^ swizzle(r): the row-wise fragments read
+// 16 rows of one slot in a cycle (ds_read_b128), the transposed ones 4 rows of four neighbouring slots, and both then touch every bank
+// once.
+template <int DP>
+__device__ __forceinline__ int tile_at(int row, int slot) {
+  const int x = DP == 128 ? ((row & 3) << 2 | (row >> 2 & 3)) : ((row >> 1 & 1) << 2 | (row >> 2 & 3));
+  return row * (DP * 2) + ((slot ^ x) << 4);
+}
+
+// rows [row0, row0 + KT) of a head into registers: zeros past `rows` and past D
+template <int DP> struct Staged { u32x4_t v[KT * DP / 8 / 256]; };
+template <int DP>
+__device__ __forceinline__ void stage_load(Staged<DP>& st, const unsigned short* base, long ts, int row0, int rows, int D, int tid) {
+#pragma unroll
+  for (int i = 0; i < KT * DP / 8 / 256; ++i) {
+    const int c = tid + i * 256, row = row0 + c / (DP / 8), col = c % (DP / 8) * 8;
+    st.v[i] = row < rows && col < D ? *(const u32x4_t*)(base + (long)row * ts + col) : (u32x4_t){0u, 0u, 0u, 0u};
+  }
+}
+template <int DP>
+__device__ __forceinline__ void stage_store(const Staged<DP>& st, char* lds, int tid) {
+#pragma unroll
+  for (int i = 0; i < KT * DP / 8 / 256; ++i) {
+    const int c = tid + i * 256;
+    *(u32x4_t*)(lds + tile_at<DP>(c / (DP / 8), c % (DP / 8))) = st.v[i];
+  }
+}
+// A operand from rows: row = 32 rb + (lane & 31), columns 16 ks + 8 (lane >> 5) ..
+template <int DP>
+__device__ __forceinline__ lpx8_t row_frag(const char* lds, int rb, int ks, int lane) {
+  return *(const lpx8_t*)(lds + tile_at<DP>(rb * 32 + (lane & 31), ks * 2 + (lane >> 5)));
+}
+// A operand from columns: column 32 cb + (lane & 31), the 16 rows 16 rk .. in the order of a 32x32 accumulator's registers
+template <int DP>
+__device__ __forceinline__ lpx8_t col_frag(const char* lds, int rk, int cb, int lane) {
+  const int i = lane & 15, col = cb * 32 + (lane >> 4 & 1) * 16 + 4 * (i & 3);
+  const int row = rk * 16 + 4 * (lane >> 5) + (i >> 2);
+  const lpx4_t lo = lds_read_tr16(lds + tile_at<DP>(row, col >> 3) + (col & 7) * 2);
+  const lpx4_t hi = lds_read_tr16(lds + tile_at<DP>(row + 8, col >> 3) + (col & 7) * 2);
+  return (lpx8_t){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+}
+// B operand kept in registers: row `row` of a head (zeros past D), columns 16 ks + 8 (lane >> 5) ..
+__device__ __forceinline__ lpx8_t global_frag(const unsigned short* base, int ks, int D, int lane) {
+  const int col = ks * 16 + 8 * (lane >> 5);
+  return col < D ? *(const lpx8_t*)(base + col) : (lpx8_t){0, 0, 0, 0, 0, 0, 0, 0};
+}
+// registers 8 rk .. 8 rk + 7 of an accumulator as the B operand of a product over its rows
+template <class E>
+__device__ __forceinline__ lpx8_t acc_frag(const f32x16& p, int rk) {
+  const u32x4_t u = {E::pack(p[8 * rk], p[8 * rk + 1]), E::pack(p[8 * rk + 2], p[8 * rk + 3]), E::pack(p[8 * rk + 4], p[8 * rk + 5]),
+                     E::pack(p[8 * rk + 6], p[8 * rk + 7])};
+  return __builtin_bit_cast(lpx8_t, u);
+}
+// row of a 32x32 accumulator's register r
+__device__ __forceinline__ int acc_row(int r, int lane) { return (r >> 2) * 8 + (lane >> 5) * 4 + (r & 3); }
+__device__ __forceinline__ f32x16 zero16() { return (f32x16){0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}; }
+
+// ---- values that are not finite in a tile that the mask crosses
+template <class E>
+__device__ __forceinline__ unsigned finite_mask(unsigned u) {          // 0xffff in each half that holds a finite value
+  const unsigned t = ~u & E::kExpMask;
+  return ((t & 0xffffu) ? 0xffffu : 0u) | ((t >> 16) ? 0xffff0000u : 0u);
+}
+template <class E, int DP>
+__device__ __forceinline__ bool tile_nonfinite(const char* lds, int lane) {      // the same answer in every lane of the wave
+  unsigned bad = 0;
+#pragma unroll
+  for (int i = 0; i < KT * DP * 2 / 1024; ++i) {
+    const u32x4_t v = *(const u32x4_t*)(lds + (i * 64 + lane) * 16);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) bad |= ~finite_mask<E>(v[j]);
+  }
+  return __any(bad != 0);
+}
+template <class E>
+__device__ __forceinline__ lpx8_t finite_only(lpx8_t f) {
+  u32x4_t u = __builtin_bit_cast(u32x4_t, f);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) u[j] &= finite_mask<E>(u[j]);
+  return __builtin_bit_cast(lpx8_t, u);
+}
+// acc[cb] holds columns 32 cb .. of the lane's row; `sees(j)`: whether that row sees row j of the tile.  What `finite_only` took out
+// comes back: as itself where it multiplies a probability, as NaN where it multiplies dS, whose sign says nothing.
+template <class E, int DP, bool NAN_ONLY, class Sees>
+__device__ __forceinline__ void add_nonfinite(f32x16 (&acc)[DP / 32], const char* lds, int lane, Sees sees) {
+#pragma unroll 1
+  for (int j = 0; j < KT; ++j) {
+    if (!sees(j)) continue;
+#pragma unroll
+    for (int cb = 0; cb < DP / 32; ++cb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int col = cb * 32 + acc_row(r, lane);
+        const unsigned short b = *(const unsigned short*)(lds + tile_at<DP>(j, col >> 3) + (col & 7) * 2);
+        const float x = E::to_f32(b);
+        if (!__builtin_isfinite(x)) acc[cb][r] += NAN_ONLY ? x - x : x;
+      }
+  }
+}
+
+struct Tile { int first, len, t, base; };
+__device__ __forceinline__ bool plan_entry(const simvg_packed_attn_args& a, int id, Tile& e) {
+  if (id >= a.plan[0]) return false;
+  const int* p = a.plan + PLAN_HEAD + 4 * id;
+  e.first = p[0]; e.len = p[1]; e.t = p[2]; e.base = p[3];
+  return true;
+}
+// a workgroup without an entry: its tile of the rows behind the last sequence, zeros; NaN everywhere where there is no valid plan
+__device__ __forceinline__ void fill_tail(const simvg_packed_attn_args& a, int id, void* out, long ts, long hs, int h, float* lse) {
+  if (!a.fill_tail) return;
+  const bool invalid = a.plan[1] < 0;
+  const int row0 = (invalid ? 0 : a.plan[1]) + (id - a.plan[0]) * QT, rows = min(QT, a.T - row0);
+  const unsigned short value = invalid ? 0x7fff : 0;         // a NaN in fp16 and in bf16
+  for (int i = threadIdx.x; i < rows * a.D; i += 256) ((unsigned short*)out)[(long)(row0 + i / a.D) * ts + (long)h * hs + i % a.D] = value;
+  if (lse)
+    for (int i = threadIdx.x; i < rows; i += 256) lse[(long)h * a.lse_hs + row0 + i] = invalid ? __builtin_nanf("") : 0.f;
+}
+// the 32 x DP block that a wave holds transposed (lane = row, registers = columns) to its rows of `out`
+template <class E, int DP>
+__device__ __forceinline__ void store_rows(const f32x16 (&acc)[DP / 32], float mul, unsigned short* out, int D, bool valid, int lane) {
+#pragma unroll
+  for (int cb = 0; cb < DP / 32; ++cb)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int col = cb * 32 + g * 8 + (lane >> 5) * 4;
+      if (valid && col < D)
+        *(u32x2_t*)(out + col) = (u32x2_t){E::pack(acc[cb][4 * g] * mul, acc[cb][4 * g + 1] * mul),
+                                           E::pack(acc[cb][4 * g + 2] * mul, acc[cb][4 * g + 3] * mul)};
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------- forward
+template <class E, int DP, bool CAUSAL>
+__global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(simvg_packed_attn_args a) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  constexpr int TILE = KT * DP * 2, DB = DP / 32, KS = DP / 16;
+  const int h = blockIdx.x % a.Hq;
+  Tile e;
+  if (!plan_entry(a, blockIdx.x / a.Hq, e)) return fill_tail(a, blockIdx.x / a.Hq, a.o, a.o_ts, a.o_hs, h, a.lse);
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int hk = h / (a.Hq / a.Hkv);
+  const int row = e.t * QT + wave * 32 + (lane & 31);        // the lane's query
+  const bool valid = row < e.len;
+  const unsigned short* qp = (const unsigned short*)a.q + (long)(e.first + min(row, e.len - 1)) * a.q_ts + (long)h * a.q_hs;
+  const unsigned short* kp = (const unsigned short*)a.k + (long)e.first * a.k_ts + (long)hk * a.k_hs;
+  const unsigned short* vp = (const unsigned short*)a.v + (long)e.first * a.v_ts + (long)hk * a.v_hs;
+  const int keys = CAUSAL ? min(e.len, (e.t + 1) * QT) : e.len, tiles = (keys + KT - 1) / KT;
+  const int wave_first = e.t * QT + wave * 32;               // the wave's first query
+  const int wave_tiles = CAUSAL ? min(tiles, (wave_first + 32 + KT - 1) / KT) : tiles;
+
+  Staged<DP> sk, sv;
+  stage_load<DP>(sk, kp, a.k_ts, 0, e.len, a.D, tid);
+  stage_load<DP>(sv, vp, a.v_ts, 0, e.len, a.D, tid);
+  lpx8_t qf[KS];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) qf[ks] = global_frag(qp, ks, a.D, lane);
+  f32x16 o[DB];
+#pragma unroll
+  for (int i = 0; i < DB; ++i) o[i] = zero16();
+  const float c = a.scale * LOG2E;
+  float m = NEG_INF, l = 0.f;                                // reference of the exponentials (raw scores), sum over this half's keys
+  stage_store<DP>(sk, smem, tid);
+  stage_store<DP>(sv, smem + 2 * TILE, tid);
+  __syncthreads();
+  for (int kt = 0; kt < tiles; ++kt) {
+    const char *lk = smem + (kt & 1) * TILE, *lv = smem + (2 + (kt & 1)) * TILE;
+    if (kt + 1 < tiles) {
+      stage_load<DP>(sk, kp, a.k_ts, (kt + 1) * KT, e.len, a.D, tid);
+      stage_load<DP>(sv, vp, a.v_ts, (kt + 1) * KT, e.len, a.D, tid);
+    }
+    if (kt < wave_tiles) {
+      f32x16 s[2];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        s[kb] = zero16();
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) s[kb] = E::mfma(row_frag<DP>(lk, kb, ks, lane), qf[ks], s[kb]);
+      }
+      const bool masked = (CAUSAL && kt * KT + KT - 1 > wave_first) || kt * KT + KT > e.len;
+      if (masked) {
+        const int last = CAUSAL ? min(row, e.len - 1) : e.len - 1;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (kt * KT + kb * 32 + acc_row(r, lane) > last) s[kb][r] = NEG_INF;
+      }
+      float top = NEG_INF;
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[kb][r]);
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      // the reference follows the maximum only where it has grown by more than 2^8: the exponentials stay below 2^8, and what is
+      // left of O and l need not be scaled at every tile
+      if (__any((top - m) * c > 8.f)) {
+        const float to = fmaxf(m, top), f = m == to ? 1.f : __builtin_amdgcn_exp2f((m - to) * c);
+        m = to;
+        l *= f;
+#pragma unroll
+        for (int i = 0; i < DB; ++i) o[i] *= f;
+      }
+      const float mc = m * c;
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[kb][r] = __builtin_amdgcn_exp2f(fmaf(s[kb][r], c, -mc));
+          l += s[kb][r];
+        }
+      const bool odd = masked && tile_nonfinite<E, DP>(lv, lane);
+#pragma unroll
+      for (int rk = 0; rk < 4; ++rk) {
+        const lpx8_t p = acc_frag<E>(s[rk >> 1], rk & 1);
+#pragma unroll
+        for (int cb = 0; cb < DB; ++cb) {
+          lpx8_t vf = col_frag<DP>(lv, rk, cb, lane);
+          if (odd) vf = finite_only<E>(vf);
+          o[cb] = E::mfma(vf, p, o[cb]);
+        }
+      }
+      if (odd) {
+        const int last = (CAUSAL ? min(row, e.len - 1) : e.len - 1) - kt * KT;
+        add_nonfinite<E, DP, false>(o, lv, lane, [&](int j) { return j <= last; });
+      }
+    }
+    if (kt + 1 < tiles) {
+      stage_store<DP>(sk, smem + ((kt + 1) & 1) * TILE, tid);
+      stage_store<DP>(sv, smem + (2 + ((kt + 1) & 1)) * TILE, tid);
+    }
+    __syncthreads();
+  }
+  l += __shfl_xor(l, 32, 64);
+  unsigned short* out = (unsigned short*)a.o + (long)(e.first + row) * a.o_ts + (long)h * a.o_hs;
+  store_rows<E, DP>(o, 1.f / l, out, a.D, valid, lane);
+  if (valid && lane < 32) a.lse[(long)h * a.lse_hs + e.first + row] = m * a.scale + __builtin_logf(l);
+}
+
+// ------------------------------------------------------------------------------------------------------------ backward
+// delta_i = sum_d dO_id O_id.  For fp16 also the largest norms of dO's and V's rows in a tile and head: |dP_ij| and |D_i| are at most
+// |dO_i| |V_j|, so with them dS can be brought to where fp16 has all its bits (`grad_power`).
+// ws: delta [Hq][T] | norms of dO [tiles][Hq] | norms of V [tiles][Hkv]
+struct Ws { float *delta, *ndo, *nv; };
+__device__ __forceinline__ Ws ws_of(const simvg_packed_attn_args& a) {
+  Ws w;
+  w.delta = a.ws;
+  w.ndo = a.ws + (long)a.Hq * a.T;
+  w.nv = w.ndo + (long)plan_capacity(a.T, a.nseq) * a.Hq;
+  return w;
+}
+template <class E>
+__device__ __forceinline__ float dot8(u32x4_t x, u32x4_t y, float s) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float a0, a1, b0, b1;
+    unpack2<E>(x[j], a0, a1);
+    unpack2<E>(y[j], b0, b1);
+    s = fmaf(a0, b0, s);
+    s = fmaf(a1, b1, s);
+  }
+  return s;
+}
+template <class E>
+__global__ __launch_bounds__(256) void packed_attn_delta_kernel(simvg_packed_attn_args a) {
+  __shared__ float most[2][4];
+  const int h = blockIdx.x % a.Hq, G = a.Hq / a.Hkv;
+  Tile e;
+  if (!plan_entry(a, blockIdx.x / a.Hq, e)) return;
+  const Ws w = ws_of(a);
+  const int lane16 = threadIdx.x & 15, n = min(QT, e.len - e.t * QT);
+  const bool with_v = E::kScaled && h % G == 0;
+  float mdo = 0.f, mv = 0.f;
+  // 16 lanes a row, 8 columns each: D <= 128
+  for (int r = threadIdx.x >> 4; r < QT; r += 16) {
+    const long row = e.first + e.t * QT + min(r, n - 1);
+    const int col = lane16 * 8;
+    float d = 0.f, sd = 0.f, sv = 0.f;
+    if (col < a.D) {
+      const u32x4_t x = *(const u32x4_t*)((const unsigned short*)a.d_o + row * a.do_ts + (long)h * a.do_hs + col);
+      const u32x4_t y = *(const u32x4_t*)((const unsigned short*)a.o + row * a.o_ts + (long)h * a.o_hs + col);
+      d = dot8<E>(x, y, 0.f);
+      if (E::kScaled) sd = dot8<E>(x, x, 0.f);
+      if (with_v) {
+        const u32x4_t z = *(const u32x4_t*)((const unsigned short*)a.v + row * a.v_ts + (long)(h / G) * a.v_hs + col);
+        sv = dot8<E>(z, z, 0.f);
+      }
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) {
+      d += __shfl_xor(d, o, 64);
+      if (E::kScaled) { sd += __shfl_xor(sd, o, 64); sv += __shfl_xor(sv, o, 64); }
+    }
+    if (r < n && lane16 == 0) w.delta[(long)h * a.T + row] = d;
+    if (__builtin_isfinite(sd)) mdo = fmaxf(mdo, sd);        // a row that is not finite has no gradient that a scale could save
+    if (__builtin_isfinite(sv)) mv = fmaxf(mv, sv);
+  }
+  if constexpr (E::kScaled) {
+    mdo = wave_max(mdo);
+    mv = wave_max(mv);
+    if ((threadIdx.x & 63) == 0) { most[0][threadIdx.x >> 6] = mdo; most[1][threadIdx.x >> 6] = mv; }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      const long tile = e.base + e.t;
+      w.ndo[tile * a.Hq + h] = sqrtf(fmaxf(fmaxf(most[0][0], most[0][1]), fmaxf(most[0][2], most[0][3])));
+      if (with_v) w.nv[tile * a.Hkv + h / G] = sqrtf(fmaxf(fmaxf(most[1][0], most[1][1]), fmaxf(most[1][2], most[1][3])));
+    }
+  }
+}
+// fp16: what is rounded to 16 bits is P 2^14 (P <= 1: the largest is 2^14) and dS 2^14 2^-x with 2^x at least the sequence's and key
+// head's largest |dO_i| |V_j|: at most 2^15.  A probability of 2^-28 then still has all its bits.  Both powers are exact and come out
+// of the sums in 32 bits.  bf16 has fp32's exponents: no scale.
+constexpr float P_POWER = 14.f;
+template <class E>
+__device__ __forceinline__ float grad_power(const simvg_packed_attn_args& a, const Tile& e, int hk, float* red) {
+  if constexpr (!E::kScaled) return 0.f;
+  const Ws w = ws_of(a);
+  const int tiles = (e.len + QT - 1) / QT, G = a.Hq / a.Hkv;
+  float mdo = 0.f, mv = 0.f;
+  for (int i = threadIdx.x; i < tiles * G; i += 256) mdo = fmaxf(mdo, w.ndo[(long)(e.base + i / G) * a.Hq + hk * G + i % G]);
+  for (int i = threadIdx.x; i < tiles; i += 256) mv = fmaxf(mv, w.nv[(long)(e.base + i) * a.Hkv + hk]);
+  mdo = wave_max(mdo);
+  mv = wave_max(mv);
+  if ((threadIdx.x & 63) == 0) { red[threadIdx.x >> 6] = mdo; red[4 + (threadIdx.x >> 6)] = mv; }
+  __syncthreads();
+  mdo = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  mv = fmaxf(fmaxf(red[4], red[5]), fmaxf(red[6], red[7]));
+  const float most = mdo * mv;
+  if (!(most > 0.f)) return 0.f;
+  return fminf(fmaxf(-ceilf(__builtin_log2f(most) + 1e-3f), -60.f), 60.f);
+}
+
+// dQ: a workgroup's 128 queries against the tiles of their keys, as in the forward pass
+template <class E, int DP, bool CAUSAL>
+__global__ __launch_bounds__(256, 2) void packed_attn_dq_kernel(simvg_packed_attn_args a) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  __shared__ float red[8];
+  constexpr int TILE = KT * DP * 2, DB = DP / 32, KS = DP / 16;
+  const int h = blockIdx.x % a.Hq;
+  Tile e;
+  if (!plan_entry(a, blockIdx.x / a.Hq, e)) return fill_tail(a, blockIdx.x / a.Hq, a.dq, a.dq_ts, a.dq_hs, h, nullptr);
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int hk = h / (a.Hq / a.Hkv);
+  const float power = grad_power<E>(a, e, hk, red), up = __builtin_amdgcn_exp2f(power), shift = E::kScaled ? P_POWER : 0.f;
+  const int row = e.t * QT + wave * 32 + (lane & 31);
+  const bool valid = row < e.len;
+  const long at = e.first + min(row, e.len - 1);
+  const unsigned short* qp = (const unsigned short*)a.q + at * a.q_ts + (long)h * a.q_hs;
+  const unsigned short* dop = (const unsigned short*)a.d_o + at * a.do_ts + (long)h * a.do_hs;
+  const unsigned short* kp = (const unsigned short*)a.k + (long)e.first * a.k_ts + (long)hk * a.k_hs;
+  const unsigned short* vp = (const unsigned short*)a.v + (long)e.first * a.v_ts + (long)hk * a.v_hs;
+  const int keys = CAUSAL ? min(e.len, (e.t + 1) * QT) : e.len, tiles = (keys + KT - 1) / KT;
+  const int wave_first = e.t * QT + wave * 32;
+  const int wave_tiles = CAUSAL ? min(tiles, (wave_first + 32 + KT - 1) / KT) : tiles;
+  Staged<DP> sk, sv;
+  stage_load<DP>(sk, kp, a.k_ts, 0, e.len, a.D, tid);
+  stage_load<DP>(sv, vp, a.v_ts, 0, e.len, a.D, tid);
+  lpx8_t qf[KS], dof[KS];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) { qf[ks] = global_frag(qp, ks, a.D, lane); dof[ks] = global_frag(dop, ks, a.D, lane); }
+  const float c = a.scale * LOG2E, lse2 = a.lse[(long)h * a.lse_hs + at] * LOG2E - shift;
+  const float delta = ws_of(a).delta[(long)h * a.T + at];
+  f32x16 dq[DB];
+#pragma unroll
+  for (int i = 0; i < DB; ++i) dq[i] = zero16();
+  stage_store<DP>(sk, smem, tid);
+  stage_store<DP>(sv, smem + 2 * TILE, tid);
+  __syncthreads();
+  for (int kt = 0; kt < tiles; ++kt) {
+    const char *lk = smem + (kt & 1) * TILE, *lv = smem + (2 + (kt & 1)) * TILE;
+    if (kt + 1 < tiles) {
+      stage_load<DP>(sk, kp, a.k_ts, (kt + 1) * KT, e.len, a.D, tid);
+      stage_load<DP>(sv, vp, a.v_ts, (kt + 1) * KT, e.len, a.D, tid);
+    }
+    if (kt < wave_tiles) {
+      const bool masked = (CAUSAL && kt * KT + KT - 1 > wave_first) || kt * KT + KT > e.len;
+      const bool odd = masked && tile_nonfinite<E, DP>(lk, lane);
+      const int last = (CAUSAL ? min(row, e.len - 1) : e.len - 1) - kt * KT;
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          s = E::mfma(row_frag<DP>(lk, kb, ks, lane), qf[ks], s);
+          dp = E::mfma(row_frag<DP>(lv, kb, ks, lane), dof[ks], dp);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float p = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse2));
+          s[r] = p * ((dp[r] - delta) * up);
+          if (masked && kb * 32 + acc_row(r, lane) > last) s[r] = 0.f;
+        }
+#pragma unroll
+        for (int rk = 0; rk < 2; ++rk) {
+          const lpx8_t ds = acc_frag<E>(s, rk);
+#pragma unroll
+          for (int cb = 0; cb < DB; ++cb) {
+            lpx8_t kf = col_frag<DP>(lk, kb * 2 + rk, cb, lane);
+            if (odd) kf = finite_only<E>(kf);
+            dq[cb] = E::mfma(kf, ds, dq[cb]);
+          }
+        }
+      }
+      if (odd) add_nonfinite<E, DP, true>(dq, lk, lane, [&](int j) { return j <= last; });
+    }
+    if (kt + 1 < tiles) {
+      stage_store<DP>(sk, smem + ((kt + 1) & 1) * TILE, tid);
+      stage_store<DP>(sv, smem + (2 + ((kt + 1) & 1)) * TILE, tid);
+    }
+    __syncthreads();
+  }
+  unsigned short* out = (unsigned short*)a.dq + (long)(e.first + row) * a.dq_ts + (long)h * a.dq_hs;
+  store_rows<E, DP>(dq, a.scale * __builtin_amdgcn_exp2f(-power - shift), out, a.D, valid, lane);
+}
+
+// dK, dV: a workgroup's 128 keys against the tiles of the queries that see them, of all heads that share the key head, one after the
+// other: the sum over heads stays in the accumulators and needs no atomics.
+template <class E, int DP, bool CAUSAL>
+__global__ __launch_bounds__(256, 1) void packed_attn_dkv_kernel(simvg_packed_attn_args a) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  __shared__ float red[8], stat[2][2][KT];
+  constexpr int TILE = KT * DP * 2, DB = DP / 32, KS = DP / 16;
+  const int hk = blockIdx.x % a.Hkv, G = a.Hq / a.Hkv;
+  Tile e;
+  if (!plan_entry(a, blockIdx.x / a.Hkv, e)) {
+    fill_tail(a, blockIdx.x / a.Hkv, a.dk, a.dk_ts, a.dk_hs, hk, nullptr);
+    return fill_tail(a, blockIdx.x / a.Hkv, a.dv, a.dv_ts, a.dv_hs, hk, nullptr);
+  }
+  const int ntile = (e.len + QT - 1) / QT;
+  if (CAUSAL) e.t = ntile - 1 - e.t;                         // the plan's order is by cost: the first keys are seen by the most queries
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const float power = grad_power<E>(a, e, hk, red), up = __builtin_amdgcn_exp2f(power), shift = E::kScaled ? P_POWER : 0.f;
+  const int key = e.t * QT + wave * 32 + (lane & 31);        // the lane's key
+  const bool valid = key < e.len;
+  const long at = e.first + min(key, e.len - 1);
+  const unsigned short* kp = (const unsigned short*)a.k + at * a.k_ts + (long)hk * a.k_hs;
+  const unsigned short* vp = (const unsigned short*)a.v + at * a.v_ts + (long)hk * a.v_hs;
+  const int first = CAUSAL ? e.t * QT / KT : 0, tiles = (e.len + KT - 1) / KT - first;       // tiles of queries, from `first`
+  const int wave_first = e.t * QT + wave * 32;
+  lpx8_t kf[KS], vf[KS];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) { kf[ks] = global_frag(kp, ks, a.D, lane); vf[ks] = global_frag(vp, ks, a.D, lane); }
+  const float c = a.scale * LOG2E;
+  const float* delta = ws_of(a).delta;
+  f32x16 dk[DB], dv[DB];
+#pragma unroll
+  for (int i = 0; i < DB; ++i) { dk[i] = zero16(); dv[i] = zero16(); }
+  Staged<DP> sq, sd;
+  float st0 = 0.f;
+  auto load = [&](int i) {                                   // step i: head hk G + i / tiles, query tile first + i % tiles
+    const int h = hk * G + i / tiles, row0 = (first + i % tiles) * KT;
+    stage_load<DP>(sq, (const unsigned short*)a.q + (long)e.first * a.q_ts + (long)h * a.q_hs, a.q_ts, row0, e.len, a.D, tid);
+    stage_load<DP>(sd, (const unsigned short*)a.d_o + (long)e.first * a.do_ts + (long)h * a.do_hs, a.do_ts, row0, e.len, a.D, tid);
+    if (tid < 2 * KT) {                                      // rows past the sequence are zeros with lse 0: P stays finite, times 0
+      const int row = row0 + (tid & (KT - 1));
+      st0 = 0.f;
+      if (row < e.len) st0 = tid < KT ? a.lse[(long)h * a.lse_hs + e.first + row] * LOG2E - shift : delta[(long)h * a.T + e.first + row];
+    }
+  };
+  auto store = [&](int buf) {
+    stage_store<DP>(sq, smem + buf * TILE, tid);
+    stage_store<DP>(sd, smem + (2 + buf) * TILE, tid);
+    if (tid < 2 * KT) stat[buf][tid / KT][tid & (KT - 1)] = st0;
+  };
+  load(0);
+  store(0);
+  __syncthreads();
+  const int steps = G * tiles;
+  for (int i = 0; i < steps; ++i) {
+    const char *lq = smem + (i & 1) * TILE, *ld = smem + (2 + (i & 1)) * TILE;
+    const float *lse = stat[i & 1][0], *del = stat[i & 1][1];
+    if (i + 1 < steps) load(i + 1);
+    const int row0 = (first + i % tiles) * KT;
+    if (!CAUSAL || row0 + KT - 1 >= wave_first) {
+      const bool masked = CAUSAL && row0 < wave_first + 31;
+      const bool odd = masked && (tile_nonfinite<E, DP>(lq, lane) || tile_nonfinite<E, DP>(ld, lane));
+      const int from = key - row0;                           // the first row of the tile that sees the lane's key
+#pragma unroll
+      for (int qb = 0; qb < 2; ++qb) {
+        f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          s = E::mfma(row_frag<DP>(lq, qb, ks, lane), kf[ks], s);
+          dp = E::mfma(row_frag<DP>(ld, qb, ks, lane), vf[ks], dp);
+        }
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const f32x4_t ls = *(const f32x4_t*)(lse + qb * 32 + g * 8 + (lane >> 5) * 4);
+          const f32x4_t dl = *(const f32x4_t*)(del + qb * 32 + g * 8 + (lane >> 5) * 4);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int x = 4 * g + r;
+            float p = __builtin_amdgcn_exp2f(fmaf(s[x], c, -ls[r]));
+            float ds = p * ((dp[x] - dl[r]) * up);
+            if (masked && qb * 32 + acc_row(x, lane) < from) { p = 0.f; ds = 0.f; }
+            s[x] = p;
+            dp[x] = ds;
+          }
+        }
+#pragma unroll
+        for (int rk = 0; rk < 2; ++rk) {
+          const lpx8_t p = acc_frag<E>(s, rk), ds = acc_frag<E>(dp, rk);
+#pragma unroll
+          for (int cb = 0; cb < DB; ++cb) {
+            lpx8_t df = col_frag<DP>(ld, qb * 2 + rk, cb, lane), qf = col_frag<DP>(lq, qb * 2 + rk, cb, lane);
+            if (odd) { df = finite_only<E>(df); qf = finite_only<E>(qf); }
+            dv[cb] = E::mfma(df, p, dv[cb]);
+            dk[cb] = E::mfma(qf, ds, dk[cb]);
+          }
+        }
+      }
+      if (odd) {
+        add_nonfinite<E, DP, false>(dv, ld, lane, [&](int j) { return j >= from; });
+        add_nonfinite<E, DP, true>(dk, lq, lane, [&](int j) { return j >= from; });
+      }
+    }
+    if (i + 1 < steps) store((i + 1) & 1);
+    __syncthreads();
+  }
+  store_rows<E, DP>(dv, __builtin_amdgcn_exp2f(-shift), (unsigned short*)a.dv + (long)(e.first + key) * a.dv_ts + (long)hk * a.dv_hs, a.D,
+                    valid, lane);
+  store_rows<E, DP>(dk, a.scale * __builtin_amdgcn_exp2f(-power - shift),
+                    (unsigned short*)a.dk + (long)(e.first + key) * a.dk_ts + (long)hk * a.dk_hs, a.D, valid, lane);
+}
+
+// ---------------------------------------------------------------------------------------------------------------- host
+bool rows16(const void* p, long ts, long hs) { return p && (uintptr_t)p % 16 == 0 && ts % 8 == 0 && hs % 8 == 0; }
+
+int attn_check(const simvg_packed_attn_args* a, bool bwd) {
+  SIMVG_CHECK_ARG(a, "packed_attn: null argument block");
+  SIMVG_CHECK_ARG(a->dtype == SEQ_F16 || a->dtype == SEQ_BF16, "packed_attn: dtype must be fp16 or bf16");
+  SIMVG_CHECK_ARG(a->T >= 0 && a->nseq >= 0 && a->nseq <= 1 << 24, "packed_attn: T and nseq must not be negative");
+  SIMVG_CHECK_ARG(a->Hkv >= 1 && a->Hq >= a->Hkv && a->Hq % a->Hkv == 0, "packed_attn: the heads of q must be a multiple of those of k and v");
+  SIMVG_CHECK_ARG(a->D >= 8 && a->D <= 128 && a->D % 8 == 0, "packed_attn: the head size must be a multiple of 8 and at most 128");
+  SIMVG_CHECK_ARG(a->scale > 0.f && a->scale < __builtin_huge_valf(), "packed_attn: scale must be positive and finite");
+  SIMVG_CHECK_ARG((long)plan_capacity(a->T, a->nseq) * a->Hq < 0x7fffffffL, "packed_attn: too many tiles for one launch");
+  if (a->T == 0) return SIMVG_OK;
+  SIMVG_CHECK_ARG(a->plan && a->lse, "packed_attn: null pointer");
+  SIMVG_CHECK_ARG((uintptr_t)a->plan % 4 == 0, "packed_attn: misaligned plan");
+  SIMVG_CHECK_ARG(rows16(a->q, a->q_ts, a->q_hs) && rows16(a->k, a->k_ts, a->k_hs) && rows16(a->v, a->v_ts, a->v_hs) &&
+                  rows16(a->o, a->o_ts, a->o_hs), "packed_attn: rows of q, k, v and out must start at multiples of 16 bytes");
+  if (bwd) {
+    SIMVG_CHECK_ARG(rows16(a->d_o, a->do_ts, a->do_hs) && rows16(a->dq, a->dq_ts, a->dq_hs) && rows16(a->dk, a->dk_ts, a->dk_hs) &&
+                    rows16(a->dv, a->dv_ts, a->dv_hs), "packed_attn: rows of the gradients must start at multiples of 16 bytes");
+    SIMVG_CHECK_ARG(a->ws, "packed_attn: the backward pass needs a workspace");
+  }
+  return SIMVG_OK;
+}
+
+template <class E, int DP, bool CAUSAL>
+void attn_launch(const simvg_packed_attn_args& a, bool bwd, hipStream_t s) {
+  const int entries = plan_capacity(a.T, a.nseq), lds = 4 * KT * DP * 2;
+  if (!bwd) {
+    hipLaunchKernelGGL((packed_attn_fwd_kernel<E, DP, CAUSAL>), dim3(entries * a.Hq), dim3(256), lds, s, a);
+    return;
+  }
+  hipLaunchKernelGGL((packed_attn_delta_kernel<E>), dim3(entries * a.Hq), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((packed_attn_dq_kernel<E, DP, CAUSAL>), dim3(entries * a.Hq), dim3(256), lds, s, a);
+  hipLaunchKernelGGL((packed_attn_dkv_kernel<E, DP, CAUSAL>), dim3(entries * a.Hkv), dim3(256), lds, s, a);
+}
+template <class E>
+void attn_dispatch(const simvg_packed_attn_args& a, bool bwd, hipStream_t s) {
+  if (a.D <= 64) a.causal ? attn_launch<E, 64, true>(a, bwd, s) : attn_launch<E, 64, false>(a, bwd, s);
+  else a.causal ? attn_launch<E, 128, true>(a, bwd, s) : attn_launch<E, 128, false>(a, bwd, s);
+}
+int attn_run(const simvg_packed_attn_args* a, bool bwd, hipStream_t s) {
+  const int rc = attn_check(a, bwd);
+  if (rc || a->T == 0) return rc;
+  if (a->dtype == SEQ_F16) attn_dispatch<F16>(*a, bwd, s);
+  else attn_dispatch<BF16>(*a, bwd, s);
+  SIMVG_LAUNCH_CHECK();
+  return SIMVG_OK;
+}
+}  // namespace
+
+extern "C" long simvg_packed_plan_ints(int T, int nseq) {
+  return T < 0 || nseq < 0 ? 0 : PLAN_HEAD + 4L * plan_capacity(T, nseq) + nseq + 1;
+}
+extern "C" int simvg_packed_plan(const int* cu_seqlens, int nseq, int T, int* plan, hipStream_t stream) {
+  SIMVG_CHECK_ARG(T >= 0 && nseq >= 0 && nseq <= 1 << 24, "packed_plan: T and nseq must not be negative");
+  SIMVG_CHECK_ARG(cu_seqlens && plan, "packed_plan: null pointer");
+  hipLaunchKernelGGL(packed_plan_kernel, dim3(1), dim3(1024), 0, stream, cu_seqlens, nseq, T, plan);
+  SIMVG_LAUNCH_CHECK();
+  return SIMVG_OK;
+}
+extern "C" long simvg_packed_attn_ws_floats(int T, int nseq, int Hq, int Hkv) {
+  return T < 0 || nseq < 0 ? 0 : (long)Hq * T + (long)plan_capacity(T, nseq) * (Hq + Hkv);
+}
+extern "C" int simvg_packed_attn_fwd(const simvg_packed_attn_args* args, hipStream_t stream) { return attn_run(args, false, stream); }
+extern "C" int simvg_packed_attn_bwd(const simvg_packed_attn_args* args, hipStream_t stream) { return attn_run(args, true, stream); }

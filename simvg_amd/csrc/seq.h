@@ -1,0 +1,70 @@
+// Shared by the sequence operators (rope.hip, packed_attn.hip, vocab_ce.hip): element types chosen per call, 32x32 MFMA fragments.
+// The encoder's kernels are built for ONE 16-bit format (common.h, "lp"); these take either of the two as an argument, because what
+// they read comes from a caller's language model and not from this library's encoder.  Rounding to 16 bits is round-to-nearest-even
+// and does not saturate: an overflow is an inf, as in torch, and a loss scaler can see it.
+#pragma once
+#include "common.h"
+
+// element types of the `dtype` arguments (include/simvg_hip.h: SIMVG_F32, SIMVG_F16, SIMVG_BF16)
+enum { SEQ_F32 = 0, SEQ_F16 = 1, SEQ_BF16 = 2 };
+
+namespace seq {
+
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((ext_vector_type(2))) float f32x2;
+
+struct F16 {
+  static constexpr bool kScaled = true;                 // 5 exponent bits: what a backward pass rounds is brought into range first
+  static constexpr unsigned kExpMask = 0x7c007c00u;
+  static __device__ __forceinline__ float to_f32(unsigned short v) { return (float)__builtin_bit_cast(_Float16, v); }
+  static __device__ __forceinline__ unsigned pack(float a, float b) {
+    return __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2){a, b}, half2v));
+  }
+  static __device__ __forceinline__ f32x16 mfma(lpx8_t a, lpx8_t b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+  }
+};
+struct BF16 {
+  static constexpr bool kScaled = false;
+  static constexpr unsigned kExpMask = 0x7f807f80u;
+  static __device__ __forceinline__ float to_f32(unsigned short v) { return __uint_as_float((unsigned)v << 16); }
+  static __device__ __forceinline__ unsigned pack(float a, float b) {
+    return __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2){a, b}, bf2));
+  }
+  static __device__ __forceinline__ f32x16 mfma(lpx8_t a, lpx8_t b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf8, a), __builtin_bit_cast(bf8, b), c, 0, 0, 0);
+  }
+};
+
+template <class E>
+__device__ __forceinline__ void unpack2(unsigned u, float& lo, float& hi) {
+  lo = E::to_f32((unsigned short)(u & 0xffffu));
+  hi = E::to_f32((unsigned short)(u >> 16));
+}
+
+// ---- HBM -> LDS without registers (LDS-DMA), 16 bytes a lane: LDS bytes [lds, lds + 1024) of the wave get what its lanes' offsets
+// name, in the lanes' order; an offset at or past `bytes` of the buffer reads zeros.  The instruction is written in asm because hipcc
+// puts `s_waitcnt vmcnt(0)` in front of every LDS read that may alias a DMA it knows of, which would wait for the tile that has just
+// been asked for; it has no register output, so nothing can be taken before it has arrived.  The caller counts: `dma_wait<N>` leaves
+// the N youngest in flight, and a barrier makes the others' pieces visible.
+__device__ __forceinline__ u32x4_t dma_buffer(const void* base, unsigned bytes) {
+  const unsigned long p = (unsigned long)base;
+  return (u32x4_t){(unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)p), (unsigned)__builtin_amdgcn_readfirstlane((int)(p >> 32) & 0xffff),
+                   (unsigned)__builtin_amdgcn_readfirstlane((int)bytes), 0x00020000u};
+}
+__device__ __forceinline__ void dma16(u32x4_t buffer, unsigned lds, unsigned offset) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane((int)lds)),
+               "v"(offset), "s"(buffer)
+               : "memory", "m0");
+}
+constexpr unsigned DMA_NOTHING = 0x80000000u;          // an offset past every buffer: zeros
+template <int N>
+__device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+// a barrier that does not drain this wave's DMA (what `__syncthreads` would wait for is the caller's business here)
+__device__ __forceinline__ void wave_barrier_only() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+}  // namespace seq
