@@ -1,3 +1,4 @@
+// simvg-build-flags: -Wno-inline-asm
 // Attention over packed sequences, forward and backward: rows [cu[s], cu[s + 1]) of q, k, v are sequence s.  A row sees the keys of its
 // own sequence, under `causal` those up to itself; Hq heads of q share Hkv heads of k and v, G = Hq / Hkv neighbours each.
 //
@@ -17,8 +18,10 @@
 //
 // Masks: rows and keys past a sequence are zeros in LDS and are never stored, so nothing of a neighbour is read.  In a tile that the
 // diagonal crosses, P is an exact 0 above it, and 0 x inf in the matrix product would still carry a later row's inf or NaN to an
-// earlier one: such a tile is looked through for values that are not finite, and if there are any they are taken out of the operand and
-// added, as themselves, to the rows that do see them (see `add_nonfinite`).
+// earlier one: such a tile is looked through for values that are not finite, and if there are any they are added, as themselves, to the
+// rows that do see them and taken out of the tile (`add_nonfinite`, `tile_clean`).
+#include <type_traits>
+
 #include "seq.h"
 
 struct simvg_packed_attn_args {
@@ -122,38 +125,56 @@ __device__ __forceinline__ int tile_at(int row, int slot) {
   return row * (DP * 2) + ((slot ^ x) << 4);
 }
 
-// rows [row0, row0 + KT) of a head into registers: zeros past `rows` and past D
-template <int DP> struct Staged { u32x4_t v[KT * DP / 8 / 256]; };
-template <int DP>
-__device__ __forceinline__ void stage_load(Staged<DP>& st, const unsigned short* base, long ts, int row0, int rows, int D, int tid) {
+// Brings tiles of KT rows of a head from HBM to LDS (LDS-DMA, seq.h): WAVES waves, `issue` asks for rows [row0, row0 + KT) with zeros
+// past `rows` and past D.
+template <int DP, int WAVES> struct Stager {
+  static constexpr int PIECES = KT * DP * 2 / 1024 / WAVES;
+  unsigned off[PIECES];
+  int wave, row[PIECES];
+  __device__ __forceinline__ void init(long ts, int D, int w, int lane) {
+    wave = w;
 #pragma unroll
-  for (int i = 0; i < KT * DP / 8 / 256; ++i) {
-    const int c = tid + i * 256, row = row0 + c / (DP / 8), col = c % (DP / 8) * 8;
-    st.v[i] = row < rows && col < D ? *(const u32x4_t*)(base + (long)row * ts + col) : (u32x4_t){0u, 0u, 0u, 0u};
+    for (int i = 0; i < PIECES; ++i) {
+      const int byte = (i * WAVES + w) * 1024 + lane * 16, phys = byte % (DP * 2) / 16;
+      row[i] = byte / (DP * 2);
+      const int slot = (tile_at<DP>(row[i], phys) - row[i] * DP * 2) >> 4;     // the permutation is its own inverse
+      off[i] = slot * 8 < D ? (unsigned)(row[i] * (int)ts * 2 + slot * 16) : DMA_NOTHING;
+    }
   }
-}
-template <int DP>
-__device__ __forceinline__ void stage_store(const Staged<DP>& st, char* lds, int tid) {
+  __device__ __forceinline__ void issue(const unsigned short* base, long ts, int row0, int rows, unsigned lds) const {
+    const u32x4_t b = dma_buffer(base + (long)row0 * ts, DMA_NOTHING - 1);
+    if (row0 + KT <= rows) {
 #pragma unroll
-  for (int i = 0; i < KT * DP / 8 / 256; ++i) {
-    const int c = tid + i * 256;
-    *(u32x4_t*)(lds + tile_at<DP>(c / (DP / 8), c % (DP / 8))) = st.v[i];
+      for (int i = 0; i < PIECES; ++i) dma16(b, lds + (i * WAVES + wave) * 1024, off[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) dma16(b, lds + (i * WAVES + wave) * 1024, row0 + row[i] < rows ? off[i] : DMA_NOTHING);
+    }
   }
-}
-// A operand from rows: row = 32 rb + (lane & 31), columns 16 ks + 8 (lane >> 5) ..
-template <int DP>
-__device__ __forceinline__ lpx8_t row_frag(const char* lds, int rb, int ks, int lane) {
-  return *(const lpx8_t*)(lds + tile_at<DP>(rb * 32 + (lane & 31), ks * 2 + (lane >> 5)));
-}
-// A operand from columns: column 32 cb + (lane & 31), the 16 rows 16 rk .. in the order of a 32x32 accumulator's registers
-template <int DP>
-__device__ __forceinline__ lpx8_t col_frag(const char* lds, int rk, int cb, int lane) {
-  const int i = lane & 15, col = cb * 32 + (lane >> 4 & 1) * 16 + 4 * (i & 3);
-  const int row = rk * 16 + 4 * (lane >> 5) + (i >> 2);
-  const lpx4_t lo = lds_read_tr16(lds + tile_at<DP>(row, col >> 3) + (col & 7) * 2);
-  const lpx4_t hi = lds_read_tr16(lds + tile_at<DP>(row + 8, col >> 3) + (col & 7) * 2);
-  return (lpx8_t){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-}
+};
+// What a lane adds to a tile's start for its part of a fragment; everything else of an address is a constant in the instruction.
+//   row(rb, ks): A operand from rows: row 32 rb + (lane & 31), columns 16 ks + 8 (lane >> 5) ..
+//   col(rk, cb): A operand from columns: column 32 cb + (lane & 31), the 16 rows 16 rk .. in the order of a 32x32 accumulator's registers
+template <int DP> struct Lanes {
+  static constexpr int ROWB = DP * 2;
+  unsigned r[DP / 16], c[DP / 32][2];
+  __device__ __forceinline__ void init(int lane) {
+    const int i = lane & 15, row = 4 * (lane >> 5) + (i >> 2);
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks) r[ks] = tile_at<DP>(lane & 31, ks * 2 + (lane >> 5));
+#pragma unroll
+    for (int cb = 0; cb < DP / 32; ++cb) {
+      const int col = cb * 32 + (lane >> 4 & 1) * 16 + 4 * (i & 3);
+      c[cb][0] = tile_at<DP>(row, col >> 3) + (col & 7) * 2;
+      c[cb][1] = tile_at<DP>(row + 8, col >> 3) + (col & 7) * 2;
+    }
+  }
+  __device__ __forceinline__ lpx8_t row(const char* tile, int rb, int ks) const { return *(const lpx8_t*)(tile + r[ks] + rb * 32 * ROWB); }
+  __device__ __forceinline__ lpx8_t col(const char* tile, int rk, int cb) const {
+    const lpx4_t lo = lds_read_tr16(tile + c[cb][0] + rk * 16 * ROWB), hi = lds_read_tr16(tile + c[cb][1] + rk * 16 * ROWB);
+    return (lpx8_t){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  }
+};
 // B operand kept in registers: row `row` of a head (zeros past D), columns 16 ks + 8 (lane >> 5) ..
 __device__ __forceinline__ lpx8_t global_frag(const unsigned short* base, int ks, int D, int lane) {
   const int col = ks * 16 + 8 * (lane >> 5);
@@ -166,9 +187,17 @@ __device__ __forceinline__ lpx8_t acc_frag(const f32x16& p, int rk) {
                      E::pack(p[8 * rk + 6], p[8 * rk + 7])};
   return __builtin_bit_cast(lpx8_t, u);
 }
+// the other half of the wave's value of v (lane ^ 32), joined with this half's
+__device__ __forceinline__ float max_halves(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
 // row of a 32x32 accumulator's register r
 __device__ __forceinline__ int acc_row(int r, int lane) { return (r >> 2) * 8 + (lane >> 5) * 4 + (r & 3); }
 __device__ __forceinline__ f32x16 zero16() { return (f32x16){0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}; }
+
+// in a branch that few tiles take: keeps hipcc from computing it for all of them and selecting
+__device__ __forceinline__ void stay_a_branch() { asm volatile(""); }
 
 // ---- values that are not finite in a tile that the mask crosses
 template <class E>
@@ -176,26 +205,34 @@ __device__ __forceinline__ unsigned finite_mask(unsigned u) {          // 0xffff
   const unsigned t = ~u & E::kExpMask;
   return ((t & 0xffffu) ? 0xffffu : 0u) | ((t >> 16) ? 0xffff0000u : 0u);
 }
+// The workgroup's 256 threads look through a tile, each its share; the same answer in all of them.  (The barrier inside also waits for
+// the tile that is on its way: this is done for the two or three tiles of a workgroup that a mask crosses, not for the others.)
 template <class E, int DP>
-__device__ __forceinline__ bool tile_nonfinite(const char* lds, int lane) {      // the same answer in every lane of the wave
+__device__ __forceinline__ bool tile_nonfinite(const char* lds) {
   unsigned bad = 0;
 #pragma unroll
-  for (int i = 0; i < KT * DP * 2 / 1024; ++i) {
-    const u32x4_t v = *(const u32x4_t*)(lds + (i * 64 + lane) * 16);
+  for (int i = 0; i < KT * DP * 2 / 4096; ++i) {
+    const u32x4_t v = *(const u32x4_t*)(lds + (i * 256 + threadIdx.x) * 16);
 #pragma unroll
     for (int j = 0; j < 4; ++j) bad |= ~finite_mask<E>(v[j]);
   }
-  return __any(bad != 0);
+  return __syncthreads_or(bad != 0);
 }
-template <class E>
-__device__ __forceinline__ lpx8_t finite_only(lpx8_t f) {
-  u32x4_t u = __builtin_bit_cast(u32x4_t, f);
+// ... and put zeros where values are not finite, once every wave has read what it needs of them
+template <class E, int DP>
+__device__ __forceinline__ void tile_clean(char* lds) {
+  __syncthreads();
+  for (int i = 0; i < KT * DP * 2 / 4096; ++i) {
+    u32x4_t* at = (u32x4_t*)(lds + (i * 256 + threadIdx.x) * 16);
+    u32x4_t v = *at;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) u[j] &= finite_mask<E>(u[j]);
-  return __builtin_bit_cast(lpx8_t, u);
+    for (int j = 0; j < 4; ++j) v[j] &= finite_mask<E>(v[j]);
+    *at = v;
+  }
+  __syncthreads();
 }
-// acc[cb] holds columns 32 cb .. of the lane's row; `sees(j)`: whether that row sees row j of the tile.  What `finite_only` took out
-// comes back: as itself where it multiplies a probability, as NaN where it multiplies dS, whose sign says nothing.
+// acc[cb] holds columns 32 cb .. of the lane's row; `sees(j)`: whether that row sees row j of the tile.  What `tile_clean` will take out
+// is added here: as itself where it multiplies a probability, as NaN where it multiplies dS, whose sign says nothing.
 template <class E, int DP, bool NAN_ONLY, class Sees>
 __device__ __forceinline__ void add_nonfinite(f32x16 (&acc)[DP / 32], const char* lds, int lane, Sees sees) {
 #pragma unroll 1
@@ -252,7 +289,7 @@ __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(simvg_packed_at
   const int h = blockIdx.x % a.Hq;
   Tile e;
   if (!plan_entry(a, blockIdx.x / a.Hq, e)) return fill_tail(a, blockIdx.x / a.Hq, a.o, a.o_ts, a.o_hs, h, a.lse);
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int hk = h / (a.Hq / a.Hkv);
   const int row = e.t * QT + wave * 32 + (lane & 31);        // the lane's query
   const bool valid = row < e.len;
@@ -261,51 +298,62 @@ __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(simvg_packed_at
   const unsigned short* vp = (const unsigned short*)a.v + (long)e.first * a.v_ts + (long)hk * a.v_hs;
   const int keys = CAUSAL ? min(e.len, (e.t + 1) * QT) : e.len, tiles = (keys + KT - 1) / KT;
   const int wave_first = e.t * QT + wave * 32;               // the wave's first query
+  // tiles that no mask touches come first, then those that the diagonal or the sequence's end crosses, then (for the wave) nothing
+  const int whole = min(CAUSAL ? (e.t * QT + 1) / KT : tiles, e.len / KT);                     // of all four waves
+  const int wave_whole = min(CAUSAL ? (wave_first + 1) / KT : tiles, e.len / KT);
   const int wave_tiles = CAUSAL ? min(tiles, (wave_first + 32 + KT - 1) / KT) : tiles;
 
-  Staged<DP> sk, sv;
-  stage_load<DP>(sk, kp, a.k_ts, 0, e.len, a.D, tid);
-  stage_load<DP>(sv, vp, a.v_ts, 0, e.len, a.D, tid);
+  Stager<DP, 4> gk, gv;
+  gk.init(a.k_ts, a.D, wave, lane);
+  gv.init(a.v_ts, a.D, wave, lane);
+  const unsigned lds = lds_addr(smem);
+  auto issue = [&](int kt, int buf) {
+    gk.issue(kp, a.k_ts, kt * KT, e.len, lds + buf * TILE);
+    gv.issue(vp, a.v_ts, kt * KT, e.len, lds + (2 + buf) * TILE);
+  };
+  issue(0, 0);
   lpx8_t qf[KS];
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) qf[ks] = global_frag(qp, ks, a.D, lane);
+  Lanes<DP> at;
+  at.init(lane);
   f32x16 o[DB];
 #pragma unroll
   for (int i = 0; i < DB; ++i) o[i] = zero16();
   const float c = a.scale * LOG2E;
   float m = NEG_INF, l = 0.f;                                // reference of the exponentials (raw scores), sum over this half's keys
-  stage_store<DP>(sk, smem, tid);
-  stage_store<DP>(sv, smem + 2 * TILE, tid);
-  __syncthreads();
-  for (int kt = 0; kt < tiles; ++kt) {
-    const char *lk = smem + (kt & 1) * TILE, *lv = smem + (2 + (kt & 1)) * TILE;
-    if (kt + 1 < tiles) {
-      stage_load<DP>(sk, kp, a.k_ts, (kt + 1) * KT, e.len, a.D, tid);
-      stage_load<DP>(sv, vp, a.v_ts, (kt + 1) * KT, e.len, a.D, tid);
-    }
-    if (kt < wave_tiles) {
-      f32x16 s[2];
+
+  // one tile; the buffer's number is a constant, so that every LDS address is a lane's register and a constant
+  auto tile = [&](int kt, auto which) {
+    constexpr int BUF = decltype(which)::value;
+    char *lk = smem + BUF * TILE, *lv = smem + (2 + BUF) * TILE;
+    dma_wait<0>();                                           // this wave's pieces of the tile
+    wave_barrier_only();                                     // everybody's; and everybody is done with the other buffer
+    if (kt + 1 < tiles) issue(kt + 1, BUF ^ 1);
+    const bool odd = kt >= whole && tile_nonfinite<E, DP>(lv), mine = kt < wave_tiles;
+    const int last = (CAUSAL ? min(row, e.len - 1) : e.len - 1) - kt * KT;     // of the tile's keys, the last that the lane's query sees
+    f32x16 s[2];
+    if (mine) {
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) {
         s[kb] = zero16();
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) s[kb] = E::mfma(row_frag<DP>(lk, kb, ks, lane), qf[ks], s[kb]);
+        for (int ks = 0; ks < KS; ++ks) s[kb] = E::mfma(at.row(lk, kb, ks), qf[ks], s[kb]);
       }
-      const bool masked = (CAUSAL && kt * KT + KT - 1 > wave_first) || kt * KT + KT > e.len;
-      if (masked) {
-        const int last = CAUSAL ? min(row, e.len - 1) : e.len - 1;
+      if (kt >= wave_whole) {
+        stay_a_branch();
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
           for (int r = 0; r < 16; ++r)
-            if (kt * KT + kb * 32 + acc_row(r, lane) > last) s[kb][r] = NEG_INF;
+            if (kb * 32 + acc_row(r, lane) > last) s[kb][r] = NEG_INF;
       }
       float top = NEG_INF;
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int r = 0; r < 16; ++r) top = fmaxf(top, s[kb][r]);
-      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      top = max_halves(top);
       // the reference follows the maximum only where it has grown by more than 2^8: the exponentials stay below 2^8, and what is
       // left of O and l need not be scaled at every tile
       if (__any((top - m) * c > 8.f)) {
@@ -323,27 +371,23 @@ __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(simvg_packed_at
           s[kb][r] = __builtin_amdgcn_exp2f(fmaf(s[kb][r], c, -mc));
           l += s[kb][r];
         }
-      const bool odd = masked && tile_nonfinite<E, DP>(lv, lane);
+    }
+    if (odd) {
+      if (mine) add_nonfinite<E, DP, false>(o, lv, lane, [&](int j) { return j <= last; });
+      tile_clean<E, DP>(lv);
+    }
+    if (mine) {
 #pragma unroll
       for (int rk = 0; rk < 4; ++rk) {
         const lpx8_t p = acc_frag<E>(s[rk >> 1], rk & 1);
 #pragma unroll
-        for (int cb = 0; cb < DB; ++cb) {
-          lpx8_t vf = col_frag<DP>(lv, rk, cb, lane);
-          if (odd) vf = finite_only<E>(vf);
-          o[cb] = E::mfma(vf, p, o[cb]);
-        }
-      }
-      if (odd) {
-        const int last = (CAUSAL ? min(row, e.len - 1) : e.len - 1) - kt * KT;
-        add_nonfinite<E, DP, false>(o, lv, lane, [&](int j) { return j <= last; });
+        for (int cb = 0; cb < DB; ++cb) o[cb] = E::mfma(at.col(lv, rk, cb), p, o[cb]);
       }
     }
-    if (kt + 1 < tiles) {
-      stage_store<DP>(sk, smem + ((kt + 1) & 1) * TILE, tid);
-      stage_store<DP>(sv, smem + (2 + ((kt + 1) & 1)) * TILE, tid);
-    }
-    __syncthreads();
+  };
+  for (int kt = 0; kt < tiles; kt += 2) {
+    tile(kt, std::integral_constant<int, 0>{});
+    if (kt + 1 < tiles) tile(kt + 1, std::integral_constant<int, 1>{});
   }
   l += __shfl_xor(l, 32, 64);
   unsigned short* out = (unsigned short*)a.o + (long)(e.first + row) * a.o_ts + (long)h * a.o_hs;
@@ -453,75 +497,88 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dq_kernel(simvg_packed_att
   const int h = blockIdx.x % a.Hq;
   Tile e;
   if (!plan_entry(a, blockIdx.x / a.Hq, e)) return fill_tail(a, blockIdx.x / a.Hq, a.dq, a.dq_ts, a.dq_hs, h, nullptr);
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int hk = h / (a.Hq / a.Hkv);
   const float power = grad_power<E>(a, e, hk, red), up = __builtin_amdgcn_exp2f(power), shift = E::kScaled ? P_POWER : 0.f;
   const int row = e.t * QT + wave * 32 + (lane & 31);
   const bool valid = row < e.len;
-  const long at = e.first + min(row, e.len - 1);
-  const unsigned short* qp = (const unsigned short*)a.q + at * a.q_ts + (long)h * a.q_hs;
-  const unsigned short* dop = (const unsigned short*)a.d_o + at * a.do_ts + (long)h * a.do_hs;
+  const long here = e.first + min(row, e.len - 1);
+  const unsigned short* qp = (const unsigned short*)a.q + here * a.q_ts + (long)h * a.q_hs;
+  const unsigned short* dop = (const unsigned short*)a.d_o + here * a.do_ts + (long)h * a.do_hs;
   const unsigned short* kp = (const unsigned short*)a.k + (long)e.first * a.k_ts + (long)hk * a.k_hs;
   const unsigned short* vp = (const unsigned short*)a.v + (long)e.first * a.v_ts + (long)hk * a.v_hs;
   const int keys = CAUSAL ? min(e.len, (e.t + 1) * QT) : e.len, tiles = (keys + KT - 1) / KT;
   const int wave_first = e.t * QT + wave * 32;
+  const int whole = min(CAUSAL ? (e.t * QT + 1) / KT : tiles, e.len / KT);
+  const int wave_whole = min(CAUSAL ? (wave_first + 1) / KT : tiles, e.len / KT);
   const int wave_tiles = CAUSAL ? min(tiles, (wave_first + 32 + KT - 1) / KT) : tiles;
-  Staged<DP> sk, sv;
-  stage_load<DP>(sk, kp, a.k_ts, 0, e.len, a.D, tid);
-  stage_load<DP>(sv, vp, a.v_ts, 0, e.len, a.D, tid);
+  Stager<DP, 4> gk, gv;
+  gk.init(a.k_ts, a.D, wave, lane);
+  gv.init(a.v_ts, a.D, wave, lane);
+  const unsigned lds = lds_addr(smem);
+  auto issue = [&](int kt, int buf) {
+    gk.issue(kp, a.k_ts, kt * KT, e.len, lds + buf * TILE);
+    gv.issue(vp, a.v_ts, kt * KT, e.len, lds + (2 + buf) * TILE);
+  };
+  issue(0, 0);
   lpx8_t qf[KS], dof[KS];
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) { qf[ks] = global_frag(qp, ks, a.D, lane); dof[ks] = global_frag(dop, ks, a.D, lane); }
-  const float c = a.scale * LOG2E, lse2 = a.lse[(long)h * a.lse_hs + at] * LOG2E - shift;
-  const float delta = ws_of(a).delta[(long)h * a.T + at];
+  Lanes<DP> at;
+  at.init(lane);
+  const float c = a.scale * LOG2E, lse2 = a.lse[(long)h * a.lse_hs + here] * LOG2E - shift;
+  const float delta = ws_of(a).delta[(long)h * a.T + here];
   f32x16 dq[DB];
 #pragma unroll
   for (int i = 0; i < DB; ++i) dq[i] = zero16();
-  stage_store<DP>(sk, smem, tid);
-  stage_store<DP>(sv, smem + 2 * TILE, tid);
-  __syncthreads();
-  for (int kt = 0; kt < tiles; ++kt) {
-    const char *lk = smem + (kt & 1) * TILE, *lv = smem + (2 + (kt & 1)) * TILE;
-    if (kt + 1 < tiles) {
-      stage_load<DP>(sk, kp, a.k_ts, (kt + 1) * KT, e.len, a.D, tid);
-      stage_load<DP>(sv, vp, a.v_ts, (kt + 1) * KT, e.len, a.D, tid);
-    }
-    if (kt < wave_tiles) {
-      const bool masked = (CAUSAL && kt * KT + KT - 1 > wave_first) || kt * KT + KT > e.len;
-      const bool odd = masked && tile_nonfinite<E, DP>(lk, lane);
-      const int last = (CAUSAL ? min(row, e.len - 1) : e.len - 1) - kt * KT;
+
+  auto tile = [&](int kt, auto which) {
+    constexpr int BUF = decltype(which)::value;
+    char *lk = smem + BUF * TILE, *lv = smem + (2 + BUF) * TILE;
+    dma_wait<0>();
+    wave_barrier_only();
+    if (kt + 1 < tiles) issue(kt + 1, BUF ^ 1);
+    const bool odd = kt >= whole && tile_nonfinite<E, DP>(lk), mine = kt < wave_tiles;
+    const int last = (CAUSAL ? min(row, e.len - 1) : e.len - 1) - kt * KT;
+    lpx8_t ds[4];
+    if (mine) {
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) {
         f32x16 s = zero16(), dp = zero16();
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-          s = E::mfma(row_frag<DP>(lk, kb, ks, lane), qf[ks], s);
-          dp = E::mfma(row_frag<DP>(lv, kb, ks, lane), dof[ks], dp);
+          s = E::mfma(at.row(lk, kb, ks), qf[ks], s);
+          dp = E::mfma(at.row(lv, kb, ks), dof[ks], dp);
         }
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const float p = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse2));
-          s[r] = p * ((dp[r] - delta) * up);
-          if (masked && kb * 32 + acc_row(r, lane) > last) s[r] = 0.f;
+          s[r] = E::kScaled ? p * ((dp[r] - delta) * up) : p * (dp[r] - delta);
         }
+        if (kt >= wave_whole) {
+          stay_a_branch();
 #pragma unroll
-        for (int rk = 0; rk < 2; ++rk) {
-          const lpx8_t ds = acc_frag<E>(s, rk);
-#pragma unroll
-          for (int cb = 0; cb < DB; ++cb) {
-            lpx8_t kf = col_frag<DP>(lk, kb * 2 + rk, cb, lane);
-            if (odd) kf = finite_only<E>(kf);
-            dq[cb] = E::mfma(kf, ds, dq[cb]);
-          }
+          for (int r = 0; r < 16; ++r)
+            if (kb * 32 + acc_row(r, lane) > last) s[r] = 0.f;
         }
+        ds[2 * kb] = acc_frag<E>(s, 0);
+        ds[2 * kb + 1] = acc_frag<E>(s, 1);
       }
-      if (odd) add_nonfinite<E, DP, true>(dq, lk, lane, [&](int j) { return j <= last; });
     }
-    if (kt + 1 < tiles) {
-      stage_store<DP>(sk, smem + ((kt + 1) & 1) * TILE, tid);
-      stage_store<DP>(sv, smem + (2 + ((kt + 1) & 1)) * TILE, tid);
+    if (odd) {
+      if (mine) add_nonfinite<E, DP, true>(dq, lk, lane, [&](int j) { return j <= last; });
+      tile_clean<E, DP>(lk);
     }
-    __syncthreads();
+    if (mine) {
+#pragma unroll
+      for (int rk = 0; rk < 4; ++rk)
+#pragma unroll
+        for (int cb = 0; cb < DB; ++cb) dq[cb] = E::mfma(at.col(lk, rk, cb), ds[rk], dq[cb]);
+    }
+  };
+  for (int kt = 0; kt < tiles; kt += 2) {
+    tile(kt, std::integral_constant<int, 0>{});
+    if (kt + 1 < tiles) tile(kt + 1, std::integral_constant<int, 1>{});
   }
   unsigned short* out = (unsigned short*)a.dq + (long)(e.first + row) * a.dq_ts + (long)h * a.dq_hs;
   store_rows<E, DP>(dq, a.scale * __builtin_amdgcn_exp2f(-power - shift), out, a.D, valid, lane);
@@ -542,60 +599,78 @@ __global__ __launch_bounds__(256, 1) void packed_attn_dkv_kernel(simvg_packed_at
   }
   const int ntile = (e.len + QT - 1) / QT;
   if (CAUSAL) e.t = ntile - 1 - e.t;                         // the plan's order is by cost: the first keys are seen by the most queries
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const float power = grad_power<E>(a, e, hk, red), up = __builtin_amdgcn_exp2f(power), shift = E::kScaled ? P_POWER : 0.f;
   const int key = e.t * QT + wave * 32 + (lane & 31);        // the lane's key
   const bool valid = key < e.len;
-  const long at = e.first + min(key, e.len - 1);
-  const unsigned short* kp = (const unsigned short*)a.k + at * a.k_ts + (long)hk * a.k_hs;
-  const unsigned short* vp = (const unsigned short*)a.v + at * a.v_ts + (long)hk * a.v_hs;
+  const long here = e.first + min(key, e.len - 1);
+  const unsigned short* kp = (const unsigned short*)a.k + here * a.k_ts + (long)hk * a.k_hs;
+  const unsigned short* vp = (const unsigned short*)a.v + here * a.v_ts + (long)hk * a.v_hs;
   const int first = CAUSAL ? e.t * QT / KT : 0, tiles = (e.len + KT - 1) / KT - first;       // tiles of queries, from `first`
-  const int wave_first = e.t * QT + wave * 32;
+  const int wave_first = e.t * QT + wave * 32, steps = G * tiles;
+  Stager<DP, 4> gq, gd;
+  gq.init(a.q_ts, a.D, wave, lane);
+  gd.init(a.do_ts, a.D, wave, lane);
+  const unsigned lds = lds_addr(smem);
+  const float* delta = ws_of(a).delta;
+  // step i: head hk G + i / tiles, query tile first + i % tiles.  The rows' lse and delta are loaded into registers a step ahead:
+  // rows past the sequence are zeros with lse 0: P stays finite, times 0
+  int load_h = hk * G, load_t = first;
+  float st0 = 0.f;
+  auto issue = [&](int buf) {
+    const int row0 = load_t * KT;
+    gq.issue((const unsigned short*)a.q + (long)e.first * a.q_ts + (long)load_h * a.q_hs, a.q_ts, row0, e.len, lds + buf * TILE);
+    gd.issue((const unsigned short*)a.d_o + (long)e.first * a.do_ts + (long)load_h * a.do_hs, a.do_ts, row0, e.len, lds + (2 + buf) * TILE);
+    if (tid < 2 * KT) {
+      const int row = row0 + (tid & (KT - 1));
+      st0 = 0.f;
+      if (row < e.len) st0 = tid < KT ? a.lse[(long)load_h * a.lse_hs + e.first + row] * LOG2E - shift : delta[(long)load_h * a.T + e.first + row];
+    }
+    if (++load_t == first + tiles) { load_t = first; ++load_h; }
+  };
+  issue(0);
   lpx8_t kf[KS], vf[KS];
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) { kf[ks] = global_frag(kp, ks, a.D, lane); vf[ks] = global_frag(vp, ks, a.D, lane); }
+  Lanes<DP> at;
+  at.init(lane);
   const float c = a.scale * LOG2E;
-  const float* delta = ws_of(a).delta;
   f32x16 dk[DB], dv[DB];
 #pragma unroll
   for (int i = 0; i < DB; ++i) { dk[i] = zero16(); dv[i] = zero16(); }
-  Staged<DP> sq, sd;
-  float st0 = 0.f;
-  auto load = [&](int i) {                                   // step i: head hk G + i / tiles, query tile first + i % tiles
-    const int h = hk * G + i / tiles, row0 = (first + i % tiles) * KT;
-    stage_load<DP>(sq, (const unsigned short*)a.q + (long)e.first * a.q_ts + (long)h * a.q_hs, a.q_ts, row0, e.len, a.D, tid);
-    stage_load<DP>(sd, (const unsigned short*)a.d_o + (long)e.first * a.do_ts + (long)h * a.do_hs, a.do_ts, row0, e.len, a.D, tid);
-    if (tid < 2 * KT) {                                      // rows past the sequence are zeros with lse 0: P stays finite, times 0
-      const int row = row0 + (tid & (KT - 1));
-      st0 = 0.f;
-      if (row < e.len) st0 = tid < KT ? a.lse[(long)h * a.lse_hs + e.first + row] * LOG2E - shift : delta[(long)h * a.T + e.first + row];
+
+  int row0 = first * KT;
+  auto tile = [&](int i, auto which) {
+    constexpr int BUF = decltype(which)::value;
+    char *lq = smem + BUF * TILE, *ld = smem + (2 + BUF) * TILE;
+    const float *lse = stat[BUF][0], *del = stat[BUF][1];
+    if (tid < 2 * KT) stat[BUF][tid / KT][tid & (KT - 1)] = st0;
+    dma_wait<0>();
+    wave_barrier_only();
+    if (i + 1 < steps) issue(BUF ^ 1);
+    const int from = key - row0;                             // the first row of the tile that sees the lane's key
+    const bool mine = !CAUSAL || row0 + KT - 1 >= wave_first, whole = !CAUSAL || row0 >= wave_first + 31;
+    // Rows that are not finite lose nothing by being cleaned before the scores: their lse (of q) or delta (of dO) is not finite either,
+    // and carries that to P and dS of every key they see
+    if (CAUSAL && row0 < e.t * QT + QT - 1) {
+      const bool odd_q = tile_nonfinite<E, DP>(lq), odd_d = tile_nonfinite<E, DP>(ld);
+      if (odd_d) {
+        if (mine) add_nonfinite<E, DP, false>(dv, ld, lane, [&](int j) { return j >= from; });
+        tile_clean<E, DP>(ld);
+      }
+      if (odd_q) {
+        if (mine) add_nonfinite<E, DP, true>(dk, lq, lane, [&](int j) { return j >= from; });
+        tile_clean<E, DP>(lq);
+      }
     }
-  };
-  auto store = [&](int buf) {
-    stage_store<DP>(sq, smem + buf * TILE, tid);
-    stage_store<DP>(sd, smem + (2 + buf) * TILE, tid);
-    if (tid < 2 * KT) stat[buf][tid / KT][tid & (KT - 1)] = st0;
-  };
-  load(0);
-  store(0);
-  __syncthreads();
-  const int steps = G * tiles;
-  for (int i = 0; i < steps; ++i) {
-    const char *lq = smem + (i & 1) * TILE, *ld = smem + (2 + (i & 1)) * TILE;
-    const float *lse = stat[i & 1][0], *del = stat[i & 1][1];
-    if (i + 1 < steps) load(i + 1);
-    const int row0 = (first + i % tiles) * KT;
-    if (!CAUSAL || row0 + KT - 1 >= wave_first) {
-      const bool masked = CAUSAL && row0 < wave_first + 31;
-      const bool odd = masked && (tile_nonfinite<E, DP>(lq, lane) || tile_nonfinite<E, DP>(ld, lane));
-      const int from = key - row0;                           // the first row of the tile that sees the lane's key
+    if (mine) {
 #pragma unroll
       for (int qb = 0; qb < 2; ++qb) {
         f32x16 s = zero16(), dp = zero16();
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-          s = E::mfma(row_frag<DP>(lq, qb, ks, lane), kf[ks], s);
-          dp = E::mfma(row_frag<DP>(ld, qb, ks, lane), vf[ks], dp);
+          s = E::mfma(at.row(lq, qb, ks), kf[ks], s);
+          dp = E::mfma(at.row(ld, qb, ks), vf[ks], dp);
         }
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
@@ -604,32 +679,33 @@ __global__ __launch_bounds__(256, 1) void packed_attn_dkv_kernel(simvg_packed_at
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const int x = 4 * g + r;
-            float p = __builtin_amdgcn_exp2f(fmaf(s[x], c, -ls[r]));
-            float ds = p * ((dp[x] - dl[r]) * up);
-            if (masked && qb * 32 + acc_row(x, lane) < from) { p = 0.f; ds = 0.f; }
-            s[x] = p;
-            dp[x] = ds;
+            s[x] = __builtin_amdgcn_exp2f(fmaf(s[x], c, -ls[r]));
+            dp[x] = E::kScaled ? s[x] * ((dp[x] - dl[r]) * up) : s[x] * (dp[x] - dl[r]);
           }
+        }
+        if (!whole) {
+          stay_a_branch();
+#pragma unroll
+          for (int x = 0; x < 16; ++x)
+            if (qb * 32 + acc_row(x, lane) < from) { s[x] = 0.f; dp[x] = 0.f; }
         }
 #pragma unroll
         for (int rk = 0; rk < 2; ++rk) {
           const lpx8_t p = acc_frag<E>(s, rk), ds = acc_frag<E>(dp, rk);
 #pragma unroll
           for (int cb = 0; cb < DB; ++cb) {
-            lpx8_t df = col_frag<DP>(ld, qb * 2 + rk, cb, lane), qf = col_frag<DP>(lq, qb * 2 + rk, cb, lane);
-            if (odd) { df = finite_only<E>(df); qf = finite_only<E>(qf); }
-            dv[cb] = E::mfma(df, p, dv[cb]);
-            dk[cb] = E::mfma(qf, ds, dk[cb]);
+            dv[cb] = E::mfma(at.col(ld, qb * 2 + rk, cb), p, dv[cb]);
+            dk[cb] = E::mfma(at.col(lq, qb * 2 + rk, cb), ds, dk[cb]);
           }
         }
       }
-      if (odd) {
-        add_nonfinite<E, DP, false>(dv, ld, lane, [&](int j) { return j >= from; });
-        add_nonfinite<E, DP, true>(dk, lq, lane, [&](int j) { return j >= from; });
-      }
     }
-    if (i + 1 < steps) store((i + 1) & 1);
-    __syncthreads();
+    row0 += KT;
+    if (row0 >= (first + tiles) * KT) row0 = first * KT;
+  };
+  for (int i = 0; i < steps; i += 2) {
+    tile(i, std::integral_constant<int, 0>{});
+    if (i + 1 < steps) tile(i + 1, std::integral_constant<int, 1>{});
   }
   store_rows<E, DP>(dv, __builtin_amdgcn_exp2f(-shift), (unsigned short*)a.dv + (long)(e.first + key) * a.dv_ts + (long)hk * a.dv_hs, a.D,
                     valid, lane);
@@ -638,7 +714,9 @@ __global__ __launch_bounds__(256, 1) void packed_attn_dkv_kernel(simvg_packed_at
 }
 
 // ---------------------------------------------------------------------------------------------------------------- host
+// rows in 16-byte chunks; a tile's offsets fit 31 bits
 bool rows16(const void* p, long ts, long hs) { return p && (uintptr_t)p % 16 == 0 && ts % 8 == 0 && hs % 8 == 0; }
+bool in_reach(long ts) { return ts >= 0 && ts < 1L << 24; }
 
 int attn_check(const simvg_packed_attn_args* a, bool bwd) {
   SIMVG_CHECK_ARG(a, "packed_attn: null argument block");
@@ -653,6 +731,8 @@ int attn_check(const simvg_packed_attn_args* a, bool bwd) {
   SIMVG_CHECK_ARG((uintptr_t)a->plan % 4 == 0, "packed_attn: misaligned plan");
   SIMVG_CHECK_ARG(rows16(a->q, a->q_ts, a->q_hs) && rows16(a->k, a->k_ts, a->k_hs) && rows16(a->v, a->v_ts, a->v_hs) &&
                   rows16(a->o, a->o_ts, a->o_hs), "packed_attn: rows of q, k, v and out must start at multiples of 16 bytes");
+  SIMVG_CHECK_ARG(in_reach(a->q_ts) && in_reach(a->k_ts) && in_reach(a->v_ts) && (!bwd || in_reach(a->do_ts)),
+                  "packed_attn: token strides must be below 2^24 elements");
   if (bwd) {
     SIMVG_CHECK_ARG(rows16(a->d_o, a->do_ts, a->do_hs) && rows16(a->dq, a->dq_ts, a->dq_hs) && rows16(a->dk, a->dk_ts, a->dk_hs) &&
                     rows16(a->dv, a->dv_ts, a->dv_hs), "packed_attn: rows of the gradients must start at multiples of 16 bytes");

@@ -61,7 +61,7 @@ __device__ __forceinline__ void dma16(u32x4_t buffer, unsigned lds, unsigned off
                "v"(offset), "s"(buffer)
                : "memory", "m0");
 }
-constexpr unsigned DMA_NOTHING = 0x80000000u;          // an offset past every buffer: zeros
+constexpr unsigned DMA_NOTHING = 0x80000000u;          // an offset past every buffer (which is at most one byte shorter): zeros
 template <int N>
 __device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 // a barrier that does not drain this wave's DMA (what `__syncthreads` would wait for is the caller's business here)
