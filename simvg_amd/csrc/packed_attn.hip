@@ -21,6 +21,7 @@
 // earlier one: such a tile is looked through for values that are not finite, and if there are any they are added, as themselves, to the
 // rows that do see them and taken out of the tile (`add_nonfinite`, `tile_clean`).
 #include <type_traits>
+#include <utility>
 
 #include "seq.h"
 
@@ -125,31 +126,48 @@ __device__ __forceinline__ int tile_at(int row, int slot) {
   return row * (DP * 2) + ((slot ^ x) << 4);
 }
 
-// Brings tiles of KT rows of a head from HBM to LDS (LDS-DMA, seq.h): WAVES waves, `issue` asks for rows [row0, row0 + KT) with zeros
-// past `rows` and past D.
-template <int DP, int WAVES> struct Stager {
-  static constexpr int PIECES = KT * DP * 2 / 1024 / WAVES;
-  unsigned off[PIECES];
-  int wave, row[PIECES];
-  __device__ __forceinline__ void init(long ts, int D, int w, int lane) {
-    wave = w;
+// in a branch that few tiles take: keeps hipcc from computing it for all of them and selecting
+__device__ __forceinline__ void stay_a_branch() { asm volatile(""); }
+
+// Brings tiles of KT rows of a head from HBM to LDS (LDS-DMA, seq.h), one after the other, the work of four waves: zeros past the
+// sequence's rows and past D.  LDS0: where the array's tiles of this operand start.
+template <int DP, int LDS0> struct Stager {
+  static constexpr int PIECES = KT * DP * 2 / 4096;
+  unsigned off[PIECES], lds;                                 // lds: of the wave's first piece
+  unsigned long base;                                        // the next tile's first row
+  unsigned step;                                             // bytes from tile to tile
+  int row, left;                                             // the lane's row of its first piece; the sequence's rows from the next tile on
+  __device__ __forceinline__ void init(const void* first, long ts, int rows, int D, const char* smem, int wave, int lane) {
+    const int r0 = (wave * 1024 + lane * 16) / (DP * 2);
+    base = (unsigned long)first;
+    step = (unsigned)(KT * 2) * (unsigned)ts;
+    lds = lds_addr(smem) + LDS0 + wave * 1024;
+    left = rows;
+    row = r0;
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
-      const int byte = (i * WAVES + w) * 1024 + lane * 16, phys = byte % (DP * 2) / 16;
-      row[i] = byte / (DP * 2);
-      const int slot = (tile_at<DP>(row[i], phys) - row[i] * DP * 2) >> 4;     // the permutation is its own inverse
-      off[i] = slot * 8 < D ? (unsigned)(row[i] * (int)ts * 2 + slot * 16) : DMA_NOTHING;
+      const int byte = (i * 4 + wave) * 1024 + lane * 16, r = byte / (DP * 2);
+      const int slot = (tile_at<DP>(r, byte % (DP * 2) / 16) - r * DP * 2) >> 4;       // the permutation is its own inverse
+      off[i] = slot * 8 < D ? (unsigned)(r * (int)ts * 2 + slot * 16) : DMA_NOTHING;
     }
   }
-  __device__ __forceinline__ void issue(const unsigned short* base, long ts, int row0, int rows, unsigned lds) const {
-    const u32x4_t b = dma_buffer(base + (long)row0 * ts, DMA_NOTHING - 1);
-    if (row0 + KT <= rows) {
+  template <int BUF> __device__ __forceinline__ void next() {
+    const u32x4_t b = {(unsigned)base, (unsigned)(base >> 32) & 0xffffu, DMA_NOTHING - 1, 0x00020000u};
+    unsigned o[PIECES];
 #pragma unroll
-      for (int i = 0; i < PIECES; ++i) dma16(b, lds + (i * WAVES + wave) * 1024, off[i]);
-    } else {
+    for (int i = 0; i < PIECES; ++i) o[i] = off[i];
+    if (left < KT) {
+      stay_a_branch();
 #pragma unroll
-      for (int i = 0; i < PIECES; ++i) dma16(b, lds + (i * WAVES + wave) * 1024, row0 + row[i] < rows ? off[i] : DMA_NOTHING);
+      for (int i = 0; i < PIECES; ++i)
+        if (row + i * (2048 / DP) >= left) o[i] = DMA_NOTHING;
     }
+    issue<BUF>(b, o, std::make_integer_sequence<int, PIECES>{});
+    base += step;
+    left -= KT;
+  }
+  template <int BUF, int... I> __device__ __forceinline__ void issue(u32x4_t b, const unsigned (&o)[PIECES], std::integer_sequence<int, I...>) {
+    (dma16_at<BUF * KT * DP * 2 + I * 4096>(b, lds, o[I]), ...);
   }
 };
 // What a lane adds to a tile's start for its part of a fragment; everything else of an address is a constant in the instruction.
@@ -157,21 +175,28 @@ template <int DP, int WAVES> struct Stager {
 //   col(rk, cb): A operand from columns: column 32 cb + (lane & 31), the 16 rows 16 rk .. in the order of a 32x32 accumulator's registers
 template <int DP> struct Lanes {
   static constexpr int ROWB = DP * 2;
-  unsigned r[DP / 16], c[DP / 32][2];
-  __device__ __forceinline__ void init(int lane) {
+  typedef __attribute__((address_space(3))) const char* Lds;
+  Lds r[DP / 16], c[DP / 32][2];
+  __device__ __forceinline__ void init(const char* smem, int lane) {
     const int i = lane & 15, row = 4 * (lane >> 5) + (i >> 2);
+    const Lds base = (Lds)(const __attribute__((address_space(3))) void*)LDS_PTR(smem);
 #pragma unroll
-    for (int ks = 0; ks < DP / 16; ++ks) r[ks] = tile_at<DP>(lane & 31, ks * 2 + (lane >> 5));
+    for (int ks = 0; ks < DP / 16; ++ks) r[ks] = base + tile_at<DP>(lane & 31, ks * 2 + (lane >> 5));
 #pragma unroll
     for (int cb = 0; cb < DP / 32; ++cb) {
       const int col = cb * 32 + (lane >> 4 & 1) * 16 + 4 * (i & 3);
-      c[cb][0] = tile_at<DP>(row, col >> 3) + (col & 7) * 2;
-      c[cb][1] = tile_at<DP>(row + 8, col >> 3) + (col & 7) * 2;
+      c[cb][0] = base + tile_at<DP>(row, col >> 3) + (col & 7) * 2;
+      c[cb][1] = base + tile_at<DP>(row + 8, col >> 3) + (col & 7) * 2;
     }
   }
-  __device__ __forceinline__ lpx8_t row(const char* tile, int rb, int ks) const { return *(const lpx8_t*)(tile + r[ks] + rb * 32 * ROWB); }
-  __device__ __forceinline__ lpx8_t col(const char* tile, int rk, int cb) const {
-    const lpx4_t lo = lds_read_tr16(tile + c[cb][0] + rk * 16 * ROWB), hi = lds_read_tr16(tile + c[cb][1] + rk * 16 * ROWB);
+  // `tile`: bytes from the start of the LDS array
+  __device__ __forceinline__ lpx8_t row(int tile, int rb, int ks) const {
+    return *(const __attribute__((address_space(3))) lpx8_t*)(r[ks] + tile + rb * 32 * ROWB);
+  }
+  __device__ __forceinline__ lpx8_t col(int tile, int rk, int cb) const {
+    typedef __attribute__((address_space(3))) lpx4_t* P;
+    const lpx4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(c[cb][0] + tile + rk * 16 * ROWB));
+    const lpx4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(c[cb][1] + tile + rk * 16 * ROWB));
     return (lpx8_t){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
   }
 };
@@ -180,6 +205,13 @@ __device__ __forceinline__ lpx8_t global_frag(const unsigned short* base, int ks
   const int col = ks * 16 + 8 * (lane >> 5);
   return col < D ? *(const lpx8_t*)(base + col) : (lpx8_t){0, 0, 0, 0, 0, 0, 0, 0};
 }
+// Loaded before a loop that has DMA in flight: taken here, so that hipcc's wait for the load stands here and not at the first use in
+// the loop, where it would wait for the tile that has just been asked for, at every tile
+template <int N> __device__ __forceinline__ void arrived(lpx8_t (&f)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(f[i]));
+}
+__device__ __forceinline__ void arrived(float& f) { asm volatile("" : "+v"(f)); }
 // registers 8 rk .. 8 rk + 7 of an accumulator as the B operand of a product over its rows
 template <class E>
 __device__ __forceinline__ lpx8_t acc_frag(const f32x16& p, int rk) {
@@ -196,14 +228,12 @@ __device__ __forceinline__ float max_halves(float v) {
 __device__ __forceinline__ int acc_row(int r, int lane) { return (r >> 2) * 8 + (lane >> 5) * 4 + (r & 3); }
 __device__ __forceinline__ f32x16 zero16() { return (f32x16){0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}; }
 
-// in a branch that few tiles take: keeps hipcc from computing it for all of them and selecting
-__device__ __forceinline__ void stay_a_branch() { asm volatile(""); }
-
 // ---- values that are not finite in a tile that the mask crosses
+// (integer arithmetic and no comparisons: unrolled, their results would fill the scalar registers)
 template <class E>
-__device__ __forceinline__ unsigned finite_mask(unsigned u) {          // 0xffff in each half that holds a finite value
-  const unsigned t = ~u & E::kExpMask;
-  return ((t & 0xffffu) ? 0xffffu : 0u) | ((t >> 16) ? 0xffff0000u : 0u);
+__device__ __forceinline__ unsigned finite_mask(unsigned u) {          // all bits of each half that holds a finite value
+  const int lo = (int)(u & 0x7fffu) - E::kInf, hi = (int)(u >> 16 & 0x7fffu) - E::kInf;
+  return ((unsigned)(lo >> 31) & 0xffffu) | ((unsigned)(hi >> 31) << 16);
 }
 // The workgroup's 256 threads look through a tile, each its share; the same answer in all of them.  (The barrier inside also waits for
 // the tile that is on its way: this is done for the two or three tiles of a workgroup that a mask crosses, not for the others.)
@@ -244,8 +274,8 @@ __device__ __forceinline__ void add_nonfinite(f32x16 (&acc)[DP / 32], const char
       for (int r = 0; r < 16; ++r) {
         const int col = cb * 32 + acc_row(r, lane);
         const unsigned short b = *(const unsigned short*)(lds + tile_at<DP>(j, col >> 3) + (col & 7) * 2);
-        const float x = E::to_f32(b);
-        if (!__builtin_isfinite(x)) acc[cb][r] += NAN_ONLY ? x - x : x;
+        const float x = E::to_f32((unsigned short)(b & ~finite_mask<E>(b)));           // 0 where it is finite
+        acc[cb][r] += NAN_ONLY ? x - x : x;
       }
   }
 }
@@ -283,7 +313,7 @@ __device__ __forceinline__ void store_rows(const f32x16 (&acc)[DP / 32], float m
 
 // ------------------------------------------------------------------------------------------------------------- forward
 template <class E, int DP, bool CAUSAL>
-__global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(simvg_packed_attn_args a) {
+__global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_fwd_kernel(simvg_packed_attn_args a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   constexpr int TILE = KT * DP * 2, DB = DP / 32, KS = DP / 16;
   const int h = blockIdx.x % a.Hq;
@@ -303,20 +333,18 @@ __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(simvg_packed_at
   const int wave_whole = min(CAUSAL ? (wave_first + 1) / KT : tiles, e.len / KT);
   const int wave_tiles = CAUSAL ? min(tiles, (wave_first + 32 + KT - 1) / KT) : tiles;
 
-  Stager<DP, 4> gk, gv;
-  gk.init(a.k_ts, a.D, wave, lane);
-  gv.init(a.v_ts, a.D, wave, lane);
-  const unsigned lds = lds_addr(smem);
-  auto issue = [&](int kt, int buf) {
-    gk.issue(kp, a.k_ts, kt * KT, e.len, lds + buf * TILE);
-    gv.issue(vp, a.v_ts, kt * KT, e.len, lds + (2 + buf) * TILE);
-  };
-  issue(0, 0);
+  Stager<DP, 0> gk;
+  Stager<DP, 2 * TILE> gv;
+  gk.init(kp, a.k_ts, e.len, a.D, smem, wave, lane);
+  gv.init(vp, a.v_ts, e.len, a.D, smem, wave, lane);
+  gk.template next<0>();
+  gv.template next<0>();
   lpx8_t qf[KS];
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) qf[ks] = global_frag(qp, ks, a.D, lane);
+  arrived(qf);
   Lanes<DP> at;
-  at.init(lane);
+  at.init(smem, lane);
   f32x16 o[DB];
 #pragma unroll
   for (int i = 0; i < DB; ++i) o[i] = zero16();
@@ -325,21 +353,27 @@ __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(simvg_packed_at
 
   // one tile; the buffer's number is a constant, so that every LDS address is a lane's register and a constant
   auto tile = [&](int kt, auto which) {
-    constexpr int BUF = decltype(which)::value;
-    char *lk = smem + BUF * TILE, *lv = smem + (2 + BUF) * TILE;
+    constexpr int BUF = decltype(which)::value, K0 = BUF * TILE, V0 = (2 + BUF) * TILE;
+    char *lk = smem + K0, *lv = smem + V0;
+    (void)lk; (void)lv;
     dma_wait<0>();                                           // this wave's pieces of the tile
     wave_barrier_only();                                     // everybody's; and everybody is done with the other buffer
-    if (kt + 1 < tiles) issue(kt + 1, BUF ^ 1);
+    if (kt + 1 < tiles) {
+      gk.template next<BUF ^ 1>();
+      gv.template next<BUF ^ 1>();
+    }
     const bool odd = kt >= whole && tile_nonfinite<E, DP>(lv), mine = kt < wave_tiles;
     const int last = (CAUSAL ? min(row, e.len - 1) : e.len - 1) - kt * KT;     // of the tile's keys, the last that the lane's query sees
     f32x16 s[2];
     if (mine) {
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) {
         s[kb] = zero16();
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) s[kb] = E::mfma(at.row(lk, kb, ks), qf[ks], s[kb]);
+        for (int ks = 0; ks < KS; ++ks) s[kb] = E::mfma(at.row(K0, kb, ks), qf[ks], s[kb]);
       }
+      __builtin_amdgcn_s_setprio(0);
       if (kt >= wave_whole) {
         stay_a_branch();
 #pragma unroll
@@ -377,12 +411,14 @@ __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(simvg_packed_at
       tile_clean<E, DP>(lv);
     }
     if (mine) {
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int rk = 0; rk < 4; ++rk) {
         const lpx8_t p = acc_frag<E>(s[rk >> 1], rk & 1);
 #pragma unroll
-        for (int cb = 0; cb < DB; ++cb) o[cb] = E::mfma(at.col(lv, rk, cb), p, o[cb]);
+        for (int cb = 0; cb < DB; ++cb) o[cb] = E::mfma(at.col(V0, rk, cb), p, o[cb]);
       }
+      __builtin_amdgcn_s_setprio(0);
     }
   };
   for (int kt = 0; kt < tiles; kt += 2) {
@@ -390,9 +426,10 @@ __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(simvg_packed_at
     if (kt + 1 < tiles) tile(kt + 1, std::integral_constant<int, 1>{});
   }
   l += __shfl_xor(l, 32, 64);
-  unsigned short* out = (unsigned short*)a.o + (long)(e.first + row) * a.o_ts + (long)h * a.o_hs;
-  store_rows<E, DP>(o, 1.f / l, out, a.D, valid, lane);
-  if (valid && lane < 32) a.lse[(long)h * a.lse_hs + e.first + row] = m * a.scale + __builtin_logf(l);
+  const auto z = late_args<simvg_packed_attn_args>();
+  unsigned short* out = (unsigned short*)z->o + (long)(e.first + row) * z->o_ts + (long)h * z->o_hs;
+  store_rows<E, DP>(o, 1.f / l, out, z->D, valid, lane);
+  if (valid && lane < 32) z->lse[(long)h * z->lse_hs + e.first + row] = m * z->scale + __builtin_logf(l);
 }
 
 // ------------------------------------------------------------------------------------------------------------ backward
@@ -490,7 +527,7 @@ __device__ __forceinline__ float grad_power(const simvg_packed_attn_args& a, con
 
 // dQ: a workgroup's 128 queries against the tiles of their keys, as in the forward pass
 template <class E, int DP, bool CAUSAL>
-__global__ __launch_bounds__(256, 2) void packed_attn_dq_kernel(simvg_packed_attn_args a) {
+__global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_dq_kernel(simvg_packed_attn_args a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ float red[8];
   constexpr int TILE = KT * DP * 2, DB = DP / 32, KS = DP / 16;
@@ -512,32 +549,37 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dq_kernel(simvg_packed_att
   const int whole = min(CAUSAL ? (e.t * QT + 1) / KT : tiles, e.len / KT);
   const int wave_whole = min(CAUSAL ? (wave_first + 1) / KT : tiles, e.len / KT);
   const int wave_tiles = CAUSAL ? min(tiles, (wave_first + 32 + KT - 1) / KT) : tiles;
-  Stager<DP, 4> gk, gv;
-  gk.init(a.k_ts, a.D, wave, lane);
-  gv.init(a.v_ts, a.D, wave, lane);
-  const unsigned lds = lds_addr(smem);
-  auto issue = [&](int kt, int buf) {
-    gk.issue(kp, a.k_ts, kt * KT, e.len, lds + buf * TILE);
-    gv.issue(vp, a.v_ts, kt * KT, e.len, lds + (2 + buf) * TILE);
-  };
-  issue(0, 0);
+  Stager<DP, 0> gk;
+  Stager<DP, 2 * TILE> gv;
+  gk.init(kp, a.k_ts, e.len, a.D, smem, wave, lane);
+  gv.init(vp, a.v_ts, e.len, a.D, smem, wave, lane);
+  gk.template next<0>();
+  gv.template next<0>();
   lpx8_t qf[KS], dof[KS];
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) { qf[ks] = global_frag(qp, ks, a.D, lane); dof[ks] = global_frag(dop, ks, a.D, lane); }
   Lanes<DP> at;
-  at.init(lane);
-  const float c = a.scale * LOG2E, lse2 = a.lse[(long)h * a.lse_hs + here] * LOG2E - shift;
-  const float delta = ws_of(a).delta[(long)h * a.T + here];
+  at.init(smem, lane);
+  const float c = a.scale * LOG2E;
+  float lse2 = a.lse[(long)h * a.lse_hs + here] * LOG2E - shift, delta = ws_of(a).delta[(long)h * a.T + here];
+  arrived(qf);
+  arrived(dof);
+  arrived(lse2);
+  arrived(delta);
   f32x16 dq[DB];
 #pragma unroll
   for (int i = 0; i < DB; ++i) dq[i] = zero16();
 
   auto tile = [&](int kt, auto which) {
-    constexpr int BUF = decltype(which)::value;
-    char *lk = smem + BUF * TILE, *lv = smem + (2 + BUF) * TILE;
+    constexpr int BUF = decltype(which)::value, K0 = BUF * TILE, V0 = (2 + BUF) * TILE;
+    char *lk = smem + K0, *lv = smem + V0;
+    (void)lk; (void)lv;
     dma_wait<0>();
     wave_barrier_only();
-    if (kt + 1 < tiles) issue(kt + 1, BUF ^ 1);
+    if (kt + 1 < tiles) {
+      gk.template next<BUF ^ 1>();
+      gv.template next<BUF ^ 1>();
+    }
     const bool odd = kt >= whole && tile_nonfinite<E, DP>(lk), mine = kt < wave_tiles;
     const int last = (CAUSAL ? min(row, e.len - 1) : e.len - 1) - kt * KT;
     lpx8_t ds[4];
@@ -547,8 +589,8 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dq_kernel(simvg_packed_att
         f32x16 s = zero16(), dp = zero16();
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-          s = E::mfma(at.row(lk, kb, ks), qf[ks], s);
-          dp = E::mfma(at.row(lv, kb, ks), dof[ks], dp);
+          s = E::mfma(at.row(K0, kb, ks), qf[ks], s);
+          dp = E::mfma(at.row(V0, kb, ks), dof[ks], dp);
         }
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
@@ -573,21 +615,22 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dq_kernel(simvg_packed_att
 #pragma unroll
       for (int rk = 0; rk < 4; ++rk)
 #pragma unroll
-        for (int cb = 0; cb < DB; ++cb) dq[cb] = E::mfma(at.col(lk, rk, cb), ds[rk], dq[cb]);
+        for (int cb = 0; cb < DB; ++cb) dq[cb] = E::mfma(at.col(K0, rk, cb), ds[rk], dq[cb]);
     }
   };
   for (int kt = 0; kt < tiles; kt += 2) {
     tile(kt, std::integral_constant<int, 0>{});
     if (kt + 1 < tiles) tile(kt + 1, std::integral_constant<int, 1>{});
   }
-  unsigned short* out = (unsigned short*)a.dq + (long)(e.first + row) * a.dq_ts + (long)h * a.dq_hs;
-  store_rows<E, DP>(dq, a.scale * __builtin_amdgcn_exp2f(-power - shift), out, a.D, valid, lane);
+  const auto z = late_args<simvg_packed_attn_args>();
+  unsigned short* out = (unsigned short*)z->dq + (long)(e.first + row) * z->dq_ts + (long)h * z->dq_hs;
+  store_rows<E, DP>(dq, z->scale * __builtin_amdgcn_exp2f(-power - shift), out, z->D, valid, lane);
 }
 
 // dK, dV: a workgroup's 128 keys against the tiles of the queries that see them, of all heads that share the key head, one after the
 // other: the sum over heads stays in the accumulators and needs no atomics.
 template <class E, int DP, bool CAUSAL>
-__global__ __launch_bounds__(256, 1) void packed_attn_dkv_kernel(simvg_packed_attn_args a) {
+__global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void packed_attn_dkv_kernel(simvg_packed_attn_args a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ float red[8], stat[2][2][KT];
   constexpr int TILE = KT * DP * 2, DB = DP / 32, KS = DP / 16;
@@ -608,32 +651,46 @@ __global__ __launch_bounds__(256, 1) void packed_attn_dkv_kernel(simvg_packed_at
   const unsigned short* vp = (const unsigned short*)a.v + here * a.v_ts + (long)hk * a.v_hs;
   const int first = CAUSAL ? e.t * QT / KT : 0, tiles = (e.len + KT - 1) / KT - first;       // tiles of queries, from `first`
   const int wave_first = e.t * QT + wave * 32, steps = G * tiles;
-  Stager<DP, 4> gq, gd;
-  gq.init(a.q_ts, a.D, wave, lane);
-  gd.init(a.do_ts, a.D, wave, lane);
-  const unsigned lds = lds_addr(smem);
-  const float* delta = ws_of(a).delta;
-  // step i: head hk G + i / tiles, query tile first + i % tiles.  The rows' lse and delta are loaded into registers a step ahead:
-  // rows past the sequence are zeros with lse 0: P stays finite, times 0
-  int load_h = hk * G, load_t = first;
+  // step i: head hk G + i / tiles, query tile first + i % tiles
+  const long row_first = e.first + (long)first * KT;
+  Stager<DP, 0> gq;
+  Stager<DP, 2 * TILE> gd;
+  gq.init((const unsigned short*)a.q + row_first * a.q_ts + (long)hk * G * a.q_hs, a.q_ts, e.len - first * KT, a.D, smem, wave, lane);
+  gd.init((const unsigned short*)a.d_o + row_first * a.do_ts + (long)hk * G * a.do_hs, a.do_ts, e.len - first * KT, a.D, smem, wave, lane);
+  const long q_wrap = a.q_hs * 2 - (long)tiles * gq.step, d_wrap = a.do_hs * 2 - (long)tiles * gd.step;
+  // the rows' lse and delta, one value a thread, are loaded into a register a step ahead: rows past the sequence are zeros with lse
+  // 0, their P stays finite, times 0
+  const bool is_lse = tid < KT;
+  const float* stat_at = (is_lse ? a.lse + (long)hk * G * a.lse_hs : ws_of(a).delta + (long)hk * G * a.T) + row_first + (tid & (KT - 1));
+  const long stat_wrap = (is_lse ? a.lse_hs : (long)a.T) - (long)tiles * KT;
   float st0 = 0.f;
-  auto issue = [&](int buf) {
-    const int row0 = load_t * KT;
-    gq.issue((const unsigned short*)a.q + (long)e.first * a.q_ts + (long)load_h * a.q_hs, a.q_ts, row0, e.len, lds + buf * TILE);
-    gd.issue((const unsigned short*)a.d_o + (long)e.first * a.do_ts + (long)load_h * a.do_hs, a.do_ts, row0, e.len, lds + (2 + buf) * TILE);
+  int load_t = 0;
+  auto issue = [&](auto buf) {
+    constexpr int B = decltype(buf)::value;
     if (tid < 2 * KT) {
-      const int row = row0 + (tid & (KT - 1));
       st0 = 0.f;
-      if (row < e.len) st0 = tid < KT ? a.lse[(long)load_h * a.lse_hs + e.first + row] * LOG2E - shift : delta[(long)load_h * a.T + e.first + row];
+      if ((tid & (KT - 1)) < gq.left) st0 = *stat_at;
+      stat_at += KT;
     }
-    if (++load_t == first + tiles) { load_t = first; ++load_h; }
+    gq.template next<B>();
+    gd.template next<B>();
+    if (++load_t == tiles) {                                 // the next head
+      load_t = 0;
+      gq.base += q_wrap;
+      gd.base += d_wrap;
+      gq.left += tiles * KT;
+      gd.left += tiles * KT;
+      stat_at += stat_wrap;
+    }
   };
-  issue(0);
+  issue(std::integral_constant<int, 0>{});
   lpx8_t kf[KS], vf[KS];
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) { kf[ks] = global_frag(kp, ks, a.D, lane); vf[ks] = global_frag(vp, ks, a.D, lane); }
+  arrived(kf);
+  arrived(vf);
   Lanes<DP> at;
-  at.init(lane);
+  at.init(smem, lane);
   const float c = a.scale * LOG2E;
   f32x16 dk[DB], dv[DB];
 #pragma unroll
@@ -641,13 +698,13 @@ __global__ __launch_bounds__(256, 1) void packed_attn_dkv_kernel(simvg_packed_at
 
   int row0 = first * KT;
   auto tile = [&](int i, auto which) {
-    constexpr int BUF = decltype(which)::value;
-    char *lq = smem + BUF * TILE, *ld = smem + (2 + BUF) * TILE;
+    constexpr int BUF = decltype(which)::value, Q0 = BUF * TILE, D0 = (2 + BUF) * TILE;
+    char *lq = smem + Q0, *ld = smem + D0;
     const float *lse = stat[BUF][0], *del = stat[BUF][1];
-    if (tid < 2 * KT) stat[BUF][tid / KT][tid & (KT - 1)] = st0;
+    if (tid < 2 * KT) stat[BUF][tid / KT][tid & (KT - 1)] = is_lse ? st0 * LOG2E - shift : st0;
     dma_wait<0>();
     wave_barrier_only();
-    if (i + 1 < steps) issue(BUF ^ 1);
+    if (i + 1 < steps) issue(std::integral_constant<int, (BUF ^ 1)>{});
     const int from = key - row0;                             // the first row of the tile that sees the lane's key
     const bool mine = !CAUSAL || row0 + KT - 1 >= wave_first, whole = !CAUSAL || row0 >= wave_first + 31;
     // Rows that are not finite lose nothing by being cleaned before the scores: their lse (of q) or delta (of dO) is not finite either,
@@ -664,14 +721,29 @@ __global__ __launch_bounds__(256, 1) void packed_attn_dkv_kernel(simvg_packed_at
       }
     }
     if (mine) {
+      // one wave to a SIMD (its accumulators and its keys' operands are 192 registers): nobody else covers a wait, so every LDS
+      // read is asked for one step before the products that take it, and the scheduler may not move it back
+      lpx8_t rq[KS], rd[KS];
+      auto rows = [&](int qb) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) { rq[ks] = at.row(Q0, qb, ks); rd[ks] = at.row(D0, qb, ks); }
+      };
+      rows(0);
 #pragma unroll
       for (int qb = 0; qb < 2; ++qb) {
         f32x16 s = zero16(), dp = zero16();
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-          s = E::mfma(at.row(lq, qb, ks), kf[ks], s);
-          dp = E::mfma(at.row(ld, qb, ks), vf[ks], dp);
+          s = E::mfma(rq[ks], kf[ks], s);
+          dp = E::mfma(rd[ks], vf[ks], dp);
         }
+        __builtin_amdgcn_sched_barrier(0);
+        lpx8_t cd[2][DB], cq[2][DB];
+#pragma unroll
+        for (int rk = 0; rk < 2; ++rk)
+#pragma unroll
+          for (int cb = 0; cb < DB; ++cb) { cd[rk][cb] = at.col(D0, qb * 2 + rk, cb); cq[rk][cb] = at.col(Q0, qb * 2 + rk, cb); }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const f32x4_t ls = *(const f32x4_t*)(lse + qb * 32 + g * 8 + (lane >> 5) * 4);
@@ -689,13 +761,16 @@ __global__ __launch_bounds__(256, 1) void packed_attn_dkv_kernel(simvg_packed_at
           for (int x = 0; x < 16; ++x)
             if (qb * 32 + acc_row(x, lane) < from) { s[x] = 0.f; dp[x] = 0.f; }
         }
+        __builtin_amdgcn_sched_barrier(0);
+        if (qb == 0) rows(1);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int rk = 0; rk < 2; ++rk) {
           const lpx8_t p = acc_frag<E>(s, rk), ds = acc_frag<E>(dp, rk);
 #pragma unroll
           for (int cb = 0; cb < DB; ++cb) {
-            dv[cb] = E::mfma(at.col(ld, qb * 2 + rk, cb), p, dv[cb]);
-            dk[cb] = E::mfma(at.col(lq, qb * 2 + rk, cb), ds, dk[cb]);
+            dv[cb] = E::mfma(cd[rk][cb], p, dv[cb]);
+            dk[cb] = E::mfma(cq[rk][cb], ds, dk[cb]);
           }
         }
       }
@@ -707,10 +782,11 @@ __global__ __launch_bounds__(256, 1) void packed_attn_dkv_kernel(simvg_packed_at
     tile(i, std::integral_constant<int, 0>{});
     if (i + 1 < steps) tile(i + 1, std::integral_constant<int, 1>{});
   }
-  store_rows<E, DP>(dv, __builtin_amdgcn_exp2f(-shift), (unsigned short*)a.dv + (long)(e.first + key) * a.dv_ts + (long)hk * a.dv_hs, a.D,
+  const auto z = late_args<simvg_packed_attn_args>();
+  store_rows<E, DP>(dv, __builtin_amdgcn_exp2f(-shift), (unsigned short*)z->dv + (long)(e.first + key) * z->dv_ts + (long)hk * z->dv_hs, z->D,
                     valid, lane);
-  store_rows<E, DP>(dk, a.scale * __builtin_amdgcn_exp2f(-power - shift),
-                    (unsigned short*)a.dk + (long)(e.first + key) * a.dk_ts + (long)hk * a.dk_hs, a.D, valid, lane);
+  store_rows<E, DP>(dk, z->scale * __builtin_amdgcn_exp2f(-power - shift),
+                    (unsigned short*)z->dk + (long)(e.first + key) * z->dk_ts + (long)hk * z->dk_hs, z->D, valid, lane);
 }
 
 // ---------------------------------------------------------------------------------------------------------------- host

@@ -19,7 +19,7 @@ typedef __attribute__((ext_vector_type(2))) float f32x2;
 
 struct F16 {
   static constexpr bool kScaled = true;                 // 5 exponent bits: what a backward pass rounds is brought into range first
-  static constexpr unsigned kExpMask = 0x7c007c00u;
+  static constexpr int kInf = 0x7c00;
   static __device__ __forceinline__ float to_f32(unsigned short v) { return (float)__builtin_bit_cast(_Float16, v); }
   static __device__ __forceinline__ unsigned pack(float a, float b) {
     return __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2){a, b}, half2v));
@@ -30,7 +30,7 @@ struct F16 {
 };
 struct BF16 {
   static constexpr bool kScaled = false;
-  static constexpr unsigned kExpMask = 0x7f807f80u;
+  static constexpr int kInf = 0x7f80;
   static __device__ __forceinline__ float to_f32(unsigned short v) { return __uint_as_float((unsigned)v << 16); }
   static __device__ __forceinline__ unsigned pack(float a, float b) {
     return __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2){a, b}, bf2));
@@ -60,6 +60,20 @@ __device__ __forceinline__ void dma16(u32x4_t buffer, unsigned lds, unsigned off
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane((int)lds)),
                "v"(offset), "s"(buffer)
                : "memory", "m0");
+}
+// the same at LDS byte `lds` + PLUS: one scalar register serves all pieces of a wave
+template <int PLUS>
+__device__ __forceinline__ void dma16_at(u32x4_t buffer, unsigned lds, unsigned offset) {
+  asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(buffer), "n"(PLUS)
+               : "memory", "m0", "scc");
+}
+// The kernel's arguments read again from the kernarg segment: what only the end of a kernel needs does not sit in scalar registers
+// through its loop (hipcc loads all arguments at the start and then spills them)
+template <class A>
+__device__ __forceinline__ const __attribute__((address_space(4))) A* late_args() {
+  auto p = (const __attribute__((address_space(4))) A*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return p;
 }
 constexpr unsigned DMA_NOTHING = 0x80000000u;          // an offset past every buffer (which is at most one byte shorter): zeros
 template <int N>
