@@ -107,7 +107,7 @@ class VocabCeArgs(C.Structure):         # simvg_vocab_ce_args
 _SIZES = {
     "simvg_qk_norm_rope_ws_floats": [c_int, c_int],
     "simvg_packed_plan_ints": [c_int, c_int],
-    "simvg_packed_attn_ws_floats": [c_int, c_int, c_int, c_int],
+    "simvg_packed_attn_ws_floats": [c_int, c_int, c_int, c_int, c_int],
     "simvg_vocab_ce_ws_bytes": [c_int, c_int, c_int, c_int, c_int],
 }
 

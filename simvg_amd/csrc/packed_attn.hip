@@ -311,6 +311,18 @@ __device__ __forceinline__ void store_rows(const f32x16 (&acc)[DP / 32], float m
     }
 }
 
+// ... in 32 bits
+template <int DP>
+__device__ __forceinline__ void store_sums(const f32x16 (&acc)[DP / 32], float mul, float* out, int D, bool valid, int lane) {
+#pragma unroll
+  for (int cb = 0; cb < DP / 32; ++cb)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int col = cb * 32 + g * 8 + (lane >> 5) * 4;
+      if (valid && col < D) *(f32x4_t*)(out + col) = (f32x4_t){acc[cb][4 * g], acc[cb][4 * g + 1], acc[cb][4 * g + 2], acc[cb][4 * g + 3]} * mul;
+    }
+}
+
 // ------------------------------------------------------------------------------------------------------------- forward
 template <class E, int DP, bool CAUSAL>
 __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_fwd_kernel(simvg_packed_attn_args a) {
@@ -351,31 +363,27 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_fwd_kernel(
   const float c = a.scale * LOG2E;
   float m = NEG_INF, l = 0.f;                                // reference of the exponentials (raw scores), sum over this half's keys
 
-  // one tile; the buffer's number is a constant, so that every LDS address is a lane's register and a constant
-  auto tile = [&](int kt, auto which) {
+  // One tile.  The buffer's number is a constant, so that every LDS address is a lane's register and a constant; MASKED: a mask crosses
+  // it for some wave.
+  auto tile = [&](int kt, auto which, auto crossed) {
     constexpr int BUF = decltype(which)::value, K0 = BUF * TILE, V0 = (2 + BUF) * TILE;
-    char *lk = smem + K0, *lv = smem + V0;
-    (void)lk; (void)lv;
+    constexpr bool MASKED = decltype(crossed)::value;
     dma_wait<0>();                                           // this wave's pieces of the tile
     wave_barrier_only();                                     // everybody's; and everybody is done with the other buffer
     if (kt + 1 < tiles) {
       gk.template next<BUF ^ 1>();
       gv.template next<BUF ^ 1>();
     }
-    const bool odd = kt >= whole && tile_nonfinite<E, DP>(lv), mine = kt < wave_tiles;
+    const bool odd = MASKED && tile_nonfinite<E, DP>(smem + V0), mine = !MASKED || kt < wave_tiles;
     const int last = (CAUSAL ? min(row, e.len - 1) : e.len - 1) - kt * KT;     // of the tile's keys, the last that the lane's query sees
     f32x16 s[2];
     if (mine) {
-      __builtin_amdgcn_s_setprio(1);
+      s[0] = s[1] = zero16();                                // two chains of products, one waits for its own result less often
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-        s[kb] = zero16();
+      for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) s[kb] = E::mfma(at.row(K0, kb, ks), qf[ks], s[kb]);
-      }
-      __builtin_amdgcn_s_setprio(0);
-      if (kt >= wave_whole) {
-        stay_a_branch();
+        for (int kb = 0; kb < 2; ++kb) s[kb] = E::mfma(at.row(K0, kb, ks), qf[ks], s[kb]);
+      if (MASKED && kt >= wave_whole) {
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -397,33 +405,44 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_fwd_kernel(
 #pragma unroll
         for (int i = 0; i < DB; ++i) o[i] *= f;
       }
-      const float mc = m * c;
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          s[kb][r] = __builtin_amdgcn_exp2f(fmaf(s[kb][r], c, -mc));
-          l += s[kb][r];
-        }
     }
     if (odd) {
-      if (mine) add_nonfinite<E, DP, false>(o, lv, lane, [&](int j) { return j <= last; });
-      tile_clean<E, DP>(lv);
+      if (mine) add_nonfinite<E, DP, false>(o, smem + V0, lane, [&](int j) { return j <= last; });
+      tile_clean<E, DP>(smem + V0);
     }
     if (mine) {
-      __builtin_amdgcn_s_setprio(1);
+      // the exponentials of 16 keys and the products of the 16 before: vector and matrix pipes at the same time
+      const float mc = m * c;
+      lpx8_t p[4];
+      auto exps = [&](int rk) {
+        f32x16& x = s[rk >> 1];
+#pragma unroll
+        for (int r = 8 * (rk & 1); r < 8 * (rk & 1) + 8; ++r) {
+          x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], c, -mc));
+          l += x[r];
+        }
+        p[rk] = acc_frag<E>(x, rk & 1);
+      };
+      exps(0);
 #pragma unroll
       for (int rk = 0; rk < 4; ++rk) {
-        const lpx8_t p = acc_frag<E>(s[rk >> 1], rk & 1);
+        lpx8_t v[DB];
 #pragma unroll
-        for (int cb = 0; cb < DB; ++cb) o[cb] = E::mfma(at.col(V0, rk, cb), p, o[cb]);
+        for (int cb = 0; cb < DB; ++cb) v[cb] = at.col(V0, rk, cb);
+#pragma unroll
+        for (int cb = 0; cb < DB; ++cb) o[cb] = E::mfma(v[cb], p[rk], o[cb]);
+        if (rk < 3) exps(rk + 1);
       }
-      __builtin_amdgcn_s_setprio(0);
     }
   };
-  for (int kt = 0; kt < tiles; kt += 2) {
-    tile(kt, std::integral_constant<int, 0>{});
-    if (kt + 1 < tiles) tile(kt + 1, std::integral_constant<int, 1>{});
+  int kt = 0;
+  for (; kt + 1 < whole; kt += 2) {
+    tile(kt, std::integral_constant<int, 0>{}, std::false_type{});
+    tile(kt + 1, std::integral_constant<int, 1>{}, std::false_type{});
+  }
+  for (; kt < tiles; kt += 2) {                              // at most three tiles more
+    tile(kt, std::integral_constant<int, 0>{}, std::true_type{});
+    if (kt + 1 < tiles) tile(kt + 1, std::integral_constant<int, 1>{}, std::true_type{});
   }
   l += __shfl_xor(l, 32, 64);
   const auto z = late_args<simvg_packed_attn_args>();
@@ -435,13 +454,17 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_fwd_kernel(
 // ------------------------------------------------------------------------------------------------------------ backward
 // delta_i = sum_d dO_id O_id.  For fp16 also the largest norms of dO's and V's rows in a tile and head: |dP_ij| and |D_i| are at most
 // |dO_i| |V_j|, so with them dS can be brought to where fp16 has all its bits (`grad_power`).
-// ws: delta [Hq][T] | norms of dO [tiles][Hq] | norms of V [tiles][Hkv]
-struct Ws { float *delta, *ndo, *nv; };
+// ws: delta [Hq][T] | norms of dO [tiles][Hq] | norms of V [tiles][Hkv] | dk, dv of the parts [parts][2][T][Hkv][D]
+__host__ __device__ __forceinline__ long ws_fixed(int T, int nseq, int Hq, int Hkv) {
+  return ((long)Hq * T + (long)plan_capacity(T, nseq) * (Hq + Hkv) + 3) / 4 * 4;
+}
+struct Ws { float *delta, *ndo, *nv, *parts; };
 __device__ __forceinline__ Ws ws_of(const simvg_packed_attn_args& a) {
   Ws w;
   w.delta = a.ws;
   w.ndo = a.ws + (long)a.Hq * a.T;
   w.nv = w.ndo + (long)plan_capacity(a.T, a.nseq) * a.Hq;
+  w.parts = a.ws + ws_fixed(a.T, a.nseq, a.Hq, a.Hkv);
   return w;
 }
 template <class E>
@@ -546,7 +569,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_dq_kernel(s
   const unsigned short* vp = (const unsigned short*)a.v + (long)e.first * a.v_ts + (long)hk * a.v_hs;
   const int keys = CAUSAL ? min(e.len, (e.t + 1) * QT) : e.len, tiles = (keys + KT - 1) / KT;
   const int wave_first = e.t * QT + wave * 32;
-  const int whole = min(CAUSAL ? (e.t * QT + 1) / KT : tiles, e.len / KT);
+  const int whole = min(CAUSAL ? (e.t * QT + 1) / KT : tiles, e.len / KT);                     // of all four waves
   const int wave_whole = min(CAUSAL ? (wave_first + 1) / KT : tiles, e.len / KT);
   const int wave_tiles = CAUSAL ? min(tiles, (wave_first + 32 + KT - 1) / KT) : tiles;
   Stager<DP, 0> gk;
@@ -570,57 +593,70 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_dq_kernel(s
 #pragma unroll
   for (int i = 0; i < DB; ++i) dq[i] = zero16();
 
-  auto tile = [&](int kt, auto which) {
+  auto tile = [&](int kt, auto which, auto crossed) {
     constexpr int BUF = decltype(which)::value, K0 = BUF * TILE, V0 = (2 + BUF) * TILE;
-    char *lk = smem + K0, *lv = smem + V0;
-    (void)lk; (void)lv;
+    constexpr bool MASKED = decltype(crossed)::value;
     dma_wait<0>();
     wave_barrier_only();
     if (kt + 1 < tiles) {
       gk.template next<BUF ^ 1>();
       gv.template next<BUF ^ 1>();
     }
-    const bool odd = kt >= whole && tile_nonfinite<E, DP>(lk), mine = kt < wave_tiles;
+    const bool odd = MASKED && tile_nonfinite<E, DP>(smem + K0), mine = !MASKED || kt < wave_tiles;
     const int last = (CAUSAL ? min(row, e.len - 1) : e.len - 1) - kt * KT;
     lpx8_t ds[4];
-    if (mine) {
+    f32x16 s, dp;
+    auto scores = [&](int kb) {
+      s = dp = zero16();
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-        f32x16 s = zero16(), dp = zero16();
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          s = E::mfma(at.row(K0, kb, ks), qf[ks], s);
-          dp = E::mfma(at.row(V0, kb, ks), dof[ks], dp);
-        }
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float p = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse2));
-          s[r] = E::kScaled ? p * ((dp[r] - delta) * up) : p * (dp[r] - delta);
-        }
-        if (kt >= wave_whole) {
-          stay_a_branch();
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (kb * 32 + acc_row(r, lane) > last) s[r] = 0.f;
-        }
-        ds[2 * kb] = acc_frag<E>(s, 0);
-        ds[2 * kb + 1] = acc_frag<E>(s, 1);
+      for (int ks = 0; ks < KS; ++ks) {
+        s = E::mfma(at.row(K0, kb, ks), qf[ks], s);
+        dp = E::mfma(at.row(V0, kb, ks), dof[ks], dp);
       }
-    }
-    if (odd) {
-      if (mine) add_nonfinite<E, DP, true>(dq, lk, lane, [&](int j) { return j <= last; });
-      tile_clean<E, DP>(lk);
-    }
-    if (mine) {
+    };
+    auto gradients = [&](int kb) {
 #pragma unroll
-      for (int rk = 0; rk < 4; ++rk)
+      for (int r = 0; r < 16; ++r) {
+        const float p = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse2));
+        s[r] = E::kScaled ? p * ((dp[r] - delta) * up) : p * (dp[r] - delta);
+      }
+      if (MASKED && kt >= wave_whole) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (kb * 32 + acc_row(r, lane) > last) s[r] = 0.f;
+      }
+      ds[2 * kb] = acc_frag<E>(s, 0);
+      ds[2 * kb + 1] = acc_frag<E>(s, 1);
+    };
+    auto products = [&](int kb) {
+#pragma unroll
+      for (int rk = 2 * kb; rk < 2 * kb + 2; ++rk)
 #pragma unroll
         for (int cb = 0; cb < DB; ++cb) dq[cb] = E::mfma(at.col(K0, rk, cb), ds[rk], dq[cb]);
+    };
+    if (mine) { scores(0); gradients(0); }
+    if (MASKED) {                                            // both halves' dS before the tile may be cleaned
+      if (mine) { scores(1); gradients(1); }
+      if (odd) {
+        if (mine) add_nonfinite<E, DP, true>(dq, smem + K0, lane, [&](int j) { return j <= last; });
+        tile_clean<E, DP>(smem + K0);
+      }
+      if (mine) { products(0); products(1); }
+    } else {
+      products(0);
+      scores(1);
+      gradients(1);
+      products(1);
     }
   };
-  for (int kt = 0; kt < tiles; kt += 2) {
-    tile(kt, std::integral_constant<int, 0>{});
-    if (kt + 1 < tiles) tile(kt + 1, std::integral_constant<int, 1>{});
+  int kt = 0;
+  for (; kt + 1 < whole; kt += 2) {
+    tile(kt, std::integral_constant<int, 0>{}, std::false_type{});
+    tile(kt + 1, std::integral_constant<int, 1>{}, std::false_type{});
+  }
+  for (; kt < tiles; kt += 2) {
+    tile(kt, std::integral_constant<int, 0>{}, std::true_type{});
+    if (kt + 1 < tiles) tile(kt + 1, std::integral_constant<int, 1>{}, std::true_type{});
   }
   const auto z = late_args<simvg_packed_attn_args>();
   unsigned short* out = (unsigned short*)z->dq + (long)(e.first + row) * z->dq_ts + (long)h * z->dq_hs;
@@ -628,17 +664,19 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_dq_kernel(s
 }
 
 // dK, dV: a workgroup's 128 keys against the tiles of the queries that see them, of all heads that share the key head, one after the
-// other: the sum over heads stays in the accumulators and needs no atomics.
+// other: the sum over heads stays in the accumulators and needs no atomics.  Where that makes few workgroups (long sequences, few key
+// heads) each of them is cut into `parts` of equal length, whose sums in 32 bits go to the workspace and are joined in their order.
 template <class E, int DP, bool CAUSAL>
-__global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void packed_attn_dkv_kernel(simvg_packed_attn_args a) {
+__global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void packed_attn_dkv_kernel(simvg_packed_attn_args a, int parts) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ float red[8], stat[2][2][KT];
   constexpr int TILE = KT * DP * 2, DB = DP / 32, KS = DP / 16;
-  const int hk = blockIdx.x % a.Hkv, G = a.Hq / a.Hkv;
+  const int hk = blockIdx.x % a.Hkv, G = a.Hq / a.Hkv, part = blockIdx.x / a.Hkv % parts, id = blockIdx.x / a.Hkv / parts;
   Tile e;
-  if (!plan_entry(a, blockIdx.x / a.Hkv, e)) {
-    fill_tail(a, blockIdx.x / a.Hkv, a.dk, a.dk_ts, a.dk_hs, hk, nullptr);
-    return fill_tail(a, blockIdx.x / a.Hkv, a.dv, a.dv_ts, a.dv_hs, hk, nullptr);
+  if (!plan_entry(a, id, e)) {
+    if (part) return;
+    fill_tail(a, id, a.dk, a.dk_ts, a.dk_hs, hk, nullptr);
+    return fill_tail(a, id, a.dv, a.dv_ts, a.dv_hs, hk, nullptr);
   }
   const int ntile = (e.len + QT - 1) / QT;
   if (CAUSAL) e.t = ntile - 1 - e.t;                         // the plan's order is by cost: the first keys are seen by the most queries
@@ -650,21 +688,22 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void packed_attn_dkv_kernel(
   const unsigned short* kp = (const unsigned short*)a.k + here * a.k_ts + (long)hk * a.k_hs;
   const unsigned short* vp = (const unsigned short*)a.v + here * a.v_ts + (long)hk * a.v_hs;
   const int first = CAUSAL ? e.t * QT / KT : 0, tiles = (e.len + KT - 1) / KT - first;       // tiles of queries, from `first`
-  const int wave_first = e.t * QT + wave * 32, steps = G * tiles;
-  // step i: head hk G + i / tiles, query tile first + i % tiles
-  const long row_first = e.first + (long)first * KT;
+  // step i of G tiles: head hk G + i / tiles, query tile first + i % tiles; this part's are [s0, s1)
+  const int wave_first = e.t * QT + wave * 32, s0 = (int)((long)G * tiles * part / parts), s1 = (int)((long)G * tiles * (part + 1) / parts);
+  const int steps = s1 - s0, h0 = hk * G + s0 / tiles, t0 = s0 % tiles;
+  const long row_first = e.first + (long)(first + t0) * KT;
   Stager<DP, 0> gq;
   Stager<DP, 2 * TILE> gd;
-  gq.init((const unsigned short*)a.q + row_first * a.q_ts + (long)hk * G * a.q_hs, a.q_ts, e.len - first * KT, a.D, smem, wave, lane);
-  gd.init((const unsigned short*)a.d_o + row_first * a.do_ts + (long)hk * G * a.do_hs, a.do_ts, e.len - first * KT, a.D, smem, wave, lane);
+  gq.init((const unsigned short*)a.q + row_first * a.q_ts + (long)h0 * a.q_hs, a.q_ts, e.len - (first + t0) * KT, a.D, smem, wave, lane);
+  gd.init((const unsigned short*)a.d_o + row_first * a.do_ts + (long)h0 * a.do_hs, a.do_ts, e.len - (first + t0) * KT, a.D, smem, wave, lane);
   const long q_wrap = a.q_hs * 2 - (long)tiles * gq.step, d_wrap = a.do_hs * 2 - (long)tiles * gd.step;
   // the rows' lse and delta, one value a thread, are loaded into a register a step ahead: rows past the sequence are zeros with lse
   // 0, their P stays finite, times 0
   const bool is_lse = tid < KT;
-  const float* stat_at = (is_lse ? a.lse + (long)hk * G * a.lse_hs : ws_of(a).delta + (long)hk * G * a.T) + row_first + (tid & (KT - 1));
+  const float* stat_at = (is_lse ? a.lse + h0 * a.lse_hs : ws_of(a).delta + (long)h0 * a.T) + row_first + (tid & (KT - 1));
   const long stat_wrap = (is_lse ? a.lse_hs : (long)a.T) - (long)tiles * KT;
   float st0 = 0.f;
-  int load_t = 0;
+  int load_t = t0;
   auto issue = [&](auto buf) {
     constexpr int B = decltype(buf)::value;
     if (tid < 2 * KT) {
@@ -683,7 +722,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void packed_attn_dkv_kernel(
       stat_at += stat_wrap;
     }
   };
-  issue(std::integral_constant<int, 0>{});
+  if (steps > 0) issue(std::integral_constant<int, 0>{});
   lpx8_t kf[KS], vf[KS];
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) { kf[ks] = global_frag(kp, ks, a.D, lane); vf[ks] = global_frag(vp, ks, a.D, lane); }
@@ -696,7 +735,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void packed_attn_dkv_kernel(
 #pragma unroll
   for (int i = 0; i < DB; ++i) { dk[i] = zero16(); dv[i] = zero16(); }
 
-  int row0 = first * KT;
+  int row0 = (first + t0) * KT;
   auto tile = [&](int i, auto which) {
     constexpr int BUF = decltype(which)::value, Q0 = BUF * TILE, D0 = (2 + BUF) * TILE;
     char *lq = smem + Q0, *ld = smem + D0;
@@ -783,10 +822,37 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void packed_attn_dkv_kernel(
     if (i + 1 < steps) tile(i + 1, std::integral_constant<int, 1>{});
   }
   const auto z = late_args<simvg_packed_attn_args>();
-  store_rows<E, DP>(dv, __builtin_amdgcn_exp2f(-shift), (unsigned short*)z->dv + (long)(e.first + key) * z->dv_ts + (long)hk * z->dv_hs, z->D,
-                    valid, lane);
-  store_rows<E, DP>(dk, z->scale * __builtin_amdgcn_exp2f(-power - shift),
-                    (unsigned short*)z->dk + (long)(e.first + key) * z->dk_ts + (long)hk * z->dk_hs, z->D, valid, lane);
+  const float mk = z->scale * __builtin_amdgcn_exp2f(-power - shift), mv = __builtin_amdgcn_exp2f(-shift);
+  if (parts == 1) {
+    store_rows<E, DP>(dv, mv, (unsigned short*)z->dv + (long)(e.first + key) * z->dv_ts + (long)hk * z->dv_hs, z->D, valid, lane);
+    store_rows<E, DP>(dk, mk, (unsigned short*)z->dk + (long)(e.first + key) * z->dk_ts + (long)hk * z->dk_hs, z->D, valid, lane);
+  } else {
+    const long n = (long)z->T * z->Hkv * z->D;
+    float* out = z->ws + ws_fixed(z->T, z->nseq, z->Hq, z->Hkv) + 2 * part * n + ((long)(e.first + key) * z->Hkv + hk) * z->D;
+    store_sums<DP>(dk, mk, out, z->D, valid, lane);
+    store_sums<DP>(dv, mv, out + n, z->D, valid, lane);
+  }
+}
+// the parts of dk and dv, joined: one thread for 8 columns of a row (rows behind the last sequence were done by the parts' kernel)
+template <class E>
+__global__ __launch_bounds__(256) void packed_attn_join_kernel(simvg_packed_attn_args a, int parts) {
+  const int per = a.D / 8, rows = a.plan[1];
+  const long n = (long)a.T * a.Hkv * a.D;
+  for (long i = blockIdx.x * 256L + threadIdx.x; i < (long)rows * a.Hkv * per; i += gridDim.x * 256L) {
+    const int c = (int)(i % per) * 8, hk = (int)(i / per % a.Hkv);
+    const long row = i / per / a.Hkv;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const float* src = ws_of(a).parts + w * n + (row * a.Hkv + hk) * a.D + c;
+      f32x4_t lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
+      for (int p = 0; p < parts; ++p) {
+        lo += *(const f32x4_t*)(src + 2 * p * n);
+        hi += *(const f32x4_t*)(src + 2 * p * n + 4);
+      }
+      unsigned short* out = w ? (unsigned short*)a.dv + row * a.dv_ts + (long)hk * a.dv_hs : (unsigned short*)a.dk + row * a.dk_ts + (long)hk * a.dk_hs;
+      *(u32x4_t*)(out + c) = (u32x4_t){E::pack(lo[0], lo[1]), E::pack(lo[2], lo[3]), E::pack(hi[0], hi[1]), E::pack(hi[2], hi[3])};
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------------------------------------------- host
@@ -812,9 +878,18 @@ int attn_check(const simvg_packed_attn_args* a, bool bwd) {
   if (bwd) {
     SIMVG_CHECK_ARG(rows16(a->d_o, a->do_ts, a->do_hs) && rows16(a->dq, a->dq_ts, a->dq_hs) && rows16(a->dk, a->dk_ts, a->dk_hs) &&
                     rows16(a->dv, a->dv_ts, a->dv_hs), "packed_attn: rows of the gradients must start at multiples of 16 bytes");
-    SIMVG_CHECK_ARG(a->ws, "packed_attn: the backward pass needs a workspace");
+    SIMVG_CHECK_ARG(a->ws && (uintptr_t)a->ws % 16 == 0, "packed_attn: the backward pass needs a workspace, aligned to 16 bytes");
   }
   return SIMVG_OK;
+}
+
+// Parts of a dK / dV workgroup: so many that the launch has four workgroups for each of the 256 compute units (one fits at a time, and
+// under `causal` they are of very different length), and that a part still has eight tiles of queries on average.
+// (16 k prompt, 2 key heads: 258 workgroups, backward pass 5.95 ms without, see below with)
+int dkv_parts(int T, int nseq, int Hq, int Hkv) {
+  const long groups = (long)plan_capacity(T, nseq) * Hkv, tiles = (long)(Hq / Hkv) * (T / (nseq > 0 ? nseq : 1)) / KT;
+  const long p = min(1024 / groups, tiles / 16);
+  return (int)max(1L, min(p, 32L));
 }
 
 template <class E, int DP, bool CAUSAL>
@@ -826,7 +901,12 @@ void attn_launch(const simvg_packed_attn_args& a, bool bwd, hipStream_t s) {
   }
   hipLaunchKernelGGL((packed_attn_delta_kernel<E>), dim3(entries * a.Hq), dim3(256), 0, s, a);
   hipLaunchKernelGGL((packed_attn_dq_kernel<E, DP, CAUSAL>), dim3(entries * a.Hq), dim3(256), lds, s, a);
-  hipLaunchKernelGGL((packed_attn_dkv_kernel<E, DP, CAUSAL>), dim3(entries * a.Hkv), dim3(256), lds, s, a);
+  const int parts = dkv_parts(a.T, a.nseq, a.Hq, a.Hkv);
+  hipLaunchKernelGGL((packed_attn_dkv_kernel<E, DP, CAUSAL>), dim3(entries * a.Hkv * parts), dim3(256), lds, s, a, parts);
+  if (parts > 1) {
+    const long work = (long)a.T * a.Hkv * a.D / 8;
+    hipLaunchKernelGGL((packed_attn_join_kernel<E>), dim3((int)min((work + 255) / 256, 4096L)), dim3(256), 0, s, a, parts);
+  }
 }
 template <class E>
 void attn_dispatch(const simvg_packed_attn_args& a, bool bwd, hipStream_t s) {
@@ -853,8 +933,10 @@ extern "C" int simvg_packed_plan(const int* cu_seqlens, int nseq, int T, int* pl
   SIMVG_LAUNCH_CHECK();
   return SIMVG_OK;
 }
-extern "C" long simvg_packed_attn_ws_floats(int T, int nseq, int Hq, int Hkv) {
-  return T < 0 || nseq < 0 ? 0 : (long)Hq * T + (long)plan_capacity(T, nseq) * (Hq + Hkv);
+extern "C" long simvg_packed_attn_ws_floats(int T, int nseq, int Hq, int Hkv, int D) {
+  if (T < 0 || nseq < 0 || Hkv < 1 || Hq < Hkv || D < 0) return 0;
+  const int parts = dkv_parts(T, nseq, Hq, Hkv);
+  return ws_fixed(T, nseq, Hq, Hkv) + (parts > 1 ? 2L * parts * T * Hkv * D : 0);
 }
 extern "C" int simvg_packed_attn_fwd(const simvg_packed_attn_args* args, hipStream_t stream) { return attn_run(args, false, stream); }
 extern "C" int simvg_packed_attn_bwd(const simvg_packed_attn_args* args, hipStream_t stream) { return attn_run(args, true, stream); }

@@ -1473,7 +1473,7 @@ def packed_attn_bwd(q, k, v, out, lse, dout, plan, causal=True, scale=None, dq=N
     _heads(a, _seq_out("dq", dq, q.shape, q.dtype, dev), "dq", "dq")
     _heads(a, _seq_out("dk", dk, k.shape, q.dtype, dev), "dk", "dk")
     _heads(a, _seq_out("dv", dv, v.shape, q.dtype, dev), "dv", "dv")
-    ws = torch.empty(max(1, lib.simvg_packed_attn_ws_floats(a.T, a.nseq, a.Hq, a.Hkv)), device=dev, dtype=torch.float32)
+    ws = torch.empty(max(1, lib.simvg_packed_attn_ws_floats(a.T, a.nseq, a.Hq, a.Hkv, a.D)), device=dev, dtype=torch.float32)
     a.lse, a.lse_hs, a.ws = lse.data_ptr(), a.T, ws.data_ptr()
     with _on_device(dev):
         t0 = _timer.start("packed_attn_bwd") if _timer is not None else None

@@ -185,6 +185,22 @@ def test_attention_long_and_large_scores(dt):
     check_attn(q, k, v, do, cu, [300], False, scale=0.01)
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dt", [F16, BF16])
+def test_attention_few_key_heads(dt, causal):
+    # one key head, long sequences: the queries of a workgroup's keys are cut into parts, over tiles and heads
+    for lens, Hq, D in (([2100], 3, 64), ([3000], 1, 128), ([1500, 2, 1400], 5, 40)):
+        q, k, v, do, cu = attn_case(lens, Hq, 1, D, dt, tail=70)
+        n = sum(lens)
+        plan = ops.packed_plan(cu, n + 70)
+        o, lse = ops.packed_attn_fwd(q, k, v, plan, causal)
+        dq, dk, dv = ops.packed_attn_bwd(q, k, v, o, lse, do, plan, causal)
+        ref = R.attention(q[:n], k[:n], v[:n], lens, causal, D ** -0.5, do[:n])
+        worst = {name: R.off(t[:n], ref[name], ref["tol"][name]) for name, t in dict(o=o, dq=dq, dk=dk, dv=dv).items()}
+        assert max(worst.values()) <= 1, worst
+        assert not any(t[n:].any() for t in (o, dq, dk, dv))
+
+
 @pytest.mark.parametrize("gstd", [1e-4, 300.0])
 def test_attention_small_and_large_gradients_in_fp16(gstd):
     # dS of a long row is far below fp16's normal range unless it is brought up
