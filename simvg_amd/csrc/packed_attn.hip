@@ -745,7 +745,8 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void packed_attn_dkv_kernel(
     wave_barrier_only();
     if (i + 1 < steps) issue(std::integral_constant<int, (BUF ^ 1)>{});
     const int from = key - row0;                             // the first row of the tile that sees the lane's key
-    const bool mine = !CAUSAL || row0 + KT - 1 >= wave_first, whole = !CAUSAL || row0 >= wave_first + 31;
+    // (without a mask row0 + KT is always above 0: a branch all the same, or hipcc keeps the operands of two steps at once and spills)
+    const bool mine = row0 + KT > (CAUSAL ? wave_first : 0), whole = !CAUSAL || row0 >= wave_first + 31;
     // Rows that are not finite lose nothing by being cleaned before the scores: their lse (of q) or delta (of dO) is not finite either,
     // and carries that to P and dS of every key they see
     if (CAUSAL && row0 < e.t * QT + QT - 1) {

@@ -6,7 +6,7 @@
 //     dx_i = g_i sum_v e_iv w_v,   dw_v = sum_i e_iv g_i x_i,   db_v = sum_i g_i e_iv
 //
 // Bound by the matrix pipes (2 M V K forward, 6 M V K backward: the logits are computed again, they are never kept), for few rows by
-// reading w once.  Forward: a matrix product whose epilogue keeps, for each row and each 32..128 words, the maximum and the sum of the
+// reading w once.  Forward: a matrix product whose epilogue keeps, for each row and each 128 or 256 words, the maximum and the sum of the
 // exponentials; a second kernel joins them.  Backward, in pieces of the vocabulary: (1) the logits of the piece again, as e rounded to
 // 16 bits into a workspace that stays near the caches; (2) its share of dx, added to sums in 32 bits; (3) its rows of dw.  (2) and (3)
 // are products over the vocabulary and over the rows: their operands lie "the other way round" in memory and are read from LDS with
@@ -16,6 +16,8 @@
 // keeps all its bits) and g x / max|g| where the rows' gradients differ (where they are equal or 0 the factor is 1 or 0: exact).
 // Everything that is summed is summed in 32 bits; db is summed before the rounding.
 #include <atomic>
+#include <type_traits>
+#include <utility>
 
 #include "seq.h"
 
@@ -36,121 +38,166 @@ using namespace seq;
 
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 constexpr float NEG_INF = -__builtin_huge_valf();
-constexpr int BK = 64;                                       // contracted values of a stage
+constexpr int BK = 32;                                       // contracted values of a stage
+constexpr int STAGES = 3;
 
 __device__ __forceinline__ f32x16 zero16() { return (f32x16){0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}; }
 __device__ __forceinline__ int acc_row(int r, int lane) { return (r >> 2) * 8 + (lane >> 5) * 4 + (r & 3); }
+// in a branch that few tiles take: keeps hipcc from computing it for all of them and selecting
+__device__ __forceinline__ void stay_a_branch() { asm volatile(""); }
 
 // ------------------------------------------------------------------------------------------------- the matrix product
+// A workgroup of four waves, a wave on each SIMD, two workgroups to a compute unit: what one does not keep the matrix pipes busy with
+// (its epilogue of exponentials, its first stage, its barriers) the other does.  A wave's tile of 128 x 64 is 128 accumulators and 6
+// fragments of 1 KiB for 8 MFMAs of 32 cycles.
+//
 // One operand of a workgroup's tile: R rows (or columns) of the result by BK contracted values per stage.
-//   T = false: memory [R][contracted], a stage is R rows of 128 bytes;  T = true: memory [contracted][R], BK rows of 2 R bytes.
+//   T = false: memory [R][contracted], a stage is R rows of 64 bytes;  T = true: memory [contracted][R], BK rows of 2 R bytes.
 // In LDS, slots of 16 bytes are permuted within a row so that the fragment reads touch every bank once: 16 rows of one slot
 // (ds_read_b128) or 4 rows of 4 neighbouring slots (ds_read_b64_tr_b16) are one cycle's.
 template <int R, bool T> struct Operand {
-  static constexpr int BYTES = R * BK * 2;
-  static constexpr int ROW = T ? R * 2 : BK * 2;
-  static __device__ __forceinline__ int at(int row, int slot) {
-    int x;
-    if (T && R >= 128) x = (row & 3) << 2;
-    else x = (row >> 1 & 1) << 2 | (row >> 2 & 3);            // rows of 128 bytes: a pair of rows shares the banks' 256
-    return row * ROW + ((slot ^ x) << 4);
-  }
-  // the 32 x 16 fragment `f` (rows 32 f ..) of contracted values 16 ks ..
-  static __device__ __forceinline__ lpx8_t frag(const char* lds, int f, int ks, int lane) {
-    if constexpr (!T) {
-      return *(const lpx8_t*)(lds + at(f * 32 + (lane & 31), ks * 2 + (lane >> 5)));
+  static constexpr int BYTES = R * BK * 2, ROW = T ? R * 2 : BK * 2, PIECES = BYTES / 4096;
+  static_assert(PIECES >= 1 && (!T || R >= 128), "tile of an operand");
+  static __device__ __forceinline__ int at(int row, int slot) { return row * ROW + ((slot ^ (T ? (row & 3) << 2 : row >> 2 & 3)) << 4); }
+
+  // what a lane adds to a stage's start for its part of a fragment; the rest of an address is a constant in the instruction
+  typedef __attribute__((address_space(3))) const char* Lds;
+  Lds lane_at[T ? 4 : BK / 16];
+  // the wave's fragments are first .. (in units of 32 rows); `base`: where the operand's stages start
+  __device__ __forceinline__ void init_reads(const char* base, int first, int lane) {
+    const Lds b = (Lds)(const __attribute__((address_space(3))) void*)LDS_PTR(base);
+    if constexpr (T) {
+      const int i = lane & 15, row = 8 * (lane >> 5) + (i >> 2);
+#pragma unroll
+      for (int f = 0; f < 4; ++f) {
+        const int col = (first + f) * 32 + (lane >> 4 & 1) * 16 + 4 * (i & 3);
+        lane_at[f] = b + at(row, col >> 3) + (col & 7) * 2;
+      }
     } else {
-      const int i = lane & 15, col = f * 32 + (lane >> 4 & 1) * 16 + 4 * (i & 3);
-      const int row = ks * 16 + 8 * (lane >> 5) + (i >> 2);
-      const lpx4_t lo = lds_read_tr16(lds + at(row, col >> 3) + (col & 7) * 2);
-      const lpx4_t hi = lds_read_tr16(lds + at(row + 4, col >> 3) + (col & 7) * 2);
-      return (lpx8_t){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+#pragma unroll
+      for (int ks = 0; ks < BK / 16; ++ks) lane_at[ks] = b + at(first * 32 + (lane & 31), ks * 2 + (lane >> 5));
     }
   }
-};
-// The source of an operand: base of the tile's first row / column, what is there of rows (R direction) and of contracted values
-struct Source { const unsigned short* base; long ld; int rows, depth; };
+  // fragment f of the wave's, contracted values 16 ks .. of stage `st`
+  __device__ __forceinline__ lpx8_t frag(int st, int f, int ks) const {
+    if constexpr (T) {
+      typedef __attribute__((address_space(3))) lpx4_t* P;
+      const lpx4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(lane_at[f] + st * BYTES + ks * 16 * ROW));
+      const lpx4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(lane_at[f] + st * BYTES + (ks * 16 + 4) * ROW));
+      return (lpx8_t){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    } else {
+      return *(const __attribute__((address_space(3))) lpx8_t*)(lane_at[ks] + st * BYTES + f * 32 * ROW);
+    }
+  }
 
-template <int R, bool T, int WAVES> struct Stager {
-  using Op = Operand<R, T>;
-  static constexpr int PIECES = Op::BYTES / 1024 / WAVES;    // 1 KiB each
-  static_assert(PIECES >= 1, "a wave stages at least one piece");
-  unsigned off[PIECES];
-  int inner[PIECES];                                         // T = false: first contracted value of the lane's 16 bytes
-  __device__ __forceinline__ void init(const Source& s, int wave, int lane) {
+  // HBM -> LDS, 1 KiB a piece, wave w's pieces are w, w + 4 ..
+  unsigned off[PIECES], lds, step;
+  unsigned long next;                                        // the next stage's first value
+  int inner, left;                                           // the lane's first contracted value of a stage (T: of its first piece); how many are left
+  // rows: what there is of the tile's rows, depth: of contracted values from `base` on; `keep(row)`: whether a row is read (T = false)
+  template <class Keep>
+  __device__ __forceinline__ void init_stages(const unsigned short* base, long ld, int rows, int depth, const char* to, int wave, int lane, Keep keep) {
+    next = (unsigned long)base;
+    step = T ? (unsigned)(BK * 2) * (unsigned)ld : BK * 2;
+    lds = lds_addr(to) + wave * 1024;
+    left = depth;
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
-      const int byte = (wave * PIECES + i) * 1024 + lane * 16, row = byte / Op::ROW, phys = byte % Op::ROW / 16;
-      const int slot = (Op::at(row, phys) - row * Op::ROW) >> 4;               // the permutation is its own inverse
-      inner[i] = slot * 8;
-      if (T) off[i] = slot * 8 < s.rows ? (unsigned)(row * s.ld * 2 + slot * 16) : DMA_NOTHING;
-      else off[i] = row < s.rows ? (unsigned)(row * s.ld * 2 + slot * 16) : DMA_NOTHING;
+      const int byte = (i * 4 + wave) * 1024 + lane * 16, row = byte / ROW;
+      const int slot = (at(row, byte % ROW / 16) - row * ROW) >> 4;            // the permutation is its own inverse
+      if (i == 0) inner = T ? row : slot * 8;                // T = false: the same in every piece (16 rows apart)
+      off[i] = (T ? slot * 8 < rows : row < rows && keep(row)) ? (unsigned)row * (unsigned)ld * 2 + slot * 16 : DMA_NOTHING;
     }
   }
-  // stage `kt` of the contraction into LDS at `lds`
-  __device__ __forceinline__ void issue(const Source& s, int kt, unsigned lds, int wave) {
-    const int left = s.depth - kt * BK;                      // contracted values from this stage on
-    if (T) {
-      // rows past the depth lie past the buffer; columns past the tile's were ruled out in init
-      const unsigned bytes = left > 0 ? (unsigned)((min(left, BK) - 1) * s.ld * 2 + ((s.rows + 7) & ~7) * 2) : 0u;
-      const u32x4_t b = dma_buffer(s.base + (long)kt * BK * s.ld, bytes);
+  template <int ST> __device__ __forceinline__ void stage() {
+    const u32x4_t b = {(unsigned)next, (unsigned)(next >> 32) & 0xffffu, DMA_NOTHING - 1, 0x00020000u};
+    unsigned o[PIECES];
 #pragma unroll
-      for (int i = 0; i < PIECES; ++i) dma16(b, lds + (wave * PIECES + i) * 1024, off[i]);
-    } else {
-      const u32x4_t b = dma_buffer(s.base + kt * BK, left > 0 ? (unsigned)((s.rows - 1) * s.ld * 2 + ((min(left, BK) + 7) & ~7) * 2) : 0u);
-      if (left >= BK) {
+    for (int i = 0; i < PIECES; ++i) o[i] = off[i];
+    if (left < BK) {                                         // zeros behind the last contracted value
+      stay_a_branch();
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i) dma16(b, lds + (wave * PIECES + i) * 1024, off[i]);
-      } else {                                               // the row's tail: what follows it is another row
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i) dma16(b, lds + (wave * PIECES + i) * 1024, inner[i] < left ? off[i] : DMA_NOTHING);
-      }
+      for (int i = 0; i < PIECES; ++i)
+        if (inner + (T ? i * 4096 / ROW : 0) >= left) o[i] = DMA_NOTHING;
     }
+    issue<ST>(b, o, std::make_integer_sequence<int, PIECES>{});
+    next += step;
+    left -= BK;
+  }
+  template <int ST, int... I> __device__ __forceinline__ void issue(u32x4_t b, const unsigned (&o)[PIECES], std::integer_sequence<int, I...>) {
+    (dma16_at<ST * BYTES + I * 4096>(b, lds, o[I]), ...);
   }
 };
+struct KeepAll { __device__ __forceinline__ bool operator()(int) const { return true; } };
 
-// acc[i][j] += A rows (wa + 32 i ..) x B rows (wb + 32 j ..) over stages [k0, k1): registers run over A's rows, lanes over B's
+// acc[i][j] += A rows (WA of the wave's, 32 i ..) x B rows (WB, 32 j ..): registers run over A's rows, lanes over B's
 template <class E, int RA, bool TA, int RB, bool TB, int WA, int WB>
 struct Product {
-  static constexpr int WAVES = (RA / WA) * (RB / WB), THREADS = WAVES * 64, NA = WA / 32, NB = WB / 32;
+  static_assert((RA / WA) * (RB / WB) == 4, "four waves");
+  static constexpr int THREADS = 256, NA = WA / 32, NB = WB / 32;
   using OA = Operand<RA, TA>;
   using OB = Operand<RB, TB>;
-  static constexpr int STAGE = OA::BYTES + OB::BYTES, LDS = 2 * STAGE;
-  static __device__ __forceinline__ void run(f32x16 (&acc)[NA][NB], const Source& sa, const Source& sb, int k0, int k1, char* smem) {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int fa = wave / (RB / WB) * NA, fb = wave % (RB / WB) * NB;
-    Stager<RA, TA, WAVES> ga;
-    Stager<RB, TB, WAVES> gb;
-    ga.init(sa, wave, lane);
-    gb.init(sb, wave, lane);
-    const unsigned lds = lds_addr(smem);
-    if (k0 < k1) {
-      ga.issue(sa, k0, lds, wave);
-      gb.issue(sb, k0, lds + OA::BYTES, wave);
-    }
-    for (int kt = k0; kt < k1; ++kt) {
-      const int buf = (kt - k0) & 1;
-      dma_wait<0>();                                         // this wave's pieces of the stage
-      wave_barrier_only();                                   // everybody's; and everybody is done with the other buffer
-      if (kt + 1 < k1) {
-        ga.issue(sa, kt + 1, lds + (buf ^ 1) * STAGE, wave);
-        gb.issue(sb, kt + 1, lds + (buf ^ 1) * STAGE + OA::BYTES, wave);
+  static constexpr int LDS = STAGES * (OA::BYTES + OB::BYTES), IN_FLIGHT = OA::PIECES + OB::PIECES;
+  static __device__ __forceinline__ int wave_a(int wave) { return wave / (RB / WB) * WA; }
+  static __device__ __forceinline__ int wave_b(int wave) { return wave % (RB / WB) * WB; }
+
+  // Three stages in LDS: one is multiplied, the next has arrived, the one after is on its way.  The fragments of a step are read while the
+  // step before is multiplied, across the stages' border too: the barrier that makes a stage visible stands before the products
+  // of the last step of the stage before, so the matrix pipes have work behind it.
+  static __device__ __forceinline__ void run(f32x16 (&acc)[NA][NB], OA& oa, OB& ob, int stages) {
+    if (stages <= 0) return;
+    lpx8_t a[2][NA], b[2][NB];
+    auto ask = [&](auto st) { oa.template stage<decltype(st)::value>(); ob.template stage<decltype(st)::value>(); };
+    auto read = [&](auto st, auto ks) {
+      constexpr int S = decltype(st)::value, K = decltype(ks)::value;
+#pragma unroll
+      for (int j = 0; j < NB; ++j) b[K & 1][j] = ob.frag(S, j, K);
+#pragma unroll
+      for (int i = 0; i < NA; ++i) a[K & 1][i] = oa.frag(S, i, K);
+    };
+    auto multiply = [&](int k) {
+#pragma unroll
+      for (int i = 0; i < NA; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) acc[i][j] = E::mfma(a[k][i], b[k][j], acc[i][j]);
+    };
+    using I0 = std::integral_constant<int, 0>;
+    using I1 = std::integral_constant<int, 1>;
+    ask(I0{});
+    if (stages > 1) { ask(I1{}); dma_wait<IN_FLIGHT>(); } else dma_wait<0>();
+    wave_barrier_only();
+    read(I0{}, I0{});
+    auto stage = [&](int kt, auto st) {
+      constexpr int S = decltype(st)::value;
+      if (kt + 2 < stages) ask(std::integral_constant<int, (S + 2) % 3>{});    // whose stage everybody has left at the last barrier
+      read(st, I1{});
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(0);
+      __builtin_amdgcn_sched_barrier(0);
+      if (kt + 1 < stages) {
+        if (kt + 2 < stages) dma_wait<IN_FLIGHT>(); else dma_wait<0>();
+        wave_barrier_only();
+        read(std::integral_constant<int, (S + 1) % 3>{}, I0{});
       }
-      const char *la = smem + buf * STAGE, *lb = la + OA::BYTES;
-#pragma unroll
-      for (int ks = 0; ks < BK / 16; ++ks) {
-        lpx8_t a[NA], b[NB];
-#pragma unroll
-        for (int j = 0; j < NB; ++j) b[j] = OB::frag(lb, fb + j, ks, lane);
-#pragma unroll
-        for (int i = 0; i < NA; ++i) a[i] = OA::frag(la, fa + i, ks, lane);
-#pragma unroll
-        for (int i = 0; i < NA; ++i)
-#pragma unroll
-          for (int j = 0; j < NB; ++j) acc[i][j] = E::mfma(a[i], b[j], acc[i][j]);
-      }
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(1);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    for (int kt = 0;;) {
+      stage(kt, I0{});
+      if (++kt >= stages) break;
+      stage(kt, I1{});
+      if (++kt >= stages) break;
+      stage(kt, std::integral_constant<int, 2>{});
+      if (++kt >= stages) break;
     }
     __syncthreads();                                         // the epilogues use the LDS
+  }
+  static __device__ __forceinline__ void zero(f32x16 (&acc)[NA][NB]) {
+#pragma unroll
+    for (int i = 0; i < NA; ++i)
+#pragma unroll
+      for (int j = 0; j < NB; ++j) acc[i][j] = zero16();
   }
 };
 
@@ -168,40 +215,53 @@ __device__ __forceinline__ void tile_of(int id, int n, int outer, int inner, int
 __device__ __forceinline__ bool is_word(const simvg_vocab_ce_args& a, long t) { return t != a.ignore_index && t >= 0 && t < a.V; }
 
 // ------------------------------------------------------------------------------------------------------------- forward
-// words in registers, rows in lanes: [word group of WA][M] (maximum, sum of exp2) and the targets' logits
-template <class E, int RB, int WA, int WB>
-__global__ __launch_bounds__((256 / WA) * (RB / WB) * 64) void ce_fwd_kernel(simvg_vocab_ce_args a, float2* part, float* zt) {
-  using P = Product<E, 256, false, RB, false, WA, WB>;
+// words in registers, rows in lanes: [tile of RA words][M] (maximum, sum of exp2) and the targets' logits
+template <class E, int RA, int RB, int WA, int WB>
+__global__ __launch_bounds__(256, 2) void ce_fwd_kernel(simvg_vocab_ce_args a, float2* part, float* zt) {
+  using P = Product<E, RA, false, RB, false, WA, WB>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int tv = cdiv(a.V, 256), tm = cdiv(a.M, RB);
+  const int tv = cdiv(a.V, RA), tm = cdiv(a.M, RB);
   int iv, im;
-  tile_of(blockIdx.x, tv * tm, tv, tm, 4, iv, im);
-  const int v0 = iv * 256, m0 = im * RB;
+  tile_of(blockIdx.x, tv * tm, tv, tm, 8, iv, im);
+  const int v0 = iv * RA, m0 = im * RB, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   f32x16 acc[P::NA][P::NB];
+  P::zero(acc);
+  typename P::OA oa;
+  typename P::OB ob;
+  oa.init_stages((const unsigned short*)a.w + (long)v0 * a.ldw, a.ldw, min(RA, a.V - v0), a.K, smem, wave, lane, KeepAll{});
+  ob.init_stages((const unsigned short*)a.x + (long)m0 * a.ldx, a.ldx, min(RB, a.M - m0), a.K, smem + STAGES * P::OA::BYTES, wave, lane, KeepAll{});
+  oa.init_reads(smem, P::wave_a(wave) / 32, lane);
+  ob.init_reads(smem + STAGES * P::OA::BYTES, P::wave_b(wave) / 32, lane);
+  P::run(acc, oa, ob, cdiv(a.K, BK));
+  const int wv = v0 + P::wave_a(wave), wm = P::wave_b(wave);
+  if (a.bias) {
 #pragma unroll
-  for (int i = 0; i < P::NA; ++i)
+    for (int i = 0; i < P::NA; ++i)
 #pragma unroll
-    for (int j = 0; j < P::NB; ++j) acc[i][j] = zero16();
-  const Source sa = {(const unsigned short*)a.w + (long)v0 * a.ldw, a.ldw, min(256, a.V - v0), a.K};
-  const Source sb = {(const unsigned short*)a.x + (long)m0 * a.ldx, a.ldx, min(RB, a.M - m0), a.K};
-  P::run(acc, sa, sb, 0, cdiv(a.K, BK), smem);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int wv = v0 + wave / (RB / WB) * WA, wm = m0 + wave % (RB / WB) * WB;
+      for (int r = 0; r < 16; ++r) {
+        const float b = a.bias[min(wv + i * 32 + acc_row(r, lane), a.V - 1)];
 #pragma unroll
-  for (int i = 0; i < P::NA; ++i)
+        for (int j = 0; j < P::NB; ++j) acc[i][j][r] += b;
+      }
+  }
+  if (wv + WA > a.V) {
+    stay_a_branch();
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int v = wv + i * 32 + acc_row(r, lane);
-      const float b = a.bias && v < a.V ? a.bias[v] : 0.f;
+    for (int i = 0; i < P::NA; ++i)
 #pragma unroll
-      for (int j = 0; j < P::NB; ++j) acc[i][j][r] = v < a.V ? acc[i][j][r] + b : NEG_INF;
-    }
+      for (int r = 0; r < 16; ++r)
+#pragma unroll
+        for (int j = 0; j < P::NB; ++j)
+          if (wv + i * 32 + acc_row(r, lane) >= a.V) acc[i][j][r] = NEG_INF;
+  }
+  float2* joined = (float2*)smem;                            // [RA / WA][RB]
 #pragma unroll
   for (int j = 0; j < P::NB; ++j) {
-    const int m = wm + j * 32 + (lane & 31);
+    const int mr = wm + j * 32 + (lane & 31), m = m0 + mr;
     const long t = m < a.M ? a.target[m] : -1;
     const int local = t >= wv && t < wv + WA && t < a.V ? (int)(t - wv) : -1;
     if (__any(local >= 0)) {
+      stay_a_branch();
 #pragma unroll
       for (int i = 0; i < P::NA; ++i)
 #pragma unroll
@@ -220,31 +280,51 @@ __global__ __launch_bounds__((256 / WA) * (RB / WB) * 64) void ce_fwd_kernel(sim
 #pragma unroll
       for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], LOG2E, -ref));
     sum += __shfl_xor(sum, 32, 64);
-    if (lane < 32 && m < a.M && wv < a.V) part[(long)(wv / WA) * a.M + m] = make_float2(top, sum);
+    if (lane < 32) joined[wave / (RB / WB) * RB + mr] = make_float2(top, sum);
+  }
+  __syncthreads();
+  if (threadIdx.x < RB && m0 + (int)threadIdx.x < a.M) {
+    float top = NEG_INF, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < RA / WA; ++w) top = fmaxf(top, joined[w * RB + threadIdx.x].x);
+    const float ref = top == NEG_INF ? 0.f : top;
+#pragma unroll
+    for (int w = 0; w < RA / WA; ++w) {
+      const float2 p = joined[w * RB + threadIdx.x];
+      sum += p.y * __builtin_amdgcn_exp2f((p.x - ref) * LOG2E);
+    }
+    part[(long)iv * a.M + m0 + threadIdx.x] = make_float2(top, sum);
   }
 }
-// 32 rows and 32 strands of word groups to a workgroup
+// 8 rows and 128 strands of word tiles to a workgroup
 __global__ __launch_bounds__(1024) void ce_join_kernel(simvg_vocab_ce_args a, const float2* part, const float* zt, int groups) {
-  __shared__ float tops[32][33], sums[32][33];
-  const int c = threadIdx.x & 31, s = threadIdx.x >> 5, m = blockIdx.x * 32 + c;
+  __shared__ float tops[128][9], sums[128][9];
+  const int c = threadIdx.x & 7, s = threadIdx.x >> 3, m = blockIdx.x * 8 + c;
   float top = NEG_INF, sum = 0.f;
-  if (m < a.M)
-    for (int g = s; g < groups; g += 32) {
+  if (m < a.M) {
+#pragma unroll 4
+    for (int g = s; g < groups; g += 128) {
       const float2 p = part[(long)g * a.M + m];
       const float to = fmaxf(top, p.x), ref = to == NEG_INF ? 0.f : to;
       sum = sum * __builtin_amdgcn_exp2f((top - ref) * LOG2E) + p.y * __builtin_amdgcn_exp2f((p.x - ref) * LOG2E);
       top = to;
     }
+  }
   tops[s][c] = top;
   sums[s][c] = sum;
   __syncthreads();
+  for (int n = 64; n > 0; n >>= 1) {
+    if (s < n) {
+      const float t1 = tops[s + n][c], to = fmaxf(top, t1), ref = to == NEG_INF ? 0.f : to;
+      sum = sum * __builtin_amdgcn_exp2f((top - ref) * LOG2E) + sums[s + n][c] * __builtin_amdgcn_exp2f((t1 - ref) * LOG2E);
+      top = to;
+      tops[s][c] = top;
+      sums[s][c] = sum;
+    }
+    __syncthreads();
+  }
   if (s == 0 && m < a.M) {
-    float t = NEG_INF;
-    for (int i = 0; i < 32; ++i) t = fmaxf(t, tops[i][c]);
-    const float ref = t == NEG_INF ? 0.f : t;
-    float total = 0.f;
-    for (int i = 0; i < 32; ++i) total += sums[i][c] * __builtin_amdgcn_exp2f((tops[i][c] - ref) * LOG2E);
-    const float lse = ref + __builtin_logf(total);
+    const float lse = (top == NEG_INF ? 0.f : top) + __builtin_logf(sum);
     const long target = a.target[m];
     a.lse[m] = lse;
     // a target that is neither a word nor ignored is a mistake of the caller's: its loss says so
@@ -253,22 +333,23 @@ __global__ __launch_bounds__(1024) void ce_join_kernel(simvg_vocab_ce_args a, co
 }
 
 // ------------------------------------------------------------------------------------------------------------ backward
-// ws: max|g| | row factors g / max|g| [M] | g x / max|g| [M][K] 16 bit | e [M][piece] 16 bit | dx sums [splits][M][K] | db sums [rows / RA][V]
+// ws: max|g| | row factors g / max|g| [M] | g x / max|g| [M][K] 16 bit | e [M][piece] 16 bit | dx sums [splits][M][K] | db sums [waves' rows][V]
 struct Plan { int piece, splits, small; long o_factor, o_x, o_e, o_dx, o_db, bytes; };
 constexpr long E_BYTES = 256L << 20;                         // of e at a time: what the memory-side cache holds
+constexpr int SMALL_M = 64;                                  // up to here one tile of 64 rows, beyond tiles of 128
 
 Plan ce_plan(int M, int V, int K, bool bias) {
   Plan p;
-  p.small = M <= 64;
+  p.small = M <= SMALL_M;
   const long words = cdiv(V, 256) * 256L;
   long piece = E_BYTES / 2 / M / 256 * 256;
   if (piece < 1024) piece = 1024;
   if (piece > words) piece = words;
   const long n = (words + piece - 1) / piece;                // even pieces
   p.piece = (int)(((words + n - 1) / n + 255) / 256 * 256);
-  // dx is M x K: few tiles.  The piece's words are shared out so that the chip's 256 compute units have a tile each
-  const int tiles = cdiv(K, 256) * cdiv(M, p.small ? 64 : 256), most = p.piece / 256;
-  p.splits = 256 / tiles < 1 ? 1 : 256 / tiles > most ? most : 256 / tiles;
+  // dx is M x K: few tiles.  The piece's words are shared out so that the chip's 512 workgroups have a tile each, of 256 words at least
+  const int tiles = cdiv(K, 256) * cdiv(M, p.small ? 64 : 128), most = p.piece / 256;
+  p.splits = 512 / tiles < 1 ? 1 : 512 / tiles > most ? most : 512 / tiles;
   auto up = [](long n) { return (n + 255) / 256 * 256; };
   long o = 256;
   p.o_factor = o; o += up(M * 4L);
@@ -316,85 +397,149 @@ __global__ __launch_bounds__(256) void ce_scale_kernel(simvg_vocab_ce_args a, co
 constexpr float E_POWER = 14.f;
 template <class E> __device__ __forceinline__ float e_scale() { return E::kScaled ? 16384.f : 1.f; }
 
-// (1) rows in registers, words in lanes: e of words [v_begin, v_begin + piece) and db's sums over the workgroup's rows
-template <class E, int RA, int WA, int WB>
-__global__ __launch_bounds__((RA / WA) * (256 / WB) * 64) void ce_e_kernel(simvg_vocab_ce_args a, const float* factor, unsigned short* e,
-                                                                           int piece, int v_begin, float* db) {
-  using P = Product<E, RA, false, 256, false, WA, WB>;
+// the sum of v over a half wave's 16-lane row, in all its lanes' last
+template <int CTRL> __device__ __forceinline__ float dpp_add(float v) {
+  return v + __uint_as_float((unsigned)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float row16_sum(float v) {
+  v = dpp_add<0xb1>(v);                                      // lane ^ 1 (quad_perm 1, 0, 3, 2)
+  v = dpp_add<0x4e>(v);                                      // lane ^ 2 (quad_perm 2, 3, 0, 1)
+  v = dpp_add<0x141>(v);                                     // the other four of eight (row_half_mirror)
+  return dpp_add<0x140>(v);                                  // the other eight (row_mirror)
+}
+
+// (1) words in registers, rows in lanes: e of words [v_begin, v_begin + piece), and db's sums over the wave's rows.  Ignored rows of x
+// are not read: their logits are 0 whatever they hold, and with an lse of +inf so are their probabilities.
+template <class E, int RA, int RB, int WA, int WB, bool BIAS>
+__global__ __launch_bounds__(256, 2) void ce_e_kernel(simvg_vocab_ce_args a, const float* factor, unsigned short* e, int piece, int v_begin,
+                                                      float* db) {
+  using P = Product<E, RA, false, RB, false, WA, WB>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int tv = piece / 256, tm = cdiv(a.M, RA);
+  const int tv = piece / RA, tm = cdiv(a.M, RB);
   int iv, im;
-  tile_of(blockIdx.x, tv * tm, tv, tm, 4, iv, im);
-  const int l0 = iv * 256, v0 = v_begin + l0, m0 = im * RA;
+  tile_of(blockIdx.x, tv * tm, tv, tm, 8, iv, im);
+  const int l0 = iv * RA, v0 = v_begin + l0, m0 = im * RB, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   f32x16 acc[P::NA][P::NB];
-#pragma unroll
-  for (int i = 0; i < P::NA; ++i)
-#pragma unroll
-    for (int j = 0; j < P::NB; ++j) acc[i][j] = zero16();
-  const int words = min(256, a.V - v0);                      // may be <= 0 in the last piece: e is zeros there
-  const Source sa = {(const unsigned short*)a.x + (long)m0 * a.ldx, a.ldx, min(RA, a.M - m0), a.K};
-  const Source sb = {(const unsigned short*)a.w + (words > 0 ? (long)v0 * a.ldw : 0L), a.ldw, max(words, 0), a.K};
-  if (words > 0) P::run(acc, sa, sb, 0, cdiv(a.K, BK), smem);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int wl = wave % (256 / WB) * WB, wm = m0 + wave / (256 / WB) * WA;
-  const float up = e_scale<E>();
-  float bias[P::NB], sum[P::NB];
+  P::zero(acc);
+  const int words = min(RA, a.V - v0);                       // may be <= 0 in the last piece: e is zeros there
+  if (words > 0) {
+    typename P::OA oa;
+    typename P::OB ob;
+    oa.init_stages((const unsigned short*)a.w + (long)v0 * a.ldw, a.ldw, words, a.K, smem, wave, lane, KeepAll{});
+    ob.init_stages((const unsigned short*)a.x + (long)m0 * a.ldx, a.ldx, min(RB, a.M - m0), a.K, smem + STAGES * P::OA::BYTES, wave, lane,
+                   [&](int row) { return is_word(a, a.target[m0 + row]); });
+    oa.init_reads(smem, P::wave_a(wave) / 32, lane);
+    ob.init_reads(smem + STAGES * P::OA::BYTES, P::wave_b(wave) / 32, lane);
+    P::run(acc, oa, ob, cdiv(a.K, BK));
+  }
+  const int wl = P::wave_a(wave), wv = v0 + wl, wm = P::wave_b(wave);
+  float less[P::NB], g[P::NB];
+  int local[P::NB];
+  bool any = false;
 #pragma unroll
   for (int j = 0; j < P::NB; ++j) {
-    const int v = v0 + wl + j * 32 + (lane & 31);
-    bias[j] = a.bias && v < a.V ? a.bias[v] : 0.f;
-    sum[j] = 0.f;
+    const int m = m0 + wm + j * 32 + (lane & 31), mc = min(m, a.M - 1);
+    const long t = a.target[mc];
+    const bool on = m < a.M && is_word(a, t);
+    less[j] = on ? (E::kScaled ? E_POWER : 0.f) - a.lse[mc] * LOG2E : NEG_INF;
+    g[j] = BIAS && on ? factor[mc] : 0.f;
+    local[j] = on && t >= wv && t < wv + WA ? (int)(t - wv) : -1;
+    any = any || local[j] >= 0;
+  }
+  if (BIAS) {
+#pragma unroll
+    for (int i = 0; i < P::NA; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float b = a.bias[min(wv + i * 32 + acc_row(r, lane), a.V - 1)];
+#pragma unroll
+        for (int j = 0; j < P::NB; ++j) acc[i][j][r] += b;
+      }
   }
 #pragma unroll
   for (int i = 0; i < P::NA; ++i)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int m = wm + i * 32 + acc_row(r, lane), mc = min(m, a.M - 1);
-      const long t = a.target[mc];
-      const bool on = m < a.M && is_word(a, t);
-      const float lse = a.lse[mc] * LOG2E, g = a.dbias ? factor[mc] : 0.f;
+    for (int j = 0; j < P::NB; ++j)
 #pragma unroll
-      for (int j = 0; j < P::NB; ++j) {
-        const int v = v0 + wl + j * 32 + (lane & 31);
-        float p = __builtin_amdgcn_exp2f(fmaf(acc[i][j][r] + bias[j], LOG2E, -lse));
-        if (t == v) p -= 1.f;
-        p = on && v < a.V ? p : 0.f;
-        sum[j] += on ? p * g : 0.f;
-        if (m < a.M) e[(long)m * piece + l0 + wl + j * 32 + (lane & 31)] = (unsigned short)E::pack(p * up, 0.f);
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], LOG2E, less[j]));
+  if (wv + WA > a.V) {
+    stay_a_branch();
+#pragma unroll
+    for (int i = 0; i < P::NA; ++i)
+#pragma unroll
+      for (int j = 0; j < P::NB; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (wv + i * 32 + acc_row(r, lane) >= a.V) acc[i][j][r] = 0.f;
+  }
+  if (__any(any)) {                                          // a target of the wave's rows is among the wave's words
+    stay_a_branch();
+#pragma unroll
+    for (int i = 0; i < P::NA; ++i)
+#pragma unroll
+      for (int j = 0; j < P::NB; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (local[j] == i * 32 + acc_row(r, lane)) acc[i][j][r] -= e_scale<E>();
+  }
+  if (BIAS) {
+    const float down = 1.f / e_scale<E>();
+#pragma unroll
+    for (int i = 0; i < P::NA; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        float s = 0.f;
+#pragma unroll
+        for (int j = 0; j < P::NB; ++j) s += g[j] == 0.f ? 0.f : acc[i][j][r] * g[j];
+        s = row16_sum(s);
+        s += __shfl_xor(s, 16, 64);
+        const int v = wv + i * 32 + acc_row(r, lane);
+        if ((lane & 31) == 0 && v < a.V && m0 + wm < a.M) db[(long)((m0 + wm) / WB) * a.V + v] = s * down;
       }
-    }
-  if (a.dbias) {
+  }
+  // through LDS, so that a row's words leave in whole lines: [row of the wave][WA words], rows 16 bytes longer than the words
+  constexpr int LD = WA * 2 + 16;
+  static_assert(4 * WB * LD <= P::LDS, "the waves' blocks of e fit the stages' LDS");
+  char* mine = smem + wave * WB * LD;
 #pragma unroll
-    for (int j = 0; j < P::NB; ++j) {
-      const int v = v0 + wl + j * 32 + (lane & 31);
-      sum[j] += __shfl_xor(sum[j], 32, 64);
-      if (lane < 32 && v < a.V && wm < a.M) db[(long)(wm / WA) * a.V + v] = sum[j];
-    }
+  for (int j = 0; j < P::NB; ++j)
+#pragma unroll
+    for (int i = 0; i < P::NA; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *(u32x2_t*)(mine + (j * 32 + (lane & 31)) * LD + (i * 32 + q * 8 + (lane >> 5) * 4) * 2) =
+            (u32x2_t){E::pack(acc[i][j][4 * q], acc[i][j][4 * q + 1]), E::pack(acc[i][j][4 * q + 2], acc[i][j][4 * q + 3])};
+  constexpr int PER = WA / 8, ROWS = 64 / PER;               // lanes to a row, rows at a time
+#pragma unroll 4
+  for (int r = 0; r < WB; r += ROWS) {
+    const int row = r + lane / PER, m = m0 + wm + row;
+    const u32x4_t v = *(const u32x4_t*)(mine + row * LD + lane % PER * 16);
+    if (m < a.M) *(u32x4_t*)(e + (long)m * piece + l0 + wl + lane % PER * 8) = v;
   }
 }
 // (2) K in registers, rows in lanes: the piece's share of dx into this split's sums
 template <class E, int RB, int WA, int WB>
-__global__ __launch_bounds__((256 / WA) * (RB / WB) * 64) void ce_dx_kernel(simvg_vocab_ce_args a, const unsigned short* e, int piece,
-                                                                            int v_begin, int splits, float* sums) {
+__global__ __launch_bounds__(256, 2) void ce_dx_kernel(simvg_vocab_ce_args a, const unsigned short* e, int piece, int v_begin, int splits,
+                                                       float* sums) {
   using P = Product<E, 256, true, RB, false, WA, WB>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tk = cdiv(a.K, 256), tm = cdiv(a.M, RB), tiles = tk * tm;
   int ik, im;
   const int split = blockIdx.x / tiles;
   tile_of(blockIdx.x % tiles, tiles, tm, tk, tk, im, ik);
-  const int k0 = ik * 256, m0 = im * RB;
+  const int k0 = ik * 256, m0 = im * RB, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   f32x16 acc[P::NA][P::NB];
-#pragma unroll
-  for (int i = 0; i < P::NA; ++i)
-#pragma unroll
-    for (int j = 0; j < P::NB; ++j) acc[i][j] = zero16();
+  P::zero(acc);
   const int words = min(piece, a.V - v_begin), stages = cdiv(words, BK);
   const int s0 = (int)((long)stages * split / splits), s1 = (int)((long)stages * (split + 1) / splits);
-  const Source sa = {(const unsigned short*)a.w + (long)v_begin * a.ldw + k0, a.ldw, min(256, a.K - k0), words};
-  const Source sb = {e + (long)m0 * piece, piece, min(RB, a.M - m0), words};
-  P::run(acc, sa, sb, s0, s1, smem);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int wk = k0 + wave / (RB / WB) * WA, wm = m0 + wave % (RB / WB) * WB;
+  typename P::OA oa;
+  typename P::OB ob;
+  oa.init_stages((const unsigned short*)a.w + ((long)v_begin + s0 * BK) * a.ldw + k0, a.ldw, min(256, a.K - k0), words - s0 * BK, smem, wave, lane, KeepAll{});
+  ob.init_stages(e + (long)m0 * piece + s0 * BK, piece, min(RB, a.M - m0), words - s0 * BK, smem + STAGES * P::OA::BYTES, wave, lane, KeepAll{});
+  oa.init_reads(smem, P::wave_a(wave) / 32, lane);
+  ob.init_reads(smem + STAGES * P::OA::BYTES, P::wave_b(wave) / 32, lane);
+  P::run(acc, oa, ob, s1 - s0);
+  const int wk = k0 + P::wave_a(wave), wm = m0 + P::wave_b(wave);
 #pragma unroll
   for (int j = 0; j < P::NB; ++j) {
     const int m = wm + j * 32 + (lane & 31);
@@ -413,25 +558,26 @@ __global__ __launch_bounds__((256 / WA) * (RB / WB) * 64) void ce_dx_kernel(simv
   }
 }
 // (3) K in registers, words in lanes: the piece's rows of dw
-template <class E, int RB, int WA, int WB>
-__global__ __launch_bounds__((256 / WA) * (RB / WB) * 64) void ce_dw_kernel(simvg_vocab_ce_args a, const unsigned short* xs,
-                                                                            const unsigned short* e, int piece, int v_begin, const float* gmax) {
-  using P = Product<E, 256, true, RB, true, WA, WB>;
+template <class E>
+__global__ __launch_bounds__(256, 2) void ce_dw_kernel(simvg_vocab_ce_args a, const unsigned short* xs, const unsigned short* e, int piece,
+                                                       int v_begin, const float* gmax) {
+  constexpr int RB = 128;
+  using P = Product<E, 256, true, RB, true, 128, 64>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int words = min(piece, a.V - v_begin), tk = cdiv(a.K, 256), tv = cdiv(words, RB);
   int ik, iv;
   tile_of(blockIdx.x, tk * tv, tv, tk, tk, iv, ik);
-  const int k0 = ik * 256, l0 = iv * RB;
+  const int k0 = ik * 256, l0 = iv * RB, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   f32x16 acc[P::NA][P::NB];
-#pragma unroll
-  for (int i = 0; i < P::NA; ++i)
-#pragma unroll
-    for (int j = 0; j < P::NB; ++j) acc[i][j] = zero16();
-  const Source sa = {xs + k0, a.K, min(256, a.K - k0), a.M};
-  const Source sb = {e + l0, piece, min(RB, piece - l0), a.M};
-  P::run(acc, sa, sb, 0, cdiv(a.M, BK), smem);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int wk = k0 + wave / (RB / WB) * WA, wl = l0 + wave % (RB / WB) * WB;
+  P::zero(acc);
+  typename P::OA oa;
+  typename P::OB ob;
+  oa.init_stages(xs + k0, a.K, min(256, a.K - k0), a.M, smem, wave, lane, KeepAll{});
+  ob.init_stages(e + l0, piece, min(RB, piece - l0), a.M, smem + STAGES * P::OA::BYTES, wave, lane, KeepAll{});
+  oa.init_reads(smem, P::wave_a(wave) / 32, lane);
+  ob.init_reads(smem + STAGES * P::OA::BYTES, P::wave_b(wave) / 32, lane);
+  P::run(acc, oa, ob, cdiv(a.M, BK));
+  const int wk = k0 + P::wave_a(wave), wl = l0 + P::wave_b(wave);
   const float mul = gmax[0] / e_scale<E>();
 #pragma unroll
   for (int j = 0; j < P::NB; ++j) {
@@ -455,6 +601,7 @@ __global__ __launch_bounds__(256) void ce_dx_join_kernel(simvg_vocab_ce_args a, 
   for (long i = blockIdx.x * 256L + threadIdx.x; i < (long)a.M * per; i += (long)gridDim.x * 256) {
     const int m = (int)(i / per), c = (int)(i % per) * 4;
     f32x4_t v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
     for (int s = 0; s < splits; ++s) v += *(const f32x4_t*)(sums + ((long)s * a.M + m) * a.K + c);
     const bool on = is_word(a, a.target[m]);
     const float g = on ? a.dloss[m] / e_scale<E>() : 0.f;
@@ -466,6 +613,7 @@ __global__ __launch_bounds__(256) void ce_db_join_kernel(simvg_vocab_ce_args a, 
   const int v = blockIdx.x * 256 + threadIdx.x;
   if (v >= a.V) return;
   float s = 0.f;
+#pragma unroll 8
   for (int g = 0; g < groups; ++g) s += db[(long)g * a.V + v];
   a.dbias[v] = s * gmax[0];
 }
@@ -506,23 +654,22 @@ void allow_lds(const void* kernel, int bytes, std::atomic<unsigned long>& done) 
     hipLaunchKernelGGL((KERNEL), dim3(GRID), dim3(P::THREADS), P::LDS, s, __VA_ARGS__);  \
   } while (0)
 
-long ce_fwd_groups(int V, bool small) { return (long)cdiv(V, 256) * (small ? 8 : 2); }
+int ce_fwd_groups(int V, int M) { return cdiv(V, M <= SMALL_M ? 128 : 256); }
 
 template <class E>
 int ce_fwd(const simvg_vocab_ce_args& a, hipStream_t s) {
-  const bool small = a.M <= 64;
-  const int wa = small ? 32 : 128, groups = cdiv(a.V, wa);
+  const int groups = ce_fwd_groups(a.V, a.M);
   float* zt = (float*)a.ws;
   float2* part = (float2*)((char*)a.ws + (a.M * 4L + 255) / 256 * 256);
-  if (small) {
-    using P = Product<E, 256, false, 64, false, 32, 64>;
-    CE_LAUNCH(P, (ce_fwd_kernel<E, 64, 32, 64>), cdiv(a.V, 256) * cdiv(a.M, 64), a, part, zt);
+  if (a.M <= SMALL_M) {                                      // a row of tiles: bound by reading w, half as high tiles keep both workgroups of a CU busy
+    using P = Product<E, 128, false, 64, false, 32, 64>;
+    CE_LAUNCH(P, (ce_fwd_kernel<E, 128, 64, 32, 64>), groups, a, part, zt);
   } else {
-    using P = Product<E, 256, false, 256, false, 128, 64>;
-    CE_LAUNCH(P, (ce_fwd_kernel<E, 256, 128, 64>), cdiv(a.V, 256) * cdiv(a.M, 256), a, part, zt);
+    using P = Product<E, 256, false, 128, false, 128, 64>;
+    CE_LAUNCH(P, (ce_fwd_kernel<E, 256, 128, 128, 64>), groups * cdiv(a.M, 128), a, part, zt);
   }
   SIMVG_LAUNCH_CHECK();
-  hipLaunchKernelGGL(ce_join_kernel, dim3(cdiv(a.M, 32)), dim3(1024), 0, s, a, part, zt, groups);
+  hipLaunchKernelGGL(ce_join_kernel, dim3(cdiv(a.M, 8)), dim3(1024), 0, s, a, part, zt, groups);
   SIMVG_LAUNCH_CHECK();
   return SIMVG_OK;
 }
@@ -544,25 +691,29 @@ int ce_bwd(const simvg_vocab_ce_args& a, hipStream_t s) {
   hipLaunchKernelGGL(ce_scale_kernel<E>, dim3(min(2048, cdiv(a.M, 2) )), dim3(256), 0, s, a, factor, xs);
   SIMVG_LAUNCH_CHECK();
   const int tk = cdiv(a.K, 256);
-  for (int v = 0; v < a.V; v += p.piece) {
+  const auto piece = [&](auto bias, int v) {
+    constexpr bool B = decltype(bias)::value;
     const int words = min(p.piece, a.V - v);
     if (p.small) {
-      using P1 = Product<E, 64, false, 256, false, 64, 32>;
-      using P2 = Product<E, 256, true, 64, false, 32, 64>;
-      CE_LAUNCH(P1, (ce_e_kernel<E, 64, 64, 32>), cdiv(a.M, 64) * (p.piece / 256), a, factor, e, p.piece, v, db);
-      CE_LAUNCH(P2, (ce_dx_kernel<E, 64, 32, 64>), cdiv(a.M, 64) * tk * p.splits, a, e, p.piece, v, p.splits, sums);
+      using P1 = Product<E, 128, false, 64, false, 32, 64>;
+      using P2 = Product<E, 256, true, 64, false, 64, 64>;
+      CE_LAUNCH(P1, (ce_e_kernel<E, 128, 64, 32, 64, B>), p.piece / 128, a, factor, e, p.piece, v, db);
+      CE_LAUNCH(P2, (ce_dx_kernel<E, 64, 64, 64>), tk * p.splits, a, e, p.piece, v, p.splits, sums);
     } else {
-      using P1 = Product<E, 256, false, 256, false, 128, 64>;
-      using P2 = Product<E, 256, true, 256, false, 128, 64>;
-      CE_LAUNCH(P1, (ce_e_kernel<E, 256, 128, 64>), cdiv(a.M, 256) * (p.piece / 256), a, factor, e, p.piece, v, db);
-      CE_LAUNCH(P2, (ce_dx_kernel<E, 256, 128, 64>), cdiv(a.M, 256) * tk * p.splits, a, e, p.piece, v, p.splits, sums);
+      using P1 = Product<E, 256, false, 128, false, 128, 64>;
+      using P2 = Product<E, 256, true, 128, false, 128, 64>;
+      CE_LAUNCH(P1, (ce_e_kernel<E, 256, 128, 128, 64, B>), cdiv(a.M, 128) * (p.piece / 256), a, factor, e, p.piece, v, db);
+      CE_LAUNCH(P2, (ce_dx_kernel<E, 128, 128, 64>), cdiv(a.M, 128) * tk * p.splits, a, e, p.piece, v, p.splits, sums);
     }
-    using P3 = Product<E, 256, true, 256, true, 128, 64>;
-    CE_LAUNCH(P3, (ce_dw_kernel<E, 256, 128, 64>), tk * cdiv(words, 256), a, xs, e, p.piece, v, gmax);
+    using P3 = Product<E, 256, true, 128, true, 128, 64>;
+    CE_LAUNCH(P3, ce_dw_kernel<E>, tk * cdiv(words, 128), a, xs, e, p.piece, v, gmax);
+  };
+  for (int v = 0; v < a.V; v += p.piece) {
+    if (a.bias) piece(std::true_type{}, v); else piece(std::false_type{}, v);
     SIMVG_LAUNCH_CHECK();
   }
   hipLaunchKernelGGL(ce_dx_join_kernel<E>, dim3(min(2048, cdiv(a.M, 2))), dim3(256), 0, s, a, sums, p.splits);
-  if (a.dbias) hipLaunchKernelGGL(ce_db_join_kernel, dim3(cdiv(a.V, 256)), dim3(256), 0, s, a, db, cdiv(a.M, p.small ? 64 : 128), gmax);
+  if (a.dbias) hipLaunchKernelGGL(ce_db_join_kernel, dim3(cdiv(a.V, 256)), dim3(256), 0, s, a, db, cdiv(a.M, 64), gmax);
   SIMVG_LAUNCH_CHECK();
   return SIMVG_OK;
 }
@@ -571,7 +722,7 @@ int ce_bwd(const simvg_vocab_ce_args& a, hipStream_t s) {
 extern "C" long simvg_vocab_ce_ws_bytes(int M, int V, int K, int with_bias, int backward) {
   if (M <= 0 || V <= 0 || K <= 0) return 0;
   if (backward) return ce_plan(M, V, K, with_bias != 0).bytes;
-  return (M * 4L + 255) / 256 * 256 + ce_fwd_groups(V, M <= 64) * M * 8;
+  return (M * 4L + 255) / 256 * 256 + (long)ce_fwd_groups(V, M) * M * 8;
 }
 extern "C" int simvg_vocab_ce_fwd(const simvg_vocab_ce_args* args, hipStream_t stream) {
   const int rc = ce_check(args, false);
