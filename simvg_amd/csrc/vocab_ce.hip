@@ -38,8 +38,7 @@ using namespace seq;
 
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 constexpr float NEG_INF = -__builtin_huge_valf();
-constexpr int BK = 32;                                       // contracted values of a stage
-constexpr int STAGES = 3;
+constexpr int BK = 64;                                       // contracted values of a stage: a row's are one line of 128 bytes
 
 __device__ __forceinline__ f32x16 zero16() { return (f32x16){0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}; }
 __device__ __forceinline__ int acc_row(int r, int lane) { return (r >> 2) * 8 + (lane >> 5) * 4 + (r & 3); }
@@ -47,18 +46,21 @@ __device__ __forceinline__ int acc_row(int r, int lane) { return (r >> 2) * 8 + 
 __device__ __forceinline__ void stay_a_branch() { asm volatile(""); }
 
 // ------------------------------------------------------------------------------------------------- the matrix product
-// A workgroup of four waves, a wave on each SIMD, two workgroups to a compute unit: what one does not keep the matrix pipes busy with
-// (its epilogue of exponentials, its first stage, its barriers) the other does.  A wave's tile of 128 x 64 is 128 accumulators and 6
-// fragments of 1 KiB for 8 MFMAs of 32 cycles.
+// A wave's tile of 128 x 64 is 128 accumulators and 6 fragments of 1 KiB for 8 MFMAs of 32 cycles; eight waves make 256 x 256, one
+// workgroup to a compute unit.  (256 x 128 in four waves, two workgroups to a compute unit with stages of 32 values, so that one's
+// epilogue runs beside the other's products: 1.08 against 1.01 ms for the forward pass at 8191 x 64010 x 1024, bound by the L2's
+// requests: half lines, and half as many products for each.)
 //
 // One operand of a workgroup's tile: R rows (or columns) of the result by BK contracted values per stage.
-//   T = false: memory [R][contracted], a stage is R rows of 64 bytes;  T = true: memory [contracted][R], BK rows of 2 R bytes.
+//   T = false: memory [R][contracted], a stage is R rows of 128 bytes;  T = true: memory [contracted][R], BK rows of 2 R bytes.
 // In LDS, slots of 16 bytes are permuted within a row so that the fragment reads touch every bank once: 16 rows of one slot
 // (ds_read_b128) or 4 rows of 4 neighbouring slots (ds_read_b64_tr_b16) are one cycle's.
-template <int R, bool T> struct Operand {
-  static constexpr int BYTES = R * BK * 2, ROW = T ? R * 2 : BK * 2, PIECES = BYTES / 4096;
-  static_assert(PIECES >= 1 && (!T || R >= 128), "tile of an operand");
-  static __device__ __forceinline__ int at(int row, int slot) { return row * ROW + ((slot ^ (T ? (row & 3) << 2 : row >> 2 & 3)) << 4); }
+template <int R, bool T, int WAVES> struct Operand {
+  static constexpr int BYTES = R * BK * 2, ROW = T ? R * 2 : BK * 2, PIECES = BYTES / 1024 / WAVES;
+  static_assert(PIECES >= 1 && (!T || R >= 128) && WAVES % 2 == 0, "tile of an operand");
+  static __device__ __forceinline__ int at(int row, int slot) {
+    return row * ROW + ((slot ^ (T ? (row & 3) << 2 : (row >> 1 & 1) << 2 | (row >> 2 & 3))) << 4);
+  }
 
   // what a lane adds to a stage's start for its part of a fragment; the rest of an address is a constant in the instruction
   typedef __attribute__((address_space(3))) const char* Lds;
@@ -90,7 +92,7 @@ template <int R, bool T> struct Operand {
     }
   }
 
-  // HBM -> LDS, 1 KiB a piece, wave w's pieces are w, w + 4 ..
+  // HBM -> LDS, 1 KiB a piece, wave w's pieces are w, w + WAVES ..
   unsigned off[PIECES], lds, step;
   unsigned long next;                                        // the next stage's first value
   int inner, left;                                           // the lane's first contracted value of a stage (T: of its first piece); how many are left
@@ -103,9 +105,9 @@ template <int R, bool T> struct Operand {
     left = depth;
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
-      const int byte = (i * 4 + wave) * 1024 + lane * 16, row = byte / ROW;
+      const int byte = (i * WAVES + wave) * 1024 + lane * 16, row = byte / ROW;
       const int slot = (at(row, byte % ROW / 16) - row * ROW) >> 4;            // the permutation is its own inverse
-      if (i == 0) inner = T ? row : slot * 8;                // T = false: the same in every piece (16 rows apart)
+      if (i == 0) inner = T ? row : slot * 8;                // T = false: the same in every piece (whole eights of rows apart)
       off[i] = (T ? slot * 8 < rows : row < rows && keep(row)) ? (unsigned)row * (unsigned)ld * 2 + slot * 16 : DMA_NOTHING;
     }
   }
@@ -118,78 +120,88 @@ template <int R, bool T> struct Operand {
       stay_a_branch();
 #pragma unroll
       for (int i = 0; i < PIECES; ++i)
-        if (inner + (T ? i * 4096 / ROW : 0) >= left) o[i] = DMA_NOTHING;
+        if (inner + (T ? i * WAVES * 1024 / ROW : 0) >= left) o[i] = DMA_NOTHING;
     }
     issue<ST>(b, o, std::make_integer_sequence<int, PIECES>{});
     next += step;
     left -= BK;
   }
   template <int ST, int... I> __device__ __forceinline__ void issue(u32x4_t b, const unsigned (&o)[PIECES], std::integer_sequence<int, I...>) {
-    (dma16_at<ST * BYTES + I * 4096>(b, lds, o[I]), ...);
+    (dma16_at<ST * BYTES + I * WAVES * 1024>(b, lds, o[I]), ...);
   }
 };
 struct KeepAll { __device__ __forceinline__ bool operator()(int) const { return true; } };
 
 // acc[i][j] += A rows (WA of the wave's, 32 i ..) x B rows (WB, 32 j ..): registers run over A's rows, lanes over B's
-template <class E, int RA, bool TA, int RB, bool TB, int WA, int WB>
+template <class E, int RA, bool TA, int RB, bool TB, int WA, int WB, int STAGES>
 struct Product {
-  static_assert((RA / WA) * (RB / WB) == 4, "four waves");
-  static constexpr int THREADS = 256, NA = WA / 32, NB = WB / 32;
-  using OA = Operand<RA, TA>;
-  using OB = Operand<RB, TB>;
-  static constexpr int LDS = STAGES * (OA::BYTES + OB::BYTES), IN_FLIGHT = OA::PIECES + OB::PIECES;
+  static constexpr int WAVES = (RA / WA) * (RB / WB), THREADS = WAVES * 64, NA = WA / 32, NB = WB / 32;
+  using OA = Operand<RA, TA, WAVES>;
+  using OB = Operand<RB, TB, WAVES>;
+  static constexpr int B_AT = STAGES * OA::BYTES, LDS = B_AT + STAGES * OB::BYTES, IN_FLIGHT = OA::PIECES + OB::PIECES;
   static __device__ __forceinline__ int wave_a(int wave) { return wave / (RB / WB) * WA; }
   static __device__ __forceinline__ int wave_b(int wave) { return wave % (RB / WB) * WB; }
 
-  // Three stages in LDS: one is multiplied, the next has arrived, the one after is on its way.  The fragments of a step are read while the
-  // step before is multiplied, across the stages' border too: the barrier that makes a stage visible stands before the products
-  // of the last step of the stage before, so the matrix pipes have work behind it.
+  // The fragments of a step are read while the step before is multiplied, across the stages' border too: the barrier that makes a stage
+  // visible stands before the products of the last step of the stage before, whose fragments have all been read by then -- so the
+  // matrix pipes have work behind it, and the stage's place in LDS is free for the one STAGES further on.
   static __device__ __forceinline__ void run(f32x16 (&acc)[NA][NB], OA& oa, OB& ob, int stages) {
     if (stages <= 0) return;
     lpx8_t a[2][NA], b[2][NB];
     auto ask = [&](auto st) { oa.template stage<decltype(st)::value>(); ob.template stage<decltype(st)::value>(); };
-    auto read = [&](auto st, auto ks) {
-      constexpr int S = decltype(st)::value, K = decltype(ks)::value;
+    auto read = [&](auto st, int ks) {
+      constexpr int S = decltype(st)::value;
 #pragma unroll
-      for (int j = 0; j < NB; ++j) b[K & 1][j] = ob.frag(S, j, K);
+      for (int j = 0; j < NB; ++j) b[ks & 1][j] = ob.frag(S, j, ks);
 #pragma unroll
-      for (int i = 0; i < NA; ++i) a[K & 1][i] = oa.frag(S, i, K);
+      for (int i = 0; i < NA; ++i) a[ks & 1][i] = oa.frag(S, i, ks);
     };
     auto multiply = [&](int k) {
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i = 0; i < NA; ++i)
 #pragma unroll
         for (int j = 0; j < NB; ++j) acc[i][j] = E::mfma(a[k][i], b[k][j], acc[i][j]);
+      __builtin_amdgcn_sched_barrier(0);
     };
     using I0 = std::integral_constant<int, 0>;
     using I1 = std::integral_constant<int, 1>;
+    using I2 = std::integral_constant<int, 2>;
     ask(I0{});
-    if (stages > 1) { ask(I1{}); dma_wait<IN_FLIGHT>(); } else dma_wait<0>();
+    if (stages >= STAGES) {
+      ask(I1{});
+      if constexpr (STAGES == 3) ask(I2{});
+      dma_wait<(STAGES - 1) * IN_FLIGHT>();
+    } else {
+      if (stages > 1) ask(I1{});
+      dma_wait<0>();
+    }
     wave_barrier_only();
-    read(I0{}, I0{});
+    read(I0{}, 0);
     auto stage = [&](int kt, auto st) {
       constexpr int S = decltype(st)::value;
-      if (kt + 2 < stages) ask(std::integral_constant<int, (S + 2) % 3>{});    // whose stage everybody has left at the last barrier
-      read(st, I1{});
-      __builtin_amdgcn_sched_barrier(0);
-      multiply(0);
-      __builtin_amdgcn_sched_barrier(0);
-      if (kt + 1 < stages) {
-        if (kt + 2 < stages) dma_wait<IN_FLIGHT>(); else dma_wait<0>();
-        wave_barrier_only();
-        read(std::integral_constant<int, (S + 1) % 3>{}, I0{});
+#pragma unroll
+      for (int ks = 0; ks < BK / 16 - 1; ++ks) {
+        read(st, ks + 1);
+        multiply(ks & 1);
       }
-      __builtin_amdgcn_sched_barrier(0);
-      multiply(1);
-      __builtin_amdgcn_sched_barrier(0);
+      if (kt + 1 < stages) {
+        if (kt + STAGES - 1 < stages) dma_wait<(STAGES - 2) * IN_FLIGHT>(); else dma_wait<0>();
+        wave_barrier_only();
+        if (kt + STAGES < stages) ask(st);
+        read(std::integral_constant<int, (S + 1) % STAGES>{}, 0);
+      }
+      multiply((BK / 16 - 1) & 1);
     };
     for (int kt = 0;;) {
       stage(kt, I0{});
       if (++kt >= stages) break;
       stage(kt, I1{});
       if (++kt >= stages) break;
-      stage(kt, std::integral_constant<int, 2>{});
-      if (++kt >= stages) break;
+      if constexpr (STAGES == 3) {
+        stage(kt, I2{});
+        if (++kt >= stages) break;
+      }
     }
     __syncthreads();                                         // the epilogues use the LDS
   }
@@ -216,22 +228,22 @@ __device__ __forceinline__ bool is_word(const simvg_vocab_ce_args& a, long t) { 
 
 // ------------------------------------------------------------------------------------------------------------- forward
 // words in registers, rows in lanes: [tile of RA words][M] (maximum, sum of exp2) and the targets' logits
-template <class E, int RA, int RB, int WA, int WB>
-__global__ __launch_bounds__(256, 2) void ce_fwd_kernel(simvg_vocab_ce_args a, float2* part, float* zt) {
-  using P = Product<E, RA, false, RB, false, WA, WB>;
+template <class E, int RA, int RB, int WA, int WB, int STAGES>
+__global__ __launch_bounds__((RA / WA) * (RB / WB) * 64, 2) void ce_fwd_kernel(simvg_vocab_ce_args a, float2* part, float* zt) {
+  using P = Product<E, RA, false, RB, false, WA, WB, STAGES>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tv = cdiv(a.V, RA), tm = cdiv(a.M, RB);
   int iv, im;
-  tile_of(blockIdx.x, tv * tm, tv, tm, 8, iv, im);
+  tile_of(blockIdx.x, tv * tm, tv, tm, 4, iv, im);
   const int v0 = iv * RA, m0 = im * RB, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   f32x16 acc[P::NA][P::NB];
   P::zero(acc);
   typename P::OA oa;
   typename P::OB ob;
   oa.init_stages((const unsigned short*)a.w + (long)v0 * a.ldw, a.ldw, min(RA, a.V - v0), a.K, smem, wave, lane, KeepAll{});
-  ob.init_stages((const unsigned short*)a.x + (long)m0 * a.ldx, a.ldx, min(RB, a.M - m0), a.K, smem + STAGES * P::OA::BYTES, wave, lane, KeepAll{});
+  ob.init_stages((const unsigned short*)a.x + (long)m0 * a.ldx, a.ldx, min(RB, a.M - m0), a.K, smem + P::B_AT, wave, lane, KeepAll{});
   oa.init_reads(smem, P::wave_a(wave) / 32, lane);
-  ob.init_reads(smem + STAGES * P::OA::BYTES, P::wave_b(wave) / 32, lane);
+  ob.init_reads(smem + P::B_AT, P::wave_b(wave) / 32, lane);
   P::run(acc, oa, ob, cdiv(a.K, BK));
   const int wv = v0 + P::wave_a(wave), wm = P::wave_b(wave);
   if (a.bias) {
@@ -336,7 +348,7 @@ __global__ __launch_bounds__(1024) void ce_join_kernel(simvg_vocab_ce_args a, co
 // ws: max|g| | row factors g / max|g| [M] | g x / max|g| [M][K] 16 bit | e [M][piece] 16 bit | dx sums [splits][M][K] | db sums [waves' rows][V]
 struct Plan { int piece, splits, small; long o_factor, o_x, o_e, o_dx, o_db, bytes; };
 constexpr long E_BYTES = 256L << 20;                         // of e at a time: what the memory-side cache holds
-constexpr int SMALL_M = 64;                                  // up to here one tile of 64 rows, beyond tiles of 128
+constexpr int SMALL_M = 64;                                  // up to here one tile of 64 rows, beyond tiles of 256
 
 Plan ce_plan(int M, int V, int K, bool bias) {
   Plan p;
@@ -347,9 +359,9 @@ Plan ce_plan(int M, int V, int K, bool bias) {
   if (piece > words) piece = words;
   const long n = (words + piece - 1) / piece;                // even pieces
   p.piece = (int)(((words + n - 1) / n + 255) / 256 * 256);
-  // dx is M x K: few tiles.  The piece's words are shared out so that the chip's 512 workgroups have a tile each, of 256 words at least
-  const int tiles = cdiv(K, 256) * cdiv(M, p.small ? 64 : 128), most = p.piece / 256;
-  p.splits = 512 / tiles < 1 ? 1 : 512 / tiles > most ? most : 512 / tiles;
+  // dx is M x K: few tiles.  The piece's words are shared out so that the chip's 256 compute units have a tile each, of 256 words at least
+  const int tiles = cdiv(K, 256) * cdiv(M, p.small ? 64 : 256), most = p.piece / 256;
+  p.splits = 256 / tiles < 1 ? 1 : 256 / tiles > most ? most : 256 / tiles;
   auto up = [](long n) { return (n + 255) / 256 * 256; };
   long o = 256;
   p.o_factor = o; o += up(M * 4L);
@@ -408,16 +420,18 @@ __device__ __forceinline__ float row16_sum(float v) {
   return dpp_add<0x140>(v);                                  // the other eight (row_mirror)
 }
 
+constexpr int e_ld(int words) { return words * 2 + 16; }       // bytes of a row of a wave's block of e in LDS
+
 // (1) words in registers, rows in lanes: e of words [v_begin, v_begin + piece), and db's sums over the wave's rows.  Ignored rows of x
 // are not read: their logits are 0 whatever they hold, and with an lse of +inf so are their probabilities.
-template <class E, int RA, int RB, int WA, int WB, bool BIAS>
-__global__ __launch_bounds__(256, 2) void ce_e_kernel(simvg_vocab_ce_args a, const float* factor, unsigned short* e, int piece, int v_begin,
-                                                      float* db) {
-  using P = Product<E, RA, false, RB, false, WA, WB>;
+template <class E, int RA, int RB, int WA, int WB, int STAGES, bool BIAS>
+__global__ __launch_bounds__((RA / WA) * (RB / WB) * 64, 2) void ce_e_kernel(simvg_vocab_ce_args a, const float* factor, unsigned short* e,
+                                                                             int piece, int v_begin, float* db) {
+  using P = Product<E, RA, false, RB, false, WA, WB, STAGES>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tv = piece / RA, tm = cdiv(a.M, RB);
   int iv, im;
-  tile_of(blockIdx.x, tv * tm, tv, tm, 8, iv, im);
+  tile_of(blockIdx.x, tv * tm, tv, tm, 4, iv, im);
   const int l0 = iv * RA, v0 = v_begin + l0, m0 = im * RB, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   f32x16 acc[P::NA][P::NB];
   P::zero(acc);
@@ -426,10 +440,10 @@ __global__ __launch_bounds__(256, 2) void ce_e_kernel(simvg_vocab_ce_args a, con
     typename P::OA oa;
     typename P::OB ob;
     oa.init_stages((const unsigned short*)a.w + (long)v0 * a.ldw, a.ldw, words, a.K, smem, wave, lane, KeepAll{});
-    ob.init_stages((const unsigned short*)a.x + (long)m0 * a.ldx, a.ldx, min(RB, a.M - m0), a.K, smem + STAGES * P::OA::BYTES, wave, lane,
+    ob.init_stages((const unsigned short*)a.x + (long)m0 * a.ldx, a.ldx, min(RB, a.M - m0), a.K, smem + P::B_AT, wave, lane,
                    [&](int row) { return is_word(a, a.target[m0 + row]); });
     oa.init_reads(smem, P::wave_a(wave) / 32, lane);
-    ob.init_reads(smem + STAGES * P::OA::BYTES, P::wave_b(wave) / 32, lane);
+    ob.init_reads(smem + P::B_AT, P::wave_b(wave) / 32, lane);
     P::run(acc, oa, ob, cdiv(a.K, BK));
   }
   const int wl = P::wave_a(wave), wv = v0 + wl, wm = P::wave_b(wave);
@@ -498,8 +512,7 @@ __global__ __launch_bounds__(256, 2) void ce_e_kernel(simvg_vocab_ce_args a, con
       }
   }
   // through LDS, so that a row's words leave in whole lines: [row of the wave][WA words], rows 16 bytes longer than the words
-  constexpr int LD = WA * 2 + 16;
-  static_assert(4 * WB * LD <= P::LDS, "the waves' blocks of e fit the stages' LDS");
+  constexpr int LD = e_ld(WA);
   char* mine = smem + wave * WB * LD;
 #pragma unroll
   for (int j = 0; j < P::NB; ++j)
@@ -518,10 +531,10 @@ __global__ __launch_bounds__(256, 2) void ce_e_kernel(simvg_vocab_ce_args a, con
   }
 }
 // (2) K in registers, rows in lanes: the piece's share of dx into this split's sums
-template <class E, int RB, int WA, int WB>
-__global__ __launch_bounds__(256, 2) void ce_dx_kernel(simvg_vocab_ce_args a, const unsigned short* e, int piece, int v_begin, int splits,
-                                                       float* sums) {
-  using P = Product<E, 256, true, RB, false, WA, WB>;
+template <class E, int RB, int WA, int WB, int STAGES>
+__global__ __launch_bounds__((256 / WA) * (RB / WB) * 64, 2) void ce_dx_kernel(simvg_vocab_ce_args a, const unsigned short* e, int piece,
+                                                                               int v_begin, int splits, float* sums) {
+  using P = Product<E, 256, true, RB, false, WA, WB, STAGES>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tk = cdiv(a.K, 256), tm = cdiv(a.M, RB), tiles = tk * tm;
   int ik, im;
@@ -535,9 +548,9 @@ __global__ __launch_bounds__(256, 2) void ce_dx_kernel(simvg_vocab_ce_args a, co
   typename P::OA oa;
   typename P::OB ob;
   oa.init_stages((const unsigned short*)a.w + ((long)v_begin + s0 * BK) * a.ldw + k0, a.ldw, min(256, a.K - k0), words - s0 * BK, smem, wave, lane, KeepAll{});
-  ob.init_stages(e + (long)m0 * piece + s0 * BK, piece, min(RB, a.M - m0), words - s0 * BK, smem + STAGES * P::OA::BYTES, wave, lane, KeepAll{});
+  ob.init_stages(e + (long)m0 * piece + s0 * BK, piece, min(RB, a.M - m0), words - s0 * BK, smem + P::B_AT, wave, lane, KeepAll{});
   oa.init_reads(smem, P::wave_a(wave) / 32, lane);
-  ob.init_reads(smem + STAGES * P::OA::BYTES, P::wave_b(wave) / 32, lane);
+  ob.init_reads(smem + P::B_AT, P::wave_b(wave) / 32, lane);
   P::run(acc, oa, ob, s1 - s0);
   const int wk = k0 + P::wave_a(wave), wm = m0 + P::wave_b(wave);
 #pragma unroll
@@ -559,10 +572,10 @@ __global__ __launch_bounds__(256, 2) void ce_dx_kernel(simvg_vocab_ce_args a, co
 }
 // (3) K in registers, words in lanes: the piece's rows of dw
 template <class E>
-__global__ __launch_bounds__(256, 2) void ce_dw_kernel(simvg_vocab_ce_args a, const unsigned short* xs, const unsigned short* e, int piece,
+__global__ __launch_bounds__(512, 2) void ce_dw_kernel(simvg_vocab_ce_args a, const unsigned short* xs, const unsigned short* e, int piece,
                                                        int v_begin, const float* gmax) {
-  constexpr int RB = 128;
-  using P = Product<E, 256, true, RB, true, 128, 64>;
+  constexpr int RB = 256;
+  using P = Product<E, 256, true, RB, true, 128, 64, 2>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int words = min(piece, a.V - v_begin), tk = cdiv(a.K, 256), tv = cdiv(words, RB);
   int ik, iv;
@@ -573,9 +586,9 @@ __global__ __launch_bounds__(256, 2) void ce_dw_kernel(simvg_vocab_ce_args a, co
   typename P::OA oa;
   typename P::OB ob;
   oa.init_stages(xs + k0, a.K, min(256, a.K - k0), a.M, smem, wave, lane, KeepAll{});
-  ob.init_stages(e + l0, piece, min(RB, piece - l0), a.M, smem + STAGES * P::OA::BYTES, wave, lane, KeepAll{});
+  ob.init_stages(e + l0, piece, min(RB, piece - l0), a.M, smem + P::B_AT, wave, lane, KeepAll{});
   oa.init_reads(smem, P::wave_a(wave) / 32, lane);
-  ob.init_reads(smem + STAGES * P::OA::BYTES, P::wave_b(wave) / 32, lane);
+  ob.init_reads(smem + P::B_AT, P::wave_b(wave) / 32, lane);
   P::run(acc, oa, ob, cdiv(a.M, BK));
   const int wk = k0 + P::wave_a(wave), wl = l0 + P::wave_b(wave);
   const float mul = gmax[0] / e_scale<E>();
@@ -647,11 +660,11 @@ void allow_lds(const void* kernel, int bytes, std::atomic<unsigned long>& done) 
   if (hipGetDevice(&device) != hipSuccess || (device < 64 && done.load() >> device & 1)) return;
   if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess && device < 64) done |= 1ul << device;
 }
-#define CE_LAUNCH(P, KERNEL, GRID, ...)                                                  \
-  do {                                                                                   \
-    static std::atomic<unsigned long> done{0};                                           \
-    allow_lds((const void*)(KERNEL), P::LDS, done);                                      \
-    hipLaunchKernelGGL((KERNEL), dim3(GRID), dim3(P::THREADS), P::LDS, s, __VA_ARGS__);  \
+#define CE_LAUNCH(THREADS, LDS, KERNEL, GRID, ...)                                   \
+  do {                                                                               \
+    static std::atomic<unsigned long> done{0};                                       \
+    allow_lds((const void*)(KERNEL), LDS, done);                                     \
+    hipLaunchKernelGGL((KERNEL), dim3(GRID), dim3(THREADS), LDS, s, __VA_ARGS__);    \
   } while (0)
 
 int ce_fwd_groups(int V, int M) { return cdiv(V, M <= SMALL_M ? 128 : 256); }
@@ -661,12 +674,12 @@ int ce_fwd(const simvg_vocab_ce_args& a, hipStream_t s) {
   const int groups = ce_fwd_groups(a.V, a.M);
   float* zt = (float*)a.ws;
   float2* part = (float2*)((char*)a.ws + (a.M * 4L + 255) / 256 * 256);
-  if (a.M <= SMALL_M) {                                      // a row of tiles: bound by reading w, half as high tiles keep both workgroups of a CU busy
-    using P = Product<E, 128, false, 64, false, 32, 64>;
-    CE_LAUNCH(P, (ce_fwd_kernel<E, 128, 64, 32, 64>), groups, a, part, zt);
+  if (a.M <= SMALL_M) {                                      // a row of tiles, bound by reading w: twice as many, half as high, two to a compute unit
+    using P = Product<E, 128, false, 64, false, 32, 64, 3>;
+    CE_LAUNCH(P::THREADS, P::LDS, (ce_fwd_kernel<E, 128, 64, 32, 64, 3>), groups, a, part, zt);
   } else {
-    using P = Product<E, 256, false, 128, false, 128, 64>;
-    CE_LAUNCH(P, (ce_fwd_kernel<E, 256, 128, 128, 64>), groups * cdiv(a.M, 128), a, part, zt);
+    using P = Product<E, 256, false, 256, false, 128, 64, 2>;
+    CE_LAUNCH(P::THREADS, P::LDS, (ce_fwd_kernel<E, 256, 256, 128, 64, 2>), groups * cdiv(a.M, 256), a, part, zt);
   }
   SIMVG_LAUNCH_CHECK();
   hipLaunchKernelGGL(ce_join_kernel, dim3(cdiv(a.M, 8)), dim3(1024), 0, s, a, part, zt, groups);
@@ -695,18 +708,20 @@ int ce_bwd(const simvg_vocab_ce_args& a, hipStream_t s) {
     constexpr bool B = decltype(bias)::value;
     const int words = min(p.piece, a.V - v);
     if (p.small) {
-      using P1 = Product<E, 128, false, 64, false, 32, 64>;
-      using P2 = Product<E, 256, true, 64, false, 64, 64>;
-      CE_LAUNCH(P1, (ce_e_kernel<E, 128, 64, 32, 64, B>), p.piece / 128, a, factor, e, p.piece, v, db);
-      CE_LAUNCH(P2, (ce_dx_kernel<E, 64, 64, 64>), tk * p.splits, a, e, p.piece, v, p.splits, sums);
+      using P1 = Product<E, 128, false, 64, false, 32, 64, 3>;
+      using P2 = Product<E, 256, true, 64, false, 64, 64, 2>;
+      static_assert(P1::WAVES * 64 * e_ld(32) <= P1::LDS, "the waves' blocks of e");
+      CE_LAUNCH(P1::THREADS, P1::LDS, (ce_e_kernel<E, 128, 64, 32, 64, 3, B>), p.piece / 128, a, factor, e, p.piece, v, db);
+      CE_LAUNCH(P2::THREADS, P2::LDS, (ce_dx_kernel<E, 64, 64, 64, 2>), tk * p.splits, a, e, p.piece, v, p.splits, sums);
     } else {
-      using P1 = Product<E, 256, false, 128, false, 128, 64>;
-      using P2 = Product<E, 256, true, 128, false, 128, 64>;
-      CE_LAUNCH(P1, (ce_e_kernel<E, 256, 128, 128, 64, B>), cdiv(a.M, 128) * (p.piece / 256), a, factor, e, p.piece, v, db);
-      CE_LAUNCH(P2, (ce_dx_kernel<E, 128, 128, 64>), cdiv(a.M, 128) * tk * p.splits, a, e, p.piece, v, p.splits, sums);
+      using P1 = Product<E, 256, false, 256, false, 128, 64, 2>;
+      using P2 = Product<E, 256, true, 256, false, 128, 64, 2>;
+      constexpr int lds = P1::WAVES * 64 * e_ld(128) > P1::LDS ? P1::WAVES * 64 * e_ld(128) : P1::LDS;
+      CE_LAUNCH(P1::THREADS, lds, (ce_e_kernel<E, 256, 256, 128, 64, 2, B>), cdiv(a.M, 256) * (p.piece / 256), a, factor, e, p.piece, v, db);
+      CE_LAUNCH(P2::THREADS, P2::LDS, (ce_dx_kernel<E, 256, 128, 64, 2>), cdiv(a.M, 256) * tk * p.splits, a, e, p.piece, v, p.splits, sums);
     }
-    using P3 = Product<E, 256, true, 128, true, 128, 64>;
-    CE_LAUNCH(P3, ce_dw_kernel<E>, tk * cdiv(words, 128), a, xs, e, p.piece, v, gmax);
+    using P3 = Product<E, 256, true, 256, true, 128, 64, 2>;
+    CE_LAUNCH(P3::THREADS, P3::LDS, ce_dw_kernel<E>, tk * cdiv(words, 256), a, xs, e, p.piece, v, gmax);
   };
   for (int v = 0; v < a.V; v += p.piece) {
     if (a.bias) piece(std::true_type{}, v); else piece(std::false_type{}, v);
