@@ -111,23 +111,27 @@ template <int R, bool T, int WAVES> struct Operand {
       off[i] = (T ? slot * 8 < rows : row < rows && keep(row)) ? (unsigned)row * (unsigned)ld * 2 + slot * 16 : DMA_NOTHING;
     }
   }
-  template <int ST> __device__ __forceinline__ void stage() {
+  // half Q of the next stage's pieces, to place ST
+  template <int ST, int Q> __device__ __forceinline__ void half() {
+    constexpr int FROM = PIECES * Q / 2, N = PIECES * (Q + 1) / 2 - FROM;
     const u32x4_t b = {(unsigned)next, (unsigned)(next >> 32) & 0xffffu, DMA_NOTHING - 1, 0x00020000u};
-    unsigned o[PIECES];
+    unsigned o[N > 0 ? N : 1];
 #pragma unroll
-    for (int i = 0; i < PIECES; ++i) o[i] = off[i];
+    for (int i = 0; i < N; ++i) o[i] = off[FROM + i];
     if (left < BK) {                                         // zeros behind the last contracted value
       stay_a_branch();
 #pragma unroll
-      for (int i = 0; i < PIECES; ++i)
-        if (inner + (T ? i * WAVES * 1024 / ROW : 0) >= left) o[i] = DMA_NOTHING;
+      for (int i = 0; i < N; ++i)
+        if (inner + (T ? (FROM + i) * WAVES * 1024 / ROW : 0) >= left) o[i] = DMA_NOTHING;
     }
-    issue<ST>(b, o, std::make_integer_sequence<int, PIECES>{});
-    next += step;
-    left -= BK;
+    issue<ST, FROM>(b, o, std::make_integer_sequence<int, N>{});
+    if (Q == 1) {
+      next += step;
+      left -= BK;
+    }
   }
-  template <int ST, int... I> __device__ __forceinline__ void issue(u32x4_t b, const unsigned (&o)[PIECES], std::integer_sequence<int, I...>) {
-    (dma16_at<ST * BYTES + I * WAVES * 1024>(b, lds, o[I]), ...);
+  template <int ST, int FROM, int... I> __device__ __forceinline__ void issue(u32x4_t b, const unsigned* o, std::integer_sequence<int, I...>) {
+    (dma16_at<ST * BYTES + (FROM + I) * WAVES * 1024>(b, lds, o[I]), ...);
   }
 };
 struct KeepAll { __device__ __forceinline__ bool operator()(int) const { return true; } };
@@ -148,50 +152,55 @@ struct Product {
   static __device__ __forceinline__ void run(f32x16 (&acc)[NA][NB], OA& oa, OB& ob, int stages) {
     if (stages <= 0) return;
     lpx8_t a[2][NA], b[2][NB];
-    auto ask = [&](auto st) { oa.template stage<decltype(st)::value>(); ob.template stage<decltype(st)::value>(); };
-    auto read = [&](auto st, int ks) {
+    auto ask = [&](auto st, auto q) __attribute__((always_inline)) {
+      oa.template half<decltype(st)::value, decltype(q)::value>();
+      ob.template half<decltype(st)::value, decltype(q)::value>();
+    };
+    using I0 = std::integral_constant<int, 0>;
+    using I1 = std::integral_constant<int, 1>;
+    using I2 = std::integral_constant<int, 2>;
+    auto ask_all = [&](auto st) __attribute__((always_inline)) { ask(st, I0{}); ask(st, I1{}); };
+    auto read = [&](auto st, int ks) __attribute__((always_inline)) {
       constexpr int S = decltype(st)::value;
 #pragma unroll
       for (int j = 0; j < NB; ++j) b[ks & 1][j] = ob.frag(S, j, ks);
 #pragma unroll
       for (int i = 0; i < NA; ++i) a[ks & 1][i] = oa.frag(S, i, ks);
     };
-    auto multiply = [&](int k) {
-      __builtin_amdgcn_sched_barrier(0);
+    // the products of one step
+    auto multiply = [&](int k) __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < NA; ++i)
 #pragma unroll
         for (int j = 0; j < NB; ++j) acc[i][j] = E::mfma(a[k][i], b[k][j], acc[i][j]);
       __builtin_amdgcn_sched_barrier(0);
     };
-    using I0 = std::integral_constant<int, 0>;
-    using I1 = std::integral_constant<int, 1>;
-    using I2 = std::integral_constant<int, 2>;
-    ask(I0{});
-    if (stages >= STAGES) {
-      ask(I1{});
-      if constexpr (STAGES == 3) ask(I2{});
-      dma_wait<(STAGES - 1) * IN_FLIGHT>();
-    } else {
-      if (stages > 1) ask(I1{});
-      dma_wait<0>();
-    }
+    ask_all(I0{});
+    if (stages > 1) ask_all(I1{});
+    if (STAGES == 3 && stages > 2) ask_all(I2{});
+    if (stages >= STAGES) dma_wait<(STAGES - 1) * IN_FLIGHT>(); else dma_wait<0>();
     wave_barrier_only();
     read(I0{}, 0);
-    auto stage = [&](int kt, auto st) {
+    // what goes to the place of the stage before is asked for in two halves, in two steps: the eight waves' pieces at once fill the
+    // queue of the load unit, and a wave that waits there multiplies nothing (forward pass 934 -> 900 us)
+    auto stage = [&](int kt, auto st) __attribute__((always_inline)) {
       constexpr int S = decltype(st)::value;
-#pragma unroll
-      for (int ks = 0; ks < BK / 16 - 1; ++ks) {
-        read(st, ks + 1);
-        multiply(ks & 1);
-      }
+      const std::integral_constant<int, (S + STAGES - 1) % STAGES> before;
+      const bool more = kt > 0 && kt - 1 + STAGES < stages;
+      read(st, 1);
+      if (more) ask(before, I1{});
+      multiply(0);
+      read(st, 2);
+      multiply(1);
+      read(st, 3);
+      multiply(0);
       if (kt + 1 < stages) {
         if (kt + STAGES - 1 < stages) dma_wait<(STAGES - 2) * IN_FLIGHT>(); else dma_wait<0>();
         wave_barrier_only();
-        if (kt + STAGES < stages) ask(st);
         read(std::integral_constant<int, (S + 1) % STAGES>{}, 0);
+        if (kt + STAGES < stages) ask(st, I0{});
       }
-      multiply((BK / 16 - 1) & 1);
+      multiply(1);
     };
     for (int kt = 0;;) {
       stage(kt, I0{});
