@@ -96,9 +96,8 @@ template <int R, bool T, int WAVES> struct Operand {
   unsigned off[PIECES], lds, step;
   unsigned long next;                                        // the next stage's first value
   int inner, left;                                           // the lane's first contracted value of a stage (T: of its first piece); how many are left
-  // rows: what there is of the tile's rows, depth: of contracted values from `base` on; `keep(row)`: whether a row is read (T = false)
-  template <class Keep>
-  __device__ __forceinline__ void init_stages(const unsigned short* base, long ld, int rows, int depth, const char* to, int wave, int lane, Keep keep) {
+  // rows: what there is of the tile's rows, depth: of contracted values from `base` on
+  __device__ __forceinline__ void init_stages(const unsigned short* base, long ld, int rows, int depth, const char* to, int wave, int lane) {
     next = (unsigned long)base;
     step = T ? (unsigned)(BK * 2) * (unsigned)ld : BK * 2;
     lds = lds_addr(to) + wave * 1024;
@@ -108,7 +107,7 @@ template <int R, bool T, int WAVES> struct Operand {
       const int byte = (i * WAVES + wave) * 1024 + lane * 16, row = byte / ROW;
       const int slot = (at(row, byte % ROW / 16) - row * ROW) >> 4;            // the permutation is its own inverse
       if (i == 0) inner = T ? row : slot * 8;                // T = false: the same in every piece (whole eights of rows apart)
-      off[i] = (T ? slot * 8 < rows : row < rows && keep(row)) ? (unsigned)row * (unsigned)ld * 2 + slot * 16 : DMA_NOTHING;
+      off[i] = (T ? slot * 8 < rows : row < rows) ? (unsigned)row * (unsigned)ld * 2 + slot * 16 : DMA_NOTHING;
     }
   }
   // half Q of the next stage's pieces, to place ST
@@ -134,7 +133,6 @@ template <int R, bool T, int WAVES> struct Operand {
     (dma16_at<ST * BYTES + (FROM + I) * WAVES * 1024>(b, lds, o[I]), ...);
   }
 };
-struct KeepAll { __device__ __forceinline__ bool operator()(int) const { return true; } };
 
 // acc[i][j] += A rows (WA of the wave's, 32 i ..) x B rows (WB, 32 j ..): registers run over A's rows, lanes over B's
 template <class E, int RA, bool TA, int RB, bool TB, int WA, int WB, int STAGES>
@@ -249,8 +247,8 @@ __global__ __launch_bounds__((RA / WA) * (RB / WB) * 64, 2) void ce_fwd_kernel(s
   P::zero(acc);
   typename P::OA oa;
   typename P::OB ob;
-  oa.init_stages((const unsigned short*)a.w + (long)v0 * a.ldw, a.ldw, min(RA, a.V - v0), a.K, smem, wave, lane, KeepAll{});
-  ob.init_stages((const unsigned short*)a.x + (long)m0 * a.ldx, a.ldx, min(RB, a.M - m0), a.K, smem + P::B_AT, wave, lane, KeepAll{});
+  oa.init_stages((const unsigned short*)a.w + (long)v0 * a.ldw, a.ldw, min(RA, a.V - v0), a.K, smem, wave, lane);
+  ob.init_stages((const unsigned short*)a.x + (long)m0 * a.ldx, a.ldx, min(RB, a.M - m0), a.K, smem + P::B_AT, wave, lane);
   oa.init_reads(smem, P::wave_a(wave) / 32, lane);
   ob.init_reads(smem + P::B_AT, P::wave_b(wave) / 32, lane);
   P::run(acc, oa, ob, cdiv(a.K, BK));
@@ -354,8 +352,12 @@ __global__ __launch_bounds__(1024) void ce_join_kernel(simvg_vocab_ce_args a, co
 }
 
 // ------------------------------------------------------------------------------------------------------------ backward
-// ws: max|g| | row factors g / max|g| [M] | g x / max|g| [M][K] 16 bit | e [M][piece] 16 bit | dx sums [splits][M][K] | db sums [waves' rows][V]
-struct Plan { int piece, splits, small; long o_factor, o_x, o_e, o_dx, o_db, bytes; };
+// Only the rows that take part are computed: the list of them, made on the device, is as long as `kept` says there (masked-word training
+// ignores most rows), and the kernels below go by that length; their launches and the workspace are laid out for all M.
+// ws: head | list: row of each kept one [M] | place of each row in the list or -1 [M] | g / max|g| of the kept [M] | kept rows of x, times
+// that [M][K] 16 bit | kept rows of x as they are [M][K] | e [M][piece] 16 bit | dx sums [splits][kept][K] | db sums [waves' rows][V]
+struct Head { float gmax; int kept; };
+struct Plan { int piece, grid_dx, small; long o_list, o_place, o_factor, o_x, o_xk, o_e, o_dx, o_db, bytes; };
 constexpr long E_BYTES = 256L << 20;                         // of e at a time: what the memory-side cache holds
 constexpr int SMALL_M = 64;                                  // up to here one tile of 64 rows, beyond tiles of 256
 
@@ -368,42 +370,71 @@ Plan ce_plan(int M, int V, int K, bool bias) {
   if (piece > words) piece = words;
   const long n = (words + piece - 1) / piece;                // even pieces
   p.piece = (int)(((words + n - 1) / n + 255) / 256 * 256);
-  // dx is M x K: few tiles.  The piece's words are shared out so that the chip's 256 compute units have a tile each, of 256 words at least
-  const int tiles = cdiv(K, 256) * cdiv(M, p.small ? 64 : 256), most = p.piece / 256;
-  p.splits = 256 / tiles < 1 ? 1 : 256 / tiles > most ? most : 256 / tiles;
+  const int rows = p.small ? 64 : 256, tiles = cdiv(K, 256) * cdiv(M, rows);
+  p.grid_dx = max(256, tiles);                               // see dx_splits
   auto up = [](long n) { return (n + 255) / 256 * 256; };
   long o = 256;
+  p.o_list = o; o += up(M * 4L);
+  p.o_place = o; o += up(M * 4L);
   p.o_factor = o; o += up(M * 4L);
   p.o_x = o; o += up((long)M * K * 2);
+  p.o_xk = o; o += up((long)M * K * 2);
   p.o_e = o; o += up((long)M * p.piece * 2);
-  p.o_dx = o; o += up((long)p.splits * M * K * 4);
+  p.o_dx = o; o += (long)p.grid_dx * rows * 256 * 4;
   p.o_db = o; o += bias ? up((long)cdiv(M, 64) * V * 4) : 0;
   p.bytes = o;
   return p;
 }
+// dx is kept x K: few tiles.  A piece's words are shared out in `splits`, so that each of the chip's 256 compute units has a tile, of 256
+// words at least
+__device__ __forceinline__ int dx_splits(int grid, int tiles, int piece) { return max(1, min(grid / max(1, tiles), piece / 256)); }
 
-__global__ __launch_bounds__(1024) void ce_gmax_kernel(simvg_vocab_ce_args a, float* gmax, float* factor) {
-  __shared__ float red[16];
+// the list of the rows that take part, in their order: one workgroup, a stretch of rows to a thread
+__global__ __launch_bounds__(1024) void ce_rows_kernel(simvg_vocab_ce_args a, Head* head, int* list, int* place, float* factor) {
+  __shared__ float most[16];
+  __shared__ int counts[1024];
+  const int tid = threadIdx.x, per = cdiv(a.M, 1024), m0 = min(tid * per, a.M), m1 = min(m0 + per, a.M);
   float g = 0.f;
-  for (int m = threadIdx.x; m < a.M; m += 1024)
-    if (is_word(a, a.target[m])) g = fmaxf(g, fabsf(a.dloss[m]));
+  int n = 0;
+  for (int m = m0; m < m1; ++m)
+    if (is_word(a, a.target[m])) {
+      g = fmaxf(g, fabsf(a.dloss[m]));
+      ++n;
+    }
   g = wave_max(g);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = g;
+  if ((tid & 63) == 0) most[tid >> 6] = g;
+  counts[tid] = n;
   __syncthreads();
-  g = red[0];
-  for (int i = 1; i < 16; ++i) g = fmaxf(g, red[i]);
-  if (threadIdx.x == 0) gmax[0] = g;
-  for (int m = threadIdx.x; m < a.M; m += 1024) factor[m] = !is_word(a, a.target[m]) ? 0.f : a.dloss[m] == 0.f ? 0.f : a.dloss[m] / g;
+  for (int o = 1; o < 1024; o <<= 1) {
+    const int v = tid >= o ? counts[tid - o] : 0;
+    __syncthreads();
+    counts[tid] += v;
+    __syncthreads();
+  }
+  g = most[0];
+  for (int i = 1; i < 16; ++i) g = fmaxf(g, most[i]);
+  int at = counts[tid] - n;
+  for (int m = m0; m < m1; ++m) {
+    const bool on = is_word(a, a.target[m]);
+    place[m] = on ? at : -1;
+    if (on) {
+      const float d = a.dloss[m];
+      list[at] = m;
+      factor[at++] = d == 0.f ? 0.f : d / g;
+    }
+  }
+  if (tid == 0) { head->gmax = g; head->kept = counts[1023]; }
 }
 template <class E>
-__global__ __launch_bounds__(256) void ce_scale_kernel(simvg_vocab_ce_args a, const float* factor, unsigned short* xs) {
+__global__ __launch_bounds__(256) void ce_gather_kernel(simvg_vocab_ce_args a, const Head* head, const int* list, const float* factor,
+                                                        unsigned short* xs, unsigned short* xk) {
   const int per = a.K / 8;
-  for (long i = blockIdx.x * 256L + threadIdx.x; i < (long)a.M * per; i += (long)gridDim.x * 256) {
-    const int m = (int)(i / per), c = (int)(i % per) * 8;
-    u32x4_t v = *(const u32x4_t*)((const unsigned short*)a.x + (long)m * a.ldx + c);
-    const float f = factor[m];
-    if (!is_word(a, a.target[m])) v = (u32x4_t){0u, 0u, 0u, 0u};               // whatever an ignored row holds
-    else if (f != 1.f) {
+  for (long i = blockIdx.x * 256L + threadIdx.x; i < (long)head->kept * per; i += gridDim.x * 256L) {
+    const int r = (int)(i / per), c = (int)(i % per) * 8;
+    u32x4_t v = *(const u32x4_t*)((const unsigned short*)a.x + (long)list[r] * a.ldx + c);
+    *(u32x4_t*)(xk + (long)r * a.K + c) = v;
+    const float f = factor[r];
+    if (f != 1.f) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         float lo, hi;
@@ -411,7 +442,7 @@ __global__ __launch_bounds__(256) void ce_scale_kernel(simvg_vocab_ce_args a, co
         v[j] = E::pack(lo * f, hi * f);
       }
     }
-    *(u32x4_t*)(xs + (long)m * a.K + c) = v;
+    *(u32x4_t*)(xs + (long)r * a.K + c) = v;
   }
 }
 
@@ -431,14 +462,15 @@ __device__ __forceinline__ float row16_sum(float v) {
 
 constexpr int e_ld(int words) { return words * 2 + 16; }       // bytes of a row of a wave's block of e in LDS
 
-// (1) words in registers, rows in lanes: e of words [v_begin, v_begin + piece), and db's sums over the wave's rows.  Ignored rows of x
-// are not read: their logits are 0 whatever they hold, and with an lse of +inf so are their probabilities.
+// (1) words in registers, kept rows in lanes: e of words [v_begin, v_begin + piece), and db's sums over the wave's rows
 template <class E, int RA, int RB, int WA, int WB, int STAGES, bool BIAS>
-__global__ __launch_bounds__((RA / WA) * (RB / WB) * 64, 2) void ce_e_kernel(simvg_vocab_ce_args a, const float* factor, unsigned short* e,
+__global__ __launch_bounds__((RA / WA) * (RB / WB) * 64, 2) void ce_e_kernel(simvg_vocab_ce_args a, const Head* head, const int* list,
+                                                                             const float* factor, const unsigned short* xk, unsigned short* e,
                                                                              int piece, int v_begin, float* db) {
   using P = Product<E, RA, false, RB, false, WA, WB, STAGES>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int tv = piece / RA, tm = cdiv(a.M, RB);
+  const int kept = head->kept, tv = piece / RA, tm = cdiv(kept, RB);
+  if ((int)blockIdx.x >= tv * tm) return;
   int iv, im;
   tile_of(blockIdx.x, tv * tm, tv, tm, 4, iv, im);
   const int l0 = iv * RA, v0 = v_begin + l0, m0 = im * RB, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -448,9 +480,8 @@ __global__ __launch_bounds__((RA / WA) * (RB / WB) * 64, 2) void ce_e_kernel(sim
   if (words > 0) {
     typename P::OA oa;
     typename P::OB ob;
-    oa.init_stages((const unsigned short*)a.w + (long)v0 * a.ldw, a.ldw, words, a.K, smem, wave, lane, KeepAll{});
-    ob.init_stages((const unsigned short*)a.x + (long)m0 * a.ldx, a.ldx, min(RB, a.M - m0), a.K, smem + P::B_AT, wave, lane,
-                   [&](int row) { return is_word(a, a.target[m0 + row]); });
+    oa.init_stages((const unsigned short*)a.w + (long)v0 * a.ldw, a.ldw, words, a.K, smem, wave, lane);
+    ob.init_stages(xk + (long)m0 * a.K, a.K, min(RB, kept - m0), a.K, smem + P::B_AT, wave, lane);
     oa.init_reads(smem, P::wave_a(wave) / 32, lane);
     ob.init_reads(smem + P::B_AT, P::wave_b(wave) / 32, lane);
     P::run(acc, oa, ob, cdiv(a.K, BK));
@@ -461,11 +492,11 @@ __global__ __launch_bounds__((RA / WA) * (RB / WB) * 64, 2) void ce_e_kernel(sim
   bool any = false;
 #pragma unroll
   for (int j = 0; j < P::NB; ++j) {
-    const int m = m0 + wm + j * 32 + (lane & 31), mc = min(m, a.M - 1);
-    const long t = a.target[mc];
-    const bool on = m < a.M && is_word(a, t);
-    less[j] = on ? (E::kScaled ? E_POWER : 0.f) - a.lse[mc] * LOG2E : NEG_INF;
-    g[j] = BIAS && on ? factor[mc] : 0.f;
+    const int r = m0 + wm + j * 32 + (lane & 31), m = list[min(r, kept - 1)];
+    const bool on = r < kept;
+    const long t = a.target[m];
+    less[j] = on ? (E::kScaled ? E_POWER : 0.f) - a.lse[m] * LOG2E : NEG_INF;
+    g[j] = BIAS && on ? factor[r] : 0.f;
     local[j] = on && t >= wv && t < wv + WA ? (int)(t - wv) : -1;
     any = any || local[j] >= 0;
   }
@@ -505,7 +536,7 @@ __global__ __launch_bounds__((RA / WA) * (RB / WB) * 64, 2) void ce_e_kernel(sim
         for (int r = 0; r < 16; ++r)
           if (local[j] == i * 32 + acc_row(r, lane)) acc[i][j][r] -= e_scale<E>();
   }
-  if (BIAS) {
+  if (BIAS && a.dbias) {
     const float down = 1.f / e_scale<E>();
 #pragma unroll
     for (int i = 0; i < P::NA; ++i)
@@ -513,11 +544,11 @@ __global__ __launch_bounds__((RA / WA) * (RB / WB) * 64, 2) void ce_e_kernel(sim
       for (int r = 0; r < 16; ++r) {
         float s = 0.f;
 #pragma unroll
-        for (int j = 0; j < P::NB; ++j) s += g[j] == 0.f ? 0.f : acc[i][j][r] * g[j];
+        for (int j = 0; j < P::NB; ++j) s += acc[i][j][r] * g[j];
         s = row16_sum(s);
         s += __shfl_xor(s, 16, 64);
         const int v = wv + i * 32 + acc_row(r, lane);
-        if ((lane & 31) == 0 && v < a.V && m0 + wm < a.M) db[(long)((m0 + wm) / WB) * a.V + v] = s * down;
+        if ((lane & 31) == 0 && v < a.V && m0 + wm < kept) db[(long)((m0 + wm) / WB) * a.V + v] = s * down;
       }
   }
   // through LDS, so that a row's words leave in whole lines: [row of the wave][WA words], rows 16 bytes longer than the words
@@ -536,16 +567,17 @@ __global__ __launch_bounds__((RA / WA) * (RB / WB) * 64, 2) void ce_e_kernel(sim
   for (int r = 0; r < WB; r += ROWS) {
     const int row = r + lane / PER, m = m0 + wm + row;
     const u32x4_t v = *(const u32x4_t*)(mine + row * LD + lane % PER * 16);
-    if (m < a.M) *(u32x4_t*)(e + (long)m * piece + l0 + wl + lane % PER * 8) = v;
+    if (m < kept) *(u32x4_t*)(e + (long)m * piece + l0 + wl + lane % PER * 8) = v;
   }
 }
 // (2) K in registers, rows in lanes: the piece's share of dx into this split's sums
 template <class E, int RB, int WA, int WB, int STAGES>
-__global__ __launch_bounds__((256 / WA) * (RB / WB) * 64, 2) void ce_dx_kernel(simvg_vocab_ce_args a, const unsigned short* e, int piece,
-                                                                               int v_begin, int splits, float* sums) {
+__global__ __launch_bounds__((256 / WA) * (RB / WB) * 64, 2) void ce_dx_kernel(simvg_vocab_ce_args a, const Head* head,
+                                                                               const unsigned short* e, int piece, int v_begin, float* sums) {
   using P = Product<E, 256, true, RB, false, WA, WB, STAGES>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int tk = cdiv(a.K, 256), tm = cdiv(a.M, RB), tiles = tk * tm;
+  const int kept = head->kept, tk = cdiv(a.K, 256), tm = cdiv(kept, RB), tiles = tk * tm, splits = dx_splits(gridDim.x, tiles, piece);
+  if ((int)blockIdx.x >= tiles * splits) return;
   int ik, im;
   const int split = blockIdx.x / tiles;
   tile_of(blockIdx.x % tiles, tiles, tm, tk, tk, im, ik);
@@ -556,8 +588,8 @@ __global__ __launch_bounds__((256 / WA) * (RB / WB) * 64, 2) void ce_dx_kernel(s
   const int s0 = (int)((long)stages * split / splits), s1 = (int)((long)stages * (split + 1) / splits);
   typename P::OA oa;
   typename P::OB ob;
-  oa.init_stages((const unsigned short*)a.w + ((long)v_begin + s0 * BK) * a.ldw + k0, a.ldw, min(256, a.K - k0), words - s0 * BK, smem, wave, lane, KeepAll{});
-  ob.init_stages(e + (long)m0 * piece + s0 * BK, piece, min(RB, a.M - m0), words - s0 * BK, smem + P::B_AT, wave, lane, KeepAll{});
+  oa.init_stages((const unsigned short*)a.w + ((long)v_begin + s0 * BK) * a.ldw + k0, a.ldw, min(256, a.K - k0), words - s0 * BK, smem, wave, lane);
+  ob.init_stages(e + (long)m0 * piece + s0 * BK, piece, min(RB, kept - m0), words - s0 * BK, smem + P::B_AT, wave, lane);
   oa.init_reads(smem, P::wave_a(wave) / 32, lane);
   ob.init_reads(smem + P::B_AT, P::wave_b(wave) / 32, lane);
   P::run(acc, oa, ob, s1 - s0);
@@ -565,14 +597,14 @@ __global__ __launch_bounds__((256 / WA) * (RB / WB) * 64, 2) void ce_dx_kernel(s
 #pragma unroll
   for (int j = 0; j < P::NB; ++j) {
     const int m = wm + j * 32 + (lane & 31);
-    if (m >= a.M) continue;
+    if (m >= kept) continue;
 #pragma unroll
     for (int i = 0; i < P::NA; ++i)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const int k = wk + i * 32 + g * 8 + (lane >> 5) * 4;
         if (k >= a.K) continue;
-        f32x4_t* at = (f32x4_t*)(sums + ((long)split * a.M + m) * a.K + k);
+        f32x4_t* at = (f32x4_t*)(sums + ((long)split * kept + m) * a.K + k);
         f32x4_t v = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
         if (v_begin > 0) v += *at;
         *at = v;
@@ -581,12 +613,12 @@ __global__ __launch_bounds__((256 / WA) * (RB / WB) * 64, 2) void ce_dx_kernel(s
 }
 // (3) K in registers, words in lanes: the piece's rows of dw
 template <class E>
-__global__ __launch_bounds__(512, 2) void ce_dw_kernel(simvg_vocab_ce_args a, const unsigned short* xs, const unsigned short* e, int piece,
-                                                       int v_begin, const float* gmax) {
+__global__ __launch_bounds__(512, 2) void ce_dw_kernel(simvg_vocab_ce_args a, const Head* head, const unsigned short* xs, const unsigned short* e,
+                                                       int piece, int v_begin) {
   constexpr int RB = 256;
   using P = Product<E, 256, true, RB, true, 128, 64, 2>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int words = min(piece, a.V - v_begin), tk = cdiv(a.K, 256), tv = cdiv(words, RB);
+  const int kept = head->kept, words = min(piece, a.V - v_begin), tk = cdiv(a.K, 256), tv = cdiv(words, RB);
   int ik, iv;
   tile_of(blockIdx.x, tk * tv, tv, tk, tk, iv, ik);
   const int k0 = ik * 256, l0 = iv * RB, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -594,13 +626,13 @@ __global__ __launch_bounds__(512, 2) void ce_dw_kernel(simvg_vocab_ce_args a, co
   P::zero(acc);
   typename P::OA oa;
   typename P::OB ob;
-  oa.init_stages(xs + k0, a.K, min(256, a.K - k0), a.M, smem, wave, lane, KeepAll{});
-  ob.init_stages(e + l0, piece, min(RB, piece - l0), a.M, smem + P::B_AT, wave, lane, KeepAll{});
+  oa.init_stages(xs + k0, a.K, min(256, a.K - k0), kept, smem, wave, lane);
+  ob.init_stages(e + l0, piece, min(RB, piece - l0), kept, smem + P::B_AT, wave, lane);
   oa.init_reads(smem, P::wave_a(wave) / 32, lane);
   ob.init_reads(smem + P::B_AT, P::wave_b(wave) / 32, lane);
-  P::run(acc, oa, ob, cdiv(a.M, BK));
+  P::run(acc, oa, ob, cdiv(kept, BK));
   const int wk = k0 + P::wave_a(wave), wl = l0 + P::wave_b(wave);
-  const float mul = gmax[0] / e_scale<E>();
+  const float mul = head->gmax / e_scale<E>();
 #pragma unroll
   for (int j = 0; j < P::NB; ++j) {
     const int v = wl + j * 32 + (lane & 31);
@@ -617,27 +649,29 @@ __global__ __launch_bounds__(512, 2) void ce_dw_kernel(simvg_vocab_ce_args a, co
       }
   }
 }
+// dx: the splits' sums, and zeros for the rows that take no part
 template <class E>
-__global__ __launch_bounds__(256) void ce_dx_join_kernel(simvg_vocab_ce_args a, const float* sums, int splits) {
-  const int per = a.K / 4;
-  for (long i = blockIdx.x * 256L + threadIdx.x; i < (long)a.M * per; i += (long)gridDim.x * 256) {
-    const int m = (int)(i / per), c = (int)(i % per) * 4;
+__global__ __launch_bounds__(256) void ce_dx_join_kernel(simvg_vocab_ce_args a, const Head* head, const int* place, const float* sums, int grid_dx,
+                                                         int rows, int piece) {
+  const int per = a.K / 4, kept = head->kept, splits = dx_splits(grid_dx, cdiv(a.K, 256) * cdiv(kept, rows), piece);
+  for (long i = blockIdx.x * 256L + threadIdx.x; i < (long)a.M * per; i += gridDim.x * 256L) {
+    const int m = (int)(i / per), c = (int)(i % per) * 4, r = place[m];
     f32x4_t v = {0.f, 0.f, 0.f, 0.f};
+    if (r >= 0) {
 #pragma unroll 8
-    for (int s = 0; s < splits; ++s) v += *(const f32x4_t*)(sums + ((long)s * a.M + m) * a.K + c);
-    const bool on = is_word(a, a.target[m]);
-    const float g = on ? a.dloss[m] / e_scale<E>() : 0.f;
-    if (!on) v = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-    *(u32x2_t*)((unsigned short*)a.dx + (long)m * a.lddx + c) = (u32x2_t){E::pack(v[0] * g, v[1] * g), E::pack(v[2] * g, v[3] * g)};
+      for (int s = 0; s < splits; ++s) v += *(const f32x4_t*)(sums + ((long)s * kept + r) * a.K + c);
+      v *= a.dloss[m] / e_scale<E>();
+    }
+    *(u32x2_t*)((unsigned short*)a.dx + (long)m * a.lddx + c) = (u32x2_t){E::pack(v[0], v[1]), E::pack(v[2], v[3])};
   }
 }
-__global__ __launch_bounds__(256) void ce_db_join_kernel(simvg_vocab_ce_args a, const float* db, int groups, const float* gmax) {
-  const int v = blockIdx.x * 256 + threadIdx.x;
+__global__ __launch_bounds__(256) void ce_db_join_kernel(simvg_vocab_ce_args a, const Head* head, const float* db) {
+  const int v = blockIdx.x * 256 + threadIdx.x, groups = cdiv(head->kept, 64);
   if (v >= a.V) return;
   float s = 0.f;
 #pragma unroll 8
   for (int g = 0; g < groups; ++g) s += db[(long)g * a.V + v];
-  a.dbias[v] = s * gmax[0];
+  a.dbias[v] = s * head->gmax;
 }
 
 // ---------------------------------------------------------------------------------------------------------------- host
@@ -707,10 +741,12 @@ template <class E>
 int ce_bwd(const simvg_vocab_ce_args& a, hipStream_t s) {
   const Plan p = ce_plan(a.M, a.V, a.K, a.dbias != nullptr);
   char* ws = (char*)a.ws;
-  float *gmax = (float*)ws, *factor = (float*)(ws + p.o_factor), *sums = (float*)(ws + p.o_dx), *db = (float*)(ws + p.o_db);
-  unsigned short *xs = (unsigned short*)(ws + p.o_x), *e = (unsigned short*)(ws + p.o_e);
-  hipLaunchKernelGGL(ce_gmax_kernel, dim3(1), dim3(1024), 0, s, a, gmax, factor);
-  hipLaunchKernelGGL(ce_scale_kernel<E>, dim3(min(2048, cdiv(a.M, 2) )), dim3(256), 0, s, a, factor, xs);
+  Head* head = (Head*)ws;
+  int *list = (int*)(ws + p.o_list), *place = (int*)(ws + p.o_place);
+  float *factor = (float*)(ws + p.o_factor), *sums = (float*)(ws + p.o_dx), *db = (float*)(ws + p.o_db);
+  unsigned short *xs = (unsigned short*)(ws + p.o_x), *xk = (unsigned short*)(ws + p.o_xk), *e = (unsigned short*)(ws + p.o_e);
+  hipLaunchKernelGGL(ce_rows_kernel, dim3(1), dim3(1024), 0, s, a, head, list, place, factor);
+  hipLaunchKernelGGL(ce_gather_kernel<E>, dim3(min(2048, cdiv(a.M, 2))), dim3(256), 0, s, a, head, list, factor, xs, xk);
   SIMVG_LAUNCH_CHECK();
   const int tk = cdiv(a.K, 256);
   const auto piece = [&](auto bias, int v) {
@@ -720,24 +756,26 @@ int ce_bwd(const simvg_vocab_ce_args& a, hipStream_t s) {
       using P1 = Product<E, 128, false, 64, false, 32, 64, 3>;
       using P2 = Product<E, 256, true, 64, false, 64, 64, 2>;
       static_assert(P1::WAVES * 64 * e_ld(32) <= P1::LDS, "the waves' blocks of e");
-      CE_LAUNCH(P1::THREADS, P1::LDS, (ce_e_kernel<E, 128, 64, 32, 64, 3, B>), p.piece / 128, a, factor, e, p.piece, v, db);
-      CE_LAUNCH(P2::THREADS, P2::LDS, (ce_dx_kernel<E, 64, 64, 64, 2>), tk * p.splits, a, e, p.piece, v, p.splits, sums);
+      CE_LAUNCH(P1::THREADS, P1::LDS, (ce_e_kernel<E, 128, 64, 32, 64, 3, B>), p.piece / 128, a, head, list, factor, xk, e, p.piece, v, db);
+      CE_LAUNCH(P2::THREADS, P2::LDS, (ce_dx_kernel<E, 64, 64, 64, 2>), p.grid_dx, a, head, e, p.piece, v, sums);
     } else {
       using P1 = Product<E, 256, false, 256, false, 128, 64, 2>;
       using P2 = Product<E, 256, true, 256, false, 128, 64, 2>;
       constexpr int lds = P1::WAVES * 64 * e_ld(128) > P1::LDS ? P1::WAVES * 64 * e_ld(128) : P1::LDS;
-      CE_LAUNCH(P1::THREADS, lds, (ce_e_kernel<E, 256, 256, 128, 64, 2, B>), cdiv(a.M, 256) * (p.piece / 256), a, factor, e, p.piece, v, db);
-      CE_LAUNCH(P2::THREADS, P2::LDS, (ce_dx_kernel<E, 256, 128, 64, 2>), cdiv(a.M, 256) * tk * p.splits, a, e, p.piece, v, p.splits, sums);
+      CE_LAUNCH(P1::THREADS, lds, (ce_e_kernel<E, 256, 256, 128, 64, 2, B>), cdiv(a.M, 256) * (p.piece / 256), a, head, list, factor, xk, e,
+                p.piece, v, db);
+      CE_LAUNCH(P2::THREADS, P2::LDS, (ce_dx_kernel<E, 256, 128, 64, 2>), p.grid_dx, a, head, e, p.piece, v, sums);
     }
     using P3 = Product<E, 256, true, 256, true, 128, 64, 2>;
-    CE_LAUNCH(P3::THREADS, P3::LDS, ce_dw_kernel<E>, tk * cdiv(words, 256), a, xs, e, p.piece, v, gmax);
+    CE_LAUNCH(P3::THREADS, P3::LDS, ce_dw_kernel<E>, tk * cdiv(words, 256), a, head, xs, e, p.piece, v);
   };
   for (int v = 0; v < a.V; v += p.piece) {
     if (a.bias) piece(std::true_type{}, v); else piece(std::false_type{}, v);
     SIMVG_LAUNCH_CHECK();
   }
-  hipLaunchKernelGGL(ce_dx_join_kernel<E>, dim3(min(2048, cdiv(a.M, 2))), dim3(256), 0, s, a, sums, p.splits);
-  if (a.dbias) hipLaunchKernelGGL(ce_db_join_kernel, dim3(cdiv(a.V, 256)), dim3(256), 0, s, a, db, cdiv(a.M, 64), gmax);
+  hipLaunchKernelGGL(ce_dx_join_kernel<E>, dim3(min(2048, cdiv(a.M, 2))), dim3(256), 0, s, a, head, place, sums, p.grid_dx, p.small ? 64 : 256,
+                     p.piece);
+  if (a.dbias) hipLaunchKernelGGL(ce_db_join_kernel, dim3(cdiv(a.V, 256)), dim3(256), 0, s, a, head, db);
   SIMVG_LAUNCH_CHECK();
   return SIMVG_OK;
 }
