@@ -4,6 +4,7 @@ Fails loudly when the library is missing: the product path has NO CPU / PyTorch 
 """
 import ctypes as C
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("SIMVG_HIP_LIB") or os.path.join(_HERE, "lib", "libsimvg_hip.so")   # override: dev builds
@@ -102,6 +103,16 @@ class VocabCeArgs(C.Structure):         # simvg_vocab_ce_args
                  ("ignore_index", c_long), ("loss", c_void_p), ("lse", c_void_p), ("dloss", c_void_p), ("dx", c_void_p), ("lddx", c_long),
                  ("dw", c_void_p), ("lddw", c_long), ("dbias", c_void_p), ("ws", c_void_p), ("ws_bytes", c_long)])
 
+
+def _packer(block):
+    """struct.Struct of an argument block: one call packs what setting a ctypes structure's members one by one takes 40 for"""
+    code = {c_int: "i", c_float: "f", c_void_p: "P", c_long: "l", c_int * 4: "4i"}
+    s = struct.Struct("@" + "".join(code[t] for _, t in block._fields_))
+    assert s.size == C.sizeof(block), block
+    return s
+
+
+QK_NORM_ROPE, PACKED_ATTN, VOCAB_CE = _packer(QkNormRopeArgs), _packer(PackedAttnArgs), _packer(VocabCeArgs)
 
 # entry points that return a size: {name: arguments}
 _SIZES = {

@@ -1271,80 +1271,69 @@ def _seq_dtype(t, name, only16=True):
     return code
 
 
-def _seq_chk(name, t, shape, dtype, device, contiguous=False):
-    """one operand of a sequence operator: where, which type, which shape, innermost dimension contiguous"""
+def _seq_bad(name, t, shape, dtype, device, contiguous):
+    """what is wrong with an operand of a sequence operator"""
     if not t.is_cuda:
         raise _lib.SimvgHipError(f"{name} must live in HBM (got a CPU tensor): simvg_amd has no CPU path")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, the other operands on {device}")
+    if t.get_device() != device:
+        raise ValueError(f"{name} is on {t.device}, the other operands on cuda:{device}")
     if t.dtype != dtype:
         raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
     if t.numel() and (not t.is_contiguous() if contiguous else (t.shape[-1] > 1 and t.stride(-1) != 1)):
         raise ValueError(f"{name}: {'must be contiguous' if contiguous else 'innermost dimension must be contiguous'}")
-    return t
 
 
-def _seq_out(name, t, shape, dtype, device):
-    """an output that the caller brought: as an operand, and no two of its elements in one place"""
-    _seq_chk(name, t, shape, dtype, device)
-    if any(st == 0 and n > 1 for st, n in zip(t.stride(), t.shape)):
+def _seq_flat(name, t, shape, dtype, device):
+    """address of a contiguous operand: where it has to be, of the type and shape it has to have"""
+    if t.get_device() != device or device < 0 or t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
+        _seq_bad(name, t, shape, dtype, device, True)
+    return t.data_ptr()
+
+
+def _seq_rows(name, t, shape, dtype, device, written=False):
+    """(address, strides of all dimensions but the innermost, which is contiguous)"""
+    st = t.stride()
+    if t.get_device() != device or device < 0 or t.dtype is not dtype or t.shape != shape or st[-1] != 1:
+        _seq_bad(name, t, shape, dtype, device, False)
+    if written and 0 in st and any(s == 0 and n > 1 for s, n in zip(st, shape)):
         raise ValueError(f"{name}: an expanded tensor cannot be written")
-    return t
+    return (t.data_ptr(), *st[:-1])
 
 
-class _on_device:
-    """makes a tensor's device the current one around a launch (nothing where it already is): the launch goes to that device's current
-    stream"""
-
-    def __init__(self, device):
-        self.guard = None if device.index == _raw_device() else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-
-
-def _heads(args, t, name, short):
-    """pointer, token stride and head stride of a [T, H, D] operand into an argument block"""
-    setattr(args, name, t.data_ptr())
-    setattr(args, short + "_ts", t.stride(0))
-    setattr(args, short + "_hs", t.stride(1))
+def _seq_launch(name, fn, block, device, flops=0.0, nbytes=0.0):
+    """one call of a library entry point on the current stream of `device`"""
+    if device != _raw_device():
+        with torch.cuda.device(device):
+            return _seq_launch(name, fn, block, device, flops, nbytes)
+    t0 = _timer.start(name) if _timer is not None else None
+    rc = fn(block, _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream)
+    if t0 is not None:
+        _timer.stop(name, t0, flops, nbytes)
+    if rc:
+        _lib.check(rc, "simvg_" + name)
 
 
 def _rope_args(q, k, pos, inv_freq, sections, gq, gk, eps, interleaved):
+    """the argument block's first members, those that both directions have"""
     if q.dim() != 3 or k.dim() != 3:
         raise ValueError("q and k must be [tokens, heads, head size]")
-    dev, (T, Hq, D) = q.device, q.shape
-    a = _lib.QkNormRopeArgs(dtype=_seq_dtype(q, "q", only16=False), T=T, Hq=Hq, Hkv=k.shape[1], D=D, eps=float(eps),
-                            interleaved=int(bool(interleaved)))
-    _seq_chk("q", q, q.shape, q.dtype, dev)
-    _seq_chk("k", k, (T, k.shape[1], D), q.dtype, dev)
-    sections = [int(n) for n in sections]
-    if not 1 <= len(sections) <= 4:
+    (T, Hq, D), Hkv, dt, dev = q.shape, k.shape[1], q.dtype, q.get_device()
+    code = _seq_dtype(q, "q", only16=False)
+    rq, rk = _seq_rows("q", q, q.shape, dt, dev), _seq_rows("k", k, (T, Hkv, D), dt, dev)
+    axes, pairs = len(sections), sum(sections)
+    if not 1 <= axes <= 4:
         raise ValueError("sections: one to four position axes")
-    if pos.dtype not in (torch.int32, torch.int64):
+    if pos.dtype is not torch.int32 and pos.dtype is not torch.int64:
         raise TypeError(f"pos: expected int32 or int64, got {pos.dtype}")
-    _seq_chk("pos", pos, (T, len(sections)), pos.dtype, dev)
-    _seq_chk("inv_freq", inv_freq, (sum(sections),), torch.float64, dev, contiguous=True)
+    pp, pld = _seq_rows("pos", pos, (T, axes), pos.dtype, dev)
+    pf = _seq_flat("inv_freq", inv_freq, (pairs,), torch.float64, dev)
     if (gq is None) != (gk is None):
         raise ValueError("gq and gk: both or neither")
-    if gq is not None:
-        a.gq = _seq_chk("gq", gq, (D,), torch.float32, dev, contiguous=True).data_ptr()
-        a.gk = _seq_chk("gk", gk, (D,), torch.float32, dev, contiguous=True).data_ptr()
-    a.n_axes = len(sections)
-    for i, n in enumerate(sections):
-        a.sections[i] = n
-    a.pos, a.pos_ld, a.pos_is_64 = pos.data_ptr(), max(pos.stride(0), len(sections)) if T <= 1 else pos.stride(0), int(pos.dtype == torch.int64)
-    a.inv_freq = inv_freq.data_ptr()
-    _heads(a, q, "q", "q")
-    _heads(a, k, "k", "k")
-    return a, dev
+    g = (0, 0) if gq is None else (_seq_flat("gq", gq, (D,), torch.float32, dev), _seq_flat("gk", gk, (D,), torch.float32, dev))
+    return (code, T, Hq, Hkv, D, axes, *sections, *(0,) * (4 - axes), 1 if interleaved else 0, 1 if pos.dtype is torch.int64 else 0, eps,
+            pp, pld if T > 1 else axes, pf, *g, *rq, *rk), dev
 
 
 def qk_norm_rope_fwd(q, k, pos, inv_freq, sections, gq=None, gk=None, eps=1e-6, interleaved=False, q_out=None, k_out=None):
@@ -1352,42 +1341,31 @@ def qk_norm_rope_fwd(q, k, pos, inv_freq, sections, gq=None, gk=None, eps=1e-6, 
     pos: [T, axes] int32 / int64; sections: pairs per axis, inv_freq: float64 [sum(sections)], a frequency per pair; gq, gk: float32 [D]
     norm weights (None: rotation alone).  Pairs are (j, j + sum(sections)), or neighbours with `interleaved`.  Returns (q_out, k_out),
     which may be q and k themselves."""
-    lib = _lib.load()
-    a, dev = _rope_args(q, k, pos, inv_freq, sections, gq, gk, eps, interleaved)
-    q_out = torch.empty(q.shape, device=dev, dtype=q.dtype) if q_out is None else _seq_out("q_out", q_out, q.shape, q.dtype, dev)
-    k_out = torch.empty(k.shape, device=dev, dtype=k.dtype) if k_out is None else _seq_out("k_out", k_out, k.shape, k.dtype, dev)
-    _heads(a, q_out, "q_out", "qo")
-    _heads(a, k_out, "k_out", "ko")
-    with _on_device(dev):
-        t0 = _timer.start("qk_norm_rope_fwd") if _timer is not None else None
-        rc = lib.simvg_qk_norm_rope_fwd(C.byref(a), _stream())
-        if t0 is not None:
-            _timer.stop("qk_norm_rope_fwd", t0, 0.0, 2.0 * q.element_size() * (q.numel() + k.numel()))
-    _lib.check(rc, "simvg_qk_norm_rope_fwd")
+    args, dev = _rope_args(q, k, pos, inv_freq, sections, gq, gk, eps, interleaved)
+    q_out = q.new_empty(q.shape) if q_out is None else q_out
+    k_out = k.new_empty(k.shape) if k_out is None else k_out
+    block = _lib.QK_NORM_ROPE.pack(*args, *_seq_rows("q_out", q_out, q.shape, q.dtype, dev, True),
+                                   *_seq_rows("k_out", k_out, k.shape, q.dtype, dev, True), 0, 0, 0, 0, 0, 0, 0, 0, 0)
+    _seq_launch("qk_norm_rope_fwd", _lib.load().simvg_qk_norm_rope_fwd, block, dev, 0.0, 2.0 * q.element_size() * (q.numel() + k.numel()))
     return q_out, k_out
 
 
 def qk_norm_rope_bwd(dq, dk, q, k, pos, inv_freq, sections, gq=None, gk=None, eps=1e-6, interleaved=False, dq_in=None, dk_in=None):
     """Gradients of `qk_norm_rope_fwd`: dq, dk of its outputs -> (dq_in, dk_in, dgq, dgk) of its inputs and norm weights (None without)."""
     lib = _lib.load()
-    a, dev = _rope_args(q, k, pos, inv_freq, sections, gq, gk, eps, interleaved)
-    _heads(a, _seq_chk("dq", dq, q.shape, q.dtype, dev), "dq", "dq")
-    _heads(a, _seq_chk("dk", dk, k.shape, k.dtype, dev), "dk", "dk")
-    dq_in = torch.empty(q.shape, device=dev, dtype=q.dtype) if dq_in is None else _seq_out("dq_in", dq_in, q.shape, q.dtype, dev)
-    dk_in = torch.empty(k.shape, device=dev, dtype=k.dtype) if dk_in is None else _seq_out("dk_in", dk_in, k.shape, k.dtype, dev)
-    _heads(a, dq_in, "q_out", "qo")
-    _heads(a, dk_in, "k_out", "ko")
-    dgq = dgk = None
+    args, dev = _rope_args(q, k, pos, inv_freq, sections, gq, gk, eps, interleaved)
+    dq_in = q.new_empty(q.shape) if dq_in is None else dq_in
+    dk_in = k.new_empty(k.shape) if dk_in is None else dk_in
+    dgq = dgk = ws = None
     if gq is not None:
-        dgq, dgk = torch.empty_like(gq), torch.empty_like(gk)
-        ws = torch.empty(max(1, lib.simvg_qk_norm_rope_ws_floats(a.T, a.D)), device=dev, dtype=torch.float32)
-        a.dgq, a.dgk, a.ws = dgq.data_ptr(), dgk.data_ptr(), ws.data_ptr()
-    with _on_device(dev):
-        t0 = _timer.start("qk_norm_rope_bwd") if _timer is not None else None
-        rc = lib.simvg_qk_norm_rope_bwd(C.byref(a), _stream())
-        if t0 is not None:
-            _timer.stop("qk_norm_rope_bwd", t0, 0.0, 3.0 * q.element_size() * (q.numel() + k.numel()))
-    _lib.check(rc, "simvg_qk_norm_rope_bwd")
+        D = q.shape[2]
+        n = lib.simvg_qk_norm_rope_ws_floats(q.shape[0], D)
+        dgq, dgk, ws = gq.new_empty(D), gk.new_empty(D), gq.new_empty(max(1, n))
+    block = _lib.QK_NORM_ROPE.pack(*args, *_seq_rows("dq_in", dq_in, q.shape, q.dtype, dev, True),
+                                   *_seq_rows("dk_in", dk_in, k.shape, q.dtype, dev, True), *_seq_rows("dq", dq, q.shape, q.dtype, dev),
+                                   *_seq_rows("dk", dk, k.shape, q.dtype, dev),
+                                   *((0, 0, 0) if ws is None else (dgq.data_ptr(), dgk.data_ptr(), ws.data_ptr())))
+    _seq_launch("qk_norm_rope_bwd", lib.simvg_qk_norm_rope_bwd, block, dev, 0.0, 3.0 * q.element_size() * (q.numel() + k.numel()))
     return dq_in, dk_in, dgq, dgk
 
 
@@ -1406,53 +1384,40 @@ def packed_plan(cu_seqlens, T):
     lib = _lib.load()
     if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
         raise ValueError("cu_seqlens must be a vector of at least one entry")
-    _seq_chk("cu_seqlens", cu_seqlens, cu_seqlens.shape, torch.int32, cu_seqlens.device, contiguous=True)
-    T, nseq = int(T), cu_seqlens.numel() - 1
+    T, nseq, dev = int(T), cu_seqlens.numel() - 1, cu_seqlens.get_device()
+    cu = _seq_flat("cu_seqlens", cu_seqlens, cu_seqlens.shape, torch.int32, dev)
     if T < 0:
         raise ValueError("T must not be negative")
-    table = torch.empty(lib.simvg_packed_plan_ints(T, nseq), device=cu_seqlens.device, dtype=torch.int32)
-    with _on_device(cu_seqlens.device):
-        rc = lib.simvg_packed_plan(_p(cu_seqlens), nseq, T, _p(table), _stream())
-    _lib.check(rc, "simvg_packed_plan")
+    table = cu_seqlens.new_empty(lib.simvg_packed_plan_ints(T, nseq))
+    _seq_launch("packed_plan", lambda at, stream: lib.simvg_packed_plan(cu, nseq, T, at, stream), table.data_ptr(), dev)
     return PackedPlan(cu_seqlens, nseq, T, table)
 
 
-def _packed_args(q, k, v, plan, causal, scale):
+def _packed_args(q, k, v, plan, causal, scale, fill_tail):
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
         raise ValueError("q, k and v must be [tokens, heads, head size]")
-    dev, (T, Hq, D), Hkv = q.device, q.shape, k.shape[1]
-    a = _lib.PackedAttnArgs(dtype=_seq_dtype(q, "q"), T=T, nseq=plan.nseq, Hq=Hq, Hkv=Hkv, D=D, causal=int(bool(causal)),
-                            scale=float(D ** -0.5 if scale is None else scale))
-    _seq_chk("q", q, q.shape, q.dtype, dev)
-    _seq_chk("k", k, (T, Hkv, D), q.dtype, dev)
-    _seq_chk("v", v, (T, Hkv, D), q.dtype, dev)
+    (T, Hq, D), Hkv, dt, dev = q.shape, k.shape[1], q.dtype, q.get_device()
+    code, rows = _seq_dtype(q, "q"), (T, Hkv, D)
+    rq, rk, rv = _seq_rows("q", q, q.shape, dt, dev), _seq_rows("k", k, rows, dt, dev), _seq_rows("v", v, rows, dt, dev)
     if plan.T != T:
         raise ValueError(f"the plan is for {plan.T} rows, q has {T}")
-    if plan.table.device != dev:
-        raise ValueError(f"the plan is on {plan.table.device}, the other operands on {dev}")
-    a.plan = plan.table.data_ptr()
-    for t, name in ((q, "q"), (k, "k"), (v, "v")):
-        _heads(a, t, name, name)
-    return a, dev
+    if plan.table.get_device() != dev:
+        raise ValueError(f"the plan is on {plan.table.device}, the other operands on {q.device}")
+    return (code, T, plan.nseq, Hq, Hkv, D, 1 if causal else 0, 1 if fill_tail else 0, D ** -0.5 if scale is None else scale,
+            plan.table.data_ptr(), *rq, *rk, *rv), dev
 
 
 def packed_attn_fwd(q, k, v, plan, causal=True, scale=None, out=None):
     """Attention over packed sequences (csrc/packed_attn.hip): q [T, Hq, D], k, v [T, Hkv, D], fp16 or bf16, `plan` from `packed_plan`.
     Returns (out [T, Hq, D], lse [Hq, T] fp32).  Rows behind the last sequence are zeros; in an `out` of the caller's they stay as
     they were."""
-    lib = _lib.load()
-    a, dev = _packed_args(q, k, v, plan, causal, scale)
-    a.fill_tail = int(out is None)
-    out = torch.empty(q.shape, device=dev, dtype=q.dtype) if out is None else _seq_out("out", out, q.shape, q.dtype, dev)
-    lse = (torch.empty if a.fill_tail else torch.zeros)(a.Hq, a.T, device=dev, dtype=torch.float32)
-    _heads(a, out, "o", "o")
-    a.lse, a.lse_hs = lse.data_ptr(), a.T
-    with _on_device(dev):
-        t0 = _timer.start("packed_attn_fwd") if _timer is not None else None
-        rc = lib.simvg_packed_attn_fwd(C.byref(a), _stream())
-        if t0 is not None:
-            _timer.stop("packed_attn_fwd", t0, 0.0, 2.0 * (2 * q.numel() + k.numel() + v.numel()))
-    _lib.check(rc, "simvg_packed_attn_fwd")
+    args, dev = _packed_args(q, k, v, plan, causal, scale, out is None)
+    (T, Hq, D), fill = q.shape, out is None
+    lse = q.new_empty((Hq, T), dtype=torch.float32) if fill else q.new_zeros((Hq, T), dtype=torch.float32)
+    out = q.new_empty(q.shape) if fill else out
+    block = _lib.PACKED_ATTN.pack(*args, *_seq_rows("out", out, q.shape, q.dtype, dev, True), lse.data_ptr(), T,
+                                  0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
+    _seq_launch("packed_attn_fwd", _lib.load().simvg_packed_attn_fwd, block, dev, 0.0, 2.0 * (2 * q.numel() + k.numel() + v.numel()))
     return out, lse
 
 
@@ -1460,82 +1425,53 @@ def packed_attn_bwd(q, k, v, out, lse, dout, plan, causal=True, scale=None, dq=N
     """Gradients of `packed_attn_fwd` from its inputs, its results and the gradient of `out`: (dq, dk, dv).  Rows behind the last sequence
     are zeros; in gradients of the caller's (all three or none) they stay as they were."""
     lib = _lib.load()
-    a, dev = _packed_args(q, k, v, plan, causal, scale)
-    given = [t is not None for t in (dq, dk, dv)]
-    if any(given) and not all(given):
+    fill = dq is None and dk is None and dv is None
+    if not fill and (dq is None or dk is None or dv is None):
         raise ValueError("dq, dk and dv: all three or none")
-    a.fill_tail = int(not any(given))
-    if a.fill_tail:
-        dq, dk, dv = (torch.empty(t.shape, device=dev, dtype=t.dtype) for t in (q, k, v))
-    _seq_chk("lse", lse, (a.Hq, a.T), torch.float32, dev, contiguous=True)
-    _heads(a, _seq_chk("out", out, q.shape, q.dtype, dev), "o", "o")
-    _heads(a, _seq_chk("dout", dout, q.shape, q.dtype, dev), "d_o", "do")
-    _heads(a, _seq_out("dq", dq, q.shape, q.dtype, dev), "dq", "dq")
-    _heads(a, _seq_out("dk", dk, k.shape, q.dtype, dev), "dk", "dk")
-    _heads(a, _seq_out("dv", dv, v.shape, q.dtype, dev), "dv", "dv")
-    ws = torch.empty(max(1, lib.simvg_packed_attn_ws_floats(a.T, a.nseq, a.Hq, a.Hkv, a.D)), device=dev, dtype=torch.float32)
-    a.lse, a.lse_hs, a.ws = lse.data_ptr(), a.T, ws.data_ptr()
-    with _on_device(dev):
-        t0 = _timer.start("packed_attn_bwd") if _timer is not None else None
-        rc = lib.simvg_packed_attn_bwd(C.byref(a), _stream())
-        if t0 is not None:
-            _timer.stop("packed_attn_bwd", t0, 0.0, 2.0 * (4 * q.numel() + 2 * k.numel() + 2 * v.numel()))
-    _lib.check(rc, "simvg_packed_attn_bwd")
+    args, dev = _packed_args(q, k, v, plan, causal, scale, fill)
+    (T, Hq, D), dt = q.shape, q.dtype
+    if fill:
+        dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+    ws = q.new_empty(max(1, lib.simvg_packed_attn_ws_floats(T, plan.nseq, Hq, k.shape[1], D)), dtype=torch.float32)
+    block = _lib.PACKED_ATTN.pack(*args, *_seq_rows("out", out, q.shape, dt, dev), _seq_flat("lse", lse, (Hq, T), torch.float32, dev), T,
+                                  *_seq_rows("dout", dout, q.shape, dt, dev), *_seq_rows("dq", dq, q.shape, dt, dev, True),
+                                  *_seq_rows("dk", dk, k.shape, dt, dev, True), *_seq_rows("dv", dv, k.shape, dt, dev, True), ws.data_ptr())
+    _seq_launch("packed_attn_bwd", lib.simvg_packed_attn_bwd, block, dev, 0.0, 2.0 * (4 * q.numel() + 2 * k.numel() + 2 * v.numel()))
     return dq, dk, dv
 
 
 def _ce_args(x, w, target, bias, ignore_index, backward):
     if x.dim() != 2 or w.dim() != 2:
         raise ValueError("x must be [rows, K] and w [words, K]")
-    dev, (M, K), V = x.device, x.shape, w.shape[0]
-    a = _lib.VocabCeArgs(dtype=_seq_dtype(x, "x"), M=M, V=V, K=K, ignore_index=int(ignore_index))
-    _seq_chk("x", x, (M, K), x.dtype, dev)
-    _seq_chk("w", w, (V, K), x.dtype, dev)
-    _seq_chk("target", target, (M,), torch.int64, dev, contiguous=True)
-    if bias is not None:
-        a.bias = _seq_chk("bias", bias, (V,), torch.float32, dev, contiguous=True).data_ptr()
-    a.x, a.ldx = x.data_ptr(), x.stride(0) if M > 1 else K
-    a.w, a.ldw = w.data_ptr(), w.stride(0) if V > 1 else K
-    a.target = target.data_ptr()
-    a.ws_bytes = _lib.load().simvg_vocab_ce_ws_bytes(M, V, K, int(bias is not None), int(backward))
-    ws = torch.empty(max(1, a.ws_bytes), device=dev, dtype=torch.uint8)
-    a.ws = ws.data_ptr()
-    return a, dev, ws
+    (M, K), V, dt, dev = x.shape, w.shape[0], x.dtype, x.get_device()
+    code = _seq_dtype(x, "x")
+    (px, ldx), (pw, ldw) = _seq_rows("x", x, x.shape, dt, dev), _seq_rows("w", w, (V, K), dt, dev)
+    pt = _seq_flat("target", target, (M,), torch.int64, dev)
+    pb = 0 if bias is None else _seq_flat("bias", bias, (V,), torch.float32, dev)
+    n = _lib.load().simvg_vocab_ce_ws_bytes(M, V, K, 0 if bias is None else 1, 1 if backward else 0)
+    ws = x.new_empty(max(1, n), dtype=torch.uint8)
+    return (code, M, V, K, px, ldx if M > 1 else K, pw, ldw if V > 1 else K, pb, pt, ignore_index), dev, ws, n
 
 
 def vocab_ce_fwd(x, w, target, bias=None, ignore_index=-100):
     """Softmax cross entropy of x [M, K] against the words w [V, K] (+ bias [V] fp32) without storing the logits (csrc/vocab_ce.hip).
     target: int64 [M].  Returns (loss [M], lse [M]) in fp32; a row whose target is ignore_index has loss 0, one whose target is no word
     has loss NaN."""
-    lib = _lib.load()
-    a, dev, ws = _ce_args(x, w, target, bias, ignore_index, False)
-    loss, lse = torch.empty(a.M, device=dev, dtype=torch.float32), torch.empty(a.M, device=dev, dtype=torch.float32)
-    a.loss, a.lse = loss.data_ptr(), lse.data_ptr()
-    with _on_device(dev):
-        t0 = _timer.start("vocab_ce_fwd") if _timer is not None else None
-        rc = lib.simvg_vocab_ce_fwd(C.byref(a), _stream())
-        if t0 is not None:
-            _timer.stop("vocab_ce_fwd", t0, 2.0 * a.M * a.V * a.K, 2.0 * (x.numel() + w.numel()))
-    _lib.check(rc, "simvg_vocab_ce_fwd")
+    args, dev, ws, n = _ce_args(x, w, target, bias, ignore_index, False)
+    M = x.shape[0]
+    loss, lse = x.new_empty(M, dtype=torch.float32), x.new_empty(M, dtype=torch.float32)
+    block = _lib.VOCAB_CE.pack(*args, loss.data_ptr(), lse.data_ptr(), 0, 0, 0, 0, 0, 0, ws.data_ptr(), n)
+    _seq_launch("vocab_ce_fwd", _lib.load().simvg_vocab_ce_fwd, block, dev, 2.0 * M * w.numel(), 2.0 * (x.numel() + w.numel()))
     return loss, lse
 
 
 def vocab_ce_bwd(x, w, target, lse, dloss, bias=None, ignore_index=-100):
     """Gradients of `vocab_ce_fwd` for the gradients dloss [M] of the rows' losses: (dx, dw, dbias), dbias None without a bias."""
-    lib = _lib.load()
-    a, dev, ws = _ce_args(x, w, target, bias, ignore_index, True)
-    dx = torch.empty(x.shape, device=dev, dtype=x.dtype)
-    dw = torch.empty(w.shape, device=dev, dtype=w.dtype)
-    dbias = None if bias is None else torch.empty_like(bias)
-    a.lse = _seq_chk("lse", lse, (a.M,), torch.float32, dev, contiguous=True).data_ptr()
-    a.dloss = _seq_chk("dloss", dloss, (a.M,), torch.float32, dev, contiguous=True).data_ptr()
-    a.dx, a.lddx, a.dw, a.lddw = dx.data_ptr(), a.K, dw.data_ptr(), a.K
-    if dbias is not None:
-        a.dbias = dbias.data_ptr()
-    with _on_device(dev):
-        t0 = _timer.start("vocab_ce_bwd") if _timer is not None else None
-        rc = lib.simvg_vocab_ce_bwd(C.byref(a), _stream())
-        if t0 is not None:
-            _timer.stop("vocab_ce_bwd", t0, 6.0 * a.M * a.V * a.K, 4.0 * (x.numel() + w.numel()))
-    _lib.check(rc, "simvg_vocab_ce_bwd")
+    args, dev, ws, n = _ce_args(x, w, target, bias, ignore_index, True)
+    M, K = x.shape
+    dx, dw = x.new_empty(x.shape), w.new_empty(w.shape)
+    dbias = None if bias is None else bias.new_empty(bias.shape)
+    block = _lib.VOCAB_CE.pack(*args, 0, _seq_flat("lse", lse, (M,), torch.float32, dev), _seq_flat("dloss", dloss, (M,), torch.float32, dev),
+                               dx.data_ptr(), K, dw.data_ptr(), K, 0 if dbias is None else dbias.data_ptr(), ws.data_ptr(), n)
+    _seq_launch("vocab_ce_bwd", _lib.load().simvg_vocab_ce_bwd, block, dev, 6.0 * M * w.numel(), 4.0 * (x.numel() + w.numel()))
     return dx, dw, dbias
