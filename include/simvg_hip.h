@@ -478,8 +478,8 @@ int simvg_qk_norm_rope_bwd(const simvg_qk_norm_rope_args* args, simvg_stream_t s
  * layer's forward and backward of that batch read it.  A list that is none makes a plan without entries: nothing is computed, and
  * with fill_tail the outputs are NaN.
  * Forward writes o and lse [Hq][T] (natural logarithm of the softmax's denominator, scale included).  Backward reads q, k, v, o, lse and
- * d_o, writes dq, dk, dv; ws: simvg_packed_attn_ws_floats() floats, aligned to 16 bytes.  Rows behind the last sequence are left as they were, or, with
- * fill_tail, become zeros. */
+ * d_o, writes dq, dk, dv.  ws: simvg_packed_attn_ws_floats() floats of the direction, aligned to 16 bytes (forward: none, 0, unless there
+ * are few rows with many keys).  Rows behind the last sequence are left as they were, or, with fill_tail, become zeros. */
 typedef struct simvg_packed_attn_args {
   int dtype, T, nseq, Hq, Hkv, D, causal, fill_tail;
   float scale;
@@ -493,7 +493,7 @@ typedef struct simvg_packed_attn_args {
 } simvg_packed_attn_args;
 long simvg_packed_plan_ints(int T, int nseq);
 int simvg_packed_plan(const int* cu_seqlens, int nseq, int T, int* plan, simvg_stream_t stream);
-long simvg_packed_attn_ws_floats(int T, int nseq, int Hq, int Hkv, int D);
+long simvg_packed_attn_ws_floats(int T, int nseq, int Hq, int Hkv, int D, int causal, int backward);
 int simvg_packed_attn_fwd(const simvg_packed_attn_args* args, simvg_stream_t stream);
 int simvg_packed_attn_bwd(const simvg_packed_attn_args* args, simvg_stream_t stream);
 

@@ -118,7 +118,7 @@ QK_NORM_ROPE, PACKED_ATTN, VOCAB_CE = _packer(QkNormRopeArgs), _packer(PackedAtt
 _SIZES = {
     "simvg_qk_norm_rope_ws_floats": [c_int, c_int],
     "simvg_packed_plan_ints": [c_int, c_int],
-    "simvg_packed_attn_ws_floats": [c_int, c_int, c_int, c_int, c_int],
+    "simvg_packed_attn_ws_floats": [c_int] * 7,
     "simvg_vocab_ce_ws_bytes": [c_int, c_int, c_int, c_int, c_int],
 }
 

@@ -20,6 +20,7 @@
 // diagonal crosses, P is an exact 0 above it, and 0 x inf in the matrix product would still carry a later row's inf or NaN to an
 // earlier one: such a tile is looked through for values that are not finite, and if there are any they are added, as themselves, to the
 // rows that do see them and taken out of the tile (`add_nonfinite`, `tile_clean`).
+#include <algorithm>
 #include <type_traits>
 #include <utility>
 
@@ -34,7 +35,7 @@ struct simvg_packed_attn_args {
   float* lse; long lse_hs;                                   // [Hq][T]: head stride, rows are neighbours
   const void* d_o; long do_ts, do_hs;                        // backward
   void* dq; long dq_ts, dq_hs; void* dk; long dk_ts, dk_hs; void* dv; long dv_ts, dv_hs;
-  float* ws;                                                 // backward: simvg_packed_attn_ws_floats() floats
+  float* ws;                                                 // simvg_packed_attn_ws_floats() floats
 };
 
 namespace {
@@ -54,19 +55,26 @@ constexpr int PLAN_HEAD = 4, PLAN_BINS = 1024;
 // one more than the tiles of any valid list: what a launch has left over is enough for the tiles behind the last sequence
 __host__ __device__ __forceinline__ int plan_capacity(int T, int nseq) { return T / QT + nseq + 1; }
 
-// in place: scan[i] = sum of scan[0 .. i], 1024 threads
-__device__ __forceinline__ void scan1024(long* scan, int tid) {
-  __syncthreads();
-  for (int o = 1; o < 1024; o <<= 1) {
-    const long v = tid >= o ? scan[tid - o] : 0;
-    __syncthreads();
-    scan[tid] += v;
-    __syncthreads();
+// sum of the values of threads 0 .. tid, and of all 1024
+__device__ __forceinline__ int scan1024(int v, int (&waves)[16], int tid, int& total) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int up = __shfl_up(v, o, 64);
+    if ((tid & 63) >= o) v += up;
   }
+  if ((tid & 63) == 63) waves[tid >> 6] = v;
+  __syncthreads();
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) {
+    if (w < tid >> 6) v += waves[w];
+    total += waves[w];
+  }
+  __syncthreads();
+  return v;
 }
 __global__ __launch_bounds__(1024) void packed_plan_kernel(const int* cu, int nseq, int T, int* plan) {
-  __shared__ long scan[1024];
-  __shared__ int bins[PLAN_BINS];
+  __shared__ int waves[16], bins[PLAN_BINS];
   const int tid = threadIdx.x, cap = plan_capacity(T, nseq);
   int* base = plan + PLAN_HEAD + 4 * cap;
   int bad = cu[0] != 0;
@@ -75,17 +83,14 @@ __global__ __launch_bounds__(1024) void packed_plan_kernel(const int* cu, int ns
     if (tid == 0) { plan[0] = 0; plan[1] = -1; }
     return;
   }
-  long carry = 0;
+  int total = 0;
   for (int s0 = 0; s0 < nseq; s0 += 1024) {                  // prefix sums of the sequences' tiles
-    const int s = s0 + tid;
-    const long mine = s < nseq ? (cu[s + 1] - cu[s] + QT - 1) / QT : 0;
-    scan[tid] = mine;
-    scan1024(scan, tid);
-    if (s < nseq) base[s] = (int)(carry + scan[tid] - mine);
-    carry += scan[1023];
-    __syncthreads();
+    const int s = s0 + tid, mine = s < nseq ? (cu[s + 1] - cu[s] + QT - 1) / QT : 0;
+    int all;
+    const int upto = scan1024(mine, waves, tid, all);
+    if (s < nseq) base[s] = total + upto - mine;
+    total += all;
   }
-  const int total = (int)carry;
   if (tid == 0) { base[nseq] = total; plan[0] = total; plan[1] = cu[nseq]; }
   bins[tid] = 0;
   __threadfence_block();
@@ -107,10 +112,9 @@ __global__ __launch_bounds__(1024) void packed_plan_kernel(const int* cu, int ns
     }
     __syncthreads();
     if (!pass) {                                             // counts to starting places
-      const int mine = bins[tid];
-      scan[tid] = mine;
-      scan1024(scan, tid);
-      bins[tid] = (int)scan[tid] - mine;
+      int all;
+      const int mine = bins[tid], upto = scan1024(mine, waves, tid, all);
+      bins[tid] = upto - mine;
       __syncthreads();
     }
   }
@@ -325,12 +329,15 @@ __device__ __forceinline__ void store_sums(const f32x16 (&acc)[DP / 32], float m
 
 // ------------------------------------------------------------------------------------------------------------- forward
 template <class E, int DP, bool CAUSAL>
-__global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_fwd_kernel(simvg_packed_attn_args a) {
+__global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_fwd_kernel(simvg_packed_attn_args a, int parts) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   constexpr int TILE = KT * DP * 2, DB = DP / 32, KS = DP / 16;
-  const int h = blockIdx.x % a.Hq;
+  const int h = blockIdx.x % a.Hq, part = blockIdx.x / a.Hq % parts, id = blockIdx.x / a.Hq / parts;
   Tile e;
-  if (!plan_entry(a, blockIdx.x / a.Hq, e)) return fill_tail(a, blockIdx.x / a.Hq, a.o, a.o_ts, a.o_hs, h, a.lse);
+  if (!plan_entry(a, id, e)) {
+    if (part == 0) fill_tail(a, id, a.o, a.o_ts, a.o_hs, h, a.lse);
+    return;
+  }
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int hk = h / (a.Hq / a.Hkv);
   const int row = e.t * QT + wave * 32 + (lane & 31);        // the lane's query
@@ -338,19 +345,23 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_fwd_kernel(
   const unsigned short* qp = (const unsigned short*)a.q + (long)(e.first + min(row, e.len - 1)) * a.q_ts + (long)h * a.q_hs;
   const unsigned short* kp = (const unsigned short*)a.k + (long)e.first * a.k_ts + (long)hk * a.k_hs;
   const unsigned short* vp = (const unsigned short*)a.v + (long)e.first * a.v_ts + (long)hk * a.v_hs;
-  const int keys = CAUSAL ? min(e.len, (e.t + 1) * QT) : e.len, tiles = (keys + KT - 1) / KT;
+  // the tiles of keys, and this part's of them: [kt0, tiles)
+  const int keys = CAUSAL ? min(e.len, (e.t + 1) * QT) : e.len, all_tiles = (keys + KT - 1) / KT;
+  const int kt0 = all_tiles * part / parts, tiles = all_tiles * (part + 1) / parts;
   const int wave_first = e.t * QT + wave * 32;               // the wave's first query
   // tiles that no mask touches come first, then those that the diagonal or the sequence's end crosses, then (for the wave) nothing
-  const int whole = min(CAUSAL ? (e.t * QT + 1) / KT : tiles, e.len / KT);                     // of all four waves
+  const int whole = min(tiles, min(CAUSAL ? (e.t * QT + 1) / KT : tiles, e.len / KT));         // of all four waves
   const int wave_whole = min(CAUSAL ? (wave_first + 1) / KT : tiles, e.len / KT);
   const int wave_tiles = CAUSAL ? min(tiles, (wave_first + 32 + KT - 1) / KT) : tiles;
 
   Stager<DP, 0> gk;
   Stager<DP, 2 * TILE> gv;
-  gk.init(kp, a.k_ts, e.len, a.D, smem, wave, lane);
-  gv.init(vp, a.v_ts, e.len, a.D, smem, wave, lane);
-  gk.template next<0>();
-  gv.template next<0>();
+  gk.init(kp + (long)kt0 * KT * a.k_ts, a.k_ts, e.len - kt0 * KT, a.D, smem, wave, lane);
+  gv.init(vp + (long)kt0 * KT * a.v_ts, a.v_ts, e.len - kt0 * KT, a.D, smem, wave, lane);
+  if (kt0 < tiles) {
+    gk.template next<0>();
+    gv.template next<0>();
+  }
   lpx8_t qf[KS];
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) qf[ks] = global_frag(qp, ks, a.D, lane);
@@ -435,36 +446,71 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_fwd_kernel(
       }
     }
   };
-  int kt = 0;
+  int kt = kt0;
   for (; kt + 1 < whole; kt += 2) {
     tile(kt, std::integral_constant<int, 0>{}, std::false_type{});
     tile(kt + 1, std::integral_constant<int, 1>{}, std::false_type{});
   }
-  for (; kt < tiles; kt += 2) {                              // at most three tiles more
+  for (; kt < tiles; kt += 2) {                              // a few tiles more
     tile(kt, std::integral_constant<int, 0>{}, std::true_type{});
     if (kt + 1 < tiles) tile(kt + 1, std::integral_constant<int, 1>{}, std::true_type{});
   }
   l += __shfl_xor(l, 32, 64);
   const auto z = late_args<simvg_packed_attn_args>();
-  unsigned short* out = (unsigned short*)z->o + (long)(e.first + row) * z->o_ts + (long)h * z->o_hs;
-  store_rows<E, DP>(o, 1.f / l, out, z->D, valid, lane);
-  if (valid && lane < 32) z->lse[(long)h * z->lse_hs + e.first + row] = m * z->scale + __builtin_logf(l);
+  if (parts == 1) {
+    unsigned short* out = (unsigned short*)z->o + (long)(e.first + row) * z->o_ts + (long)h * z->o_hs;
+    store_rows<E, DP>(o, 1.f / l, out, z->D, valid, lane);
+    if (valid && lane < 32) z->lse[(long)h * z->lse_hs + e.first + row] = m * z->scale + __builtin_logf(l);
+  } else {
+    // [part][T][Hq] (reference, sum) and [part][T][Hq][D] numerators
+    const long n = (long)z->T * z->Hq, at = (long)(e.first + row) * z->Hq + h;
+    store_sums<DP>(o, 1.f, z->ws + 2 * parts * n + (part * n + at) * z->D, z->D, valid, lane);
+    if (valid && lane < 32) ((float2*)z->ws)[part * n + at] = make_float2(m * z->scale * LOG2E, l);
+  }
+}
+// the parts of a row joined: out = sum O_p 2^(m_p - m) / sum l_p 2^(m_p - m); 16 lanes a row
+template <class E>
+__global__ __launch_bounds__(256) void packed_attn_fwd_join_kernel(simvg_packed_attn_args a, int parts) {
+  const int c = (threadIdx.x & 15) * 8;
+  const long n = (long)a.T * a.Hq, rows = (long)a.plan[1] * a.Hq;
+  const float2* stat = (const float2*)a.ws;
+  for (long at = blockIdx.x * 16L + (threadIdx.x >> 4); at < rows; at += gridDim.x * 16L) {
+    float m = NEG_INF, l = 0.f;
+    for (int p = 0; p < parts; ++p) m = fmaxf(m, stat[p * n + at].x);
+    f32x4_t lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
+    for (int p = 0; p < parts; ++p) {
+      const float2 s = stat[p * n + at];
+      const float f = s.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(s.x - m);       // a part without keys has no reference
+      l += s.y * f;
+      if (c < a.D) {
+        const float* src = a.ws + 2 * parts * n + (p * n + at) * a.D + c;
+        const f32x4_t x = *(const f32x4_t*)src, y = *(const f32x4_t*)(src + 4);
+        lo += x * f;
+        hi += y * f;
+      }
+    }
+    const long row = at / a.Hq, h = at % a.Hq;
+    const float r = 1.f / l;
+    if (c < a.D)
+      *(u32x4_t*)((unsigned short*)a.o + row * a.o_ts + h * a.o_hs + c) = (u32x4_t){E::pack(lo[0] * r, lo[1] * r), E::pack(lo[2] * r, lo[3] * r),
+                                                                                   E::pack(hi[0] * r, hi[1] * r), E::pack(hi[2] * r, hi[3] * r)};
+    if (c == 0) a.lse[h * a.lse_hs + row] = (m + __builtin_log2f(l)) * LN2;
+  }
 }
 
 // ------------------------------------------------------------------------------------------------------------ backward
 // delta_i = sum_d dO_id O_id.  For fp16 also the largest norms of dO's and V's rows in a tile and head: |dP_ij| and |D_i| are at most
 // |dO_i| |V_j|, so with them dS can be brought to where fp16 has all its bits (`grad_power`).
-// ws: delta [Hq][T] | norms of dO [tiles][Hq] | norms of V [tiles][Hkv] | dk, dv of the parts [parts][2][T][Hkv][D]
+// ws: delta [Hq][T] | norms of dO [tiles][Hq] | norms of V [tiles][Hkv] | the parts' sums, dQ [parts][T][Hq][D], then dK and dV [parts][2][T][Hkv][D]
 __host__ __device__ __forceinline__ long ws_fixed(int T, int nseq, int Hq, int Hkv) {
   return ((long)Hq * T + (long)plan_capacity(T, nseq) * (Hq + Hkv) + 3) / 4 * 4;
 }
-struct Ws { float *delta, *ndo, *nv, *parts; };
+struct Ws { float *delta, *ndo, *nv; };
 __device__ __forceinline__ Ws ws_of(const simvg_packed_attn_args& a) {
   Ws w;
   w.delta = a.ws;
   w.ndo = a.ws + (long)a.Hq * a.T;
   w.nv = w.ndo + (long)plan_capacity(a.T, a.nseq) * a.Hq;
-  w.parts = a.ws + ws_fixed(a.T, a.nseq, a.Hq, a.Hkv);
   return w;
 }
 template <class E>
@@ -550,13 +596,16 @@ __device__ __forceinline__ float grad_power(const simvg_packed_attn_args& a, con
 
 // dQ: a workgroup's 128 queries against the tiles of their keys, as in the forward pass
 template <class E, int DP, bool CAUSAL>
-__global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_dq_kernel(simvg_packed_attn_args a) {
+__global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_dq_kernel(simvg_packed_attn_args a, int parts) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ float red[8];
   constexpr int TILE = KT * DP * 2, DB = DP / 32, KS = DP / 16;
-  const int h = blockIdx.x % a.Hq;
+  const int h = blockIdx.x % a.Hq, part = blockIdx.x / a.Hq % parts, id = blockIdx.x / a.Hq / parts;
   Tile e;
-  if (!plan_entry(a, blockIdx.x / a.Hq, e)) return fill_tail(a, blockIdx.x / a.Hq, a.dq, a.dq_ts, a.dq_hs, h, nullptr);
+  if (!plan_entry(a, id, e)) {
+    if (part == 0) fill_tail(a, id, a.dq, a.dq_ts, a.dq_hs, h, nullptr);
+    return;
+  }
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int hk = h / (a.Hq / a.Hkv);
   const float power = grad_power<E>(a, e, hk, red), up = __builtin_amdgcn_exp2f(power), shift = E::kScaled ? P_POWER : 0.f;
@@ -567,17 +616,21 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_dq_kernel(s
   const unsigned short* dop = (const unsigned short*)a.d_o + here * a.do_ts + (long)h * a.do_hs;
   const unsigned short* kp = (const unsigned short*)a.k + (long)e.first * a.k_ts + (long)hk * a.k_hs;
   const unsigned short* vp = (const unsigned short*)a.v + (long)e.first * a.v_ts + (long)hk * a.v_hs;
-  const int keys = CAUSAL ? min(e.len, (e.t + 1) * QT) : e.len, tiles = (keys + KT - 1) / KT;
+  // the tiles of keys, and this part's of them: [kt0, tiles)
+  const int keys = CAUSAL ? min(e.len, (e.t + 1) * QT) : e.len, all_tiles = (keys + KT - 1) / KT;
+  const int kt0 = all_tiles * part / parts, tiles = all_tiles * (part + 1) / parts;
   const int wave_first = e.t * QT + wave * 32;
-  const int whole = min(CAUSAL ? (e.t * QT + 1) / KT : tiles, e.len / KT);                     // of all four waves
+  const int whole = min(tiles, min(CAUSAL ? (e.t * QT + 1) / KT : tiles, e.len / KT));         // of all four waves
   const int wave_whole = min(CAUSAL ? (wave_first + 1) / KT : tiles, e.len / KT);
   const int wave_tiles = CAUSAL ? min(tiles, (wave_first + 32 + KT - 1) / KT) : tiles;
   Stager<DP, 0> gk;
   Stager<DP, 2 * TILE> gv;
-  gk.init(kp, a.k_ts, e.len, a.D, smem, wave, lane);
-  gv.init(vp, a.v_ts, e.len, a.D, smem, wave, lane);
-  gk.template next<0>();
-  gv.template next<0>();
+  gk.init(kp + (long)kt0 * KT * a.k_ts, a.k_ts, e.len - kt0 * KT, a.D, smem, wave, lane);
+  gv.init(vp + (long)kt0 * KT * a.v_ts, a.v_ts, e.len - kt0 * KT, a.D, smem, wave, lane);
+  if (kt0 < tiles) {
+    gk.template next<0>();
+    gv.template next<0>();
+  }
   lpx8_t qf[KS], dof[KS];
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) { qf[ks] = global_frag(qp, ks, a.D, lane); dof[ks] = global_frag(dop, ks, a.D, lane); }
@@ -649,7 +702,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_dq_kernel(s
       products(1);
     }
   };
-  int kt = 0;
+  int kt = kt0;
   for (; kt + 1 < whole; kt += 2) {
     tile(kt, std::integral_constant<int, 0>{}, std::false_type{});
     tile(kt + 1, std::integral_constant<int, 1>{}, std::false_type{});
@@ -659,8 +712,11 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_dq_kernel(s
     if (kt + 1 < tiles) tile(kt + 1, std::integral_constant<int, 1>{}, std::true_type{});
   }
   const auto z = late_args<simvg_packed_attn_args>();
-  unsigned short* out = (unsigned short*)z->dq + (long)(e.first + row) * z->dq_ts + (long)h * z->dq_hs;
-  store_rows<E, DP>(dq, z->scale * __builtin_amdgcn_exp2f(-power - shift), out, z->D, valid, lane);
+  const float mul = z->scale * __builtin_amdgcn_exp2f(-power - shift);
+  if (parts == 1) store_rows<E, DP>(dq, mul, (unsigned short*)z->dq + (long)(e.first + row) * z->dq_ts + (long)h * z->dq_hs, z->D, valid, lane);
+  else
+    store_sums<DP>(dq, mul, z->ws + ws_fixed(z->T, z->nseq, z->Hq, z->Hkv) + ((part * (long)z->T + e.first + row) * z->Hq + h) * z->D, z->D,
+                   valid, lane);
 }
 
 // dK, dV: a workgroup's 128 keys against the tiles of the queries that see them, of all heads that share the key head, one after the
@@ -834,25 +890,23 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void packed_attn_dkv_kernel(
     store_sums<DP>(dv, mv, out + n, z->D, valid, lane);
   }
 }
-// the parts of dk and dv, joined: one thread for 8 columns of a row (rows behind the last sequence were done by the parts' kernel)
+// the parts of a gradient, joined: sums [part][T][H][D], `stride` apart, one thread for 8 columns of a row (rows behind the last
+// sequence were done by the parts' kernel)
 template <class E>
-__global__ __launch_bounds__(256) void packed_attn_join_kernel(simvg_packed_attn_args a, int parts) {
-  const int per = a.D / 8, rows = a.plan[1];
-  const long n = (long)a.T * a.Hkv * a.D;
-  for (long i = blockIdx.x * 256L + threadIdx.x; i < (long)rows * a.Hkv * per; i += gridDim.x * 256L) {
-    const int c = (int)(i % per) * 8, hk = (int)(i / per % a.Hkv);
-    const long row = i / per / a.Hkv;
-#pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      const float* src = ws_of(a).parts + w * n + (row * a.Hkv + hk) * a.D + c;
-      f32x4_t lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
-      for (int p = 0; p < parts; ++p) {
-        lo += *(const f32x4_t*)(src + 2 * p * n);
-        hi += *(const f32x4_t*)(src + 2 * p * n + 4);
-      }
-      unsigned short* out = w ? (unsigned short*)a.dv + row * a.dv_ts + (long)hk * a.dv_hs : (unsigned short*)a.dk + row * a.dk_ts + (long)hk * a.dk_hs;
-      *(u32x4_t*)(out + c) = (u32x4_t){E::pack(lo[0], lo[1]), E::pack(lo[2], lo[3]), E::pack(hi[0], hi[1]), E::pack(hi[2], hi[3])};
+__global__ __launch_bounds__(256) void packed_attn_join_kernel(const int* plan, const float* sums, long stride, int parts, int H, int D,
+                                                               unsigned short* out, long ts, long hs) {
+  const int per = D / 8;
+  for (long i = blockIdx.x * 256L + threadIdx.x; i < (long)plan[1] * H * per; i += gridDim.x * 256L) {
+    const int c = (int)(i % per) * 8, h = (int)(i / per % H);
+    const long row = i / per / H;
+    const float* src = sums + (row * H + h) * D + c;
+    f32x4_t lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
+#pragma unroll 4
+    for (int p = 0; p < parts; ++p) {
+      lo += *(const f32x4_t*)(src + p * stride);
+      hi += *(const f32x4_t*)(src + p * stride + 4);
     }
+    *(u32x4_t*)(out + row * ts + h * hs + c) = (u32x4_t){E::pack(lo[0], lo[1]), E::pack(lo[2], lo[3]), E::pack(hi[0], hi[1]), E::pack(hi[2], hi[3])};
   }
 }
 
@@ -861,6 +915,27 @@ __global__ __launch_bounds__(256) void packed_attn_join_kernel(simvg_packed_attn
 bool rows16(const void* p, long ts, long hs) { return p && (uintptr_t)p % 16 == 0 && ts % 8 == 0 && hs % 8 == 0; }
 bool in_reach(long ts) { return ts >= 0 && ts < 1L << 24; }
 
+// How many parts a workgroup's work is cut into where a launch has few workgroups: so many that there are four for each of the 256
+// compute units (under `causal` they are of very different length), each of at least eight tiles on average.
+int parts_of(long groups, long tiles) { return (int)std::max(1L, std::min(std::min(1024 / groups, tiles / 8), 32L)); }
+// ... of a tile of queries, over its keys (forward pass and dQ): one sequence of 8192 rows, 4 heads of 128, causal: see DESIGN.md's table
+int row_parts(int T, int nseq, int Hq, int causal) {
+  return parts_of((long)plan_capacity(T, nseq) * Hq, (long)T / std::max(nseq, 1) / KT / (causal ? 2 : 1));
+}
+// ... of a tile of keys, over the queries and heads that see it (dK, dV; 16 k causal prompt, 16 heads on 2: 5.95 ms for the backward pass
+// without, 3.84 with four parts)
+int key_parts(int T, int nseq, int Hq, int Hkv, int causal) {
+  return parts_of((long)plan_capacity(T, nseq) * Hkv, (long)T / std::max(nseq, 1) / KT * (Hq / Hkv) / (causal ? 2 : 1));
+}
+// the parts' sums of the backward pass: dQ's and then dK's and dV's use the same room
+long bwd_sums(int T, int nseq, int Hq, int Hkv, int D, int causal) {
+  const int r = row_parts(T, nseq, Hq, causal), k = key_parts(T, nseq, Hq, Hkv, causal);
+  return std::max(r > 1 ? (long)r * T * Hq * D : 0L, k > 1 ? 2L * k * T * Hkv * D : 0L);
+}
+long fwd_sums(int T, int nseq, int Hq, int D, int causal) {
+  const int r = row_parts(T, nseq, Hq, causal);
+  return r > 1 ? (long)r * T * Hq * (D + 2) : 0L;
+}
 int attn_check(const simvg_packed_attn_args* a, bool bwd) {
   SIMVG_CHECK_ARG(a, "packed_attn: null argument block");
   SIMVG_CHECK_ARG(a->dtype == SEQ_F16 || a->dtype == SEQ_BF16, "packed_attn: dtype must be fp16 or bf16");
@@ -876,6 +951,8 @@ int attn_check(const simvg_packed_attn_args* a, bool bwd) {
                   rows16(a->o, a->o_ts, a->o_hs), "packed_attn: rows of q, k, v and out must start at multiples of 16 bytes");
   SIMVG_CHECK_ARG(in_reach(a->q_ts) && in_reach(a->k_ts) && in_reach(a->v_ts) && (!bwd || in_reach(a->do_ts)),
                   "packed_attn: token strides must be below 2^24 elements");
+  SIMVG_CHECK_ARG(bwd || fwd_sums(a->T, a->nseq, a->Hq, a->D, a->causal) == 0 || (a->ws && (uintptr_t)a->ws % 16 == 0),
+                  "packed_attn: this forward pass needs a workspace, aligned to 16 bytes");
   if (bwd) {
     SIMVG_CHECK_ARG(rows16(a->d_o, a->do_ts, a->do_hs) && rows16(a->dq, a->dq_ts, a->dq_hs) && rows16(a->dk, a->dk_ts, a->dk_hs) &&
                     rows16(a->dv, a->dv_ts, a->dv_hs), "packed_attn: rows of the gradients must start at multiples of 16 bytes");
@@ -884,29 +961,32 @@ int attn_check(const simvg_packed_attn_args* a, bool bwd) {
   return SIMVG_OK;
 }
 
-// Parts of a dK / dV workgroup: so many that the launch has four workgroups for each of the 256 compute units (one fits at a time, and
-// under `causal` they are of very different length), and that a part still has eight tiles of queries on average.
-// (16 k prompt, 2 key heads: 258 workgroups, backward pass 5.95 ms without, see below with)
-int dkv_parts(int T, int nseq, int Hq, int Hkv) {
-  const long groups = (long)plan_capacity(T, nseq) * Hkv, tiles = (long)(Hq / Hkv) * (T / (nseq > 0 ? nseq : 1)) / KT;
-  const long p = min(1024 / groups, tiles / 16);
-  return (int)max(1L, min(p, 32L));
+template <class E>
+void join(const simvg_packed_attn_args& a, const float* sums, long stride, int parts, int H, void* out, long ts, long hs, hipStream_t s) {
+  const long work = (long)a.T * H * a.D / 8;
+  hipLaunchKernelGGL((packed_attn_join_kernel<E>), dim3((int)min((work + 255) / 256, 4096L)), dim3(256), 0, s, a.plan, sums, stride, parts, H, a.D,
+                     (unsigned short*)out, ts, hs);
 }
 
 template <class E, int DP, bool CAUSAL>
 void attn_launch(const simvg_packed_attn_args& a, bool bwd, hipStream_t s) {
-  const int entries = plan_capacity(a.T, a.nseq), lds = 4 * KT * DP * 2;
+  const int entries = plan_capacity(a.T, a.nseq), lds = 4 * KT * DP * 2, rparts = row_parts(a.T, a.nseq, a.Hq, a.causal);
   if (!bwd) {
-    hipLaunchKernelGGL((packed_attn_fwd_kernel<E, DP, CAUSAL>), dim3(entries * a.Hq), dim3(256), lds, s, a);
+    hipLaunchKernelGGL((packed_attn_fwd_kernel<E, DP, CAUSAL>), dim3(entries * a.Hq * rparts), dim3(256), lds, s, a, rparts);
+    if (rparts > 1)
+      hipLaunchKernelGGL((packed_attn_fwd_join_kernel<E>), dim3((int)min(((long)a.T * a.Hq + 15) / 16, 8192L)), dim3(256), 0, s, a, rparts);
     return;
   }
+  float* sums = a.ws + ws_fixed(a.T, a.nseq, a.Hq, a.Hkv);
   hipLaunchKernelGGL((packed_attn_delta_kernel<E>), dim3(entries * a.Hq), dim3(256), 0, s, a);
-  hipLaunchKernelGGL((packed_attn_dq_kernel<E, DP, CAUSAL>), dim3(entries * a.Hq), dim3(256), lds, s, a);
-  const int parts = dkv_parts(a.T, a.nseq, a.Hq, a.Hkv);
-  hipLaunchKernelGGL((packed_attn_dkv_kernel<E, DP, CAUSAL>), dim3(entries * a.Hkv * parts), dim3(256), lds, s, a, parts);
-  if (parts > 1) {
-    const long work = (long)a.T * a.Hkv * a.D / 8;
-    hipLaunchKernelGGL((packed_attn_join_kernel<E>), dim3((int)min((work + 255) / 256, 4096L)), dim3(256), 0, s, a, parts);
+  hipLaunchKernelGGL((packed_attn_dq_kernel<E, DP, CAUSAL>), dim3(entries * a.Hq * rparts), dim3(256), lds, s, a, rparts);
+  if (rparts > 1) join<E>(a, sums, (long)a.T * a.Hq * a.D, rparts, a.Hq, a.dq, a.dq_ts, a.dq_hs, s);
+  const int kparts = key_parts(a.T, a.nseq, a.Hq, a.Hkv, a.causal);
+  hipLaunchKernelGGL((packed_attn_dkv_kernel<E, DP, CAUSAL>), dim3(entries * a.Hkv * kparts), dim3(256), lds, s, a, kparts);
+  if (kparts > 1) {
+    const long n = (long)a.T * a.Hkv * a.D;
+    join<E>(a, sums, 2 * n, kparts, a.Hkv, a.dk, a.dk_ts, a.dk_hs, s);
+    join<E>(a, sums + n, 2 * n, kparts, a.Hkv, a.dv, a.dv_ts, a.dv_hs, s);
   }
 }
 template <class E>
@@ -934,10 +1014,9 @@ extern "C" int simvg_packed_plan(const int* cu_seqlens, int nseq, int T, int* pl
   SIMVG_LAUNCH_CHECK();
   return SIMVG_OK;
 }
-extern "C" long simvg_packed_attn_ws_floats(int T, int nseq, int Hq, int Hkv, int D) {
-  if (T < 0 || nseq < 0 || Hkv < 1 || Hq < Hkv || D < 0) return 0;
-  const int parts = dkv_parts(T, nseq, Hq, Hkv);
-  return ws_fixed(T, nseq, Hq, Hkv) + (parts > 1 ? 2L * parts * T * Hkv * D : 0);
+extern "C" long simvg_packed_attn_ws_floats(int T, int nseq, int Hq, int Hkv, int D, int causal, int backward) {
+  if (T <= 0 || nseq < 0 || Hkv < 1 || Hq < Hkv || D < 0) return 0;
+  return backward ? ws_fixed(T, nseq, Hq, Hkv) + bwd_sums(T, nseq, Hq, Hkv, D, causal != 0) : fwd_sums(T, nseq, Hq, D, causal != 0);
 }
 extern "C" int simvg_packed_attn_fwd(const simvg_packed_attn_args* args, hipStream_t stream) { return attn_run(args, false, stream); }
 extern "C" int simvg_packed_attn_bwd(const simvg_packed_attn_args* args, hipStream_t stream) { return attn_run(args, true, stream); }

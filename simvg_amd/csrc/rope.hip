@@ -104,6 +104,9 @@ __device__ __forceinline__ void angles(const simvg_qk_norm_rope_args& a, int P, 
   }
 }
 
+// the wave's own LDS row: written and read by this wave alone, whose LDS accesses are done in their order
+__device__ __forceinline__ void own_row_written() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
 // the rotation of one lane's two chunks by +t (forward) or -t (backward).  Partners are (lo[i], hi[i]), or neighbours of 2V
 // consecutive values in lo, hi
 template <int V>
@@ -137,9 +140,9 @@ __global__ __launch_bounds__(256) void rope_fwd_kernel(simvg_qk_norm_rope_args a
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const long t = (long)blockIdx.x * (4 / wpt) + wave / wpt;
   float2* cs = cs_all[wave];
-  if (t < a.T) angles(a, P, t, lane, cs);
-  __syncthreads();
   if (t >= a.T) return;
+  angles(a, P, t, lane, cs);
+  own_row_written();
   constexpr int GROUPS = 64 / LPR;
   const int group = lane / LPR, l = lane % LPR, n = a.D / (2 * V);
   const float inv_d = 1.f / (float)a.D;
@@ -209,13 +212,9 @@ __global__ __launch_bounds__(256) void rope_bwd_kernel(simvg_qk_norm_rope_args a
     for (int i = 0; i < NP; ++i)
 #pragma unroll
       for (int j = 0; j < 2 * V; ++j) acc[w][i][j] = 0.f;
-  // every wave makes the same number of rounds: the barriers are met by all
-  for (long t0 = (long)blockIdx.x * 4; t0 < a.T; t0 += (long)gridDim.x * 4) {
-    const long t = t0 + wave;
-    __syncthreads();
-    if (t < a.T) angles(a, P, t, lane, cs);
-    __syncthreads();
-    if (t >= a.T) continue;
+  for (long t = (long)blockIdx.x * 4 + wave; t < a.T; t += (long)gridDim.x * 4) {
+    angles(a, P, t, lane, cs);
+    own_row_written();
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
       const int H = w ? a.Hkv : a.Hq;
@@ -314,18 +313,23 @@ __global__ __launch_bounds__(256) void rope_bwd_kernel(simvg_qk_norm_rope_args a
     a.ws[(long)blockIdx.x * 2 * a.D + i] = (sum[0][i] + sum[1][i]) + (sum[2][i] + sum[3][i]);
 }
 
-// dgq | dgk = the sum of `rows` partial rows: 16 columns per workgroup, 16 strands of rows, joined in order
-__global__ __launch_bounds__(256) void rope_dg_kernel(const float* ws, int rows, int D, float* dgq, float* dgk) {
-  __shared__ float part[16][17];
+// dgq | dgk = the sum of `rows` partial rows: 16 columns per workgroup, 64 strands of rows, joined in order
+__global__ __launch_bounds__(1024) void rope_dg_kernel(const float* ws, int rows, int D, float* dgq, float* dgk) {
+  __shared__ float part[64][17];
   const int c = blockIdx.x * 16 + (threadIdx.x & 15), s = threadIdx.x >> 4;
   float v = 0.f;
-  if (c < 2 * D)
-    for (int r = s; r < rows; r += 16) v += ws[(long)r * 2 * D + c];
+  if (c < 2 * D) {
+#pragma unroll 8
+    for (int r = s; r < rows; r += 64) v += ws[(long)r * 2 * D + c];
+  }
   part[s][threadIdx.x & 15] = v;
+  __syncthreads();
+  if (s < 16) part[s][threadIdx.x & 15] = (part[s][threadIdx.x & 15] + part[s + 16][threadIdx.x & 15]) + (part[s + 32][threadIdx.x & 15] + part[s + 48][threadIdx.x & 15]);
   __syncthreads();
   if (s == 0 && c < 2 * D) {
     float total = 0.f;
-    for (int i = 0; i < 16; ++i) total += part[i][threadIdx.x & 15];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) total += part[i][threadIdx.x];
     (c < D ? dgq[c] : dgk[c - D]) = total;
   }
 }
@@ -398,7 +402,7 @@ int rope_run(const simvg_qk_norm_rope_args* args, bool bwd, hipStream_t s) {
     SIMVG_LAUNCH_CHECK();
   }
   if (bwd && a.gq) {                                          // without a token the gradients are sums of nothing: zeros
-    hipLaunchKernelGGL(rope_dg_kernel, dim3(cdiv(2 * a.D, 16)), dim3(256), 0, s, a.ws, min(cdiv(a.T, 4), ROPE_BWD_BLOCKS), a.D, a.dgq, a.dgk);
+    hipLaunchKernelGGL(rope_dg_kernel, dim3(cdiv(2 * a.D, 16)), dim3(1024), 0, s, a.ws, min(cdiv(a.T, 4), ROPE_BWD_BLOCKS), a.D, a.dgq, a.dgk);
     SIMVG_LAUNCH_CHECK();
   }
   return SIMVG_OK;

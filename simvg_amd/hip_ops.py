@@ -1411,13 +1411,16 @@ def packed_attn_fwd(q, k, v, plan, causal=True, scale=None, out=None):
     """Attention over packed sequences (csrc/packed_attn.hip): q [T, Hq, D], k, v [T, Hkv, D], fp16 or bf16, `plan` from `packed_plan`.
     Returns (out [T, Hq, D], lse [Hq, T] fp32).  Rows behind the last sequence are zeros; in an `out` of the caller's they stay as
     they were."""
+    lib = _lib.load()
     args, dev = _packed_args(q, k, v, plan, causal, scale, out is None)
     (T, Hq, D), fill = q.shape, out is None
+    n = lib.simvg_packed_attn_ws_floats(T, plan.nseq, Hq, k.shape[1], D, args[6], 0)
+    ws = None if n == 0 else q.new_empty(n, dtype=torch.float32)
     lse = q.new_empty((Hq, T), dtype=torch.float32) if fill else q.new_zeros((Hq, T), dtype=torch.float32)
     out = q.new_empty(q.shape) if fill else out
     block = _lib.PACKED_ATTN.pack(*args, *_seq_rows("out", out, q.shape, q.dtype, dev, True), lse.data_ptr(), T,
-                                  0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
-    _seq_launch("packed_attn_fwd", _lib.load().simvg_packed_attn_fwd, block, dev, 0.0, 2.0 * (2 * q.numel() + k.numel() + v.numel()))
+                                  0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0 if ws is None else ws.data_ptr())
+    _seq_launch("packed_attn_fwd", lib.simvg_packed_attn_fwd, block, dev, 0.0, 2.0 * (2 * q.numel() + k.numel() + v.numel()))
     return out, lse
 
 
@@ -1432,7 +1435,7 @@ def packed_attn_bwd(q, k, v, out, lse, dout, plan, causal=True, scale=None, dq=N
     (T, Hq, D), dt = q.shape, q.dtype
     if fill:
         dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
-    ws = q.new_empty(max(1, lib.simvg_packed_attn_ws_floats(T, plan.nseq, Hq, k.shape[1], D)), dtype=torch.float32)
+    ws = q.new_empty(max(1, lib.simvg_packed_attn_ws_floats(T, plan.nseq, Hq, k.shape[1], D, args[6], 1)), dtype=torch.float32)
     block = _lib.PACKED_ATTN.pack(*args, *_seq_rows("out", out, q.shape, dt, dev), _seq_flat("lse", lse, (Hq, T), torch.float32, dev), T,
                                   *_seq_rows("dout", dout, q.shape, dt, dev), *_seq_rows("dq", dq, q.shape, dt, dev, True),
                                   *_seq_rows("dk", dk, k.shape, dt, dev, True), *_seq_rows("dv", dv, k.shape, dt, dev, True), ws.data_ptr())

@@ -80,7 +80,7 @@ def test_attention_refuses_before_launching():
     _refused(lib.simvg_packed_attn_bwd, _lib.PackedAttnArgs(**(ok | rows | grads)), "workspace")
     assert lib.simvg_packed_plan(None, 1, 4, None, None) < 0 and lib.simvg_packed_plan(256, -1, 4, 256, None) < 0
     assert lib.simvg_packed_plan_ints(-1, 3) == 0 and lib.simvg_packed_plan_ints(1000, 3) > 0
-    assert lib.simvg_packed_attn_ws_floats(-1, 1, 1, 1, 64) == 0
+    assert lib.simvg_packed_attn_ws_floats(-1, 1, 1, 1, 64, 1, 1) == 0
 
 
 def test_vocab_ce_refuses_before_launching():
