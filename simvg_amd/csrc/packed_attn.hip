@@ -228,8 +228,9 @@ __device__ __forceinline__ float max_halves(float v) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
-// row of a 32x32 accumulator's register r
-__device__ __forceinline__ int acc_row(int r, int lane) { return (r >> 2) * 8 + (lane >> 5) * 4 + (r & 3); }
+// row of a 32x32 accumulator's register r: a constant, and 4 more in the upper half of the wave
+__device__ __forceinline__ constexpr int reg_row(int r) { return (r >> 2) * 8 + (r & 3); }
+__device__ __forceinline__ int acc_row(int r, int lane) { return reg_row(r) + (lane >> 5) * 4; }
 __device__ __forceinline__ f32x16 zero16() { return (f32x16){0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}; }
 
 // ---- values that are not finite in a tile that the mask crosses
@@ -387,6 +388,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_fwd_kernel(
     }
     const bool odd = MASKED && tile_nonfinite<E, DP>(smem + V0), mine = !MASKED || kt < wave_tiles;
     const int last = (CAUSAL ? min(row, e.len - 1) : e.len - 1) - kt * KT;     // of the tile's keys, the last that the lane's query sees
+    const int last4 = last - (lane >> 5) * 4;                // against a register's constant
     f32x16 s[2];
     if (mine) {
       s[0] = s[1] = zero16();                                // two chains of products, one waits for its own result less often
@@ -399,7 +401,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_fwd_kernel(
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
           for (int r = 0; r < 16; ++r)
-            if (kb * 32 + acc_row(r, lane) > last) s[kb][r] = NEG_INF;
+            if (kb * 32 + reg_row(r) > last4) s[kb][r] = NEG_INF;
       }
       float top = NEG_INF;
 #pragma unroll
@@ -657,6 +659,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_dq_kernel(s
     }
     const bool odd = MASKED && tile_nonfinite<E, DP>(smem + K0), mine = !MASKED || kt < wave_tiles;
     const int last = (CAUSAL ? min(row, e.len - 1) : e.len - 1) - kt * KT;
+    const int last4 = last - (lane >> 5) * 4;                // against a register's constant
     lpx8_t ds[4];
     f32x16 s, dp;
     auto scores = [&](int kb) {
@@ -676,7 +679,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_dq_kernel(s
       if (MASKED && kt >= wave_whole) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          if (kb * 32 + acc_row(r, lane) > last) s[r] = 0.f;
+          if (kb * 32 + reg_row(r) > last4) s[r] = 0.f;
       }
       ds[2 * kb] = acc_frag<E>(s, 0);
       ds[2 * kb + 1] = acc_frag<E>(s, 1);
@@ -801,6 +804,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void packed_attn_dkv_kernel(
     wave_barrier_only();
     if (i + 1 < steps) issue(std::integral_constant<int, (BUF ^ 1)>{});
     const int from = key - row0;                             // the first row of the tile that sees the lane's key
+    const int from4 = from - (lane >> 5) * 4;
     // (without a mask row0 + KT is always above 0: a branch all the same, or hipcc keeps the operands of two steps at once and spills)
     const bool mine = row0 + KT > (CAUSAL ? wave_first : 0), whole = !CAUSAL || row0 >= wave_first + 31;
     // Rows that are not finite lose nothing by being cleaned before the scores: their lse (of q) or delta (of dO) is not finite either,
@@ -855,7 +859,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void packed_attn_dkv_kernel(
           stay_a_branch();
 #pragma unroll
           for (int x = 0; x < 16; ++x)
-            if (qb * 32 + acc_row(x, lane) < from) { s[x] = 0.f; dp[x] = 0.f; }
+            if (qb * 32 + reg_row(x) < from4) { s[x] = 0.f; dp[x] = 0.f; }
         }
         __builtin_amdgcn_sched_barrier(0);
         if (qb == 0) rows(1);
