@@ -228,6 +228,10 @@ __device__ __forceinline__ float max_halves(float v) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
+__device__ __forceinline__ float add_halves(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
 // row of a 32x32 accumulator's register r: a constant, and 4 more in the upper half of the wave
 __device__ __forceinline__ constexpr int reg_row(int r) { return (r >> 2) * 8 + (r & 3); }
 __device__ __forceinline__ int acc_row(int r, int lane) { return reg_row(r) + (lane >> 5) * 4; }
@@ -501,8 +505,8 @@ __global__ __launch_bounds__(256) void packed_attn_fwd_join_kernel(simvg_packed_
 }
 
 // ------------------------------------------------------------------------------------------------------------ backward
-// delta_i = sum_d dO_id O_id.  For fp16 also the largest norms of dO's and V's rows in a tile and head: |dP_ij| and |D_i| are at most
-// |dO_i| |V_j|, so with them dS can be brought to where fp16 has all its bits (`grad_power`).
+// For fp16: delta_i = sum_d dO_id O_id, and the largest norms of dO's and V's rows in a tile and head: |dP_ij| and |delta_i| are at most
+// |dO_i| |V_j|, so with them dS can be brought to where fp16 has all its bits (`grad_power`).  (bf16: the dQ kernel takes delta along.)
 // ws: delta [Hq][T] | norms of dO [tiles][Hq] | norms of V [tiles][Hkv] | the parts' sums, dQ [parts][T][Hq][D], then dK and dV [parts][2][T][Hkv][D]
 __host__ __device__ __forceinline__ long ws_fixed(int T, int nseq, int Hq, int Hkv) {
   return ((long)Hq * T + (long)plan_capacity(T, nseq) * (Hq + Hkv) + 3) / 4 * 4;
@@ -535,7 +539,7 @@ __global__ __launch_bounds__(256) void packed_attn_delta_kernel(simvg_packed_att
   if (!plan_entry(a, blockIdx.x / a.Hq, e)) return;
   const Ws w = ws_of(a);
   const int lane16 = threadIdx.x & 15, n = min(QT, e.len - e.t * QT);
-  const bool with_v = E::kScaled && h % G == 0;
+  const bool with_v = h % G == 0;
   float mdo = 0.f, mv = 0.f;
   // 16 lanes a row, 8 columns each: D <= 128
   for (int r = threadIdx.x >> 4; r < QT; r += 16) {
@@ -546,7 +550,7 @@ __global__ __launch_bounds__(256) void packed_attn_delta_kernel(simvg_packed_att
       const u32x4_t x = *(const u32x4_t*)((const unsigned short*)a.d_o + row * a.do_ts + (long)h * a.do_hs + col);
       const u32x4_t y = *(const u32x4_t*)((const unsigned short*)a.o + row * a.o_ts + (long)h * a.o_hs + col);
       d = dot8<E>(x, y, 0.f);
-      if (E::kScaled) sd = dot8<E>(x, x, 0.f);
+      sd = dot8<E>(x, x, 0.f);
       if (with_v) {
         const u32x4_t z = *(const u32x4_t*)((const unsigned short*)a.v + row * a.v_ts + (long)(h / G) * a.v_hs + col);
         sv = dot8<E>(z, z, 0.f);
@@ -555,22 +559,21 @@ __global__ __launch_bounds__(256) void packed_attn_delta_kernel(simvg_packed_att
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) {
       d += __shfl_xor(d, o, 64);
-      if (E::kScaled) { sd += __shfl_xor(sd, o, 64); sv += __shfl_xor(sv, o, 64); }
+      sd += __shfl_xor(sd, o, 64);
+      sv += __shfl_xor(sv, o, 64);
     }
     if (r < n && lane16 == 0) w.delta[(long)h * a.T + row] = d;
     if (__builtin_isfinite(sd)) mdo = fmaxf(mdo, sd);        // a row that is not finite has no gradient that a scale could save
     if (__builtin_isfinite(sv)) mv = fmaxf(mv, sv);
   }
-  if constexpr (E::kScaled) {
-    mdo = wave_max(mdo);
-    mv = wave_max(mv);
-    if ((threadIdx.x & 63) == 0) { most[0][threadIdx.x >> 6] = mdo; most[1][threadIdx.x >> 6] = mv; }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      const long tile = e.base + e.t;
-      w.ndo[tile * a.Hq + h] = sqrtf(fmaxf(fmaxf(most[0][0], most[0][1]), fmaxf(most[0][2], most[0][3])));
-      if (with_v) w.nv[tile * a.Hkv + h / G] = sqrtf(fmaxf(fmaxf(most[1][0], most[1][1]), fmaxf(most[1][2], most[1][3])));
-    }
+  mdo = wave_max(mdo);
+  mv = wave_max(mv);
+  if ((threadIdx.x & 63) == 0) { most[0][threadIdx.x >> 6] = mdo; most[1][threadIdx.x >> 6] = mv; }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const long tile = e.base + e.t;
+    w.ndo[tile * a.Hq + h] = sqrtf(fmaxf(fmaxf(most[0][0], most[0][1]), fmaxf(most[0][2], most[0][3])));
+    if (with_v) w.nv[tile * a.Hkv + h / G] = sqrtf(fmaxf(fmaxf(most[1][0], most[1][1]), fmaxf(most[1][2], most[1][3])));
   }
 }
 // fp16: what is rounded to 16 bits is P 2^14 (P <= 1: the largest is 2^14) and dS 2^14 2^-x with 2^x at least the sequence's and key
@@ -639,7 +642,18 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_dq_kernel(s
   Lanes<DP> at;
   at.init(smem, lane);
   const float c = a.scale * LOG2E;
-  float lse2 = a.lse[(long)h * a.lse_hs + here] * LOG2E - shift, delta = ws_of(a).delta[(long)h * a.T + here];
+  float lse2 = a.lse[(long)h * a.lse_hs + here] * LOG2E - shift, delta;
+  if constexpr (E::kScaled) {
+    delta = ws_of(a).delta[(long)h * a.T + here];
+  } else {                                                   // dO's row is here already: delta needs no kernel of its own
+    const unsigned short* op = (const unsigned short*)a.o + here * a.o_ts + (long)h * a.o_hs;
+    delta = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+      delta = dot8<E>(__builtin_bit_cast(u32x4_t, dof[ks]), __builtin_bit_cast(u32x4_t, global_frag(op, ks, a.D, lane)), delta);
+    delta = add_halves(delta);
+    if (part == 0 && valid && lane < 32) ws_of(a).delta[(long)h * a.T + here] = delta;
+  }
   arrived(qf);
   arrived(dof);
   arrived(lse2);
@@ -919,17 +933,20 @@ __global__ __launch_bounds__(256) void packed_attn_join_kernel(const int* plan, 
 bool rows16(const void* p, long ts, long hs) { return p && (uintptr_t)p % 16 == 0 && ts % 8 == 0 && hs % 8 == 0; }
 bool in_reach(long ts) { return ts >= 0 && ts < 1L << 24; }
 
-// How many parts a workgroup's work is cut into where a launch has few workgroups: so many that there are four for each of the 256
-// compute units (under `causal` they are of very different length), each of at least eight tiles on average.
-int parts_of(long groups, long tiles) { return (int)std::max(1L, std::min(std::min(1024 / groups, tiles / 8), 32L)); }
-// ... of a tile of queries, over its keys (forward pass and dQ): one sequence of 8192 rows, 4 heads of 128, causal: see DESIGN.md's table
-int row_parts(int T, int nseq, int Hq, int causal) {
-  return parts_of((long)plan_capacity(T, nseq) * Hq, (long)T / std::max(nseq, 1) / KT / (causal ? 2 : 1));
+// How many parts a workgroup's work is cut into where a launch has few workgroups: so many that there are two for each of the 256
+// compute units, four under `causal`, where they are of very different length, and each of at least eight tiles on average.  (One
+// sequence of 8192 rows, 4 heads of 128 on 1, causal: forward 156 us uncut and 99 cut, backward 1246 and 351; 2048 rows, 8 heads of 128,
+// no mask: 42 and 38, 133 and 114; 8192 rows, 4 heads, no mask, 256 equal workgroups: 501 us uncut, 519 in three parts.)
+int parts_of(long groups, long tiles, int causal) {
+  return (int)std::max(1L, std::min(std::min((causal ? 1024 : 512) / groups, tiles / (causal ? 2 : 1) / 8), 32L));
 }
-// ... of a tile of keys, over the queries and heads that see it (dK, dV; 16 k causal prompt, 16 heads on 2: 5.95 ms for the backward pass
-// without, 3.84 with four parts)
+// ... of a tile of queries, over its keys (forward pass and dQ)
+int row_parts(int T, int nseq, int Hq, int causal) {
+  return parts_of((long)plan_capacity(T, nseq) * Hq, (long)T / std::max(nseq, 1) / KT, causal);
+}
+// ... of a tile of keys, over the queries and heads that see it (dK, dV)
 int key_parts(int T, int nseq, int Hq, int Hkv, int causal) {
-  return parts_of((long)plan_capacity(T, nseq) * Hkv, (long)T / std::max(nseq, 1) / KT * (Hq / Hkv) / (causal ? 2 : 1));
+  return parts_of((long)plan_capacity(T, nseq) * Hkv, (long)T / std::max(nseq, 1) / KT * (Hq / Hkv), causal);
 }
 // the parts' sums of the backward pass: dQ's and then dK's and dV's use the same room
 long bwd_sums(int T, int nseq, int Hq, int Hkv, int D, int causal) {
@@ -982,7 +999,7 @@ void attn_launch(const simvg_packed_attn_args& a, bool bwd, hipStream_t s) {
     return;
   }
   float* sums = a.ws + ws_fixed(a.T, a.nseq, a.Hq, a.Hkv);
-  hipLaunchKernelGGL((packed_attn_delta_kernel<E>), dim3(entries * a.Hq), dim3(256), 0, s, a);
+  if constexpr (E::kScaled) hipLaunchKernelGGL((packed_attn_delta_kernel<E>), dim3(entries * a.Hq), dim3(256), 0, s, a);
   hipLaunchKernelGGL((packed_attn_dq_kernel<E, DP, CAUSAL>), dim3(entries * a.Hq * rparts), dim3(256), lds, s, a, rparts);
   if (rparts > 1) join<E>(a, sums, (long)a.T * a.Hq * a.D, rparts, a.Hq, a.dq, a.dq_ts, a.dq_hs, s);
   const int kparts = key_parts(a.T, a.nseq, a.Hq, a.Hkv, a.causal);
