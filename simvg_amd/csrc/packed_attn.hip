@@ -300,9 +300,10 @@ __device__ __forceinline__ bool plan_entry(const simvg_packed_attn_args& a, int 
 __device__ __forceinline__ void fill_tail(const simvg_packed_attn_args& a, int id, void* out, long ts, long hs, int h, float* lse) {
   if (!a.fill_tail) return;
   const bool invalid = a.plan[1] < 0;
-  const int row0 = (invalid ? 0 : a.plan[1]) + (id - a.plan[0]) * QT, rows = min(QT, a.T - row0);
+  const long row0 = (invalid ? 0L : a.plan[1]) + (id - a.plan[0]) * (long)QT;
+  const int rows = (int)min((long)QT, a.T - row0);
   const unsigned short value = invalid ? 0x7fff : 0;         // a NaN in fp16 and in bf16
-  for (int i = threadIdx.x; i < rows * a.D; i += 256) ((unsigned short*)out)[(long)(row0 + i / a.D) * ts + (long)h * hs + i % a.D] = value;
+  for (int i = threadIdx.x; i < rows * a.D; i += 256) ((unsigned short*)out)[(row0 + i / a.D) * ts + (long)h * hs + i % a.D] = value;
   if (lse)
     for (int i = threadIdx.x; i < rows; i += 256) lse[(long)h * a.lse_hs + row0 + i] = invalid ? __builtin_nanf("") : 0.f;
 }
@@ -429,7 +430,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_fwd_kernel(
     }
     if (mine) {
       // the exponentials of 16 keys and the products of the 16 before: vector and matrix pipes at the same time
-      const float mc = m * c;
+      const float mc = m == NEG_INF ? 0.f : m * c;           // nothing but scores of -inf so far: exponentials of 0, not NaN
       lpx8_t p[4];
       auto exps = [&](int rk) {
         f32x16& x = s[rk >> 1];
@@ -818,9 +819,10 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void packed_attn_dkv_kernel(
     wave_barrier_only();
     if (i + 1 < steps) issue(std::integral_constant<int, (BUF ^ 1)>{});
     const int from = key - row0;                             // the first row of the tile that sees the lane's key
-    const int from4 = from - (lane >> 5) * 4;
+    // (rows past the sequence are zeros; times a key of -inf they would be NaN)
+    const int from4 = from - (lane >> 5) * 4, rows4 = e.len - row0 - (lane >> 5) * 4;
     // (without a mask row0 + KT is always above 0: a branch all the same, or hipcc keeps the operands of two steps at once and spills)
-    const bool mine = row0 + KT > (CAUSAL ? wave_first : 0), whole = !CAUSAL || row0 >= wave_first + 31;
+    const bool mine = row0 + KT > (CAUSAL ? wave_first : 0), whole = row0 + KT <= e.len && (!CAUSAL || row0 >= wave_first + 31);
     // Rows that are not finite lose nothing by being cleaned before the scores: their lse (of q) or delta (of dO) is not finite either,
     // and carries that to P and dS of every key they see
     if (CAUSAL && row0 < e.t * QT + QT - 1) {
@@ -873,7 +875,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void packed_attn_dkv_kernel(
           stay_a_branch();
 #pragma unroll
           for (int x = 0; x < 16; ++x)
-            if (qb * 32 + reg_row(x) < from4) { s[x] = 0.f; dp[x] = 0.f; }
+            if ((CAUSAL && qb * 32 + reg_row(x) < from4) || qb * 32 + reg_row(x) >= rows4) { s[x] = 0.f; dp[x] = 0.f; }
         }
         __builtin_amdgcn_sched_barrier(0);
         if (qb == 0) rows(1);
@@ -936,7 +938,7 @@ bool in_reach(long ts) { return ts >= 0 && ts < 1L << 24; }
 // How many parts a workgroup's work is cut into where a launch has few workgroups: so many that there are two for each of the 256
 // compute units, four under `causal`, where they are of very different length, and each of at least eight tiles on average.  (One
 // sequence of 8192 rows, 4 heads of 128 on 1, causal: forward 156 us uncut and 99 cut, backward 1246 and 351; 2048 rows, 8 heads of 128,
-// no mask: 42 and 38, 133 and 114; 8192 rows, 4 heads, no mask, 256 equal workgroups: 501 us uncut, 519 in three parts.)
+// no mask: 42 and 40, 133 and 123; 8192 rows, 4 heads, no mask, 256 equal workgroups: 501 us uncut, 519 in three parts.)
 int parts_of(long groups, long tiles, int causal) {
   return (int)std::max(1L, std::min(std::min((causal ? 1024 : 512) / groups, tiles / (causal ? 2 : 1) / 8), 32L));
 }
@@ -964,7 +966,7 @@ int attn_check(const simvg_packed_attn_args* a, bool bwd) {
   SIMVG_CHECK_ARG(a->Hkv >= 1 && a->Hq >= a->Hkv && a->Hq % a->Hkv == 0, "packed_attn: the heads of q must be a multiple of those of k and v");
   SIMVG_CHECK_ARG(a->D >= 8 && a->D <= 128 && a->D % 8 == 0, "packed_attn: the head size must be a multiple of 8 and at most 128");
   SIMVG_CHECK_ARG(a->scale > 0.f && a->scale < __builtin_huge_valf(), "packed_attn: scale must be positive and finite");
-  SIMVG_CHECK_ARG((long)plan_capacity(a->T, a->nseq) * a->Hq < 0x7fffffffL, "packed_attn: too many tiles for one launch");
+  SIMVG_CHECK_ARG((long)plan_capacity(a->T, a->nseq) * a->Hq < 1L << 24, "packed_attn: too many tiles for one launch");
   if (a->T == 0) return SIMVG_OK;
   SIMVG_CHECK_ARG(a->plan && a->lse, "packed_attn: null pointer");
   SIMVG_CHECK_ARG((uintptr_t)a->plan % 4 == 0, "packed_attn: misaligned plan");
@@ -991,6 +993,12 @@ void join(const simvg_packed_attn_args& a, const float* sums, long stride, int p
 
 template <class E, int DP, bool CAUSAL>
 void attn_launch(const simvg_packed_attn_args& a, bool bwd, hipStream_t s) {
+  static std::atomic<unsigned long> done[3] = {{0}, {0}, {0}};               // the tiles of 128 columns and the kernels' own few bytes pass 64 KiB
+  if (!bwd) allow_lds((const void*)packed_attn_fwd_kernel<E, DP, CAUSAL>, 4 * KT * DP * 2, done[0]);
+  else {
+    allow_lds((const void*)packed_attn_dq_kernel<E, DP, CAUSAL>, 4 * KT * DP * 2, done[1]);
+    allow_lds((const void*)packed_attn_dkv_kernel<E, DP, CAUSAL>, 4 * KT * DP * 2, done[2]);
+  }
   const int entries = plan_capacity(a.T, a.nseq), lds = 4 * KT * DP * 2, rparts = row_parts(a.T, a.nseq, a.Hq, a.causal);
   if (!bwd) {
     hipLaunchKernelGGL((packed_attn_fwd_kernel<E, DP, CAUSAL>), dim3(entries * a.Hq * rparts), dim3(256), lds, s, a, rparts);

@@ -342,6 +342,7 @@ int rope_check(const simvg_qk_norm_rope_args* a, bool bwd, int& P) {
   SIMVG_CHECK_ARG(a, "qk_norm_rope: null argument block");
   SIMVG_CHECK_ARG(a->dtype == SEQ_F32 || a->dtype == SEQ_F16 || a->dtype == SEQ_BF16, "qk_norm_rope: dtype must be fp32, fp16 or bf16");
   SIMVG_CHECK_ARG(a->T >= 0 && a->Hq >= 1 && a->Hkv >= 1, "qk_norm_rope: needs T >= 0 and at least one head of q and of k");
+  SIMVG_CHECK_ARG(a->T < 1 << 26, "qk_norm_rope: too many tokens for one launch");
   SIMVG_CHECK_ARG(a->D >= 2 && a->D <= ROPE_MAX_D && a->D % 2 == 0, "qk_norm_rope: the head size must be even and at most 256");
   SIMVG_CHECK_ARG(a->n_axes >= 1 && a->n_axes <= 4, "qk_norm_rope: one to four position axes");
   P = 0;

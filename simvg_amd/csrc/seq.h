@@ -3,6 +3,8 @@
 // they read comes from a caller's language model and not from this library's encoder.  Rounding to 16 bits is round-to-nearest-even
 // and does not saturate: an overflow is an inf, as in torch, and a loss scaler can see it.
 #pragma once
+#include <atomic>
+
 #include "common.h"
 
 // element types of the `dtype` arguments (include/simvg_hip.h: SIMVG_F32, SIMVG_F16, SIMVG_BF16)
@@ -51,17 +53,7 @@ __device__ __forceinline__ void unpack2(unsigned u, float& lo, float& hi) {
 // puts `s_waitcnt vmcnt(0)` in front of every LDS read that may alias a DMA it knows of, which would wait for the tile that has just
 // been asked for; it has no register output, so nothing can be taken before it has arrived.  The caller counts: `dma_wait<N>` leaves
 // the N youngest in flight, and a barrier makes the others' pieces visible.
-__device__ __forceinline__ u32x4_t dma_buffer(const void* base, unsigned bytes) {
-  const unsigned long p = (unsigned long)base;
-  return (u32x4_t){(unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)p), (unsigned)__builtin_amdgcn_readfirstlane((int)(p >> 32) & 0xffff),
-                   (unsigned)__builtin_amdgcn_readfirstlane((int)bytes), 0x00020000u};
-}
-__device__ __forceinline__ void dma16(u32x4_t buffer, unsigned lds, unsigned offset) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane((int)lds)),
-               "v"(offset), "s"(buffer)
-               : "memory", "m0");
-}
-// the same at LDS byte `lds` + PLUS: one scalar register serves all pieces of a wave
+// (LDS byte `lds` + PLUS: one scalar register serves all pieces of a wave.  A buffer: address, 48 bits | bytes | 0x00020000.)
 template <int PLUS>
 __device__ __forceinline__ void dma16_at(u32x4_t buffer, unsigned lds, unsigned offset) {
   asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(buffer), "n"(PLUS)
@@ -80,5 +72,12 @@ template <int N>
 __device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 // a barrier that does not drain this wave's DMA (what `__syncthreads` would wait for is the caller's business here)
 __device__ __forceinline__ void wave_barrier_only() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// more than 64 KiB of LDS has to be asked for, once on each device
+inline void allow_lds(const void* kernel, int bytes, std::atomic<unsigned long>& done) {
+  int device = 0;
+  if (hipGetDevice(&device) != hipSuccess || (device < 64 && done.load() >> device & 1)) return;
+  if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess && device < 64) done |= 1ul << device;
+}
 
 }  // namespace seq

@@ -15,7 +15,6 @@
 // Rounding to 16 bits, by choice: e (one rounding, relative 2^-9 bf16 / 2^-12 fp16; in fp16 times 2^14, so that a probability of 2^-28
 // keeps all its bits) and g x / max|g| where the rows' gradients differ (where they are equal or 0 the factor is 1 or 0: exact).
 // Everything that is summed is summed in 32 bits; db is summed before the rounding.
-#include <atomic>
 #include <type_traits>
 #include <utility>
 
@@ -36,7 +35,7 @@ struct simvg_vocab_ce_args {
 namespace {
 using namespace seq;
 
-constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+constexpr float LOG2E = 1.44269504088896340736f;
 constexpr float NEG_INF = -__builtin_huge_valf();
 constexpr int BK = 64;                                       // contracted values of a stage: a row's are one line of 128 bytes
 
@@ -683,6 +682,7 @@ int ce_check(const simvg_vocab_ce_args* a, bool bwd) {
   SIMVG_CHECK_ARG(a->M >= 0 && a->V >= 1 && a->K >= 8, "vocab_ce: needs M >= 0, V >= 1, K >= 8");
   SIMVG_CHECK_ARG(a->K % 8 == 0, "vocab_ce: K must be a multiple of 8");
   SIMVG_CHECK_ARG(a->M <= 1 << 22 && a->V <= 1 << 24 && a->K <= 1 << 16, "vocab_ce: M, V or K too large");
+  SIMVG_CHECK_ARG((long)cdiv(a->V, 256) * cdiv(a->M, 256) < 1L << 23, "vocab_ce: too many tiles for one launch");
   SIMVG_CHECK_ARG(a->ldx >= a->K && a->ldw >= a->K && a->ldx < 1 << 21 && a->ldw < 1 << 21, "vocab_ce: row strides must be at least K and below 2^21");
   SIMVG_CHECK_ARG(rows16(a->w, a->ldw), "vocab_ce: rows of w must start at multiples of 16 bytes");
   SIMVG_CHECK_ARG(a->M == 0 || rows16(a->x, a->ldx), "vocab_ce: rows of x must start at multiples of 16 bytes");
@@ -697,12 +697,6 @@ int ce_check(const simvg_vocab_ce_args* a, bool bwd) {
   return SIMVG_OK;
 }
 
-// more than 64 KiB of LDS has to be asked for, once on each device
-void allow_lds(const void* kernel, int bytes, std::atomic<unsigned long>& done) {
-  int device = 0;
-  if (hipGetDevice(&device) != hipSuccess || (device < 64 && done.load() >> device & 1)) return;
-  if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess && device < 64) done |= 1ul << device;
-}
 #define CE_LAUNCH(THREADS, LDS, KERNEL, GRID, ...)                                   \
   do {                                                                               \
     static std::atomic<unsigned long> done{0};                                       \

@@ -5,6 +5,9 @@ path's image and text tokens is trained with.  PyTorch autograd is the tape only
     q, k = qk_norm_rope(q, k, pos, inv_freq, sections, gq, gk)          # [T, H, D]
     o = packed_attention(q, k, v, plan)                                 # causal, grouped heads
     loss = vocab_cross_entropy(x, w, target, bias)                      # the logits are never stored
+
+All run on the current stream and may be captured into a HIP graph, forward and backward (a captured backward pass must not find an
+eager graph of the same leaves alive: torch ends the process then).  A second derivative is refused.
 """
 import torch
 from torch.autograd.function import once_differentiable
@@ -16,8 +19,9 @@ __all__ = ["PackedPlan", "packed_plan", "qk_norm_rope", "packed_attention", "voc
 
 
 def _rows(t):
-    """a gradient with its innermost dimension contiguous (autograd may hand over an expanded or transposed one)"""
-    return t if t.stride(-1) == 1 and all(s % 8 == 0 for s in t.stride()[:-1]) and t.data_ptr() % 16 == 0 else t.contiguous()
+    """a gradient with rows of 16-byte chunks (autograd may hand over an expanded or transposed one, or a part of a larger one)"""
+    fits = t.stride(-1) == 1 and all(s % 8 == 0 for s in t.stride()[:-1]) and t.data_ptr() % 16 == 0
+    return t if fits else t.clone(memory_format=torch.contiguous_format)
 
 
 class QKNormRope(torch.autograd.Function):

@@ -50,7 +50,7 @@ def _refused(fn, args, words):
 def test_rope_refuses_before_launching():
     lib = _lib.load()
     ok = dict(dtype=1, T=4, Hq=2, Hkv=1, D=64, n_axes=1, sections=(C.c_int * 4)(32), eps=1e-6)
-    for bad, words in ((dict(dtype=3), "dtype"), (dict(T=-1), "T >= 0"), (dict(Hkv=0), "head"), (dict(D=63), "even"), (dict(D=512), "256"),
+    for bad, words in ((dict(dtype=3), "dtype"), (dict(T=-1), "T >= 0"), (dict(T=1 << 26), "too many"), (dict(Hkv=0), "head"), (dict(D=63), "even"), (dict(D=512), "256"),
                        (dict(n_axes=0), "axes"), (dict(n_axes=5), "axes"), (dict(sections=(C.c_int * 4)(33)), "sections"),
                        (dict(sections=(C.c_int * 4)(-1)), "negative"), (dict(sections=(C.c_int * 4)(0)), "sections"),
                        (dict(gq=16), "both"), (dict(), "null pointer")):
@@ -69,7 +69,7 @@ def test_attention_refuses_before_launching():
     for bad, words in ((dict(dtype=0), "fp16 or bf16"), (dict(T=-1), "negative"), (dict(nseq=-1), "negative"), (dict(Hq=3), "multiple"),
                        (dict(Hkv=0), "multiple"), (dict(D=60), "multiple of 8"), (dict(D=136), "128"), (dict(D=0), "multiple of 8"),
                        (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"),
-                       (dict(T=1 << 30, Hq=1 << 20, Hkv=1), "too many"), (dict(), "null pointer")):
+                       (dict(T=1 << 30, Hq=1 << 20, Hkv=1), "too many"), (dict(T=1 << 20, Hq=1 << 12, Hkv=1), "too many"), (dict(), "null pointer")):
         for fn in (lib.simvg_packed_attn_fwd, lib.simvg_packed_attn_bwd):
             _refused(fn, _lib.PackedAttnArgs(**(ok | bad)), words)
     rows = {n: 256 for n in ("plan", "lse", "q", "k", "v", "o")} | {n + s: 64 for n in "qkvo" for s in ("_ts", "_hs")}
@@ -88,7 +88,7 @@ def test_vocab_ce_refuses_before_launching():
     ok = dict(dtype=1, M=4, V=100, K=64, ldx=64, ldw=64)
     ptr = dict(x=256, w=256, target=256, lse=256, loss=256)
     for bad, words in ((dict(dtype=0), "fp16 or bf16"), (dict(M=-1), "M >= 0"), (dict(V=0), "V >= 1"), (dict(K=60), "multiple of 8"), (dict(K=0), "K >= 8"),
-                       (dict(M=1 << 23), "too large"), (dict(ldx=56), "strides"), (dict(ldw=1 << 21), "strides"), (dict(w=None), "16 bytes"),
+                       (dict(M=1 << 23), "too large"), (dict(M=1 << 22, V=1 << 24), "too many"), (dict(ldx=56), "strides"), (dict(ldw=1 << 21), "strides"), (dict(w=None), "16 bytes"),
                        (dict(x=264), "16 bytes"), (dict(target=None), "null pointer"), (dict(lse=None), "null pointer")):
         for fn in (lib.simvg_vocab_ce_fwd, lib.simvg_vocab_ce_bwd):
             _refused(fn, _lib.VocabCeArgs(**(ok | ptr | bad)), words)

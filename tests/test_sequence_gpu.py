@@ -307,6 +307,52 @@ def test_attention_scores_of_minus_infinity():
     assert float((o[1:].float() - o2.float()).abs().max()) <= 4 * R.h(BF16) * float(v.float().abs().max())   # one probability each way
 
 
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("lens,Hq,Hkv", [([300], 2, 1), ([2500], 2, 1), ([70, 200, 65], 12, 4)], ids=["tiles", "parts", "batch"])
+@pytest.mark.parametrize("causal", [True, False])
+def test_attention_tiles_of_minus_infinity(causal, lens, Hq, Hkv, dt):
+    """the first keys of a sequence, whole tiles of them, have scores of -inf: what comes behind them is not lost"""
+    q, k, v, do, cu = attn_case(lens, Hq, Hkv, 64, dt)
+    q, k = q.clone(), k.clone()
+    q[..., 0] = 1
+    skip = 130 if lens[0] > 130 else 64
+    k[:skip, :, 0] = float("-inf")
+    T = sum(lens)
+    plan = ops.packed_plan(cu, T)
+    o, lse = ops.packed_attn_fwd(q, k, v, plan, causal)
+    dq, dk, dv = ops.packed_attn_bwd(q, k, v, o, lse, do, plan, causal)
+    alone = slice(0, skip if causal else 0)                                # rows that see nothing else
+    assert bool(torch.isnan(o[alone]).all()) and bool((lse[:, alone] == float("-inf")).all())
+    # the same rows without those keys, from the definition: a sequence of the rest (causal: from the first that sees it), whose other
+    # rows are those of a sequence that is cut after `skip`
+    cut = [skip, lens[0] - skip, *lens[1:]] if causal else lens
+    kk, vv = k.clone(), v.clone()
+    if causal:
+        kk[:skip, :, 0] = 0
+        ref = R.attention(q, kk, vv, cut, True, 0.125, do)
+        for name, t in dict(o=o, dq=dq, dk=dk, dv=dv).items():
+            rows = slice(skip, T)
+            if name == "dq":                                               # dS 0 times a key of -inf: NaN in that column, by the formula
+                assert R.off(t[rows][..., 1:], ref[name][rows][..., 1:], ref["tol"][name][rows][..., 1:]) <= 1
+            else:
+                assert R.off(t[rows], ref[name][rows], ref["tol"][name][rows]) <= 1, name
+        assert R.off(lse[:, skip:], ref["lse"][:, skip:], ref["tol"]["lse"][:, skip:]) <= 1
+    else:
+        x = q.double(), k.double(), v.double()
+        rows = slice(0, lens[0])
+        for h in range(Hq):
+            Q, K, V = x[0][rows, h], x[1][rows, h // (Hq // Hkv)], x[2][rows, h // (Hq // Hkv)]
+            S = 0.125 * Q @ torch.where(torch.isinf(K), 0.0, K).t()
+            S[:, :skip] = float("-inf")
+            P = S.softmax(-1)
+            # the bound of sequence_ref.attention for o, over the keys that are left
+            size = (0.125 * Q.abs() @ K[skip:].abs().t()).amax(-1) * 72 * R.U + 8 * R.U * (1 + S.logsumexp(-1).abs())
+            tol = (P @ V.abs()) * (R.h(dt) + 2 * size[:, None] + (lens[0] + 64) * R.U) + R.tiny(dt) * V.abs().sum(0) + R.rounded(P @ V, dt)
+            assert R.off(o[rows, h], P @ V, tol) <= 1
+        assert not dv[:skip].any() and not dk[:skip].any()                 # probabilities of 0
+    assert bool(torch.isfinite(dv[skip:]).all()) and bool(torch.isfinite(dk[skip:]).all())
+
+
 def test_attention_a_list_that_is_none_is_loud():
     q, k, v, do, _ = attn_case([100], 2, 1, 32, F16)
     for cu in ([0, 60, 40, 100], [0, 101], [1, 100], [0, -1, 100], [0, 2 ** 31 - 1]):
@@ -553,6 +599,13 @@ def test_refusals():
         a = dict(lse=lse, do=do, dq=None) | bad
         with pytest.raises(E):
             ops.packed_attn_bwd(q, k, v, o, a["lse"], a["do"], plan, dq=a["dq"])
+    for bad in (dict(out=k), dict(out=v)):                                 # results in the operands' memory, and in each other's
+        with pytest.raises(E):
+            ops.packed_attn_fwd(q[:, :2], k, v, plan, out=bad["out"])
+    mine = [torch.empty_like(t) for t in (q, k, v)]
+    for a, b, c in ((q, mine[1], mine[2]), (do, mine[1], mine[2]), (o, mine[1], mine[2]), (mine[0], k, mine[2]), (mine[0], mine[1], mine[1])):
+        with pytest.raises(E):
+            ops.packed_attn_bwd(q, k, v, o, lse, do, plan, dq=a, dk=b, dv=c)
     with pytest.raises(E):
         ops.packed_plan(cu.long(), 10)
     with pytest.raises(E):
