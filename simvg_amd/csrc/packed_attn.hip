@@ -141,6 +141,7 @@ template <int DP, int LDS0> struct Stager {
   unsigned long base;                                        // the next tile's first row
   unsigned step;                                             // bytes from tile to tile
   int row, left;                                             // the lane's row of its first piece; the sequence's rows from the next tile on
+  unsigned place = 0;                                        // added to LDS0, where the buffer's number is no constant
   __device__ __forceinline__ void init(const void* first, long ts, int rows, int D, const char* smem, int wave, int lane) {
     const int r0 = (wave * 1024 + lane * 16) / (DP * 2);
     base = (unsigned long)first;
@@ -171,7 +172,7 @@ template <int DP, int LDS0> struct Stager {
     left -= KT;
   }
   template <int BUF, int... I> __device__ __forceinline__ void issue(u32x4_t b, const unsigned (&o)[PIECES], std::integer_sequence<int, I...>) {
-    (dma16_at<BUF * KT * DP * 2 + I * 4096>(b, lds, o[I]), ...);
+    (dma16_at<BUF * KT * DP * 2 + I * 4096>(b, lds + place, o[I]), ...);
   }
 };
 // What a lane adds to a tile's start for its part of a fragment; everything else of an address is a constant in the instruction.
@@ -508,15 +509,16 @@ __global__ __launch_bounds__(256) void packed_attn_fwd_join_kernel(simvg_packed_
 // ------------------------------------------------------------------------------------------------------------ backward
 // For fp16: delta_i = sum_d dO_id O_id, and the largest norms of dO's and V's rows in a tile and head: |dP_ij| and |delta_i| are at most
 // |dO_i| |V_j|, so with them dS can be brought to where fp16 has all its bits (`grad_power`).  (bf16: the dQ kernel takes delta along.)
-// ws: delta [Hq][T] | norms of dO [tiles][Hq] | norms of V [tiles][Hkv] | the parts' sums, dQ [parts][T][Hq][D], then dK and dV [parts][2][T][Hkv][D]
+// ws: -delta [Hq][T] | lse log2(e) less P's power [Hq][T] | norms of dO [tiles][Hq] | norms of V [tiles][Hkv] | the parts' sums, dQ [parts][T][Hq][D], then dK and dV [parts][2][T][Hkv][D]
 __host__ __device__ __forceinline__ long ws_fixed(int T, int nseq, int Hq, int Hkv) {
-  return ((long)Hq * T + (long)plan_capacity(T, nseq) * (Hq + Hkv) + 3) / 4 * 4;
+  return (2L * Hq * T + (long)plan_capacity(T, nseq) * (Hq + Hkv) + 3) / 4 * 4;
 }
-struct Ws { float *delta, *ndo, *nv; };
+struct Ws { float *less, *lse2, *ndo, *nv; };
 __device__ __forceinline__ Ws ws_of(const simvg_packed_attn_args& a) {
   Ws w;
-  w.delta = a.ws;
-  w.ndo = a.ws + (long)a.Hq * a.T;
+  w.less = a.ws;
+  w.lse2 = a.ws + (long)a.Hq * a.T;
+  w.ndo = w.lse2 + (long)a.Hq * a.T;
   w.nv = w.ndo + (long)plan_capacity(a.T, a.nseq) * a.Hq;
   return w;
 }
@@ -563,7 +565,7 @@ __global__ __launch_bounds__(256) void packed_attn_delta_kernel(simvg_packed_att
       sd += __shfl_xor(sd, o, 64);
       sv += __shfl_xor(sv, o, 64);
     }
-    if (r < n && lane16 == 0) w.delta[(long)h * a.T + row] = d;
+    if (r < n && lane16 == 0) w.less[(long)h * a.T + row] = -d;
     if (__builtin_isfinite(sd)) mdo = fmaxf(mdo, sd);        // a row that is not finite has no gradient that a scale could save
     if (__builtin_isfinite(sv)) mv = fmaxf(mv, sv);
   }
@@ -645,7 +647,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_dq_kernel(s
   const float c = a.scale * LOG2E;
   float lse2 = a.lse[(long)h * a.lse_hs + here] * LOG2E - shift, delta;
   if constexpr (E::kScaled) {
-    delta = ws_of(a).delta[(long)h * a.T + here];
+    delta = -ws_of(a).less[(long)h * a.T + here];
   } else {                                                   // dO's row is here already: delta needs no kernel of its own
     const unsigned short* op = (const unsigned short*)a.o + here * a.o_ts + (long)h * a.o_hs;
     delta = 0.f;
@@ -653,8 +655,9 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_dq_kernel(s
     for (int ks = 0; ks < KS; ++ks)
       delta = dot8<E>(__builtin_bit_cast(u32x4_t, dof[ks]), __builtin_bit_cast(u32x4_t, global_frag(op, ks, a.D, lane)), delta);
     delta = add_halves(delta);
-    if (part == 0 && valid && lane < 32) ws_of(a).delta[(long)h * a.T + here] = delta;
+    if (part == 0 && valid && lane < 32) ws_of(a).less[(long)h * a.T + here] = -delta;
   }
+  if (part == 0 && valid && lane < 32) ws_of(a).lse2[(long)h * a.T + here] = lse2;             // for dK and dV
   arrived(qf);
   arrived(dof);
   arrived(lse2);
@@ -737,14 +740,16 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_dq_kernel(s
                    valid, lane);
 }
 
+constexpr int DKV_STAGES = 4;
 // dK, dV: a workgroup's 128 keys against the tiles of the queries that see them, of all heads that share the key head, one after the
 // other: the sum over heads stays in the accumulators and needs no atomics.  Where that makes few workgroups (long sequences, few key
 // heads) each of them is cut into `parts` of equal length, whose sums in 32 bits go to the workspace and are joined in their order.
 template <class E, int DP, bool CAUSAL>
 __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void packed_attn_dkv_kernel(simvg_packed_attn_args a, int parts) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  __shared__ float red[8], stat[2][2][KT];
-  constexpr int TILE = KT * DP * 2, DB = DP / 32, KS = DP / 16;
+  constexpr bool PIPED = DP == 128;
+  __shared__ float red[8];
+  constexpr int TILE = KT * DP * 2, DB = DP / 32, KS = DP / 16, STAGE = 2 * TILE, STAT0 = DKV_STAGES * STAGE, STAT = 2 * KT * 4;
   const int hk = blockIdx.x % a.Hkv, G = a.Hq / a.Hkv, part = blockIdx.x / a.Hkv % parts, id = blockIdx.x / a.Hkv / parts;
   Tile e;
   if (!plan_entry(a, id, e)) {
@@ -761,42 +766,48 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void packed_attn_dkv_kernel(
   const long here = e.first + min(key, e.len - 1);
   const unsigned short* kp = (const unsigned short*)a.k + here * a.k_ts + (long)hk * a.k_hs;
   const unsigned short* vp = (const unsigned short*)a.v + here * a.v_ts + (long)hk * a.v_hs;
-  const int first = CAUSAL ? e.t * QT / KT : 0, tiles = (e.len + KT - 1) / KT - first;       // tiles of queries, from `first`
-  // step i of G tiles: head hk G + i / tiles, query tile first + i % tiles; this part's are [s0, s1)
+  // Step i of the G heads' tiles: the sequence's tile of queries all - 1 - i / G, head hk G + i % G; this part's are [s0, s1).  From the
+  // last tile backwards, all heads of a tile: the workgroups of a sequence's keys, which all see its end, read the same rows at the same
+  // time and find them in the L2.
+  const int first = CAUSAL ? e.t * QT / KT : 0, all = (e.len + KT - 1) / KT, tiles = all - first;
   const int wave_first = e.t * QT + wave * 32, s0 = (int)((long)G * tiles * part / parts), s1 = (int)((long)G * tiles * (part + 1) / parts);
-  const int steps = s1 - s0, h0 = hk * G + s0 / tiles, t0 = s0 % tiles;
-  const long row_first = e.first + (long)(first + t0) * KT;
+  const int steps = s1 - s0, g0 = s0 % G, t0 = all - 1 - s0 / G;
+  const long row_first = e.first + (long)t0 * KT;
   Stager<DP, 0> gq;
-  Stager<DP, 2 * TILE> gd;
-  gq.init((const unsigned short*)a.q + row_first * a.q_ts + (long)h0 * a.q_hs, a.q_ts, e.len - (first + t0) * KT, a.D, smem, wave, lane);
-  gd.init((const unsigned short*)a.d_o + row_first * a.do_ts + (long)h0 * a.do_hs, a.do_ts, e.len - (first + t0) * KT, a.D, smem, wave, lane);
-  const long q_wrap = a.q_hs * 2 - (long)tiles * gq.step, d_wrap = a.do_hs * 2 - (long)tiles * gd.step;
-  // the rows' lse and delta, one value a thread, are loaded into a register a step ahead: rows past the sequence are zeros with lse
-  // 0, their P stays finite, times 0
-  const bool is_lse = tid < KT;
-  const float* stat_at = (is_lse ? a.lse + h0 * a.lse_hs : ws_of(a).delta + (long)h0 * a.T) + row_first + (tid & (KT - 1));
-  const long stat_wrap = (is_lse ? a.lse_hs : (long)a.T) - (long)tiles * KT;
-  float st0 = 0.f;
-  int load_t = t0;
-  auto issue = [&](auto buf) {
-    constexpr int B = decltype(buf)::value;
-    if (tid < 2 * KT) {
-      st0 = 0.f;
-      if ((tid & (KT - 1)) < gq.left) st0 = *stat_at;
-      stat_at += KT;
+  Stager<DP, TILE> gd;
+  gq.init((const unsigned short*)a.q + row_first * a.q_ts + (long)(hk * G + g0) * a.q_hs, a.q_ts, e.len - t0 * KT, a.D, smem, wave, lane);
+  gd.init((const unsigned short*)a.d_o + row_first * a.do_ts + (long)(hk * G + g0) * a.do_hs, a.do_ts, e.len - t0 * KT, a.D, smem, wave, lane);
+  // from the last head of a tile to the first of the one before (`next` has gone one tile on)
+  const long q_head = a.q_hs * 2 - (long)gq.step, d_head = a.do_hs * 2 - (long)gd.step, q_back = -(long)gq.step - G * (a.q_hs * 2), d_back = -(long)gd.step - G * (a.do_hs * 2);
+  // the rows' lse and delta, from two waves
+  unsigned long stat_at = (unsigned long)((wave ? ws_of(a).less : ws_of(a).lse2) + (long)(hk * G + g0) * a.T + row_first);
+  const long stat_head = a.T * 4L, stat_back = -G * (a.T * 4L) - KT * 4L;
+  const unsigned stat_lds = lds_addr(smem) + STAT0 + wave * KT * 4;
+  int send_g = g0, send_to = 0;                              // of the next step that is sent for: its head and its place
+  auto send = [&] {
+    gq.place = gd.place = send_to * STAGE;
+    if (wave < 2) {
+      const u32x4_t b = {(unsigned)stat_at, (unsigned)(stat_at >> 32) & 0xffffu, DMA_NOTHING - 1, 0x00020000u};
+      dma4(b, stat_lds + send_to * STAT, lane < gq.left ? lane * 4u : DMA_NOTHING);
     }
-    gq.template next<B>();
-    gd.template next<B>();
-    if (++load_t == tiles) {                                 // the next head
-      load_t = 0;
-      gq.base += q_wrap;
-      gd.base += d_wrap;
-      gq.left += tiles * KT;
-      gd.left += tiles * KT;
-      stat_at += stat_wrap;
+    gq.template next<0>();
+    gd.template next<0>();
+    gq.base += q_head;
+    gd.base += d_head;
+    gq.left += KT;
+    gd.left += KT;
+    stat_at += stat_head;
+    if (++send_g == G) {                                     // the tile before
+      send_g = 0;
+      gq.base += q_back;
+      gd.base += d_back;
+      gq.left += KT;
+      gd.left += KT;
+      stat_at += stat_back;
     }
+    if (++send_to == DKV_STAGES) send_to = 0;
   };
-  if (steps > 0) issue(std::integral_constant<int, 0>{});
+  for (int i = 0; i < DKV_STAGES - 1 && i < steps; ++i) send();
   lpx8_t kf[KS], vf[KS];
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) { kf[ks] = global_frag(kp, ks, a.D, lane); vf[ks] = global_frag(vp, ks, a.D, lane); }
@@ -809,23 +820,22 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void packed_attn_dkv_kernel(
 #pragma unroll
   for (int i = 0; i < DB; ++i) { dk[i] = zero16(); dv[i] = zero16(); }
 
-  int row0 = (first + t0) * KT;
-  auto tile = [&](int i, auto which) {
-    constexpr int BUF = decltype(which)::value, Q0 = BUF * TILE, D0 = (2 + BUF) * TILE;
-    char *lq = smem + Q0, *ld = smem + D0;
-    const float *lse = stat[BUF][0], *del = stat[BUF][1];
-    if (tid < 2 * KT) stat[BUF][tid / KT][tid & (KT - 1)] = is_lse ? st0 * LOG2E - shift : st0;
-    dma_wait<0>();
+  int row0 = t0 * KT, g_now = g0, now = 0;                   // of the step that is multiplied: its first row, head and place
+  // A step's tile becomes visible: every wave's pieces are in LDS, nobody reads the one before any more, and to its place goes the one
+  // DKV_STAGES further on
+  auto arrive = [&](int i, int row0, int place) {
+    constexpr int PIECES = 2 * Stager<DP, 0>::PIECES, AHEAD = DKV_STAGES - 2;
+    if (i + AHEAD >= steps) dma_wait<0>();
+    else if (wave < 2) dma_wait<AHEAD * (PIECES + 1)>();
+    else dma_wait<AHEAD * PIECES>();
     wave_barrier_only();
-    if (i + 1 < steps) issue(std::integral_constant<int, (BUF ^ 1)>{});
-    const int from = key - row0;                             // the first row of the tile that sees the lane's key
-    // (rows past the sequence are zeros; times a key of -inf they would be NaN)
-    const int from4 = from - (lane >> 5) * 4, rows4 = e.len - row0 - (lane >> 5) * 4;
-    // (without a mask row0 + KT is always above 0: a branch all the same, or hipcc keeps the operands of two steps at once and spills)
-    const bool mine = row0 + KT > (CAUSAL ? wave_first : 0), whole = row0 + KT <= e.len && (!CAUSAL || row0 >= wave_first + 31);
+    if (i + DKV_STAGES - 1 < steps) send();
     // Rows that are not finite lose nothing by being cleaned before the scores: their lse (of q) or delta (of dO) is not finite either,
     // and carries that to P and dS of every key they see
     if (CAUSAL && row0 < e.t * QT + QT - 1) {
+      char *lq = smem + place * STAGE, *ld = lq + TILE;
+      const bool mine = row0 + KT > wave_first;
+      const int from = key - row0;
       const bool odd_q = tile_nonfinite<E, DP>(lq), odd_d = tile_nonfinite<E, DP>(ld);
       if (odd_d) {
         if (mine) add_nonfinite<E, DP, false>(dv, ld, lane, [&](int j) { return j >= from; });
@@ -836,68 +846,143 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void packed_attn_dkv_kernel(
         tile_clean<E, DP>(lq);
       }
     }
+  };
+  // A block of 32 rows takes A: S and dP; B: P and dS from them, rounded; C: their products into dV and dK, each in N groups of two MFMAs.
+  constexpr int N = DP / 16, PER = 16 / N;
+  lpx8_t x[N], y[N];                                         // operands of q and dO, by rows (A) or columns (C)
+  auto rows = [&](int g, int stage, int qb) {
+    x[g] = at.row(stage, qb, g);
+    y[g] = at.row(stage + TILE, qb, g);
+  };
+  auto cols = [&](int g, int stage, int qb) {
+    x[g] = at.col(stage, qb * 2 + g / DB, g % DB);
+    y[g] = at.col(stage + TILE, qb * 2 + g / DB, g % DB);
+  };
+  auto step = [&](int i) {
+    const int stage = now * STAGE;
+    const float* stat = (const float*)(smem + STAT0 + now * STAT) + (lane >> 5) * 4;
+    // (without a mask row0 + KT is always above 0: a branch all the same, or hipcc keeps the operands of two steps at once and spills)
+    const bool mine = row0 + KT > (CAUSAL ? wave_first : 0), whole = row0 + KT <= e.len && (!CAUSAL || row0 >= wave_first + 31);
+    u32x4_t p[2], ds[2];
+    auto products = [&](int g) {
+      const int rk = g / DB, cb = g % DB;
+      dv[cb] = E::mfma(y[g], __builtin_bit_cast(lpx8_t, p[rk]), dv[cb]);
+      dk[cb] = E::mfma(x[g], __builtin_bit_cast(lpx8_t, ds[rk]), dk[cb]);
+    };
     if (mine) {
-      // one wave to a SIMD (its accumulators and its keys' operands are 192 registers): nobody else covers a wait, so every LDS
-      // read is asked for one step before the products that take it, and the scheduler may not move it back
-      lpx8_t rq[KS], rd[KS];
-      auto rows = [&](int qb) {
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) { rq[ks] = at.row(Q0, qb, ks); rd[ks] = at.row(D0, qb, ks); }
-      };
-      rows(0);
-#pragma unroll
-      for (int qb = 0; qb < 2; ++qb) {
-        f32x16 s = zero16(), dp = zero16();
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          s = E::mfma(rq[ks], kf[ks], s);
-          dp = E::mfma(rd[ks], vf[ks], dp);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        lpx8_t cd[2][DB], cq[2][DB];
-#pragma unroll
-        for (int rk = 0; rk < 2; ++rk)
-#pragma unroll
-          for (int cb = 0; cb < DB; ++cb) { cd[rk][cb] = at.col(D0, qb * 2 + rk, cb); cq[rk][cb] = at.col(Q0, qb * 2 + rk, cb); }
-        __builtin_amdgcn_sched_barrier(0);
+      f32x16 s[2], dp[2];
+      f32x4_t ls[2][4];
+      u32x4_t np[2], nds[2];
+      auto start = [&](int qb) {                             // dP's products start from -delta
+        s[qb] = zero16();
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const f32x4_t ls = *(const f32x4_t*)(lse + qb * 32 + g * 8 + (lane >> 5) * 4);
-          const f32x4_t dl = *(const f32x4_t*)(del + qb * 32 + g * 8 + (lane >> 5) * 4);
+          ls[qb][g] = *(const f32x4_t*)(stat + qb * 32 + g * 8);
+          const f32x4_t d = *(const f32x4_t*)(stat + KT + qb * 32 + g * 8);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int x = 4 * g + r;
-            s[x] = __builtin_amdgcn_exp2f(fmaf(s[x], c, -ls[r]));
-            dp[x] = E::kScaled ? s[x] * ((dp[x] - dl[r]) * up) : s[x] * (dp[x] - dl[r]);
-          }
+          for (int r = 0; r < 4; ++r) dp[qb][4 * g + r] = d[r];
         }
-        if (!whole) {
+      };
+      auto scores = [&](int g, int qb) {
+        s[qb] = E::mfma(x[g], kf[g], s[qb]);
+        dp[qb] = E::mfma(y[g], vf[g], dp[qb]);
+      };
+      auto gradients = [&](int g, int qb) {                  // registers PER g ..
+#pragma unroll
+        for (int r = PER * g; r < PER * (g + 1); r += 2) {
+          const float p0 = __builtin_amdgcn_exp2f(fmaf(s[qb][r], c, -ls[qb][r / 4][r % 4]));
+          const float p1 = __builtin_amdgcn_exp2f(fmaf(s[qb][r + 1], c, -ls[qb][r / 4][r % 4 + 1]));
+          np[r / 8][r % 8 / 2] = E::pack(p0, p1);
+          nds[r / 8][r % 8 / 2] = E::kScaled ? E::pack(p0 * (dp[qb][r] * up), p1 * (dp[qb][r + 1] * up)) : E::pack(p0 * dp[qb][r], p1 * dp[qb][r + 1]);
+        }
+      };
+      auto rounded = [&](int qb) {
+        if (!whole) {                                        // bits, not products: what is masked may be NaN
           stay_a_branch();
+          // the rows of the tile that see the lane's key, up to the sequence's end (rows past it are zeros; times a key of -inf, NaN)
+          const int from4 = (CAUSAL ? key - row0 : 0) - (lane >> 5) * 4, rows4 = e.len - row0 - (lane >> 5) * 4;
 #pragma unroll
-          for (int x = 0; x < 16; ++x)
-            if ((CAUSAL && qb * 32 + reg_row(x) < from4) || qb * 32 + reg_row(x) >= rows4) { s[x] = 0.f; dp[x] = 0.f; }
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        if (qb == 0) rows(1);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int rk = 0; rk < 2; ++rk) {
-          const lpx8_t p = acc_frag<E>(s, rk), ds = acc_frag<E>(dp, rk);
-#pragma unroll
-          for (int cb = 0; cb < DB; ++cb) {
-            dv[cb] = E::mfma(cd[rk][cb], p, dv[cb]);
-            dk[cb] = E::mfma(cq[rk][cb], ds, dk[cb]);
+          for (int r = 0; r < 16; r += 2) {
+            const int row = qb * 32 + reg_row(r);
+            const unsigned m = (row >= from4 && row < rows4 ? 0xffffu : 0u) | (row + 1 >= from4 && row + 1 < rows4 ? 0xffff0000u : 0u);
+            np[r / 8][r % 8 / 2] &= m;
+            nds[r / 8][r % 8 / 2] &= m;
           }
+        }
+        p[0] = np[0]; p[1] = np[1]; ds[0] = nds[0]; ds[1] = nds[1];
+      };
+      if constexpr (PIPED) {
+        start(0);
+#pragma unroll
+        for (int g = 0; g < N; ++g) {
+          scores(g, 0);
+          rows(g, stage, 1);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        start(1);
+#pragma unroll
+        for (int g = 0; g < N; ++g) {
+          scores(g, 1);
+          cols(g, stage, 0);
+          gradients(g, 0);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        rounded(0);
+#pragma unroll
+        for (int g = 0; g < N; ++g) {
+          products(g);
+          cols(g, stage, 1);
+          gradients(g, 1);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        rounded(1);
+      } else {
+#pragma unroll
+        for (int qb = 0; qb < 2; ++qb) {
+#pragma unroll
+          for (int g = 0; g < N; ++g) rows(g, stage, qb);
+          start(0);
+#pragma unroll
+          for (int g = 0; g < N; ++g) scores(g, 0);
+#pragma unroll
+          for (int g = 0; g < N; ++g) cols(g, stage, qb);
+#pragma unroll
+          for (int g = 0; g < N; ++g) gradients(g, 0);
+          rounded(qb);
+#pragma unroll
+          for (int g = 0; g < N; ++g) products(g);
+          stat += 32;
         }
       }
     }
-    row0 += KT;
-    if (row0 >= (first + tiles) * KT) row0 = first * KT;
+    if (++g_now == G) {
+      g_now = 0;
+      row0 -= KT;
+    }
+    if (++now == DKV_STAGES) now = 0;
+    if (i + 1 < steps) arrive(i + 1, row0, now);
+    if constexpr (PIPED) {
+      if (mine) {
+#pragma unroll
+        for (int g = 0; g < N; ++g) {
+          products(g);
+          rows(g, now * STAGE, 0);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      } else {
+#pragma unroll
+        for (int g = 0; g < N; ++g) rows(g, now * STAGE, 0);
+      }
+    }
   };
-  for (int i = 0; i < steps; i += 2) {
-    tile(i, std::integral_constant<int, 0>{});
-    if (i + 1 < steps) tile(i + 1, std::integral_constant<int, 1>{});
+  if (steps > 0) {
+    arrive(0, row0, 0);
+    if constexpr (PIPED) {
+#pragma unroll
+      for (int g = 0; g < N; ++g) rows(g, 0, 0);
+    }
   }
+  for (int i = 0; i < steps; ++i) step(i);
   const auto z = late_args<simvg_packed_attn_args>();
   const float mk = z->scale * __builtin_amdgcn_exp2f(-power - shift), mv = __builtin_amdgcn_exp2f(-shift);
   if (parts == 1) {
@@ -991,13 +1076,15 @@ void join(const simvg_packed_attn_args& a, const float* sums, long stride, int p
                      (unsigned short*)out, ts, hs);
 }
 
+constexpr int dkv_lds(int DP) { return DKV_STAGES * (2 * KT * DP * 2 + 2 * KT * 4); }
+
 template <class E, int DP, bool CAUSAL>
 void attn_launch(const simvg_packed_attn_args& a, bool bwd, hipStream_t s) {
   static std::atomic<unsigned long> done[3] = {{0}, {0}, {0}};               // the tiles of 128 columns and the kernels' own few bytes pass 64 KiB
   if (!bwd) allow_lds((const void*)packed_attn_fwd_kernel<E, DP, CAUSAL>, 4 * KT * DP * 2, done[0]);
   else {
     allow_lds((const void*)packed_attn_dq_kernel<E, DP, CAUSAL>, 4 * KT * DP * 2, done[1]);
-    allow_lds((const void*)packed_attn_dkv_kernel<E, DP, CAUSAL>, 4 * KT * DP * 2, done[2]);
+    allow_lds((const void*)packed_attn_dkv_kernel<E, DP, CAUSAL>, dkv_lds(DP), done[2]);
   }
   const int entries = plan_capacity(a.T, a.nseq), lds = 4 * KT * DP * 2, rparts = row_parts(a.T, a.nseq, a.Hq, a.causal);
   if (!bwd) {
@@ -1011,7 +1098,7 @@ void attn_launch(const simvg_packed_attn_args& a, bool bwd, hipStream_t s) {
   hipLaunchKernelGGL((packed_attn_dq_kernel<E, DP, CAUSAL>), dim3(entries * a.Hq * rparts), dim3(256), lds, s, a, rparts);
   if (rparts > 1) join<E>(a, sums, (long)a.T * a.Hq * a.D, rparts, a.Hq, a.dq, a.dq_ts, a.dq_hs, s);
   const int kparts = key_parts(a.T, a.nseq, a.Hq, a.Hkv, a.causal);
-  hipLaunchKernelGGL((packed_attn_dkv_kernel<E, DP, CAUSAL>), dim3(entries * a.Hkv * kparts), dim3(256), lds, s, a, kparts);
+  hipLaunchKernelGGL((packed_attn_dkv_kernel<E, DP, CAUSAL>), dim3(entries * a.Hkv * kparts), dim3(256), dkv_lds(DP), s, a, kparts);
   if (kparts > 1) {
     const long n = (long)a.T * a.Hkv * a.D;
     join<E>(a, sums, 2 * n, kparts, a.Hkv, a.dk, a.dk_ts, a.dk_hs, s);

@@ -59,6 +59,10 @@ __device__ __forceinline__ void dma16_at(u32x4_t buffer, unsigned lds, unsigned 
   asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(buffer), "n"(PLUS)
                : "memory", "m0", "scc");
 }
+// 4 bytes a lane: LDS bytes [lds, lds + 256)
+__device__ __forceinline__ void dma4(u32x4_t buffer, unsigned lds, unsigned offset) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(buffer) : "memory", "m0");
+}
 // The kernel's arguments read again from the kernarg segment: what only the end of a kernel needs does not sit in scalar registers
 // through its loop (hipcc loads all arguments at the start and then spills them)
 template <class A>
