@@ -290,6 +290,10 @@ __device__ __forceinline__ void add_nonfinite(f32x16 (&acc)[DP / 32], const char
   }
 }
 
+// Workgroup j of the Hq of a tile runs on XCD j mod 8 if 8 divides Hq: heads that share a key head go to the same one, whose L2 then
+// holds that head's k and v and not everybody's
+__device__ __forceinline__ int head_of(int j, int Hq) { return Hq % 8 ? j : j % 8 * (Hq / 8) + j / 8; }
+
 struct Tile { int first, len, t, base; };
 __device__ __forceinline__ bool plan_entry(const simvg_packed_attn_args& a, int id, Tile& e) {
   if (id >= a.plan[0]) return false;
@@ -339,7 +343,7 @@ template <class E, int DP, bool CAUSAL>
 __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_fwd_kernel(simvg_packed_attn_args a, int parts) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   constexpr int TILE = KT * DP * 2, DB = DP / 32, KS = DP / 16;
-  const int h = blockIdx.x % a.Hq, part = blockIdx.x / a.Hq % parts, id = blockIdx.x / a.Hq / parts;
+  const int h = head_of(blockIdx.x % a.Hq, a.Hq), part = blockIdx.x / a.Hq % parts, id = blockIdx.x / a.Hq / parts;
   Tile e;
   if (!plan_entry(a, id, e)) {
     if (part == 0) fill_tail(a, id, a.o, a.o_ts, a.o_hs, h, a.lse);
@@ -608,7 +612,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_dq_kernel(s
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ float red[8];
   constexpr int TILE = KT * DP * 2, DB = DP / 32, KS = DP / 16;
-  const int h = blockIdx.x % a.Hq, part = blockIdx.x / a.Hq % parts, id = blockIdx.x / a.Hq / parts;
+  const int h = head_of(blockIdx.x % a.Hq, a.Hq), part = blockIdx.x / a.Hq % parts, id = blockIdx.x / a.Hq / parts;
   Tile e;
   if (!plan_entry(a, id, e)) {
     if (part == 0) fill_tail(a, id, a.dq, a.dq_ts, a.dq_hs, h, nullptr);
