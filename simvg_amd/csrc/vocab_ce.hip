@@ -459,7 +459,26 @@ __device__ __forceinline__ float row16_sum(float v) {
   return dpp_add<0x140>(v);                                  // the other eight (row_mirror)
 }
 
-constexpr int e_ld(int words) { return words * 2 + 16; }       // bytes of a row of a wave's block of e in LDS
+// A wave's block, WB rows (lanes) of WA values (registers) times `mul`, through LDS at `mine`, so that rows leave in whole lines (from the
+// registers they would leave in halves of 16 bytes): store(row, first column, eight values).  Rows there are 16 bytes longer than the values.
+constexpr int e_ld(int values) { return values * 2 + 16; }
+template <class E, int WA, int WB, class Store>
+__device__ __forceinline__ void block_rows(const f32x16 (&acc)[WA / 32][WB / 32], float mul, char* mine, int lane, Store store) {
+  constexpr int LD = e_ld(WA), PER = WA / 8, ROWS = 64 / PER;  // lanes to a row, rows at a time
+#pragma unroll
+  for (int j = 0; j < WB / 32; ++j)
+#pragma unroll
+    for (int i = 0; i < WA / 32; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *(u32x2_t*)(mine + (j * 32 + (lane & 31)) * LD + (i * 32 + q * 8 + (lane >> 5) * 4) * 2) =
+            (u32x2_t){E::pack(acc[i][j][4 * q] * mul, acc[i][j][4 * q + 1] * mul), E::pack(acc[i][j][4 * q + 2] * mul, acc[i][j][4 * q + 3] * mul)};
+#pragma unroll 4
+  for (int r = 0; r < WB; r += ROWS) {
+    const int row = r + lane / PER, col = lane % PER * 8;
+    store(row, col, *(const u32x4_t*)(mine + row * LD + col * 2));
+  }
+}
 
 // (1) words in registers, kept rows in lanes: e of words [v_begin, v_begin + piece), and db's sums over the wave's rows
 template <class E, int RA, int RB, int WA, int WB, int STAGES, bool BIAS>
@@ -550,24 +569,10 @@ __global__ __launch_bounds__((RA / WA) * (RB / WB) * 64, 2) void ce_e_kernel(sim
         if ((lane & 31) == 0 && v < a.V && m0 + wm < kept) db[(long)((m0 + wm) / WB) * a.V + v] = s * down;
       }
   }
-  // through LDS, so that a row's words leave in whole lines: [row of the wave][WA words], rows 16 bytes longer than the words
-  constexpr int LD = e_ld(WA);
-  char* mine = smem + wave * WB * LD;
-#pragma unroll
-  for (int j = 0; j < P::NB; ++j)
-#pragma unroll
-    for (int i = 0; i < P::NA; ++i)
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        *(u32x2_t*)(mine + (j * 32 + (lane & 31)) * LD + (i * 32 + q * 8 + (lane >> 5) * 4) * 2) =
-            (u32x2_t){E::pack(acc[i][j][4 * q], acc[i][j][4 * q + 1]), E::pack(acc[i][j][4 * q + 2], acc[i][j][4 * q + 3])};
-  constexpr int PER = WA / 8, ROWS = 64 / PER;               // lanes to a row, rows at a time
-#pragma unroll 4
-  for (int r = 0; r < WB; r += ROWS) {
-    const int row = r + lane / PER, m = m0 + wm + row;
-    const u32x4_t v = *(const u32x4_t*)(mine + row * LD + lane % PER * 16);
-    if (m < kept) *(u32x4_t*)(e + (long)m * piece + l0 + wl + lane % PER * 8) = v;
-  }
+  block_rows<E, WA, WB>(acc, 1.f, smem + wave * WB * e_ld(WA), lane, [&](int row, int col, u32x4_t v) {
+    const int m = m0 + wm + row;
+    if (m < kept) *(u32x4_t*)(e + (long)m * piece + l0 + wl + col) = v;
+  });
 }
 // (2) K in registers, rows in lanes: the piece's share of dx into this split's sums
 template <class E, int RB, int WA, int WB, int STAGES>
@@ -632,21 +637,9 @@ __global__ __launch_bounds__(512, 2) void ce_dw_kernel(simvg_vocab_ce_args a, co
   P::run(acc, oa, ob, cdiv(kept, BK));
   const int wk = k0 + P::wave_a(wave), wl = l0 + P::wave_b(wave);
   const float mul = head->gmax / e_scale<E>();
-#pragma unroll
-  for (int j = 0; j < P::NB; ++j) {
-    const int v = wl + j * 32 + (lane & 31);
-    if (v >= words) continue;
-    unsigned short* out = (unsigned short*)a.dw + (long)(v_begin + v) * a.lddw;
-#pragma unroll
-    for (int i = 0; i < P::NA; ++i)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int k = wk + i * 32 + g * 8 + (lane >> 5) * 4;
-        if (k < a.K)
-          *(u32x2_t*)(out + k) = (u32x2_t){E::pack(acc[i][j][4 * g] * mul, acc[i][j][4 * g + 1] * mul),
-                                           E::pack(acc[i][j][4 * g + 2] * mul, acc[i][j][4 * g + 3] * mul)};
-      }
-  }
+  block_rows<E, 128, 64>(acc, mul, smem + wave * 64 * e_ld(128), lane, [&](int row, int col, u32x4_t v) {
+    if (wl + row < words && wk + col < a.K) *(u32x4_t*)((unsigned short*)a.dw + (long)(v_begin + wl + row) * a.lddw + wk + col) = v;
+  });
 }
 // dx: the splits' sums, and zeros for the rows that take no part
 template <class E>
@@ -761,7 +754,7 @@ int ce_bwd(const simvg_vocab_ce_args& a, hipStream_t s) {
       CE_LAUNCH(P2::THREADS, P2::LDS, (ce_dx_kernel<E, 256, 128, 64, 2>), p.grid_dx, a, head, e, p.piece, v, sums);
     }
     using P3 = Product<E, 256, true, 256, true, 128, 64, 2>;
-    CE_LAUNCH(P3::THREADS, P3::LDS, ce_dw_kernel<E>, tk * cdiv(words, 256), a, head, xs, e, p.piece, v);
+    CE_LAUNCH(P3::THREADS, max(P3::LDS, P3::WAVES * 64 * e_ld(128)), ce_dw_kernel<E>, tk * cdiv(words, 256), a, head, xs, e, p.piece, v);
   };
   for (int v = 0; v < a.V; v += p.piece) {
     if (a.bias) piece(std::true_type{}, v); else piece(std::false_type{}, v);
