@@ -385,8 +385,11 @@ Plan ce_plan(int M, int V, int K, bool bias) {
   return p;
 }
 // dx is kept x K: few tiles.  A piece's words are shared out in `splits`, so that each of the chip's 256 compute units has a tile, of 256
-// words at least
-__device__ __forceinline__ int dx_splits(int grid, int tiles, int piece) { return max(1, min(grid / max(1, tiles), piece / 256)); }
+// words at least, and eights of them go to the eight XCDs: the tiles of a split read the same words and e, through one L2
+__device__ __forceinline__ int dx_splits(int grid, int tiles, int piece) {
+  const int n = max(1, min(grid / max(1, tiles), piece / 256));
+  return n < 8 ? n : n & ~7;
+}
 
 // the list of the rows that take part, in their order: one workgroup, a stretch of rows to a thread
 __global__ __launch_bounds__(1024) void ce_rows_kernel(simvg_vocab_ce_args a, Head* head, int* list, int* place, float* factor) {
@@ -574,6 +577,7 @@ __global__ __launch_bounds__((RA / WA) * (RB / WB) * 64, 2) void ce_e_kernel(sim
     if (m < kept) *(u32x4_t*)(e + (long)m * piece + l0 + wl + col) = v;
   });
 }
+constexpr int dx_ld(int values) { return values * 4 + 16; }    // bytes of a row of a wave's sums in LDS
 // (2) K in registers, rows in lanes: the piece's share of dx into this split's sums
 template <class E, int RB, int WA, int WB, int STAGES>
 __global__ __launch_bounds__((256 / WA) * (RB / WB) * 64, 2) void ce_dx_kernel(simvg_vocab_ce_args a, const Head* head,
@@ -583,8 +587,16 @@ __global__ __launch_bounds__((256 / WA) * (RB / WB) * 64, 2) void ce_dx_kernel(s
   const int kept = head->kept, tk = cdiv(a.K, 256), tm = cdiv(kept, RB), tiles = tk * tm, splits = dx_splits(gridDim.x, tiles, piece);
   if ((int)blockIdx.x >= tiles * splits) return;
   int ik, im;
-  const int split = blockIdx.x / tiles;
-  tile_of(blockIdx.x % tiles, tiles, tm, tk, tk, im, ik);
+  int split, slot = blockIdx.x / 8;
+  if (splits >= 8) {
+    split = slot / tiles * 8 + blockIdx.x % 8;
+    slot %= tiles;
+    im = slot / tk;
+    ik = slot % tk;
+  } else {
+    split = blockIdx.x / tiles;
+    tile_of(blockIdx.x % tiles, tiles, tm, tk, tk, im, ik);
+  }
   const int k0 = ik * 256, m0 = im * RB, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   f32x16 acc[P::NA][P::NB];
   P::zero(acc);
@@ -598,21 +610,26 @@ __global__ __launch_bounds__((256 / WA) * (RB / WB) * 64, 2) void ce_dx_kernel(s
   ob.init_reads(smem + P::B_AT, P::wave_b(wave) / 32, lane);
   P::run(acc, oa, ob, s1 - s0);
   const int wk = k0 + P::wave_a(wave), wm = m0 + P::wave_b(wave);
+  // through LDS, so that rows leave in whole lines, 32 of the wave at a time
+  constexpr int LD = dx_ld(WA), PER = WA / 4, ROWS = 64 / PER;
+  char* mine = smem + wave * 32 * LD;
 #pragma unroll
   for (int j = 0; j < P::NB; ++j) {
-    const int m = wm + j * 32 + (lane & 31);
-    if (m >= kept) continue;
 #pragma unroll
     for (int i = 0; i < P::NA; ++i)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int k = wk + i * 32 + g * 8 + (lane >> 5) * 4;
-        if (k >= a.K) continue;
-        f32x4_t* at = (f32x4_t*)(sums + ((long)split * kept + m) * a.K + k);
-        f32x4_t v = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
-        if (v_begin > 0) v += *at;
-        *at = v;
-      }
+      for (int g = 0; g < 4; ++g)
+        *(f32x4_t*)(mine + (lane & 31) * LD + (i * 32 + g * 8 + (lane >> 5) * 4) * 4) =
+            (f32x4_t){acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+#pragma unroll 4
+    for (int r = 0; r < 32; r += ROWS) {
+      const int row = r + lane / PER, m = wm + j * 32 + row, k = wk + lane % PER * 4;
+      f32x4_t v = *(const f32x4_t*)(mine + row * LD + lane % PER * 16);
+      if (m >= kept || k >= a.K) continue;
+      f32x4_t* at = (f32x4_t*)(sums + ((long)split * kept + m) * a.K + k);
+      if (v_begin > 0) v += *at;
+      *at = v;
+    }
   }
 }
 // (3) K in registers, words in lanes: the piece's rows of dw
@@ -742,7 +759,7 @@ int ce_bwd(const simvg_vocab_ce_args& a, hipStream_t s) {
     if (p.small) {
       using P1 = Product<E, 128, false, 64, false, 32, 64, 3>;
       using P2 = Product<E, 256, true, 64, false, 64, 64, 2>;
-      static_assert(P1::WAVES * 64 * e_ld(32) <= P1::LDS, "the waves' blocks of e");
+      static_assert(P1::WAVES * 64 * e_ld(32) <= P1::LDS && P2::WAVES * 32 * dx_ld(64) <= P2::LDS, "the waves' blocks of results");
       CE_LAUNCH(P1::THREADS, P1::LDS, (ce_e_kernel<E, 128, 64, 32, 64, 3, B>), p.piece / 128, a, head, list, factor, xk, e, p.piece, v, db);
       CE_LAUNCH(P2::THREADS, P2::LDS, (ce_dx_kernel<E, 64, 64, 64, 2>), p.grid_dx, a, head, e, p.piece, v, sums);
     } else {
@@ -751,7 +768,7 @@ int ce_bwd(const simvg_vocab_ce_args& a, hipStream_t s) {
       constexpr int lds = P1::WAVES * 64 * e_ld(128) > P1::LDS ? P1::WAVES * 64 * e_ld(128) : P1::LDS;
       CE_LAUNCH(P1::THREADS, lds, (ce_e_kernel<E, 256, 256, 128, 64, 2, B>), cdiv(a.M, 256) * (p.piece / 256), a, head, list, factor, xk, e,
                 p.piece, v, db);
-      CE_LAUNCH(P2::THREADS, P2::LDS, (ce_dx_kernel<E, 256, 128, 64, 2>), p.grid_dx, a, head, e, p.piece, v, sums);
+      CE_LAUNCH(P2::THREADS, max(P2::LDS, P2::WAVES * 32 * dx_ld(128)), (ce_dx_kernel<E, 256, 128, 64, 2>), p.grid_dx, a, head, e, p.piece, v, sums);
     }
     using P3 = Product<E, 256, true, 256, true, 128, 64, 2>;
     CE_LAUNCH(P3::THREADS, max(P3::LDS, P3::WAVES * 64 * e_ld(128)), ce_dw_kernel<E>, tk * cdiv(words, 256), a, head, xs, e, p.piece, v);
