@@ -232,6 +232,27 @@ __device__ __forceinline__ void tile_of(int id, int n, int outer, int inner, int
 // a row takes part if its target is a word; otherwise (ignored, or no word at all) its gradient is nothing
 __device__ __forceinline__ bool is_word(const simvg_vocab_ce_args& a, long t) { return t != a.ignore_index && t >= 0 && t < a.V; }
 
+// the words' bias: to LDS before the products, and added behind them (64 loads a lane, whose wait nothing covers there, are 16 reads)
+template <int RA>
+__device__ __forceinline__ void bias_to_lds(const simvg_vocab_ce_args& a, int v0, const char* to, int wave, int lane) {
+  const unsigned long p = (unsigned long)(a.bias + v0);
+  const u32x4_t b = {(unsigned)p, (unsigned)(p >> 32) & 0xffffu, DMA_NOTHING - 1, 0x00020000u};
+  if (wave < RA / 64) dma4(b, lds_addr(to) + wave * 256, v0 + wave * 64 + lane < a.V ? (wave * 64 + lane) * 4u : DMA_NOTHING);
+}
+template <int NA, int NB>
+__device__ __forceinline__ void add_bias(f32x16 (&acc)[NA][NB], const char* from, int lane) {       // from: the wave's first word's
+#pragma unroll
+  for (int i = 0; i < NA; ++i)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const f32x4_t b = *(const f32x4_t*)(from + (i * 32 + q * 8 + (lane >> 5) * 4) * 4);
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[i][j][4 * q + r] += b[r];
+    }
+}
+
 // ------------------------------------------------------------------------------------------------------------- forward
 // words in registers, rows in lanes: [tile of RA words][M] (maximum, sum of exp2) and the targets' logits
 template <class E, int RA, int RB, int WA, int WB, int STAGES>
@@ -250,18 +271,10 @@ __global__ __launch_bounds__((RA / WA) * (RB / WB) * 64, 2) void ce_fwd_kernel(s
   ob.init_stages((const unsigned short*)a.x + (long)m0 * a.ldx, a.ldx, min(RB, a.M - m0), a.K, smem + P::B_AT, wave, lane);
   oa.init_reads(smem, P::wave_a(wave) / 32, lane);
   ob.init_reads(smem + P::B_AT, P::wave_b(wave) / 32, lane);
+  if (a.bias) bias_to_lds<RA>(a, v0, smem + P::LDS, wave, lane);
   P::run(acc, oa, ob, cdiv(a.K, BK));
   const int wv = v0 + P::wave_a(wave), wm = P::wave_b(wave);
-  if (a.bias) {
-#pragma unroll
-    for (int i = 0; i < P::NA; ++i)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float b = a.bias[min(wv + i * 32 + acc_row(r, lane), a.V - 1)];
-#pragma unroll
-        for (int j = 0; j < P::NB; ++j) acc[i][j][r] += b;
-      }
-  }
+  if (a.bias) add_bias(acc, smem + P::LDS + P::wave_a(wave) * 4, lane);
   if (wv + WA > a.V) {
     stay_a_branch();
 #pragma unroll
@@ -465,6 +478,7 @@ __device__ __forceinline__ float row16_sum(float v) {
 // A wave's block, WB rows (lanes) of WA values (registers) times `mul`, through LDS at `mine`, so that rows leave in whole lines (from the
 // registers they would leave in halves of 16 bytes): store(row, first column, eight values).  Rows there are 16 bytes longer than the values.
 constexpr int e_ld(int values) { return values * 2 + 16; }
+constexpr int max_of(int x, int y) { return x > y ? x : y; }
 template <class E, int WA, int WB, class Store>
 __device__ __forceinline__ void block_rows(const f32x16 (&acc)[WA / 32][WB / 32], float mul, char* mine, int lane, Store store) {
   constexpr int LD = e_ld(WA), PER = WA / 8, ROWS = 64 / PER;  // lanes to a row, rows at a time
@@ -483,6 +497,8 @@ __device__ __forceinline__ void block_rows(const f32x16 (&acc)[WA / 32][WB / 32]
   }
 }
 
+template <class P> constexpr int e_lds() { return max_of(P::LDS, P::WAVES * P::NB * 32 * e_ld(P::NA * 32)); }      // of (1), without the bias
+
 // (1) words in registers, kept rows in lanes: e of words [v_begin, v_begin + piece), and db's sums over the wave's rows
 template <class E, int RA, int RB, int WA, int WB, int STAGES, bool BIAS>
 __global__ __launch_bounds__((RA / WA) * (RB / WB) * 64, 2) void ce_e_kernel(simvg_vocab_ce_args a, const Head* head, const int* list,
@@ -490,6 +506,7 @@ __global__ __launch_bounds__((RA / WA) * (RB / WB) * 64, 2) void ce_e_kernel(sim
                                                                              int piece, int v_begin, float* db) {
   using P = Product<E, RA, false, RB, false, WA, WB, STAGES>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
+  constexpr int BIAS_AT = e_lds<P>();
   const int kept = head->kept, tv = piece / RA, tm = cdiv(kept, RB);
   if ((int)blockIdx.x >= tv * tm) return;
   int iv, im;
@@ -505,7 +522,9 @@ __global__ __launch_bounds__((RA / WA) * (RB / WB) * 64, 2) void ce_e_kernel(sim
     ob.init_stages(xk + (long)m0 * a.K, a.K, min(RB, kept - m0), a.K, smem + P::B_AT, wave, lane);
     oa.init_reads(smem, P::wave_a(wave) / 32, lane);
     ob.init_reads(smem + P::B_AT, P::wave_b(wave) / 32, lane);
+    if (BIAS) bias_to_lds<RA>(a, v0, smem + BIAS_AT, wave, lane);
     P::run(acc, oa, ob, cdiv(a.K, BK));
+    if (BIAS) add_bias(acc, smem + BIAS_AT + P::wave_a(wave) * 4, lane);
   }
   const int wl = P::wave_a(wave), wv = v0 + wl, wm = P::wave_b(wave);
   float less[P::NB], g[P::NB];
@@ -520,16 +539,6 @@ __global__ __launch_bounds__((RA / WA) * (RB / WB) * 64, 2) void ce_e_kernel(sim
     g[j] = BIAS && on ? factor[r] : 0.f;
     local[j] = on && t >= wv && t < wv + WA ? (int)(t - wv) : -1;
     any = any || local[j] >= 0;
-  }
-  if (BIAS) {
-#pragma unroll
-    for (int i = 0; i < P::NA; ++i)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float b = a.bias[min(wv + i * 32 + acc_row(r, lane), a.V - 1)];
-#pragma unroll
-        for (int j = 0; j < P::NB; ++j) acc[i][j][r] += b;
-      }
   }
 #pragma unroll
   for (int i = 0; i < P::NA; ++i)
@@ -723,10 +732,10 @@ int ce_fwd(const simvg_vocab_ce_args& a, hipStream_t s) {
   float2* part = (float2*)((char*)a.ws + (a.M * 4L + 255) / 256 * 256);
   if (a.M <= SMALL_M) {                                      // a row of tiles, bound by reading w: twice as many, half as high, two to a compute unit
     using P = Product<E, 128, false, 64, false, 32, 64, 3>;
-    CE_LAUNCH(P::THREADS, P::LDS, (ce_fwd_kernel<E, 128, 64, 32, 64, 3>), groups, a, part, zt);
+    CE_LAUNCH(P::THREADS, P::LDS + 128 * 4, (ce_fwd_kernel<E, 128, 64, 32, 64, 3>), groups, a, part, zt);
   } else {
     using P = Product<E, 256, false, 256, false, 128, 64, 2>;
-    CE_LAUNCH(P::THREADS, P::LDS, (ce_fwd_kernel<E, 256, 256, 128, 64, 2>), groups * cdiv(a.M, 256), a, part, zt);
+    CE_LAUNCH(P::THREADS, P::LDS + 256 * 4, (ce_fwd_kernel<E, 256, 256, 128, 64, 2>), groups * cdiv(a.M, 256), a, part, zt);
   }
   SIMVG_LAUNCH_CHECK();
   hipLaunchKernelGGL(ce_join_kernel, dim3(cdiv(a.M, 8)), dim3(1024), 0, s, a, part, zt, groups);
@@ -759,19 +768,18 @@ int ce_bwd(const simvg_vocab_ce_args& a, hipStream_t s) {
     if (p.small) {
       using P1 = Product<E, 128, false, 64, false, 32, 64, 3>;
       using P2 = Product<E, 256, true, 64, false, 64, 64, 2>;
-      static_assert(P1::WAVES * 64 * e_ld(32) <= P1::LDS && P2::WAVES * 32 * dx_ld(64) <= P2::LDS, "the waves' blocks of results");
-      CE_LAUNCH(P1::THREADS, P1::LDS, (ce_e_kernel<E, 128, 64, 32, 64, 3, B>), p.piece / 128, a, head, list, factor, xk, e, p.piece, v, db);
+      static_assert(P2::WAVES * 32 * dx_ld(64) <= P2::LDS, "the waves' blocks of results");
+      CE_LAUNCH(P1::THREADS, e_lds<P1>() + 128 * 4, (ce_e_kernel<E, 128, 64, 32, 64, 3, B>), p.piece / 128, a, head, list, factor, xk, e, p.piece, v, db);
       CE_LAUNCH(P2::THREADS, P2::LDS, (ce_dx_kernel<E, 64, 64, 64, 2>), p.grid_dx, a, head, e, p.piece, v, sums);
     } else {
       using P1 = Product<E, 256, false, 256, false, 128, 64, 2>;
       using P2 = Product<E, 256, true, 256, false, 128, 64, 2>;
-      constexpr int lds = P1::WAVES * 64 * e_ld(128) > P1::LDS ? P1::WAVES * 64 * e_ld(128) : P1::LDS;
-      CE_LAUNCH(P1::THREADS, lds, (ce_e_kernel<E, 256, 256, 128, 64, 2, B>), cdiv(a.M, 256) * (p.piece / 256), a, head, list, factor, xk, e,
+      CE_LAUNCH(P1::THREADS, e_lds<P1>() + 256 * 4, (ce_e_kernel<E, 256, 256, 128, 64, 2, B>), cdiv(a.M, 256) * (p.piece / 256), a, head, list, factor, xk, e,
                 p.piece, v, db);
-      CE_LAUNCH(P2::THREADS, max(P2::LDS, P2::WAVES * 32 * dx_ld(128)), (ce_dx_kernel<E, 256, 128, 64, 2>), p.grid_dx, a, head, e, p.piece, v, sums);
+      CE_LAUNCH(P2::THREADS, max_of(P2::LDS, P2::WAVES * 32 * dx_ld(128)), (ce_dx_kernel<E, 256, 128, 64, 2>), p.grid_dx, a, head, e, p.piece, v, sums);
     }
     using P3 = Product<E, 256, true, 256, true, 128, 64, 2>;
-    CE_LAUNCH(P3::THREADS, max(P3::LDS, P3::WAVES * 64 * e_ld(128)), ce_dw_kernel<E>, tk * cdiv(words, 256), a, head, xs, e, p.piece, v);
+    CE_LAUNCH(P3::THREADS, max_of(P3::LDS, P3::WAVES * 64 * e_ld(128)), ce_dw_kernel<E>, tk * cdiv(words, 256), a, head, xs, e, p.piece, v);
   };
   for (int v = 0; v < a.V; v += p.piece) {
     if (a.bias) piece(std::true_type{}, v); else piece(std::false_type{}, v);
