@@ -12,6 +12,13 @@
 // lane already has -- the order of the contraction's keys is free, and the transposed reads (ds_read_b64_tr_b16) that fetch V^T use
 // the order in which the accumulator holds them.  P and dS never leave registers.
 //
+// Measured, of 1.46 (fp16) and 1.44 (bf16) PFLOP/s that a library product of 8192^3 reaches: one sequence of 16384 rows, 16 heads of 128
+// on 2, causal, bf16, forward 1.01 ms, 1.09 PFLOP/s; nine of up to 4097 rows, 32 heads on 8: forward 0.49 ms, 0.92; dQ 0.72 ms and dK, dV
+// 1.04 ms, 0.94 and 0.87 of what each computes (6 D and 8 D: both need the scores).  Half of the time the matrix pipes work (the clock
+// falls to 1.7 GHz under them), a third goes to the exponentials and the rest of the vector work, which one or two waves to a SIMD
+// cover in part.  Heads of 64 (64 x 411 rows, 12 heads, no mask, fp16): forward 73 us, dQ 94, dK and dV 134: vector work, as much
+// for half the products.
+//
 // Which rows a workgroup takes stands in a plan that the caller has built once for a batch (packed_plan_kernel): one entry for each
 // tile of 128 rows of each sequence, tiles far down a sequence first, because under `causal` they cost most and the last workgroups to
 // start should be the short ones.
@@ -296,10 +303,11 @@ __device__ __forceinline__ int head_of(int j, int Hq) { return Hq % 8 ? j : j % 
 
 struct Tile { int first, len, t, base; };
 __device__ __forceinline__ bool plan_entry(const simvg_packed_attn_args& a, int id, Tile& e) {
-  if (id >= a.plan[0]) return false;
-  const int* p = a.plan + PLAN_HEAD + 4 * id;
-  e.first = p[0]; e.len = p[1]; e.t = p[2]; e.base = p[3];
-  return true;
+  const int* p = a.plan + PLAN_HEAD + 4 * id;                // the grid is as long as the table: the entry is read beside the count
+  int n = a.plan[0], first = p[0], len = p[1], t = p[2], base = p[3];
+  asm volatile("" : "+s"(n), "+s"(first), "+s"(len), "+s"(t), "+s"(base));
+  e.first = first; e.len = len; e.t = t; e.base = base;
+  return id < n;
 }
 // a workgroup without an entry: its tile of the rows behind the last sequence, zeros; NaN everywhere where there is no valid plan
 __device__ __forceinline__ void fill_tail(const simvg_packed_attn_args& a, int id, void* out, long ts, long hs, int h, float* lse) {
@@ -620,7 +628,6 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_dq_kernel(s
   }
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int hk = h / (a.Hq / a.Hkv);
-  const float power = grad_power<E>(a, e, hk, red), up = __builtin_amdgcn_exp2f(power), shift = E::kScaled ? P_POWER : 0.f;
   const int row = e.t * QT + wave * 32 + (lane & 31);
   const bool valid = row < e.len;
   const long here = e.first + min(row, e.len - 1);
@@ -643,6 +650,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_dq_kernel(s
     gk.template next<0>();
     gv.template next<0>();
   }
+  const float power = grad_power<E>(a, e, hk, red), up = __builtin_amdgcn_exp2f(power), shift = E::kScaled ? P_POWER : 0.f;
   lpx8_t qf[KS], dof[KS];
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) { qf[ks] = global_frag(qp, ks, a.D, lane); dof[ks] = global_frag(dop, ks, a.D, lane); }
@@ -744,6 +752,8 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_dq_kernel(s
                    valid, lane);
 }
 
+// Four stages: with two, asked for one tile ahead, a quarter of the time went to waiting for them (documents' backward pass 1842 us,
+// 1630 with the sending left out; 1761 with four stages and the tiles' order below).
 constexpr int DKV_STAGES = 4;
 // dK, dV: a workgroup's 128 keys against the tiles of the queries that see them, of all heads that share the key head, one after the
 // other: the sum over heads stays in the accumulators and needs no atomics.  Where that makes few workgroups (long sequences, few key
@@ -751,8 +761,8 @@ constexpr int DKV_STAGES = 4;
 template <class E, int DP, bool CAUSAL>
 __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void packed_attn_dkv_kernel(simvg_packed_attn_args a, int parts) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  constexpr bool PIPED = DP == 128;
   __shared__ float red[8];
+  constexpr bool PIPED = DP == 128;
   constexpr int TILE = KT * DP * 2, DB = DP / 32, KS = DP / 16, STAGE = 2 * TILE, STAT0 = DKV_STAGES * STAGE, STAT = 2 * KT * 4;
   const int hk = blockIdx.x % a.Hkv, G = a.Hq / a.Hkv, part = blockIdx.x / a.Hkv % parts, id = blockIdx.x / a.Hkv / parts;
   Tile e;
@@ -764,7 +774,6 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void packed_attn_dkv_kernel(
   const int ntile = (e.len + QT - 1) / QT;
   if (CAUSAL) e.t = ntile - 1 - e.t;                         // the plan's order is by cost: the first keys are seen by the most queries
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-  const float power = grad_power<E>(a, e, hk, red), up = __builtin_amdgcn_exp2f(power), shift = E::kScaled ? P_POWER : 0.f;
   const int key = e.t * QT + wave * 32 + (lane & 31);        // the lane's key
   const bool valid = key < e.len;
   const long here = e.first + min(key, e.len - 1);
@@ -812,6 +821,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void packed_attn_dkv_kernel(
     if (++send_to == DKV_STAGES) send_to = 0;
   };
   for (int i = 0; i < DKV_STAGES - 1 && i < steps; ++i) send();
+  const float power = grad_power<E>(a, e, hk, red), up = __builtin_amdgcn_exp2f(power), shift = E::kScaled ? P_POWER : 0.f;
   lpx8_t kf[KS], vf[KS];
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) { kf[ks] = global_frag(kp, ks, a.D, lane); vf[ks] = global_frag(vp, ks, a.D, lane); }
@@ -852,6 +862,11 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void packed_attn_dkv_kernel(
     }
   };
   // A block of 32 rows takes A: S and dP; B: P and dS from them, rounded; C: their products into dV and dK, each in N groups of two MFMAs.
+  // Heads of 128 leave one wave to a SIMD (its accumulators and its keys' operands are 192 registers): nobody else covers its waits or
+  // its vector work, so a tile's two blocks go through in four phases, A0, A1 beside B0, C0 beside B1, C1, and each group asks for the
+  // operands of its like in the next phase, the last one for the next step's first rows (one block
+  // after the other and two stages: 1150 us for the documents' dK and dV, now 1040).  Smaller heads have two waves to a SIMD,
+  // which cover each other, and no room for the second block's registers: one block after the other.
   constexpr int N = DP / 16, PER = 16 / N;
   lpx8_t x[N], y[N];                                         // operands of q and dO, by rows (A) or columns (C)
   auto rows = [&](int g, int stage, int qb) {
@@ -1026,8 +1041,9 @@ bool in_reach(long ts) { return ts >= 0 && ts < 1L << 24; }
 
 // How many parts a workgroup's work is cut into where a launch has few workgroups: so many that there are two for each of the 256
 // compute units, four under `causal`, where they are of very different length, and each of at least eight tiles on average.  (One
-// sequence of 8192 rows, 4 heads of 128 on 1, causal: forward 156 us uncut and 99 cut, backward 1246 and 351; 2048 rows, 8 heads of 128,
-// no mask: 42 and 40, 133 and 123; 8192 rows, 4 heads, no mask, 256 equal workgroups: 501 us uncut, 519 in three parts.)
+// sequence of 8192 rows, 4 heads of 128 on 1, causal: forward 152 us uncut and 99 cut, backward 1091 and 335; 16384 rows, 16 heads on 2:
+// backward 5.14 and 3.79 ms; 2048 rows, 8 heads of 128, no mask: 41 and 40 us, 124 and 118; 8192 rows, 4 heads, no mask, are 264 equal
+// workgroups and stay uncut: three parts took 519 us where one took 501.)
 int parts_of(long groups, long tiles, int causal) {
   return (int)std::max(1L, std::min(std::min((causal ? 1024 : 512) / groups, tiles / (causal ? 2 : 1) / 8), 32L));
 }

@@ -12,6 +12,11 @@
 // frequency keeps 2^-32 of a turn, in 32 bits it would keep 2^-4) and leave (cos, sin) in LDS for all heads; then groups of lanes
 // take a head's row each, a lane holding the two chunks of 16 bytes whose values are each other's partners, so that nothing but the
 // sum of squares crosses lanes.
+//
+// Measured (a copy of 4 GiB reaches 4.7 TB/s, one that stays in the 256 MB memory-side cache 7.2): 26944 tokens, 24 heads of 64, fp16,
+// forward: 35 us, 4.7 TB/s; 16384 tokens, 40 heads of 128, bf16: forward 56 us, 6.0 TB/s, backward 140 us, 3.6 TB/s (three waves a
+// SIMD: the weights' sums stay in 16 registers a lane and weight, and a wave has one row's loads in flight) + 4 us for the join; one
+// token: 4 us.
 #include "seq.h"
 
 struct simvg_qk_norm_rope_args {
