@@ -14,9 +14,8 @@
 // sum of squares crosses lanes.
 //
 // Measured (a copy of 4 GiB reaches 4.7 TB/s, one that stays in the 256 MB memory-side cache 7.2): 26944 tokens, 24 heads of 64, fp16,
-// forward: 35 us, 4.7 TB/s; 16384 tokens, 40 heads of 128, bf16: forward 56 us, 6.0 TB/s, backward 140 us, 3.6 TB/s (three waves a
-// SIMD: the weights' sums stay in 16 registers a lane and weight, and a wave has one row's loads in flight) + 4 us for the join; one
-// token: 4 us.
+// forward: 35 us, 4.7 TB/s; 16384 tokens, 40 heads of 128, bf16: forward 56 us, 6.0 TB/s, backward 110 us with the join of the weights'
+// gradients, 4.6 TB/s; one token: 4 us.
 #include "seq.h"
 
 struct simvg_qk_norm_rope_args {
@@ -35,7 +34,11 @@ namespace {
 using namespace seq;
 
 constexpr int ROPE_MAX_D = 256;
-constexpr int ROPE_BWD_BLOCKS = 1024;                       // workgroups of the backward pass: one partial sum of (dgq | dgk) each
+// Workgroups of the backward pass, one partial sum of (dgq | dgk) each: as many as the chip holds at once (three to a compute unit with
+// 16-bit values, four with 32-bit ones), each walking its share of the tokens.  16384 tokens, 40 heads of 128, bf16: 110 us with 768, 134
+// with 1024, 121 with 2048; 4099 tokens, fp32: 17.9, 17.0, 18.8.
+constexpr int ROPE_BWD_BLOCKS = 1024;
+int rope_bwd_blocks(int T, int dtype) { return min(cdiv(T, 4), dtype == SEQ_F32 ? ROPE_BWD_BLOCKS : 768); }
 
 // V consecutive values: 16 bytes of 16-bit values, or of 32-bit ones, or a single value
 template <int DT, int V> struct Chunk;
@@ -381,7 +384,7 @@ void rope_launch(const simvg_qk_norm_rope_args& a, int P, bool bwd, hipStream_t 
     const int wpt = a.T < 1024 ? 4 : 1;
     hipLaunchKernelGGL((rope_fwd_kernel<DT, V, LPR, NP>), dim3(cdiv(a.T, 4 / wpt)), dim3(256), 0, s, a, P, wpt);
   } else {
-    hipLaunchKernelGGL((rope_bwd_kernel<DT, V, LPR, NP>), dim3(min(cdiv(a.T, 4), ROPE_BWD_BLOCKS)), dim3(256), 0, s, a, P);
+    hipLaunchKernelGGL((rope_bwd_kernel<DT, V, LPR, NP>), dim3(rope_bwd_blocks(a.T, a.dtype)), dim3(256), 0, s, a, P);
   }
 }
 template <int DT, int V>
@@ -408,7 +411,7 @@ int rope_run(const simvg_qk_norm_rope_args* args, bool bwd, hipStream_t s) {
     SIMVG_LAUNCH_CHECK();
   }
   if (bwd && a.gq) {                                          // without a token the gradients are sums of nothing: zeros
-    hipLaunchKernelGGL(rope_dg_kernel, dim3(cdiv(2 * a.D, 16)), dim3(1024), 0, s, a.ws, min(cdiv(a.T, 4), ROPE_BWD_BLOCKS), a.D, a.dgq, a.dgk);
+    hipLaunchKernelGGL(rope_dg_kernel, dim3(cdiv(2 * a.D, 16)), dim3(1024), 0, s, a.ws, rope_bwd_blocks(a.T, a.dtype), a.D, a.dgq, a.dgk);
     SIMVG_LAUNCH_CHECK();
   }
   return SIMVG_OK;
