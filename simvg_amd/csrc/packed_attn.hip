@@ -13,10 +13,10 @@
 // the order in which the accumulator holds them.  P and dS never leave registers.
 //
 // Measured, of 1.46 (fp16) and 1.44 (bf16) PFLOP/s that a library product of 8192^3 reaches: one sequence of 16384 rows, 16 heads of 128
-// on 2, causal, bf16, forward 1.01 ms, 1.09 PFLOP/s; nine of up to 4097 rows, 32 heads on 8: forward 0.49 ms, 0.92; dQ 0.72 ms and dK, dV
-// 1.04 ms, 0.94 and 0.87 of what each computes (6 D and 8 D: both need the scores).  Half of the time the matrix pipes work (the clock
+// on 2, causal, bf16, forward 1.01 ms, 1.09 PFLOP/s; nine of up to 4097 rows, 32 heads on 8: forward 0.49 ms, 0.92; dQ 0.71 ms and dK, dV
+// 1.06 ms, 0.95 and 0.85 of what each computes (6 D and 8 D: both need the scores).  Half of the time the matrix pipes work (the clock
 // falls to 1.7 GHz under them), a third goes to the exponentials and the rest of the vector work, which one or two waves to a SIMD
-// cover in part.  Heads of 64 (64 x 411 rows, 12 heads, no mask, fp16): forward 73 us, dQ 94, dK and dV 134: vector work, as much
+// cover in part.  Heads of 64 (64 x 411 rows, 12 heads, no mask, fp16): forward 73 us, dQ 95, dK and dV 132: vector work, as much
 // for half the products.
 //
 // Which rows a workgroup takes stands in a plan that the caller has built once for a batch (packed_plan_kernel): one entry for each
@@ -864,8 +864,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void packed_attn_dkv_kernel(
   // A block of 32 rows takes A: S and dP; B: P and dS from them, rounded; C: their products into dV and dK, each in N groups of two MFMAs.
   // Heads of 128 leave one wave to a SIMD (its accumulators and its keys' operands are 192 registers): nobody else covers its waits or
   // its vector work, so a tile's two blocks go through in four phases, A0, A1 beside B0, C0 beside B1, C1, and each group asks for the
-  // operands of its like in the next phase, the last one for the next step's first rows (one block
-  // after the other and two stages: 1150 us for the documents' dK and dV, now 1040).  Smaller heads have two waves to a SIMD,
+  // operands of its like in the next phase, the last one for the next step's first rows.  Smaller heads have two waves to a SIMD,
   // which cover each other, and no room for the second block's registers: one block after the other.
   constexpr int N = DP / 16, PER = 16 / N;
   lpx8_t x[N], y[N];                                         // operands of q and dO, by rows (A) or columns (C)
