@@ -371,7 +371,8 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_fwd_kernel(
   // tiles that no mask touches come first, then those that the diagonal or the sequence's end crosses, then (for the wave) nothing
   const int whole = min(tiles, min(CAUSAL ? (e.t * QT + 1) / KT : tiles, e.len / KT));         // of all four waves
   const int wave_whole = min(CAUSAL ? (wave_first + 1) / KT : tiles, e.len / KT);
-  const int wave_tiles = CAUSAL ? min(tiles, (wave_first + 32 + KT - 1) / KT) : tiles;
+  const bool live = wave_first < e.len;                      // a wave without a row only brings its pieces of the tiles
+  const int wave_tiles = !live ? 0 : CAUSAL ? min(tiles, (wave_first + 32 + KT - 1) / KT) : tiles;
 
   Stager<DP, 0> gk;
   Stager<DP, 2 * TILE> gv;
@@ -404,7 +405,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_fwd_kernel(
       gk.template next<BUF ^ 1>();
       gv.template next<BUF ^ 1>();
     }
-    const bool odd = MASKED && tile_nonfinite<E, DP>(smem + V0), mine = !MASKED || kt < wave_tiles;
+    const bool odd = MASKED && tile_nonfinite<E, DP>(smem + V0), mine = MASKED ? kt < wave_tiles : live;
     const int last = (CAUSAL ? min(row, e.len - 1) : e.len - 1) - kt * KT;     // of the tile's keys, the last that the lane's query sees
     const int last4 = last - (lane >> 5) * 4;                // against a register's constant
     f32x16 s[2];
@@ -641,7 +642,8 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_dq_kernel(s
   const int wave_first = e.t * QT + wave * 32;
   const int whole = min(tiles, min(CAUSAL ? (e.t * QT + 1) / KT : tiles, e.len / KT));         // of all four waves
   const int wave_whole = min(CAUSAL ? (wave_first + 1) / KT : tiles, e.len / KT);
-  const int wave_tiles = CAUSAL ? min(tiles, (wave_first + 32 + KT - 1) / KT) : tiles;
+  const bool live = wave_first < e.len;                      // a wave without a row only brings its pieces of the tiles
+  const int wave_tiles = !live ? 0 : CAUSAL ? min(tiles, (wave_first + 32 + KT - 1) / KT) : tiles;
   Stager<DP, 0> gk;
   Stager<DP, 2 * TILE> gv;
   gk.init(kp + (long)kt0 * KT * a.k_ts, a.k_ts, e.len - kt0 * KT, a.D, smem, wave, lane);
@@ -687,7 +689,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_dq_kernel(s
       gk.template next<BUF ^ 1>();
       gv.template next<BUF ^ 1>();
     }
-    const bool odd = MASKED && tile_nonfinite<E, DP>(smem + K0), mine = !MASKED || kt < wave_tiles;
+    const bool odd = MASKED && tile_nonfinite<E, DP>(smem + K0), mine = MASKED ? kt < wave_tiles : live;
     const int last = (CAUSAL ? min(row, e.len - 1) : e.len - 1) - kt * KT;
     const int last4 = last - (lane >> 5) * 4;                // against a register's constant
     lpx8_t ds[4];
@@ -728,7 +730,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_dq_kernel(s
         tile_clean<E, DP>(smem + K0);
       }
       if (mine) { products(0); products(1); }
-    } else {
+    } else if (mine) {
       products(0);
       scores(1);
       gradients(1);
@@ -880,7 +882,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void packed_attn_dkv_kernel(
     const int stage = now * STAGE;
     const float* stat = (const float*)(smem + STAT0 + now * STAT) + (lane >> 5) * 4;
     // (without a mask row0 + KT is always above 0: a branch all the same, or hipcc keeps the operands of two steps at once and spills)
-    const bool mine = row0 + KT > (CAUSAL ? wave_first : 0), whole = row0 + KT <= e.len && (!CAUSAL || row0 >= wave_first + 31);
+    const bool mine = wave_first < e.len && row0 + KT > (CAUSAL ? wave_first : 0), whole = row0 + KT <= e.len && (!CAUSAL || row0 >= wave_first + 31);
     u32x4_t p[2], ds[2];
     auto products = [&](int g) {
       const int rk = g / DB, cb = g % DB;

@@ -60,8 +60,9 @@ def check_rope(q, k, pos, inv, sections, gq, gk, dq, dk, interleaved, eps=1e-6):
         tol = dn if g is None else r * (dn + n * (dn * n).mean(-1, keepdim=True))
         assert R.off(dx, want[0], (48 + D / 4) * R.U * tol + R.rounded(want[0], dt)) <= 1
         if g is not None and T:
-            # every lane adds its rows, then 64 / lanes of a row, 4 waves, workgroups by 16 strands
-            adds = (T / 4096 + 1) * x.shape[1] + 160
+            # a wave's lanes add the rows of its tokens (at least 768 workgroups of 4 waves share them), then 6 halvings of a wave, 4 waves,
+            # 1024 / 64 workgroups in each of 64 strands and 4 + 16 sums of those
+            adds = (T / 3072 + 1) * x.shape[1] + 6 + 4 + 16 + 4 + 16
             assert R.off(dg, want[1], (adds + 32 + D / 8) * R.U * (mag * n).sum((0, 1))) <= 1
         elif g is not None:
             assert not dg.any()
