@@ -354,16 +354,17 @@ def test_attention_tiles_of_minus_infinity(causal, lens, Hq, Hkv, dt):
     assert bool(torch.isfinite(dv[skip:]).all()) and bool(torch.isfinite(dk[skip:]).all())
 
 
-def test_attention_a_list_that_is_none_is_loud():
+@pytest.mark.parametrize("causal", [True, False])
+def test_attention_a_list_that_is_none_is_loud(causal):
     q, k, v, do, _ = attn_case([100], 2, 1, 32, F16)
     for cu in ([0, 60, 40, 100], [0, 101], [1, 100], [0, -1, 100], [0, 2 ** 31 - 1]):
         plan = ops.packed_plan(torch.tensor(cu, dtype=torch.int32, device=DEV), 100)
-        o, lse = ops.packed_attn_fwd(q, k, v, plan)
+        o, lse = ops.packed_attn_fwd(q, k, v, plan, causal)
         assert bool(torch.isnan(o).all()) and bool(torch.isnan(lse).all()), cu
-        grads = ops.packed_attn_bwd(q, k, v, o, lse, do, plan)
+        grads = ops.packed_attn_bwd(q, k, v, o, lse, do, plan, causal)
         assert all(bool(torch.isnan(t).all()) for t in grads), cu
         keep = torch.full_like(q, 3.0)
-        ops.packed_attn_fwd(q, k, v, plan, out=keep)
+        ops.packed_attn_fwd(q, k, v, plan, causal, out=keep)
         assert bool((keep == 3).all())
 
 
