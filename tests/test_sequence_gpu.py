@@ -309,6 +309,27 @@ def test_attention_scores_of_minus_infinity():
 
 
 @pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("lens,Hq,Hkv,D", [([1, 20, 5, 128, 127], 4, 2, 64), ([2300], 2, 1, 128), ([64] * 7, 3, 3, 40)], ids=["short", "parts", "tiles"])
+def test_attention_rows_with_one_key_have_no_gradient(lens, Hq, Hkv, D, dt):
+    """P is 1 and dP is delta: dQ is nothing but what fp32 leaves of their difference, not the output's rounding to 16 bits"""
+    q, k, v, do, cu = attn_case(lens, Hq, Hkv, D, dt)
+    plan = ops.packed_plan(cu, sum(lens))
+    o, lse = ops.packed_attn_fwd(q, k, v, plan, True)
+    dq, _, _ = ops.packed_attn_bwd(q, k, v, o, lse, do, plan, True)
+    scale, first = D ** -0.5, 0
+    for n in lens:
+        for h in range(Hq):
+            Q, K, V, dO = (t[first:first + n].double() for t in (q[:, h], k[:, h // (Hq // Hkv)], v[:, h // (Hq // Hkv)], do[:, h]))
+            # the score: as in sequence_ref.attention; P is off by its error, dP and delta (a sum of it alone) by D products and sums each
+            ds = scale * (Q[0].abs() * K[0].abs()).sum() * (D + 8) * R.U + 8 * R.U * (1 + lse[h, first].double().abs())
+            at = (dO[0].abs() * V[0].abs()).sum() * (2 * (D + 8) * R.U + 2 * ds)
+            if dt == F16:                                                  # the least that dS is rounded to
+                at = at + 4 * 2.0 ** -39 * dO.norm(dim=-1).max() * V.norm(dim=-1).max()
+            assert bool((dq[first, h].double().abs() <= scale * at * K[0].abs() * (1 + 2 * R.h(dt)) + R.tiny(dt)).all()), (n, h)
+        first += n
+
+
+@pytest.mark.parametrize("dt", [F16, BF16])
 @pytest.mark.parametrize("lens,Hq,Hkv", [([300], 2, 1), ([2500], 2, 1), ([70, 200, 65], 12, 4)], ids=["tiles", "parts", "batch"])
 @pytest.mark.parametrize("causal", [True, False])
 def test_attention_tiles_of_minus_infinity(causal, lens, Hq, Hkv, dt):
