@@ -410,60 +410,106 @@ __device__ __forceinline__ int dx_splits(int grid, int tiles, int piece) {
   return n < 8 ? n : n & ~7;
 }
 
-// the list of the rows that take part, in their order: one workgroup, a stretch of rows to a thread
-__global__ __launch_bounds__(1024) void ce_rows_kernel(simvg_vocab_ce_args a, Head* head, int* list, int* place, float* factor) {
+// A workgroup of 1024 counts the rows that take part, a stretch of rows to a thread: the thread's first place in their list, how many
+// there are, and the largest |gradient| among them
+struct Counted { int m0, m1, at, kept; float g; };
+__device__ __forceinline__ Counted count_rows(const simvg_vocab_ce_args& a) {
   __shared__ float most[16];
-  __shared__ int counts[1024];
-  const int tid = threadIdx.x, per = cdiv(a.M, 1024), m0 = min(tid * per, a.M), m1 = min(m0 + per, a.M);
-  float g = 0.f;
+  __shared__ int counts[16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, per = cdiv(a.M, 1024);
+  Counted c = {min(tid * per, a.M), min(tid * per + per, a.M), 0, 0, 0.f};
   int n = 0;
-  for (int m = m0; m < m1; ++m)
+  for (int m = c.m0; m < c.m1; ++m)
     if (is_word(a, a.target[m])) {
-      g = fmaxf(g, fabsf(a.dloss[m]));
+      c.g = fmaxf(c.g, fabsf(a.dloss[m]));
       ++n;
     }
-  g = wave_max(g);
-  if ((tid & 63) == 0) most[tid >> 6] = g;
-  counts[tid] = n;
-  __syncthreads();
-  for (int o = 1; o < 1024; o <<= 1) {
-    const int v = tid >= o ? counts[tid - o] : 0;
-    __syncthreads();
-    counts[tid] += v;
-    __syncthreads();
+  c.g = wave_max(c.g);
+  int upto = n;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int before = __shfl_up(upto, o, 64);
+    if (lane >= o) upto += before;
   }
-  g = most[0];
-  for (int i = 1; i < 16; ++i) g = fmaxf(g, most[i]);
-  int at = counts[tid] - n;
-  for (int m = m0; m < m1; ++m) {
+  if (lane == 63) { most[wave] = c.g; counts[wave] = upto; }
+  __syncthreads();
+  c.at = upto - n;
+  c.g = most[0];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    c.g = fmaxf(c.g, most[i]);
+    if (i < wave) c.at += counts[i];
+    c.kept += counts[i];
+  }
+  return c;
+}
+__device__ __forceinline__ float row_factor(float d, float g) { return d == 0.f ? 0.f : d / g; }
+// the list of the rows that take part, in their order: one workgroup
+__global__ __launch_bounds__(1024) void ce_rows_kernel(simvg_vocab_ce_args a, Head* head, int* list, int* place, float* factor) {
+  const Counted c = count_rows(a);
+  int at = c.at;
+  for (int m = c.m0; m < c.m1; ++m) {
     const bool on = is_word(a, a.target[m]);
     place[m] = on ? at : -1;
     if (on) {
-      const float d = a.dloss[m];
       list[at] = m;
-      factor[at++] = d == 0.f ? 0.f : d / g;
+      factor[at++] = row_factor(a.dloss[m], c.g);
     }
   }
-  if (tid == 0) { head->gmax = g; head->kept = counts[1023]; }
+  if (threadIdx.x == 0) { head->gmax = c.g; head->kept = c.kept; }
+}
+// eight values of kept row r, row m of x: as they are, and times the row's factor
+template <class E>
+__device__ __forceinline__ void gather8(const simvg_vocab_ce_args& a, int r, int m, int c, float f, unsigned short* xs, unsigned short* xk) {
+  u32x4_t v = *(const u32x4_t*)((const unsigned short*)a.x + (long)m * a.ldx + c);
+  *(u32x4_t*)(xk + (long)r * a.K + c) = v;
+  if (f != 1.f) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float lo, hi;
+      unpack2<E>(v[j], lo, hi);
+      v[j] = E::pack(lo * f, hi * f);
+    }
+  }
+  *(u32x4_t*)(xs + (long)r * a.K + c) = v;
 }
 template <class E>
 __global__ __launch_bounds__(256) void ce_gather_kernel(simvg_vocab_ce_args a, const Head* head, const int* list, const float* factor,
                                                         unsigned short* xs, unsigned short* xk) {
   const int per = a.K / 8;
   for (long i = blockIdx.x * 256L + threadIdx.x; i < (long)head->kept * per; i += gridDim.x * 256L) {
-    const int r = (int)(i / per), c = (int)(i % per) * 8;
-    u32x4_t v = *(const u32x4_t*)((const unsigned short*)a.x + (long)list[r] * a.ldx + c);
-    *(u32x4_t*)(xk + (long)r * a.K + c) = v;
-    const float f = factor[r];
-    if (f != 1.f) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float lo, hi;
-        unpack2<E>(v[j], lo, hi);
-        v[j] = E::pack(lo * f, hi * f);
-      }
+    const int r = (int)(i / per);
+    gather8<E>(a, r, list[r], (int)(i % per) * 8, factor[r], xs, xk);
+  }
+}
+// Both in one launch: every workgroup counts for itself, the first one writes the list down.  (Up to a few thousand rows the count costs less
+// than a launch: backward pass of 1280 rows 215 -> 211 us, of 40 rows, 8003 words 40.5 -> 37.9.)
+constexpr int ROWS_AT_ONCE = 4096;
+template <class E>
+__global__ __launch_bounds__(1024) void ce_rows_gather_kernel(simvg_vocab_ce_args a, Head* head, int* list, int* place, float* factor,
+                                                              unsigned short* xs, unsigned short* xk) {
+  __shared__ int rows[ROWS_AT_ONCE];
+  __shared__ float factors[ROWS_AT_ONCE];
+  const Counted c = count_rows(a);
+  const bool first = blockIdx.x == 0;
+  int at = c.at;
+  for (int m = c.m0; m < c.m1; ++m) {
+    const bool on = is_word(a, a.target[m]);
+    if (first) place[m] = on ? at : -1;
+    if (on) {
+      const float f = row_factor(a.dloss[m], c.g);
+      rows[at] = m;
+      factors[at] = f;
+      if (first) { list[at] = m; factor[at] = f; }
+      ++at;
     }
-    *(u32x4_t*)(xs + (long)r * a.K + c) = v;
+  }
+  if (first && threadIdx.x == 0) { head->gmax = c.g; head->kept = c.kept; }
+  __syncthreads();
+  const int per = a.K / 8;
+  for (int i = blockIdx.x * 1024 + threadIdx.x; i < c.kept * per; i += gridDim.x * 1024) {
+    const int r = i / per;
+    gather8<E>(a, r, rows[r], i % per * 8, factors[r], xs, xk);
   }
 }
 
@@ -764,8 +810,12 @@ int ce_bwd(const simvg_vocab_ce_args& a, hipStream_t s) {
   int *list = (int*)(ws + p.o_list), *place = (int*)(ws + p.o_place);
   float *factor = (float*)(ws + p.o_factor), *sums = (float*)(ws + p.o_dx), *db = (float*)(ws + p.o_db);
   unsigned short *xs = (unsigned short*)(ws + p.o_x), *xk = (unsigned short*)(ws + p.o_xk), *e = (unsigned short*)(ws + p.o_e);
-  hipLaunchKernelGGL(ce_rows_kernel, dim3(1), dim3(1024), 0, s, a, head, list, place, factor);
-  hipLaunchKernelGGL(ce_gather_kernel<E>, dim3(min(2048, cdiv(a.M, 2))), dim3(256), 0, s, a, head, list, factor, xs, xk);
+  if (a.M <= ROWS_AT_ONCE) {
+    hipLaunchKernelGGL(ce_rows_gather_kernel<E>, dim3(min(256, cdiv(a.M * (a.K / 8), 1024))), dim3(1024), 0, s, a, head, list, place, factor, xs, xk);
+  } else {
+    hipLaunchKernelGGL(ce_rows_kernel, dim3(1), dim3(1024), 0, s, a, head, list, place, factor);
+    hipLaunchKernelGGL(ce_gather_kernel<E>, dim3(min(2048, cdiv(a.M, 2))), dim3(256), 0, s, a, head, list, factor, xs, xk);
+  }
   SIMVG_LAUNCH_CHECK();
   const int tk = cdiv(a.K, 256);
   const auto piece = [&](auto bias, int v) {

@@ -459,6 +459,11 @@ def test_vocab_ce_rows_of_unequal_weight(dt):
     check_ce(*ce_case(40, 1500, 256, dt, uniform=False))
 
 
+@pytest.mark.parametrize("M", [1023, 1025, 4096, 4097])               # rows to a thread of the list's workgroup; a list in one launch or two
+def test_vocab_ce_lists_of_rows(M):
+    check_ce(*ce_case(M, 270, 72, F16, ignored=0.5, uniform=False))
+
+
 @pytest.mark.parametrize("dt", [F16, BF16])
 def test_vocab_ce_in_several_pieces(dt):
     # 2^27 / 40000 words to a piece: eight pieces, the last one partly empty
