@@ -13,10 +13,10 @@
 // the order in which the accumulator holds them.  P and dS never leave registers.
 //
 // Measured, of 1.46 (fp16) and 1.44 (bf16) PFLOP/s that a library product of 8192^3 reaches: one sequence of 16384 rows, 16 heads of 128
-// on 2, causal, bf16, forward 1.01 ms, 1.09 PFLOP/s; nine of up to 4097 rows, 32 heads on 8: forward 0.49 ms, 0.92; dQ 0.71 ms and dK, dV
-// 1.06 ms, 0.95 and 0.85 of what each computes (6 D and 8 D: both need the scores).  Half of the time the matrix pipes work (the clock
+// on 2, causal, bf16, forward 1.01 ms, 1.09 PFLOP/s; nine of up to 4097 rows, 32 heads on 8: forward 0.49 ms, 0.92; dQ 0.69 ms and dK, dV
+// 1.06 ms, 0.98 and 0.85 of what each computes (6 D and 8 D: both need the scores).  Half of the time the matrix pipes work (the clock
 // falls to 1.7 GHz under them), a third goes to the exponentials and the rest of the vector work, which one or two waves to a SIMD
-// cover in part.  Heads of 64 (64 x 411 rows, 12 heads, no mask, fp16): forward 73 us, dQ 95, dK and dV 132: vector work, as much
+// cover in part.  Heads of 64 (64 x 411 rows, 12 heads, no mask, fp16): forward 68 us, dQ 92, dK and dV 132: vector work, as much
 // for half the products.
 //
 // Which rows a workgroup takes stands in a plan that the caller has built once for a batch (packed_plan_kernel): one entry for each
@@ -56,7 +56,8 @@ constexpr float NEG_INF = -__builtin_huge_valf();
 // ---------------------------------------------------------------------------------------------------------------- the plan
 // ints: [0] entries, [1] the row after the last sequence (-1: `cu` is no such list, there are no entries), [2..3] unused, then int4
 // {first row, rows, tile of the sequence, tiles of all sequences before} per entry, tiles far down their sequence first, then the same
-// entries in their natural order, then nseq + 1 prefix sums of tiles (used while building).  A list that does not start at 0, falls, or passes T is found here, so the kernels below stay inside their tensors
+// entries in their natural order, then nseq + 1 prefix sums of tiles (used while building).  A list that does not start at 0, falls, or
+// passes T is found here, so the kernels below stay inside their tensors
 // whatever it holds.
 constexpr int PLAN_HEAD = 4, PLAN_BINS = 1024;
 // one more than the tiles of any valid list: what a launch has left over is enough for the tiles behind the last sequence
@@ -550,7 +551,8 @@ __global__ __launch_bounds__(256) void packed_attn_fwd_join_kernel(simvg_packed_
 // ------------------------------------------------------------------------------------------------------------ backward
 // For fp16: delta_i = sum_d dO_id O_id, and the largest norms of dO's and V's rows in a tile and head: |dP_ij| and |delta_i| are at most
 // |dO_i| |V_j|, so with them dS can be brought to where fp16 has all its bits (`grad_power`).  (bf16: the dQ kernel takes delta along.)
-// ws: -delta [Hq][T] | lse log2(e) less P's power [Hq][T] | norms of dO [tiles][Hq] | norms of V [tiles][Hkv] | the parts' sums, dQ [parts][T][Hq][D], then dK and dV [parts][2][T][Hkv][D]
+// ws: -delta [Hq][T] | lse log2(e) less P's power [Hq][T] | norms of dO [tiles][Hq] | norms of V [tiles][Hkv] |
+// the parts' sums: dQ [parts][T][Hq][D], then dK and dV [parts][2][T][Hkv][D]
 __host__ __device__ __forceinline__ long ws_fixed(int T, int nseq, int Hq, int Hkv) {
   return (2L * Hq * T + (long)plan_capacity(T, nseq) * (Hq + Hkv) + 3) / 4 * 4;
 }
@@ -849,7 +851,8 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void packed_attn_dkv_kernel(
   gq.init((const unsigned short*)a.q + row_first * a.q_ts + (long)(hk * G + g0) * a.q_hs, a.q_ts, e.len - t0 * KT, a.D, smem, wave, lane);
   gd.init((const unsigned short*)a.d_o + row_first * a.do_ts + (long)(hk * G + g0) * a.do_hs, a.do_ts, e.len - t0 * KT, a.D, smem, wave, lane);
   // from the last head of a tile to the first of the one before (`next` has gone one tile on)
-  const long q_head = a.q_hs * 2 - (long)gq.step, d_head = a.do_hs * 2 - (long)gd.step, q_back = -(long)gq.step - G * (a.q_hs * 2), d_back = -(long)gd.step - G * (a.do_hs * 2);
+  const long q_head = a.q_hs * 2 - (long)gq.step, d_head = a.do_hs * 2 - (long)gd.step;
+  const long q_back = -(long)gq.step - G * (a.q_hs * 2), d_back = -(long)gd.step - G * (a.do_hs * 2);
   // the rows' lse and delta, from two waves
   unsigned long stat_at = (unsigned long)((wave ? ws_of(a).less : ws_of(a).lse2) + (long)(hk * G + g0) * a.T + row_first);
   const long stat_head = a.T * 4L, stat_back = -G * (a.T * 4L) - KT * 4L;
@@ -969,7 +972,8 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void packed_attn_dkv_kernel(
           const float p0 = __builtin_amdgcn_exp2f(fmaf(s[qb][r], c, -ls[qb][r / 4][r % 4]));
           const float p1 = __builtin_amdgcn_exp2f(fmaf(s[qb][r + 1], c, -ls[qb][r / 4][r % 4 + 1]));
           np[r / 8][r % 8 / 2] = E::pack(p0, p1);
-          nds[r / 8][r % 8 / 2] = E::kScaled ? E::pack(p0 * (dp[qb][r] * up), p1 * (dp[qb][r + 1] * up)) : E::pack(p0 * dp[qb][r], p1 * dp[qb][r + 1]);
+          nds[r / 8][r % 8 / 2] = E::kScaled ? E::pack(p0 * (dp[qb][r] * up), p1 * (dp[qb][r + 1] * up))
+                                             : E::pack(p0 * dp[qb][r], p1 * dp[qb][r + 1]);
         }
       };
       auto rounded = [&](int qb) {

@@ -332,7 +332,8 @@ __global__ __launch_bounds__(1024) void rope_dg_kernel(const float* ws, int rows
   }
   part[s][threadIdx.x & 15] = v;
   __syncthreads();
-  if (s < 16) part[s][threadIdx.x & 15] = (part[s][threadIdx.x & 15] + part[s + 16][threadIdx.x & 15]) + (part[s + 32][threadIdx.x & 15] + part[s + 48][threadIdx.x & 15]);
+  const int l = threadIdx.x & 15;
+  if (s < 16) part[s][l] = (part[s][l] + part[s + 16][l]) + (part[s + 32][l] + part[s + 48][l]);
   __syncthreads();
   if (s == 0 && c < 2 * D) {
     float total = 0.f;

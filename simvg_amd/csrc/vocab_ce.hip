@@ -413,17 +413,32 @@ __device__ __forceinline__ int dx_splits(int grid, int tiles, int piece) {
 // A workgroup of 1024 counts the rows that take part, a stretch of rows to a thread: the thread's first place in their list, how many
 // there are, and the largest |gradient| among them
 struct Counted { int m0, m1, at, kept; float g; };
+// f(row, whether it takes part, its gradient) of rows m0 .. m1 - 1, the loads of four at a time
+template <class F> __device__ __forceinline__ void each_row(const simvg_vocab_ce_args& a, int m0, int m1, F f) {
+  for (int m = m0; m < m1; m += 4) {
+    long t[4];
+    float d[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      t[i] = a.target[min(m + i, m1 - 1)];
+      d[i] = a.dloss[min(m + i, m1 - 1)];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (m + i < m1) f(m + i, is_word(a, t[i]), d[i]);
+  }
+}
 __device__ __forceinline__ Counted count_rows(const simvg_vocab_ce_args& a) {
   __shared__ float most[16];
   __shared__ int counts[16];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, per = cdiv(a.M, 1024);
   Counted c = {min(tid * per, a.M), min(tid * per + per, a.M), 0, 0, 0.f};
   int n = 0;
-  for (int m = c.m0; m < c.m1; ++m)
-    if (is_word(a, a.target[m])) {
-      c.g = fmaxf(c.g, fabsf(a.dloss[m]));
-      ++n;
-    }
+  each_row(a, c.m0, c.m1, [&](int, bool on, float d) {
+    if (!on) return;
+    c.g = fmaxf(c.g, fabsf(d));
+    ++n;
+  });
   c.g = wave_max(c.g);
   int upto = n;
 #pragma unroll
@@ -448,14 +463,13 @@ __device__ __forceinline__ float row_factor(float d, float g) { return d == 0.f 
 __global__ __launch_bounds__(1024) void ce_rows_kernel(simvg_vocab_ce_args a, Head* head, int* list, int* place, float* factor) {
   const Counted c = count_rows(a);
   int at = c.at;
-  for (int m = c.m0; m < c.m1; ++m) {
-    const bool on = is_word(a, a.target[m]);
+  each_row(a, c.m0, c.m1, [&](int m, bool on, float d) {
     place[m] = on ? at : -1;
     if (on) {
       list[at] = m;
-      factor[at++] = row_factor(a.dloss[m], c.g);
+      factor[at++] = row_factor(d, c.g);
     }
-  }
+  });
   if (threadIdx.x == 0) { head->gmax = c.g; head->kept = c.kept; }
 }
 // eight values of kept row r, row m of x: as they are, and times the row's factor
@@ -493,17 +507,16 @@ __global__ __launch_bounds__(1024) void ce_rows_gather_kernel(simvg_vocab_ce_arg
   const Counted c = count_rows(a);
   const bool first = blockIdx.x == 0;
   int at = c.at;
-  for (int m = c.m0; m < c.m1; ++m) {
-    const bool on = is_word(a, a.target[m]);
+  each_row(a, c.m0, c.m1, [&](int m, bool on, float d) {
     if (first) place[m] = on ? at : -1;
     if (on) {
-      const float f = row_factor(a.dloss[m], c.g);
+      const float f = row_factor(d, c.g);
       rows[at] = m;
       factors[at] = f;
       if (first) { list[at] = m; factor[at] = f; }
       ++at;
     }
-  }
+  });
   if (first && threadIdx.x == 0) { head->gmax = c.g; head->kept = c.kept; }
   __syncthreads();
   const int per = a.K / 8;
@@ -857,8 +870,8 @@ extern "C" long simvg_vocab_ce_ws_bytes(int M, int V, int K, int with_bias, int 
 extern "C" int simvg_vocab_ce_fwd(const simvg_vocab_ce_args* args, hipStream_t stream) {
   const int rc = ce_check(args, false);
   if (rc || args->M == 0) return rc;
-  SIMVG_CHECK_ARG(args->ws && (uintptr_t)args->ws % 256 == 0 && args->ws_bytes >= simvg_vocab_ce_ws_bytes(args->M, args->V, args->K, args->bias != nullptr, 0),
-                  "vocab_ce: the workspace is too small or misaligned");
+  const long need = simvg_vocab_ce_ws_bytes(args->M, args->V, args->K, args->bias != nullptr, 0);
+  SIMVG_CHECK_ARG(args->ws && (uintptr_t)args->ws % 256 == 0 && args->ws_bytes >= need, "vocab_ce: the workspace is too small or misaligned");
   return args->dtype == SEQ_F16 ? ce_fwd<F16>(*args, stream) : ce_fwd<BF16>(*args, stream);
 }
 extern "C" int simvg_vocab_ce_bwd(const simvg_vocab_ce_args* args, hipStream_t stream) {
@@ -869,7 +882,7 @@ extern "C" int simvg_vocab_ce_bwd(const simvg_vocab_ce_args* args, hipStream_t s
     SIMVG_LAUNCH_CHECK();
     return SIMVG_OK;
   }
-  SIMVG_CHECK_ARG(args->ws && (uintptr_t)args->ws % 256 == 0 && args->ws_bytes >= simvg_vocab_ce_ws_bytes(args->M, args->V, args->K, args->dbias != nullptr, 1),
-                  "vocab_ce: the workspace is too small or misaligned");
+  const long need = simvg_vocab_ce_ws_bytes(args->M, args->V, args->K, args->dbias != nullptr, 1);
+  SIMVG_CHECK_ARG(args->ws && (uintptr_t)args->ws % 256 == 0 && args->ws_bytes >= need, "vocab_ce: the workspace is too small or misaligned");
   return args->dtype == SEQ_F16 ? ce_bwd<F16>(*args, stream) : ce_bwd<BF16>(*args, stream);
 }

@@ -62,7 +62,7 @@ def check_rope(q, k, pos, inv, sections, gq, gk, dq, dk, interleaved, eps=1e-6):
         if g is not None and T:
             # a wave's lanes add the rows of its tokens (at least 768 workgroups of 4 waves share them), then 6 halvings of a wave, 4 waves,
             # 1024 / 64 workgroups in each of 64 strands and 4 + 16 sums of those
-            adds = (T / 3072 + 1) * x.shape[1] + 6 + 4 + 16 + 4 + 16
+            adds = (T / (4 * 768) + 1) * x.shape[1] + 6 + 4 + 16 + 4 + 16
             assert R.off(dg, want[1], (adds + 32 + D / 8) * R.U * (mag * n).sum((0, 1))) <= 1
         elif g is not None:
             assert not dg.any()
