@@ -4,6 +4,7 @@ Pointers are `tensor.data_ptr()` of caller-owned PyTorch-ROCm tensors; every cal
 current HIP stream and never synchronises.  PyTorch here is device memory + streams only.
 """
 import ctypes as C
+import functools
 
 import numpy
 
@@ -1302,6 +1303,12 @@ def _seq_rows(name, t, shape, dtype, device, written=False):
     return (t.data_ptr(), *st[:-1])
 
 
+@functools.lru_cache(maxsize=1024)
+def _seq_size(name, *sizes):
+    """what a workspace or table of these sizes takes (a call into the library is most of a microsecond)"""
+    return getattr(_lib.load(), name)(*sizes)
+
+
 def _seq_launch(name, fn, block, device, flops=0.0, nbytes=0.0):
     """one call of a library entry point on the current stream of `device`"""
     if device != _raw_device():
@@ -1359,7 +1366,7 @@ def qk_norm_rope_bwd(dq, dk, q, k, pos, inv_freq, sections, gq=None, gk=None, ep
     dgq = dgk = ws = None
     if gq is not None:
         D = q.shape[2]
-        n = lib.simvg_qk_norm_rope_ws_floats(q.shape[0], D)
+        n = _seq_size("simvg_qk_norm_rope_ws_floats", q.shape[0], D)
         dgq, dgk, ws = gq.new_empty(D), gk.new_empty(D), gq.new_empty(max(1, n))
     block = _lib.QK_NORM_ROPE.pack(*args, *_seq_rows("dq_in", dq_in, q.shape, q.dtype, dev, True),
                                    *_seq_rows("dk_in", dk_in, k.shape, q.dtype, dev, True), *_seq_rows("dq", dq, q.shape, q.dtype, dev),
@@ -1388,7 +1395,7 @@ def packed_plan(cu_seqlens, T):
     cu = _seq_flat("cu_seqlens", cu_seqlens, cu_seqlens.shape, torch.int32, dev)
     if T < 0:
         raise ValueError("T must not be negative")
-    table = cu_seqlens.new_empty(lib.simvg_packed_plan_ints(T, nseq))
+    table = cu_seqlens.new_empty(_seq_size("simvg_packed_plan_ints", T, nseq))
     _seq_launch("packed_plan", lambda at, stream: lib.simvg_packed_plan(cu, nseq, T, at, stream), table.data_ptr(), dev)
     return PackedPlan(cu_seqlens, nseq, T, table)
 
@@ -1423,7 +1430,7 @@ def packed_attn_fwd(q, k, v, plan, causal=True, scale=None, out=None):
     lib = _lib.load()
     args, dev = _packed_args(q, k, v, plan, causal, scale, out is None)
     (T, Hq, D), fill = q.shape, out is None
-    n = lib.simvg_packed_attn_ws_floats(T, plan.nseq, Hq, k.shape[1], D, args[6], 0)
+    n = _seq_size("simvg_packed_attn_ws_floats", T, plan.nseq, Hq, k.shape[1], D, args[6], 0)
     ws = None if n == 0 else q.new_empty(n, dtype=torch.float32)
     lse = q.new_empty((Hq, T), dtype=torch.float32) if fill else q.new_zeros((Hq, T), dtype=torch.float32)
     out = q.new_empty(q.shape) if fill else out
@@ -1449,7 +1456,7 @@ def packed_attn_bwd(q, k, v, out, lse, dout, plan, causal=True, scale=None, dq=N
         dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
     else:
         _seq_apart({"dq": dq, "dk": dk, "dv": dv}, q, k, v, out, dout)
-    ws = q.new_empty(max(1, lib.simvg_packed_attn_ws_floats(T, plan.nseq, Hq, k.shape[1], D, args[6], 1)), dtype=torch.float32)
+    ws = q.new_empty(max(1, _seq_size("simvg_packed_attn_ws_floats", T, plan.nseq, Hq, k.shape[1], D, args[6], 1)), dtype=torch.float32)
     block = _lib.PACKED_ATTN.pack(*args, *_seq_rows("out", out, q.shape, dt, dev), _seq_flat("lse", lse, (Hq, T), torch.float32, dev), T,
                                   *_seq_rows("dout", dout, q.shape, dt, dev), *_seq_rows("dq", dq, q.shape, dt, dev, True),
                                   *_seq_rows("dk", dk, k.shape, dt, dev, True), *_seq_rows("dv", dv, k.shape, dt, dev, True), ws.data_ptr())
@@ -1465,7 +1472,7 @@ def _ce_args(x, w, target, bias, ignore_index, backward):
     (px, ldx), (pw, ldw) = _seq_rows("x", x, x.shape, dt, dev), _seq_rows("w", w, (V, K), dt, dev)
     pt = _seq_flat("target", target, (M,), torch.int64, dev)
     pb = 0 if bias is None else _seq_flat("bias", bias, (V,), torch.float32, dev)
-    n = _lib.load().simvg_vocab_ce_ws_bytes(M, V, K, 0 if bias is None else 1, 1 if backward else 0)
+    n = _seq_size("simvg_vocab_ce_ws_bytes", M, V, K, 0 if bias is None else 1, 1 if backward else 0)
     ws = x.new_empty(max(1, n), dtype=torch.uint8)
     return (code, M, V, K, px, ldx if M > 1 else K, pw, ldw if V > 1 else K, pb, pt, ignore_index), dev, ws, n
 
