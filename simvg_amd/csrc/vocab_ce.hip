@@ -43,6 +43,7 @@ using namespace seq;
 
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr float NEG_INF = -__builtin_huge_valf();
+constexpr float FAR = 4096.f;                                // logits beyond it have their maximum subtracted before the scaling, not in its fma
 constexpr int BK = 64;                                       // contracted values of a stage: a row's are one line of 128 bytes
 
 __device__ __forceinline__ f32x16 zero16() { return (f32x16){0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}; }
@@ -311,7 +312,18 @@ __global__ __launch_bounds__((RA / WA) * (RB / WB) * 64, 2) void ce_fwd_kernel(s
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, acc[i][j][r]);
     top = fmaxf(top, __shfl_xor(top, 32, 64));
-    const float ref = top == NEG_INF ? 0.f : top * LOG2E;
+    float ref = top == NEG_INF ? 0.f : top * LOG2E;
+    // `ref` is rounded, and off by hundreds of powers of two in a tile of words that a bias of -1e10 takes out, by all of them at -1e38:
+    // the exponentials there would be inf, not 1
+    if (__any(top != NEG_INF && fabsf(top) > FAR)) {
+      stay_a_branch();
+      const float base = top == NEG_INF ? 0.f : top;
+#pragma unroll
+      for (int i = 0; i < P::NA; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][j][r] -= base;
+      ref = 0.f;
+    }
 #pragma unroll
     for (int i = 0; i < P::NA; ++i)
 #pragma unroll
@@ -600,7 +612,16 @@ __global__ __launch_bounds__((RA / WA) * (RB / WB) * 64, 2) void ce_e_kernel(sim
     const int r = m0 + wm + j * 32 + (lane & 31), m = list[min(r, kept - 1)];
     const bool on = r < kept;
     const long t = a.target[m];
-    less[j] = on ? (E::kScaled ? E_POWER : 0.f) - a.lse[m] * LOG2E : NEG_INF;
+    const float lse = a.lse[m], power = E::kScaled ? E_POWER : 0.f;
+    less[j] = on ? power - lse * LOG2E : NEG_INF;
+    if (__any(on && fabsf(lse) > FAR)) {                     // as in the forward pass
+      stay_a_branch();
+#pragma unroll
+      for (int i = 0; i < P::NA; ++i)
+#pragma unroll
+        for (int q = 0; q < 16; ++q) acc[i][j][q] -= lse;
+      if (on) less[j] = power;
+    }
     g[j] = BIAS && on ? factor[r] : 0.f;
     local[j] = on && t >= wv && t < wv + WA ? (int)(t - wv) : -1;
     any = any || local[j] >= 0;

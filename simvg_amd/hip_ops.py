@@ -1480,7 +1480,7 @@ def _ce_args(x, w, target, bias, ignore_index, backward):
 def vocab_ce_fwd(x, w, target, bias=None, ignore_index=-100):
     """Softmax cross entropy of x [M, K] against the words w [V, K] (+ bias [V] fp32) without storing the logits (csrc/vocab_ce.hip).
     target: int64 [M].  Returns (loss [M], lse [M]) in fp32; a row whose target is ignore_index has loss 0, one whose target is no word
-    has loss NaN."""
+    has loss NaN.  A bias of -inf, or a finite one that leaves nothing of a word's probability, takes the word out, as long as one is left."""
     args, dev, ws, n = _ce_args(x, w, target, bias, ignore_index, False)
     M = x.shape[0]
     loss, lse = x.new_empty(M, dtype=torch.float32), x.new_empty(M, dtype=torch.float32)

@@ -1,0 +1,58 @@
+"""The sequence operators at calls that their documentation allows and that are easily got wrong."""
+import pytest
+import torch
+
+import sequence_ref as R
+from simvg_amd import hip_ops as ops
+from test_sequence_gpu import BF16, DEV, F16, F32, ce_case
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------------------------------------------------------ vocabulary loss
+
+@pytest.mark.parametrize("value", [torch.finfo(F32).min, -1e30, -1e10, -1e6])
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("M,V", [(20, 900), (300, 1500)])
+def test_words_masked_by_a_large_finite_bias(M, V, dt, value):
+    """whole tiles of words whose bias is the type's lowest value, or any that leaves nothing of them: the loss and the gradients are those
+    of the words that are left"""
+    x, w, t, b, gl = ce_case(M, V, 64, dt, ignored=0.1)
+    left = torch.zeros(V, dtype=torch.bool, device=DEV)
+    left[:7] = left[500:600] = True
+    words = left.nonzero().squeeze(1)
+    t = torch.where(t == -100, t, words[t.clamp(min=0) % len(words)])
+    place = torch.full((V,), -1, device=DEV)
+    place[words] = torch.arange(len(words), device=DEV)
+    b = torch.where(left, b, value)
+    loss, lse = ops.vocab_ce_fwd(x, w, t, b)
+    dx, dw, db = ops.vocab_ce_bwd(x, w, t, lse, gl, b)
+    ref = R.vocab_ce(x, w[words], torch.where(t == -100, t, place[t.clamp(min=0)]), b[words], gl)
+    got = dict(loss=loss, lse=lse, dx=dx, dw=dw[words], dbias=db[words])
+    worst = {n: R.off(v, ref[n], ref["tol"][n]) for n, v in got.items()}
+    assert max(worst.values()) <= 1, worst
+    assert not dw[~left].any() and not db[~left].any()
+
+
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("M", [20, 300])
+@pytest.mark.parametrize("value", [1e5, 1e10, 1e30])
+def test_a_word_far_above_the_others(M, dt, value):
+    """its probability is 1, to the last bit: e is 1 there, -1 at the target and 0 elsewhere, all exact in 16 bits"""
+    x, w, t, b, gl = ce_case(M, 900, 64, dt, ignored=0.0)
+    word = 333
+    b[word] = value
+    loss, lse = ops.vocab_ce_fwd(x, w, t, b)
+    dx, dw, db = ops.vocab_ce_bwd(x, w, t, lse, gl, b)
+    e = torch.zeros(M, 900, device=DEV, dtype=torch.float64)
+    e[:, word] = 1
+    e[torch.arange(M, device=DEV), t] -= 1
+    g, X, W = gl.double()[:, None], x.double(), w.double()
+    # lse is the word's logit, rounded after 64 products and sums; a probability is off by that difference's exponential where the logits are
+    # held to less than a unit, and is 1 or 0 where they are not (1e10 is a multiple of 1024)
+    p = 0.0 if value > 1e9 else 4 * (64 + 8) * R.U * float((X.abs() @ W.abs().t()).max()) + 16 * R.U * value
+    want, size = (g * (e @ W), (g * e).t() @ X, (g * e).sum(0)), (g * (e.abs() @ W.abs()), (g * e.abs()).t() @ X.abs(), (g * e.abs()).sum(0))
+    assert R.off(dx, want[0], (p + (R.h(dt) if p else 0) + 300 * R.U) * size[0] + p * g * W[word].abs() + R.rounded(want[0], dt)) <= 1
+    assert R.off(dw, want[1], (p + (R.h(dt) if p else 0) + 400 * R.U) * size[1] + p * (g * X.abs()).sum(0) + R.rounded(want[1], dt)) <= 1
+    assert R.off(db, want[2], (p + 400 * R.U) * size[2] + p * g.sum()) <= 1
+    assert bool((lse.double() - value).abs().max() <= 64 + 2 * R.U * value) and bool(torch.isfinite(loss).all())
