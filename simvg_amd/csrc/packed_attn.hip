@@ -50,8 +50,9 @@ using namespace seq;
 
 constexpr int QT = 128;                                      // rows of a plan entry
 constexpr int KT = 64;                                       // rows of a tile in LDS
-constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+constexpr float LOG2E = 1.44269504088896340736f;
 constexpr float NEG_INF = -__builtin_huge_valf();
+constexpr float FAR = 4096.f;                                // exponents beyond it: the reference is subtracted before the scaling, not in its fma
 
 // ---------------------------------------------------------------------------------------------------------------- the plan
 // ints: [0] entries, [1] the row after the last sequence (-1: `cu` is no such list, there are no entries), [2..3] unused, then int4
@@ -473,7 +474,16 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_fwd_kernel(
     }
     if (mine) {
       // the exponentials of 16 keys and the products of the 16 before: vector and matrix pipes at the same time
-      const float mc = m == NEG_INF ? 0.f : m * c;           // nothing but scores of -inf so far: exponentials of 0, not NaN
+      float mc = m == NEG_INF ? 0.f : m * c;                 // nothing but scores of -inf so far: exponentials of 0, not NaN
+      // m c is rounded, and off by hundreds of powers of two while a row has seen nothing but scores of -1e10 (keys that a feature takes
+      // out): its exponentials would be inf, not 1
+      if (__any(fabsf(mc) > FAR)) {
+        stay_a_branch();
+        const bool far = fabsf(mc) > FAR;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) s[kb] -= far ? m : 0.f;
+        if (far) mc = 0.f;
+      }
       lpx8_t p[4];
       auto exps = [&](int rk) {
         f32x16& x = s[rk >> 1];
@@ -515,22 +525,23 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_fwd_kernel(
     // [part][T][Hq] (reference, sum) and [part][T][Hq][D] numerators
     const long n = (long)z->T * z->Hq, at = (long)(e.first + row) * z->Hq + h;
     store_sums<DP>(o, 1.f, z->ws + 2 * parts * n + (part * n + at) * z->D, z->D, valid, lane);
-    if (valid && lane < 32) ((float2*)z->ws)[part * n + at] = make_float2(m * z->scale * LOG2E, l);
+    if (valid && lane < 32) ((float2*)z->ws)[part * n + at] = make_float2(m, l);
   }
 }
-// the parts of a row joined: out = sum O_p 2^(m_p - m) / sum l_p 2^(m_p - m); 16 lanes a row
+// the parts of a row joined: out = sum O_p 2^((m_p - m) c) / sum l_p 2^((m_p - m) c), c = scale log2(e); 16 lanes a row
 template <class E>
 __global__ __launch_bounds__(256) void packed_attn_fwd_join_kernel(simvg_packed_attn_args a, int parts) {
   const int c = (threadIdx.x & 15) * 8;
   const long n = (long)a.T * a.Hq, rows = (long)a.plan[1] * a.Hq;
   const float2* stat = (const float2*)a.ws;
+  const float scale2 = a.scale * LOG2E;
   for (long at = blockIdx.x * 16L + (threadIdx.x >> 4); at < rows; at += gridDim.x * 16L) {
     float m = NEG_INF, l = 0.f;
     for (int p = 0; p < parts; ++p) m = fmaxf(m, stat[p * n + at].x);
     f32x4_t lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
     for (int p = 0; p < parts; ++p) {
       const float2 s = stat[p * n + at];
-      const float f = s.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(s.x - m);       // a part without keys has no reference
+      const float f = s.y == 0.f ? 0.f : __builtin_amdgcn_exp2f((s.x - m) * scale2);       // a part without keys has no reference
       l += s.y * f;
       if (c < a.D) {
         const float* src = a.ws + 2 * parts * n + (p * n + at) * a.D + c;
@@ -544,7 +555,7 @@ __global__ __launch_bounds__(256) void packed_attn_fwd_join_kernel(simvg_packed_
     if (c < a.D)
       *(u32x4_t*)((unsigned short*)a.o + row * a.o_ts + h * a.o_hs + c) = (u32x4_t){E::pack(lo[0] * r, lo[1] * r), E::pack(lo[2] * r, lo[3] * r),
                                                                                    E::pack(hi[0] * r, hi[1] * r), E::pack(hi[2] * r, hi[3] * r)};
-    if (c == 0) a.lse[h * a.lse_hs + row] = (m + __builtin_log2f(l)) * LN2;
+    if (c == 0) a.lse[h * a.lse_hs + row] = m * a.scale + __builtin_logf(l);
   }
 }
 

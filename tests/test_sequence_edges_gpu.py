@@ -4,7 +4,7 @@ import torch
 
 import sequence_ref as R
 from simvg_amd import hip_ops as ops
-from test_sequence_gpu import BF16, DEV, F16, F32, ce_case
+from test_sequence_gpu import BF16, DEV, F16, F32, attn_case, ce_case
 
 pytestmark = pytest.mark.gpu
 
@@ -56,3 +56,33 @@ def test_a_word_far_above_the_others(M, dt, value):
     assert R.off(dw, want[1], (p + (R.h(dt) if p else 0) + 400 * R.U) * size[1] + p * (g * X.abs()).sum(0) + R.rounded(want[1], dt)) <= 1
     assert R.off(db, want[2], (p + 400 * R.U) * size[2] + p * g.sum()) <= 1
     assert bool((lse.double() - value).abs().max() <= 64 + 2 * R.U * value) and bool(torch.isfinite(loss).all())
+
+
+# ------------------------------------------------------------------------------------------------------------------------ attention
+
+@pytest.mark.parametrize("scale", [None, 1.0])
+@pytest.mark.parametrize("dt,value", [(F16, torch.finfo(F16).min), (BF16, -1e10), (BF16, -1e30), (BF16, torch.finfo(BF16).min)])
+@pytest.mark.parametrize("lens,Hq,Hkv", [([300], 2, 1), ([2500], 2, 1), ([70, 200, 65], 12, 4)], ids=["tiles", "parts", "batch"])
+@pytest.mark.parametrize("causal", [True, False])
+def test_tiles_of_large_negative_scores(causal, lens, Hq, Hkv, dt, value, scale):
+    """the first keys of a sequence, whole tiles of them, have scores that leave nothing of their probability: every row that sees another
+    key gets the bits that it gets where those scores are -inf"""
+    q, k, v, do, cu = attn_case(lens, Hq, Hkv, 64, dt)
+    q, k = q.clone(), k.clone()
+    q[..., 0] = 1
+    skip, T = 130 if lens[0] > 130 else 64, sum(lens)
+    plan = ops.packed_plan(cu, T)
+
+    def run(masked):
+        k[:skip, :, 0] = masked
+        o, lse = ops.packed_attn_fwd(q, k, v, plan, causal, scale)
+        return (o, lse, *ops.packed_attn_bwd(q, k, v, o, lse, do, plan, causal, scale))
+    o, lse, dq, dk, dv = run(value)
+    wo, wlse, wdq, wdk, wdv = run(float("-inf"))
+    rows = slice(skip if causal else 0, T)                                  # those that see another key
+    assert bool(torch.isfinite(wo[rows]).all()) and bool(torch.isfinite(wdk[skip:]).all())
+    assert torch.equal(o[rows], wo[rows]) and torch.equal(lse[:, rows], wlse[:, rows])
+    assert torch.equal(dk[skip:], wdk[skip:]) and torch.equal(dv[skip:], wdv[skip:])
+    assert torch.equal(dq[rows][..., 1:], wdq[rows][..., 1:]) and bool(torch.isfinite(dq[rows]).all())
+    # the others: some weighted mean of the rows of v
+    assert bool(torch.isfinite(o).all()) and float(o.float().abs().max()) <= float(v.float().abs().max()) * (1 + 2 * R.h(dt))
