@@ -315,14 +315,14 @@ __global__ __launch_bounds__((RA / WA) * (RB / WB) * 64, 2) void ce_fwd_kernel(s
     float ref = top == NEG_INF ? 0.f : top * LOG2E;
     // `ref` is rounded, and off by hundreds of powers of two in a tile of words that a bias of -1e10 takes out, by all of them at -1e38:
     // the exponentials there would be inf, not 1
-    if (__any(top != NEG_INF && fabsf(top) > FAR)) {
+    if (__any(fabsf(ref) > FAR)) {
       stay_a_branch();
-      const float base = top == NEG_INF ? 0.f : top;
+      const bool far = fabsf(ref) > FAR;                     // each row by itself: what another one is far off changes no bit of it
 #pragma unroll
       for (int i = 0; i < P::NA; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) acc[i][j][r] -= base;
-      ref = 0.f;
+        for (int r = 0; r < 16; ++r) acc[i][j][r] -= far ? top : 0.f;
+      if (far) ref = 0.f;
     }
 #pragma unroll
     for (int i = 0; i < P::NA; ++i)
@@ -614,13 +614,14 @@ __global__ __launch_bounds__((RA / WA) * (RB / WB) * 64, 2) void ce_e_kernel(sim
     const long t = a.target[m];
     const float lse = a.lse[m], power = E::kScaled ? E_POWER : 0.f;
     less[j] = on ? power - lse * LOG2E : NEG_INF;
-    if (__any(on && fabsf(lse) > FAR)) {                     // as in the forward pass
+    const bool far = on && fabsf(lse) > FAR;
+    if (__any(far)) {                                        // as in the forward pass
       stay_a_branch();
 #pragma unroll
       for (int i = 0; i < P::NA; ++i)
 #pragma unroll
-        for (int q = 0; q < 16; ++q) acc[i][j][q] -= lse;
-      if (on) less[j] = power;
+        for (int q = 0; q < 16; ++q) acc[i][j][q] -= far ? lse : 0.f;
+      if (far) less[j] = power;
     }
     g[j] = BIAS && on ? factor[r] : 0.f;
     local[j] = on && t >= wv && t < wv + WA ? (int)(t - wv) : -1;

@@ -58,6 +58,23 @@ def test_a_word_far_above_the_others(M, dt, value):
     assert bool((lse.double() - value).abs().max() <= 64 + 2 * R.U * value) and bool(torch.isfinite(loss).all())
 
 
+@pytest.mark.parametrize("M", [20, 300])
+def test_a_row_far_off_changes_no_bit_of_the_others(M):
+    x, w, t, b, gl = ce_case(M, 900, 64, BF16, ignored=0.0)
+    loss, lse = ops.vocab_ce_fwd(x, w, t, b)
+    dx, _, _ = ops.vocab_ce_bwd(x, w, t, lse, gl, b)
+    x2 = x.clone()
+    x2[3] = x[3] * 2.0 ** 12                                               # logits of thousands
+    loss2, lse2 = ops.vocab_ce_fwd(x2, w, t, b)
+    dx2, _, _ = ops.vocab_ce_bwd(x2, w, t, lse2, gl, b)
+    others = torch.arange(M, device=DEV) != 3
+    assert float(lse2[3]) > 4096 and bool(torch.isfinite(dx2).all())
+    assert torch.equal(loss2[others], loss[others]) and torch.equal(lse2[others], lse[others]) and torch.equal(dx2[others], dx[others])
+    ref = R.vocab_ce(x2, w, t, b, gl)
+    assert R.off(lse2, ref["lse"], ref["tol"]["lse"]) <= 1 and R.off(loss2, ref["loss"], ref["tol"]["loss"]) <= 1
+    assert R.off(dx2, ref["dx"], ref["tol"]["dx"]) <= 1
+
+
 # ------------------------------------------------------------------------------------------------------------------------ attention
 
 @pytest.mark.parametrize("scale", [None, 1.0])
