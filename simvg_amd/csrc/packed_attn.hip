@@ -459,13 +459,21 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_fwd_kernel(
         for (int r = 0; r < 16; ++r) top = fmaxf(top, s[kb][r]);
       top = max_halves(top);
       // the reference follows the maximum only where it has grown by more than 2^8: the exponentials stay below 2^8, and what is
-      // left of O and l need not be scaled at every tile
-      if (__any((top - m) * c > 8.f)) {
-        const float to = fmaxf(m, top), f = m == to ? 1.f : __builtin_amdgcn_exp2f((m - to) * c);
+      // left of O and l need not be scaled at every tile.  (Each row by itself: its neighbours in the wave change no bit of it.)
+      if (__any((top - m) * c > 8.f || fabsf(m * c) > FAR)) {
+        const float to = (top - m) * c > 8.f ? top : m, f = m == to ? 1.f : __builtin_amdgcn_exp2f((m - to) * c);
         m = to;
         l *= f;
 #pragma unroll
         for (int i = 0; i < DB; ++i) o[i] *= f;
+        // m c is rounded, and off by hundreds of powers of two while a row has seen nothing but scores of -1e10 (keys that a feature takes
+        // out): its exponentials would be inf, not 1
+        const bool far = fabsf(m * c) > FAR && m != NEG_INF;
+        if (__any(far)) {
+          stay_a_branch();
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb) s[kb] -= far ? m : 0.f;
+        }
       }
     }
     if (odd) {
@@ -474,16 +482,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_fwd_kernel(
     }
     if (mine) {
       // the exponentials of 16 keys and the products of the 16 before: vector and matrix pipes at the same time
-      float mc = m == NEG_INF ? 0.f : m * c;                 // nothing but scores of -inf so far: exponentials of 0, not NaN
-      // m c is rounded, and off by hundreds of powers of two while a row has seen nothing but scores of -1e10 (keys that a feature takes
-      // out): its exponentials would be inf, not 1
-      if (__any(fabsf(mc) > FAR)) {
-        stay_a_branch();
-        const bool far = fabsf(mc) > FAR;
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) s[kb] -= far ? m : 0.f;
-        if (far) mc = 0.f;
-      }
+      const float mc = fabsf(m * c) > FAR ? 0.f : m * c;     // (nothing but scores of -inf so far: exponentials of 0, not NaN)
       lpx8_t p[4];
       auto exps = [&](int rk) {
         f32x16& x = s[rk >> 1];

@@ -103,3 +103,18 @@ def test_tiles_of_large_negative_scores(causal, lens, Hq, Hkv, dt, value, scale)
     assert torch.equal(dq[rows][..., 1:], wdq[rows][..., 1:]) and bool(torch.isfinite(dq[rows]).all())
     # the others: some weighted mean of the rows of v
     assert bool(torch.isfinite(o).all()) and float(o.float().abs().max()) <= float(v.float().abs().max()) * (1 + 2 * R.h(dt))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("causal", [True, False])
+def test_a_query_changes_no_bit_of_the_others(causal, D):
+    """each row's maximum is followed by itself, not by its neighbours in a wave"""
+    q, k, v, do, cu = attn_case([400], 2, 1, D, BF16)
+    plan = ops.packed_plan(cu, 400)
+    o, lse = ops.packed_attn_fwd(q, k, v, plan, causal)
+    q2 = q.clone()
+    q2[37] = q[37] * 64                                                    # its maximum moves at many tiles
+    o2, lse2 = ops.packed_attn_fwd(q2, k, v, plan, causal)
+    others = torch.arange(400, device=DEV) != 37
+    assert torch.equal(o2[others], o[others]) and torch.equal(lse2[:, others], lse[:, others])
+    assert not torch.equal(lse2[:, 37], lse[:, 37])
