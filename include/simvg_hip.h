@@ -476,10 +476,11 @@ int simvg_qk_norm_rope_bwd(const simvg_qk_norm_rope_args* args, simvg_stream_t s
  * of 8, <= 128; fp16 / bf16.
  * simvg_packed_plan lays a batch's lengths out for the kernels once (cu: device int32 [nseq + 1], cu[0] = 0, rising, at most T); every
  * layer's forward and backward of that batch read it.  A list that is none makes a plan without entries: nothing is computed, and
- * with fill_tail the outputs are NaN.
+ * what fill_tail names is NaN.
  * Forward writes o and lse [Hq][T] (natural logarithm of the softmax's denominator, scale included).  Backward reads q, k, v, o, lse and
  * d_o, writes dq, dk, dv.  ws: simvg_packed_attn_ws_floats() floats of the direction, aligned to 16 bytes (forward: none, 0, unless there
- * are few rows with many keys).  Rows behind the last sequence are left as they were, or, with fill_tail, become zeros. */
+ * are few rows with many keys).  Rows behind the last sequence are left as they were, or, with fill_tail 1, become zeros (fill_tail 2: those
+ * of the forward pass's lse alone). */
 typedef struct simvg_packed_attn_args {
   int dtype, T, nseq, Hq, Hkv, D, causal, fill_tail;
   float scale;

@@ -34,7 +34,7 @@
 #include "seq.h"
 
 struct simvg_packed_attn_args {
-  int dtype, T, nseq, Hq, Hkv, D, causal, fill_tail;        // fill_tail: rows past the last sequence become zeros (else: as they were)
+  int dtype, T, nseq, Hq, Hkv, D, causal, fill_tail;        // fill_tail: rows past the last sequence become zeros (else: as they were); 2: lse's alone
   float scale;
   const int* plan;
   const void* q; long q_ts, q_hs; const void* k; long k_ts, k_hs; const void* v; long v_ts, v_hs;
@@ -60,6 +60,7 @@ constexpr float FAR = 4096.f;                                // exponents beyond
 // entries in their natural order, then nseq + 1 prefix sums of tiles (used while building).  A list that does not start at 0, falls, or
 // passes T is found here, so the kernels below stay inside their tensors
 // whatever it holds.
+constexpr int FILL_LSE = 2;                                  // fill_tail of a forward pass into a result of the caller's
 constexpr int PLAN_HEAD = 4, PLAN_BINS = 1024;
 // one more than the tiles of any valid list: what a launch has left over is enough for the tiles behind the last sequence
 __host__ __device__ __forceinline__ int plan_capacity(int T, int nseq) { return T / QT + nseq + 1; }
@@ -341,12 +342,13 @@ __device__ __forceinline__ bool workgroup(const simvg_packed_attn_args& a, int H
 }
 // a workgroup without an entry: its tile of the rows behind the last sequence, zeros; NaN everywhere where there is no valid plan
 __device__ __forceinline__ void fill_tail(const simvg_packed_attn_args& a, int id, void* out, long ts, long hs, int h, float* lse) {
-  if (!a.fill_tail) return;
+  if (!a.fill_tail || (a.fill_tail == FILL_LSE && !lse)) return;
   const bool invalid = a.plan[1] < 0;
   const long row0 = (invalid ? 0L : a.plan[1]) + (id - a.plan[0]) * (long)QT;
   const int rows = (int)min((long)QT, a.T - row0);
   const unsigned short value = invalid ? 0x7fff : 0;         // a NaN in fp16 and in bf16
-  for (int i = threadIdx.x; i < rows * a.D; i += 256) ((unsigned short*)out)[(row0 + i / a.D) * ts + (long)h * hs + i % a.D] = value;
+  if (a.fill_tail != FILL_LSE)
+    for (int i = threadIdx.x; i < rows * a.D; i += 256) ((unsigned short*)out)[(row0 + i / a.D) * ts + (long)h * hs + i % a.D] = value;
   if (lse)
     for (int i = threadIdx.x; i < rows; i += 256) lse[(long)h * a.lse_hs + row0 + i] = invalid ? __builtin_nanf("") : 0.f;
 }

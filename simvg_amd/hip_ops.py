@@ -1419,21 +1419,22 @@ def _packed_args(q, k, v, plan, causal, scale, fill_tail):
         raise ValueError(f"the plan is for {plan.T} rows, q has {T}")
     if plan.table.get_device() != dev:
         raise ValueError(f"the plan is on {plan.table.device}, the other operands on {q.device}")
-    return (code, T, plan.nseq, Hq, Hkv, D, 1 if causal else 0, 1 if fill_tail else 0, D ** -0.5 if scale is None else scale,
+    return (code, T, plan.nseq, Hq, Hkv, D, 1 if causal else 0, fill_tail, D ** -0.5 if scale is None else scale,
             plan.table.data_ptr(), *rq, *rk, *rv), dev
 
 
 def packed_attn_fwd(q, k, v, plan, causal=True, scale=None, out=None):
     """Attention over packed sequences (csrc/packed_attn.hip): q [T, Hq, D], k, v [T, Hkv, D], fp16 or bf16, `plan` from `packed_plan`.
     Returns (out [T, Hq, D], lse [Hq, T] fp32).  Rows behind the last sequence are zeros; in an `out` of the caller's, which may not
-    overlap the operands, they stay as they were.  A row whose visible scores are all -inf is NaN.  Scores of any finite size are right here;
+    overlap the operands, they stay as they were (lse's are zeros; NaN where `cu_seqlens` was no valid list).  A row whose visible scores are all -inf is NaN.  Scores of any finite size are right here;
     `packed_attn_bwd` takes the probabilities from lse, which holds them to one part in 2^24 of a row's largest |scale q k|."""
     lib = _lib.load()
-    args, dev = _packed_args(q, k, v, plan, causal, scale, out is None)
-    (T, Hq, D), fill = q.shape, out is None
+    fill = out is None
+    args, dev = _packed_args(q, k, v, plan, causal, scale, 1 if fill else 2)
+    T, Hq, D = q.shape
     n = _seq_size("simvg_packed_attn_ws_floats", T, plan.nseq, Hq, k.shape[1], D, args[6], 0)
     ws = None if n == 0 else q.new_empty(n, dtype=torch.float32)
-    lse = q.new_empty((Hq, T), dtype=torch.float32) if fill else q.new_zeros((Hq, T), dtype=torch.float32)
+    lse = q.new_empty((Hq, T), dtype=torch.float32)
     out = q.new_empty(q.shape) if fill else out
     if not fill:
         _seq_apart({"out": out}, q, k, v)
@@ -1451,7 +1452,7 @@ def packed_attn_bwd(q, k, v, out, lse, dout, plan, causal=True, scale=None, dq=N
     fill = dq is None and dk is None and dv is None
     if not fill and (dq is None or dk is None or dv is None):
         raise ValueError("dq, dk and dv: all three or none")
-    args, dev = _packed_args(q, k, v, plan, causal, scale, fill)
+    args, dev = _packed_args(q, k, v, plan, causal, scale, 1 if fill else 0)
     (T, Hq, D), dt = q.shape, q.dtype
     if fill:
         dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)

@@ -118,3 +118,17 @@ def test_a_query_changes_no_bit_of_the_others(causal, D):
     others = torch.arange(400, device=DEV) != 37
     assert torch.equal(o2[others], o[others]) and torch.equal(lse2[:, others], lse[:, others])
     assert not torch.equal(lse2[:, 37], lse[:, 37])
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_a_list_that_is_none_shows_in_lse_beside_a_result_of_the_callers(causal):
+    q, k, v, do, _ = attn_case([100], 2, 1, 32, F16)
+    for cu in ([0, 60, 40, 100], [0, 101], [1, 100], [0, -1, 100]):
+        plan = ops.packed_plan(torch.tensor(cu, dtype=torch.int32, device=DEV), 100)
+        keep = torch.full_like(q, 3.0)
+        o, lse = ops.packed_attn_fwd(q, k, v, plan, causal, out=keep)
+        assert o is keep and bool((keep == 3).all()) and bool(torch.isnan(lse).all()), cu
+    # rows behind the last sequence: the result's stay, lse's are zeros
+    plan = ops.packed_plan(torch.tensor([0, 60], dtype=torch.int32, device=DEV), 100)
+    _, lse = ops.packed_attn_fwd(q, k, v, plan, causal, out=keep)
+    assert bool((keep[60:] == 3).all()) and not lse[:, 60:].any() and bool(torch.isfinite(lse).all()) and bool((lse[:, :60] != 0).any())
