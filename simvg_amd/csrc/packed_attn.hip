@@ -379,6 +379,8 @@ __device__ __forceinline__ void store_sums(const f32x16 (&acc)[DP / 32], float m
 }
 
 // ------------------------------------------------------------------------------------------------------------- forward
+// ws, where the keys are cut into parts: (reference, sum) [parts][T][Hq], a multiple of 16 bytes, then numerators [parts][T][Hq][D]
+__host__ __device__ __forceinline__ long ws_stats(long parts, long T, long Hq) { return (2 * parts * T * Hq + 3) / 4 * 4; }
 template <class E, int DP, bool CAUSAL>
 __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_fwd_kernel(simvg_packed_attn_args a, int parts) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -523,9 +525,8 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_fwd_kernel(
     store_rows<E, DP>(o, 1.f / l, out, z->D, valid, lane);
     if (valid && lane < 32) z->lse[(long)h * z->lse_hs + e.first + row] = m * z->scale + __builtin_logf(l);
   } else {
-    // [part][T][Hq] (reference, sum) and [part][T][Hq][D] numerators
     const long n = (long)z->T * z->Hq, at = (long)(e.first + row) * z->Hq + h;
-    store_sums<DP>(o, 1.f, z->ws + 2 * parts * n + (part * n + at) * z->D, z->D, valid, lane);
+    store_sums<DP>(o, 1.f, z->ws + ws_stats(parts, z->T, z->Hq) + (part * n + at) * z->D, z->D, valid, lane);
     if (valid && lane < 32) ((float2*)z->ws)[part * n + at] = make_float2(m, l);
   }
 }
@@ -545,7 +546,7 @@ __global__ __launch_bounds__(256) void packed_attn_fwd_join_kernel(simvg_packed_
       const float f = s.y == 0.f ? 0.f : __builtin_amdgcn_exp2f((s.x - m) * scale2);       // a part without keys has no reference
       l += s.y * f;
       if (c < a.D) {
-        const float* src = a.ws + 2 * parts * n + (p * n + at) * a.D + c;
+        const float* src = a.ws + ws_stats(parts, a.T, a.Hq) + (p * n + at) * a.D + c;
         const f32x4_t x = *(const f32x4_t*)src, y = *(const f32x4_t*)(src + 4);
         lo += x * f;
         hi += y * f;
@@ -1135,7 +1136,7 @@ long bwd_sums(int T, int nseq, int Hq, int Hkv, int D, int causal) {
 }
 long fwd_sums(int T, int nseq, int Hq, int D, int causal) {
   const int r = row_parts(T, nseq, Hq, causal);
-  return r > 1 ? (long)r * T * Hq * (D + 2) : 0L;
+  return r > 1 ? ws_stats(r, T, Hq) + (long)r * T * Hq * D : 0L;
 }
 int attn_check(const simvg_packed_attn_args* a, bool bwd) {
   SIMVG_CHECK_ARG(a, "packed_attn: null argument block");

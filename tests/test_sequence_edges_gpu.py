@@ -132,3 +132,15 @@ def test_a_list_that_is_none_shows_in_lse_beside_a_result_of_the_callers(causal)
     plan = ops.packed_plan(torch.tensor([0, 60], dtype=torch.int32, device=DEV), 100)
     _, lse = ops.packed_attn_fwd(q, k, v, plan, causal, out=keep)
     assert bool((keep[60:] == 3).all()) and not lse[:, 60:].any() and bool(torch.isfinite(lse).all()) and bool((lse[:, :60] != 0).any())
+
+
+@pytest.mark.parametrize("lens,Hq,causal", [([1571], 3, False), ([2501], 1, True), ([1667], 1, True)])
+def test_attention_cut_over_keys_with_odd_sizes(lens, Hq, causal):
+    """sequences long enough to be cut into parts, an odd number of rows and heads: o, lse and gradients"""
+    q, k, v, do, cu = attn_case(lens, Hq, 1, 64, BF16)
+    plan = ops.packed_plan(cu, lens[0])
+    o, lse = ops.packed_attn_fwd(q, k, v, plan, causal)
+    dq, dk, dv = ops.packed_attn_bwd(q, k, v, o, lse, do, plan, causal)
+    ref = R.attention(q, k, v, lens, causal, 0.125, do)
+    worst = {n: R.off(t, ref[n], ref["tol"][n]) for n, t in dict(o=o, lse=lse, dq=dq, dk=dk, dv=dv).items()}
+    assert max(worst.values()) <= 1, worst
