@@ -453,9 +453,9 @@ int simvg_philox4x32(const unsigned* ctr, const unsigned* key, unsigned* out);
  *   t_j = pos[row][axis(j)] * inv_freq[j] (in 64 bits),  j < P = sum(sections), axis(j) = the section that j falls into,
  *   (a_j, b_j) = (j, j + P) or, interleaved, (2j, 2j + 1); values from 2P on are normalised and not rotated.
  * x: [T][H][D], D even and <= 256, fp32 / fp16 / bf16; pos: [T][n_axes] int32 or (pos_is_64) int64; gq, gk: fp32 [D], both or
- * neither (rotation alone).  Forward writes q_out / k_out (which may be q / k themselves).  Backward reads q, k and the gradients
+ * neither (rotation alone).  Forward writes q_out / k_out.  Backward reads q, k and the gradients
  * dq, dk of the outputs, writes the inputs' gradients to q_out / k_out and the weights' to dgq / dgk (sums over rows and heads,
- * written, not added); ws: simvg_qk_norm_rope_ws_floats(T, D) floats. */
+ * written, not added).  q_out / k_out may be q / k themselves (backward: dq / dk too) and may not overlap anything else; ws: simvg_qk_norm_rope_ws_floats(T, D) floats. */
 typedef struct simvg_qk_norm_rope_args {
   int dtype, T, Hq, Hkv, D, n_axes, sections[4], interleaved, pos_is_64;
   float eps;

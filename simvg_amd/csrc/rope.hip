@@ -366,6 +366,15 @@ int rope_check(const simvg_qk_norm_rope_args* a, bool bwd, int& P) {
   SIMVG_CHECK_ARG(!bwd || a->T == 0 || (a->dq && a->dk), "qk_norm_rope: null pointer");
   SIMVG_CHECK_ARG(!bwd || !a->gq || (a->dgq && a->dgk && a->ws), "qk_norm_rope: the weights' gradients need outputs and a workspace");
   SIMVG_CHECK_ARG(a->pos_ld >= a->n_axes || a->T <= 1, "qk_norm_rope: rows of positions are shorter than the axes");
+  // a row is read whole before it is written: results may lie where their own operands do, row on row, and nowhere else on an operand
+  const Rows q = {a->q, a->q_ts, a->q_hs, a->Hq}, k = {a->k, a->k_ts, a->k_hs, a->Hkv}, dq = {a->dq, a->dq_ts, a->dq_hs, a->Hq},
+             dk = {a->dk, a->dk_ts, a->dk_hs, a->Hkv}, qo = {a->q_out, a->qo_ts, a->qo_hs, a->Hq}, ko = {a->k_out, a->ko_ts, a->ko_hs, a->Hkv};
+  const auto apart = [&](const Rows& x, const Rows& y) { return rows_apart(x, y, a->T, a->D, a->dtype == SEQ_F32 ? 4 : 2); };
+  const auto over = [&](const Rows& out, const Rows& in) { return out.same(in) || apart(out, in); };
+  SIMVG_CHECK_ARG(apart(qo, ko) && over(qo, q) && over(ko, k) && apart(qo, k) && apart(ko, q),
+                  "qk_norm_rope: a result overlaps another result or an operand (only its own one, row on row, may it replace)");
+  SIMVG_CHECK_ARG(!bwd || (over(qo, dq) && over(ko, dk) && apart(qo, dk) && apart(ko, dq)),
+                  "qk_norm_rope: a result overlaps another result or an operand (only its own one, row on row, may it replace)");
   return SIMVG_OK;
 }
 

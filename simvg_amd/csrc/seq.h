@@ -3,7 +3,13 @@
 // they read comes from a caller's language model and not from this library's encoder.  Rounding to 16 bits is round-to-nearest-even
 // and does not saturate: an overflow is an inf, as in torch, and a loss scaler can see it.
 #pragma once
+#include <climits>
+
+#include <algorithm>
 #include <atomic>
+#include <cstdlib>
+#include <initializer_list>
+#include <numeric>
 
 #include "common.h"
 
@@ -76,6 +82,42 @@ template <int N>
 __device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 // a barrier that does not drain this wave's DMA (what `__syncthreads` would wait for is the caller's business here)
 __device__ __forceinline__ void wave_barrier_only() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// ---- where an operand [T][H][D] lies, for the host's checks that results have memory of their own
+struct Rows {
+  const void* p; long ts, hs; int H;
+  bool same(const Rows& o) const { return p == o.p && ts == o.ts && hs == o.hs && H == o.H; }
+};
+// Whether two operands of the same T, D and size of a value have no value in common.  Slices of one buffer lie in each other's range and
+// are told apart by their rows: the distance of two heads' rows is d + i ts for tokens i apart.  Exact where the token strides are the
+// same; where they are not, rows that could meet in an endless tensor (a multiple of the strides' common divisor apart) count as meeting.
+inline bool rows_apart(Rows a, Rows b, int T, int D, int size) {
+  if (T <= 0 || a.H <= 0 || b.H <= 0 || !a.p || !b.p) return true;
+  for (Rows* r : {&a, &b}) {                                 // strides that are never walked
+    if (T == 1) r->ts = 0;
+    if (r->H == 1) r->hs = 0;
+  }
+  const long start = ((intptr_t)b.p - (intptr_t)a.p), row = (long)D * size;
+  const auto low = [&](const Rows& r) { return std::min(0L, (T - 1) * r.ts * size) + std::min(0L, (r.H - 1) * r.hs * size); };
+  const auto high = [&](const Rows& r) { return std::max(0L, (T - 1) * r.ts * size) + std::max(0L, (r.H - 1) * r.hs * size) + row; };
+  if (start + low(b) >= high(a) || low(a) >= start + high(b)) return true;
+  const long step = std::gcd(a.ts, b.ts) * size, reach = a.ts == b.ts ? T - 1 : LONG_MAX;
+  const auto meet = [&](long d) {                            // some |i| <= reach with |d + i step| < row
+    if (step == 0) return std::abs(d) < row;
+    const long i = std::abs(d) / step, rest = std::abs(d) % step;
+    return (i <= reach && rest < row) || (i < reach && step - rest < row) || (i > reach && std::abs(d) - reach * step < row);
+  };
+  if (a.hs == b.hs) {                                        // the heads' distances are few
+    for (long h = 1 - a.H; h < b.H; ++h)
+      if (meet(start + h * b.hs * size)) return false;
+    return true;
+  }
+  if ((long)a.H * b.H > 1 << 16) return false;
+  for (int i = 0; i < a.H; ++i)
+    for (int j = 0; j < b.H; ++j)
+      if (meet(start + (j * b.hs - i * a.hs) * size)) return false;
+  return true;
+}
 
 // more than 64 KiB of LDS has to be asked for, once on each device
 inline void allow_lds(const void* kernel, int bytes, std::atomic<unsigned long>& done) {

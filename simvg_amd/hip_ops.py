@@ -1347,7 +1347,7 @@ def qk_norm_rope_fwd(q, k, pos, inv_freq, sections, gq=None, gk=None, eps=1e-6, 
     """Norm of every head of q [T, Hq, D] and k [T, Hkv, D], then the rotation by up to four position axes, in one pass (csrc/rope.hip).
     pos: [T, axes] int32 / int64; sections: pairs per axis, inv_freq: float64 [sum(sections)], a frequency per pair; gq, gk: float32 [D]
     norm weights (None: rotation alone).  Pairs are (j, j + sum(sections)), or neighbours with `interleaved`.  Returns (q_out, k_out),
-    which may be q and k themselves."""
+    which may be q and k themselves and overlap nothing else."""
     args, dev = _rope_args(q, k, pos, inv_freq, sections, gq, gk, eps, interleaved)
     q_out = q.new_empty(q.shape) if q_out is None else q_out
     k_out = k.new_empty(k.shape) if k_out is None else k_out

@@ -3,8 +3,8 @@ import pytest
 import torch
 
 import sequence_ref as R
-from simvg_amd import hip_ops as ops
-from test_sequence_gpu import BF16, DEV, F16, F32, attn_case, ce_case
+from simvg_amd import _lib, hip_ops as ops
+from test_sequence_gpu import BF16, DEV, F16, F32, attn_case, ce_case, gen, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -144,3 +144,26 @@ def test_attention_cut_over_keys_with_odd_sizes(lens, Hq, causal):
     ref = R.attention(q, k, v, lens, causal, 0.125, do)
     worst = {n: R.off(t, ref[n], ref["tol"][n]) for n, t in dict(o=o, lse=lse, dq=dq, dk=dk, dv=dv).items()}
     assert max(worst.values()) <= 1, worst
+
+
+# ------------------------------------------------------------------------------------------------------------------ results' memory
+
+def test_rotation_in_one_buffer():
+    """q and k of a fused projection rotated where they are; results on anything else are refused"""
+    T, H, D, sections = 57, 4, 64, (8, 24)
+    qkv = randn(gen(4), T, 3 * H * D, dt=BF16)
+    q, k, v = (t.view(T, H, D) for t in qkv.split(H * D, dim=1))
+    pos = torch.arange(2 * T, device=DEV, dtype=torch.int32).view(T, 2)
+    inv = 100.0 ** (-torch.arange(32, device=DEV, dtype=torch.float64) / 32)
+    g = 1 + randn(gen(5), D, std=0.1)
+    args = (pos, inv, sections, g, g)
+    want, values = ops.qk_norm_rope_fwd(q, k, *args), v.clone()
+    for bad in (dict(q_out=k), dict(k_out=q), dict(q_out=qkv[:, 8:8 + H * D].view(T, H, D)), dict(q_out=torch.empty_like(q), k_out=q[1:]),
+                dict(q_out=v, k_out=v)):
+        with pytest.raises((ValueError, _lib.SimvgHipError)):
+            ops.qk_norm_rope_fwd(q, k, *args, **bad)
+    for bad in (dict(dq_in=k), dict(dq_in=values), dict(dk_in=q), dict(dq_in=q, dk_in=q)):
+        with pytest.raises((ValueError, _lib.SimvgHipError)):
+            ops.qk_norm_rope_bwd(want[0], values, q, k, *args, **bad)
+    ops.qk_norm_rope_fwd(q, k, *args, q_out=q, k_out=k)
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1]) and torch.equal(v, values)
