@@ -480,7 +480,7 @@ int simvg_qk_norm_rope_bwd(const simvg_qk_norm_rope_args* args, simvg_stream_t s
  * Forward writes o and lse [Hq][T] (natural logarithm of the softmax's denominator, scale included).  Backward reads q, k, v, o, lse and
  * d_o, writes dq, dk, dv.  ws: simvg_packed_attn_ws_floats() floats of the direction, aligned to 16 bytes (forward: none, 0, unless there
  * are few rows with many keys).  Rows behind the last sequence are left as they were, or, with fill_tail 1, become zeros (fill_tail 2: those
- * of the forward pass's lse alone). */
+ * of the forward pass's lse alone).  Results overlap neither the operands nor each other; slices of one buffer do not overlap. */
 typedef struct simvg_packed_attn_args {
   int dtype, T, nseq, Hq, Hkv, D, causal, fill_tail;
   float scale;

@@ -1400,15 +1400,6 @@ def packed_plan(cu_seqlens, T):
     return PackedPlan(cu_seqlens, nseq, T, table)
 
 
-def _seq_apart(written, *read):
-    """results that start where an operand or another result does would be written while they are still read (numel 0: nothing is)"""
-    taken = {t.data_ptr() for t in read if t.numel()}
-    for name, t in written.items():
-        if t.numel() and t.data_ptr() in taken:
-            raise ValueError(f"{name} must have memory of its own")
-        taken.add(t.data_ptr())
-
-
 def _packed_args(q, k, v, plan, causal, scale, fill_tail):
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
         raise ValueError("q, k and v must be [tokens, heads, head size]")
@@ -1436,8 +1427,6 @@ def packed_attn_fwd(q, k, v, plan, causal=True, scale=None, out=None):
     ws = None if n == 0 else q.new_empty(n, dtype=torch.float32)
     lse = q.new_empty((Hq, T), dtype=torch.float32)
     out = q.new_empty(q.shape) if fill else out
-    if not fill:
-        _seq_apart({"out": out}, q, k, v)
     block = _lib.PACKED_ATTN.pack(*args, *_seq_rows("out", out, q.shape, q.dtype, dev, True), lse.data_ptr(), T,
                                   0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0 if ws is None else ws.data_ptr())
     _seq_launch("packed_attn_fwd", lib.simvg_packed_attn_fwd, block, dev, 0.0, 2.0 * (2 * q.numel() + k.numel() + v.numel()))
@@ -1456,8 +1445,6 @@ def packed_attn_bwd(q, k, v, out, lse, dout, plan, causal=True, scale=None, dq=N
     (T, Hq, D), dt = q.shape, q.dtype
     if fill:
         dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
-    else:
-        _seq_apart({"dq": dq, "dk": dk, "dv": dv}, q, k, v, out, dout)
     ws = q.new_empty(max(1, _seq_size("simvg_packed_attn_ws_floats", T, plan.nseq, Hq, k.shape[1], D, args[6], 1)), dtype=torch.float32)
     block = _lib.PACKED_ATTN.pack(*args, *_seq_rows("out", out, q.shape, dt, dev), _seq_flat("lse", lse, (Hq, T), torch.float32, dev), T,
                                   *_seq_rows("dout", dout, q.shape, dt, dev), *_seq_rows("dq", dq, q.shape, dt, dev, True),

@@ -81,3 +81,33 @@ def test_overlap_is_told_exactly():
         assert no if common else (T > 1 and ts != ts2) or not no, (T, Hq, Hkv, D, ts, hs, ts2, hs2, p2 - base)
         seen[common] += 1
     assert min(seen) > 500
+
+
+def attn_args(**over):
+    names = ("q", "k", "v", "o", "d_o", "dq", "dk", "dv")
+    at = {n: (i + 1) << 16 for i, n in enumerate(names)}
+    strides = {p + s: v for p in ("q", "k", "v", "o", "do", "dq", "dk", "dv") for s, v in (("_ts", 4 * 64), ("_hs", 64))}
+    return _lib.PackedAttnArgs(**(dict(dtype=2, T=20, nseq=1, Hq=4, Hkv=2, D=64, causal=1, scale=0.125, plan=1 << 20, lse=1 << 21, lse_hs=20,
+                                       ws=1 << 22) | at | strides | over))
+
+
+def test_attention_refuses_results_on_operands():
+    lib = _lib.load()
+    q, k, v, o, do, dq, dk, dv = (i << 16 for i in range(1, 9))
+    for bad in (dict(o=q), dict(o=k), dict(o=v), dict(o=q + 128), dict(o=k + 16), dict(o=v - 64)):
+        assert refused(lib.simvg_packed_attn_fwd, attn_args(**bad), "overlaps"), bad
+    for bad in (dict(dq=q), dict(dq=do), dict(dq=o + 128), dict(dk=k), dict(dk=v + 128), dict(dv=v), dict(dv=q + 256), dict(dk=dv), dict(dq=dk + 128),
+                dict(dv=dq + 16), dict(dk=do + 32)):
+        assert refused(lib.simvg_packed_attn_bwd, attn_args(**bad), "overlaps"), bad
+
+
+@NO_DEVICE
+def test_attention_takes_slices_of_one_buffer():
+    lib = _lib.load()
+    q, dq = 1 << 16, 6 << 16
+    fused = {p + "_ts": 16 * 64 for p in ("q", "k", "v", "o", "do", "dq", "dk", "dv")}
+    heads = {p + s: v for p in ("q", "k", "v", "o") for s, v in (("_ts", 64), ("_hs", 20 * 64))}       # [heads][tokens][D]
+    for ok in (dict(k=q + 512, v=q + 768, o=q + 1024, **fused), dict(k=q + 4 * 2560, v=q + 6 * 2560, o=q + 8 * 2560, **heads)):
+        assert not refused(lib.simvg_packed_attn_fwd, attn_args(**ok), "overlaps"), ok
+    for ok in (dict(dk=dq + 512, dv=dq + 768, **fused), dict(k=q + 512, v=q + 768, dq=q + 1024, dk=q + 1536, dv=q + 1792, **fused)):
+        assert not refused(lib.simvg_packed_attn_bwd, attn_args(**ok), "overlaps"), ok

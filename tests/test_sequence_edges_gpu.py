@@ -167,3 +167,30 @@ def test_rotation_in_one_buffer():
             ops.qk_norm_rope_bwd(want[0], values, q, k, *args, **bad)
     ops.qk_norm_rope_fwd(q, k, *args, q_out=q, k_out=k)
     assert torch.equal(q, want[0]) and torch.equal(k, want[1]) and torch.equal(v, values)
+
+
+def test_attention_and_its_gradients_in_one_buffer():
+    """out beside q, k and v in one buffer, the gradients in another; results on an operand are refused"""
+    lens, Hq, Hkv, D = [90, 41], 4, 2, 64
+    q0, k0, v0, do, cu = attn_case(lens, Hq, Hkv, D, F16)
+    T, cuts = sum(lens), [Hq * D, Hkv * D, Hkv * D, Hq * D]
+    plan = ops.packed_plan(cu, T)
+    want = ops.packed_attn_fwd(q0, k0, v0, plan)
+    grads = ops.packed_attn_bwd(q0, k0, v0, *want, do, plan)
+    room, rest = torch.zeros(T, sum(cuts), dtype=F16, device=DEV), torch.zeros(T, sum(cuts[:3]), dtype=F16, device=DEV)
+    q, k, v, o = (t.view(T, -1, D) for t in room.split(cuts, dim=1))
+    mine = [t.view(T, -1, D) for t in rest.split(cuts[:3], dim=1)]
+    for a, b in ((q, q0), (k, k0), (v, v0)):
+        a.copy_(b)
+    for bad in (q, room[:, 8:8 + Hq * D].view(T, Hq, D), room[:, Hkv * D:(Hkv + Hq) * D].view(T, Hq, D)):
+        with pytest.raises((ValueError, _lib.SimvgHipError)):
+            ops.packed_attn_fwd(q, k, v, plan, out=bad)
+    _, lse = ops.packed_attn_fwd(q, k, v, plan, out=o)
+    assert torch.equal(o, want[0]) and torch.equal(lse, want[1])
+    for bad in (mine[:2] + [v], [q, *mine[1:]], [o, *mine[1:]], [mine[0], mine[1], mine[0][:, :Hkv]], [mine[0], mine[1], mine[0][:, 1:1 + Hkv]],
+                [rest[:, 8:8 + Hq * D].view(T, Hq, D), *mine[1:]]):
+        with pytest.raises((ValueError, _lib.SimvgHipError)):
+            ops.packed_attn_bwd(q, k, v, o, lse, do, plan, dq=bad[0], dk=bad[1], dv=bad[2])
+    ops.packed_attn_bwd(q, k, v, o, lse, do, plan, dq=mine[0], dk=mine[1], dv=mine[2])
+    assert all(torch.equal(a, b) for a, b in zip(mine, grads))
+    assert all(torch.equal(a, b) for a, b in ((q, q0), (k, k0), (v, v0), (o, want[0])))
