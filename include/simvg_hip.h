@@ -519,6 +519,10 @@ typedef struct simvg_vocab_ce_args {
 long simvg_vocab_ce_ws_bytes(int M, int V, int K, int with_bias, int backward);
 int simvg_vocab_ce_fwd(const simvg_vocab_ce_args* args, simvg_stream_t stream);
 int simvg_vocab_ce_bwd(const simvg_vocab_ce_args* args, simvg_stream_t stream);
+/* total = the sum of the M rows' losses, or, with `mean`, that over the number of targets that are not ignore_index (NaN without one);
+ * count = that number (a sum: 1), what the gradient of `total` is divided by for a row's dloss.  No memset: fit for a captured graph. */
+int simvg_vocab_ce_reduce(const float* loss, const long* target, long ignore_index, int M, int mean, float* total, float* count,
+                          simvg_stream_t stream);
 
 #ifdef __cplusplus
 }

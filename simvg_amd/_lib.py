@@ -130,6 +130,7 @@ _SIGS = {
     "simvg_packed_attn_bwd": [c_void_p, c_void_p],
     "simvg_vocab_ce_fwd": [c_void_p, c_void_p],
     "simvg_vocab_ce_bwd": [c_void_p, c_void_p],
+    "simvg_vocab_ce_reduce": [c_void_p, c_void_p, c_long, c_int, c_int, c_void_p, c_void_p, c_void_p],
     "simvg_text_filt_fwd": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p],
     "simvg_text_filt_bwd": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p],
     "simvg_query_mix_fwd": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p],

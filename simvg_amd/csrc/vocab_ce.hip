@@ -381,6 +381,34 @@ __global__ __launch_bounds__(1024) void ce_join_kernel(simvg_vocab_ce_args a, co
   }
 }
 
+// The rows' losses to one: their sum, or their mean over the rows that are not ignored, and how many those are (1 for a sum: what a
+// row's gradient is divided by).  One workgroup, every run adds in the same order, in 64 bits; no counters to be cleared, so that a captured
+// graph holds nothing but kernels (torch's sum over some hundred thousand rows clears one by a memset).
+__global__ __launch_bounds__(1024) void ce_reduce_kernel(const float* loss, const long* target, long ignore_index, int M, int mean, float* total,
+                                                         float* count) {
+  __shared__ double sums[16];
+  __shared__ int counts[16];
+  double sum = 0.;
+  int n = 0;
+#pragma unroll 8
+  for (int m = threadIdx.x; m < M; m += 1024) {
+    sum += loss[m];
+    n += target[m] != ignore_index;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    sum += __shfl_xor(sum, o, 64);
+    n += __shfl_xor(n, o, 64);
+  }
+  if ((threadIdx.x & 63) == 0) { sums[threadIdx.x >> 6] = sum; counts[threadIdx.x >> 6] = n; }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 16; ++i) { sum += sums[i]; n += counts[i]; }
+    *total = (float)(mean ? sum / n : sum);
+    *count = mean ? (float)n : 1.f;
+  }
+}
+
 // ------------------------------------------------------------------------------------------------------------ backward
 // Only the rows that take part are computed: the list of them, made on the device, is as long as `kept` says there (masked-word training
 // ignores most rows), and the kernels below go by that length; their launches and the workspace are laid out for all M.
@@ -895,6 +923,14 @@ extern "C" int simvg_vocab_ce_fwd(const simvg_vocab_ce_args* args, hipStream_t s
   const long need = simvg_vocab_ce_ws_bytes(args->M, args->V, args->K, args->bias != nullptr, 0);
   SIMVG_CHECK_ARG(args->ws && (uintptr_t)args->ws % 256 == 0 && args->ws_bytes >= need, "vocab_ce: the workspace is too small or misaligned");
   return args->dtype == SEQ_F16 ? ce_fwd<F16>(*args, stream) : ce_fwd<BF16>(*args, stream);
+}
+extern "C" int simvg_vocab_ce_reduce(const float* loss, const long* target, long ignore_index, int M, int mean, float* total, float* count,
+                                     hipStream_t stream) {
+  SIMVG_CHECK_ARG(M >= 0 && M <= 1 << 22, "vocab_ce_reduce: M must be between 0 and 2^22");
+  SIMVG_CHECK_ARG((M == 0 || (loss && target)) && total && count, "vocab_ce_reduce: null pointer");
+  hipLaunchKernelGGL(ce_reduce_kernel, dim3(1), dim3(1024), 0, stream, loss, target, ignore_index, M, mean, total, count);
+  SIMVG_LAUNCH_CHECK();
+  return SIMVG_OK;
 }
 extern "C" int simvg_vocab_ce_bwd(const simvg_vocab_ce_args* args, hipStream_t stream) {
   const int rc = ce_check(args, true);

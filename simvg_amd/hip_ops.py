@@ -1478,6 +1478,20 @@ def vocab_ce_fwd(x, w, target, bias=None, ignore_index=-100):
     return loss, lse
 
 
+def vocab_ce_reduce(loss, target, ignore_index=-100, mean=True):
+    """(total, count): the sum of the rows' losses, or their mean over the `count` rows that are not ignored (NaN without any; a sum's count
+    is 1), fp32 scalars.  dloss of a row is the gradient of `total` over `count`."""
+    if loss.dim() != 1:
+        raise ValueError("loss must be a vector")
+    dev, M = loss.get_device(), loss.shape[0]
+    pl, pt = _seq_flat("loss", loss, (M,), torch.float32, dev), _seq_flat("target", target, (M,), torch.int64, dev)
+    total, count = loss.new_empty(()), loss.new_empty(())
+    lib = _lib.load()
+    _seq_launch("vocab_ce_reduce", lambda out, stream: lib.simvg_vocab_ce_reduce(pl, pt, ignore_index, M, 1 if mean else 0, out, count.data_ptr(), stream),
+                total.data_ptr(), dev, 0.0, 12.0 * M)
+    return total, count
+
+
 def vocab_ce_bwd(x, w, target, lse, dloss, bias=None, ignore_index=-100):
     """Gradients of `vocab_ce_fwd` for the gradients dloss [M] of the rows' losses: (dx, dw, dbias), dbias None without a bias."""
     args, dev, ws, n = _ce_args(x, w, target, bias, ignore_index, True)

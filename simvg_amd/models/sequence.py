@@ -72,6 +72,20 @@ class VocabCrossEntropy(torch.autograd.Function):
         return dx, dw, None, dbias, None
 
 
+class ReducedLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, loss, target, ignore_index, mean):
+        total, count = ops.vocab_ce_reduce(loss, target, ignore_index, mean)
+        ctx.save_for_backward(count)
+        ctx.rows = loss.shape
+        return total
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dtotal):
+        return (dtotal / ctx.saved_tensors[0]).expand(ctx.rows), None, None, None
+
+
 def qk_norm_rope(q, k, pos, inv_freq, sections, gq=None, gk=None, eps=1e-6, interleaved=False):
     """`hip_ops.qk_norm_rope_fwd` with gradients for q, k and the norm weights"""
     return QKNormRope.apply(q, k, pos, inv_freq, tuple(sections), gq, gk, eps, interleaved)
@@ -88,7 +102,4 @@ def vocab_cross_entropy(x, w, target, bias=None, ignore_index=-100, reduction="m
     if reduction not in ("mean", "sum", "none"):
         raise ValueError(f"reduction must be mean, sum or none, got {reduction!r}")
     loss = VocabCrossEntropy.apply(x, w, target, bias, ignore_index)
-    if reduction == "none":
-        return loss
-    total = loss.sum()
-    return total if reduction == "sum" else total / (target != ignore_index).sum()
+    return loss if reduction == "none" else ReducedLoss.apply(loss, target, ignore_index, reduction == "mean")

@@ -111,3 +111,10 @@ def test_attention_takes_slices_of_one_buffer():
         assert not refused(lib.simvg_packed_attn_fwd, attn_args(**ok), "overlaps"), ok
     for ok in (dict(dk=dq + 512, dv=dq + 768, **fused), dict(k=q + 512, v=q + 768, dq=q + 1024, dk=q + 1536, dv=q + 1792, **fused)):
         assert not refused(lib.simvg_packed_attn_bwd, attn_args(**ok), "overlaps"), ok
+
+
+def test_reduced_loss_refuses_before_launching():
+    fn = _lib.load().simvg_vocab_ce_reduce
+    for bad in (dict(M=-1), dict(M=(1 << 22) + 1), dict(loss=None), dict(target=None), dict(total=None), dict(count=None)):
+        a = dict(loss=256, target=512, ignore_index=-100, M=4, mean=1, total=768, count=1024) | bad
+        assert fn(*a.values(), None) < 0 and b"vocab_ce_reduce" in _lib.load().simvg_last_error(), bad

@@ -1,9 +1,12 @@
 """The sequence operators at calls that their documentation allows and that are easily got wrong."""
+import ctypes as C
+
 import pytest
 import torch
 
 import sequence_ref as R
 from simvg_amd import _lib, hip_ops as ops
+from simvg_amd.models import sequence as S
 from test_sequence_gpu import BF16, DEV, F16, F32, attn_case, ce_case, gen, randn
 
 pytestmark = pytest.mark.gpu
@@ -194,3 +197,74 @@ def test_attention_and_its_gradients_in_one_buffer():
     ops.packed_attn_bwd(q, k, v, o, lse, do, plan, dq=mine[0], dk=mine[1], dv=mine[2])
     assert all(torch.equal(a, b) for a, b in zip(mine, grads))
     assert all(torch.equal(a, b) for a, b in ((q, q0), (k, k0), (v, v0), (o, want[0])))
+
+
+# -------------------------------------------------------------------------------------------------------------------- captured graphs
+
+def graph_nodes(graph):
+    """the types of a captured graph's nodes (0 kernel, 1 copy, 2 memset ..), from the HIP library that torch has loaded"""
+    path = next(ln.split()[-1] for ln in open("/proc/self/maps") if "libamdhip64" in ln)
+    hip, raw, n = C.CDLL(path), C.c_void_p(graph.raw_cuda_graph()), C.c_size_t(0)
+    assert hip.hipGraphGetNodes(raw, None, C.byref(n)) == 0
+    nodes, kind = (C.c_void_p * n.value)(), C.c_int(-1)
+    assert hip.hipGraphGetNodes(raw, nodes, C.byref(n)) == 0
+    kinds = []
+    for node in nodes:
+        assert hip.hipGraphNodeGetType(C.c_void_p(node), C.byref(kind)) == 0
+        kinds.append(kind.value)
+    return kinds
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum"])
+@pytest.mark.parametrize("M", [90, 1 << 20])
+def test_reduced_loss_in_a_captured_graph(M, reduction):
+    """the sum over many rows is a kernel of the library's: torch's own, from some hundred thousand rows on, clears its counters by a memset,
+    which replays wrongly"""
+    x, w, t, b, _ = ce_case(M, 60, 16, BF16, ignored=0.3)
+    leaves = [z.clone().requires_grad_() for z in (x, w, b)]
+
+    def step():
+        loss = S.vocab_cross_entropy(leaves[0], leaves[1], t, leaves[2], reduction=reduction)
+        return (loss.detach(), *torch.autograd.grad(loss, leaves))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        out = step()
+    kinds = graph_nodes(graph)
+    assert kinds and set(kinds) == {0}, kinds
+    graph.instantiate()
+    for i in range(3):
+        with torch.no_grad():
+            leaves[0].mul_(0.75)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert bool(torch.isfinite(out[0])) and all(torch.equal(p, r) for p, r in zip(out, step())), i
+        torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("M", [0, 1, 333, 40000])
+def test_reduced_loss_and_its_gradients(M):
+    x, w, t, b, _ = ce_case(M, 300, 64, F16, ignored=0.3)
+    if M == 1:
+        t.fill_(7)
+    rows = S.vocab_cross_entropy(x, w, t, b, reduction="none").detach().double()
+    n = int((t != -100).sum())
+    for reduction in ("sum", "mean"):
+        leaves = [z.clone().requires_grad_() for z in (x, w, b)]
+        loss = S.vocab_cross_entropy(leaves[0], leaves[1], t, leaves[2], reduction=reduction)
+        assert loss.shape == () and loss.dtype == F32
+        if n == 0 and reduction == "mean":
+            assert bool(torch.isnan(loss))
+            continue
+        want = rows.sum() if reduction == "sum" else rows.sum() / n
+        assert abs(float(loss.detach()) - float(want)) <= 4 * R.U * float(want)       # rounded once, and the quotient once more
+        got = torch.autograd.grad(loss * 512, leaves)
+        _, lse = ops.vocab_ce_fwd(x, w, t, b)
+        each = torch.full((M,), 512.0 if reduction == "sum" else 512.0 / n, device=DEV)
+        for a, c in zip(got, ops.vocab_ce_bwd(x, w, t, lse, each, b)):
+            assert torch.equal(a, c)
