@@ -1139,7 +1139,6 @@ long fwd_sums(int T, int nseq, int Hq, int D, int causal) {
   return r > 1 ? ws_stats(r, T, Hq) + (long)r * T * Hq * D : 0L;
 }
 int attn_check(const simvg_packed_attn_args* a, bool bwd) {
-  SIMVG_CHECK_ARG(a, "packed_attn: null argument block");
   SIMVG_CHECK_ARG(a->dtype == SEQ_F16 || a->dtype == SEQ_BF16, "packed_attn: dtype must be fp16 or bf16");
   SIMVG_CHECK_ARG(a->T >= 0 && a->nseq >= 0 && a->nseq <= 1 << 24, "packed_attn: T and nseq must not be negative");
   SIMVG_CHECK_ARG(a->Hkv >= 1 && a->Hq >= a->Hkv && a->Hq % a->Hkv == 0, "packed_attn: the heads of q must be a multiple of those of k and v");
@@ -1214,11 +1213,17 @@ void attn_dispatch(const simvg_packed_attn_args& a, bool bwd, hipStream_t s) {
   if (a.D <= 64) a.causal ? attn_launch<E, 64, true>(a, bwd, s) : attn_launch<E, 64, false>(a, bwd, s);
   else a.causal ? attn_launch<E, 128, true>(a, bwd, s) : attn_launch<E, 128, false>(a, bwd, s);
 }
-int attn_run(const simvg_packed_attn_args* a, bool bwd, hipStream_t s) {
-  const int rc = attn_check(a, bwd);
-  if (rc || a->T == 0) return rc;
-  if (a->dtype == SEQ_F16) attn_dispatch<F16>(*a, bwd, s);
-  else attn_dispatch<BF16>(*a, bwd, s);
+int attn_run(const simvg_packed_attn_args* args, bool bwd, hipStream_t s) {
+  SIMVG_CHECK_ARG(args, "packed_attn: null argument block");
+  simvg_packed_attn_args a = *args;
+  // the token stride of one token and the head stride of one head are never walked: whatever a view has there is no reason to refuse it
+  if (a.T == 1) a.q_ts = a.k_ts = a.v_ts = a.o_ts = a.do_ts = a.dq_ts = a.dk_ts = a.dv_ts = 0;
+  if (a.Hq == 1) a.q_hs = a.o_hs = a.do_hs = a.dq_hs = 0;
+  if (a.Hkv == 1) a.k_hs = a.v_hs = a.dk_hs = a.dv_hs = 0;
+  const int rc = attn_check(&a, bwd);
+  if (rc || a.T == 0) return rc;
+  if (a.dtype == SEQ_F16) attn_dispatch<F16>(a, bwd, s);
+  else attn_dispatch<BF16>(a, bwd, s);
   SIMVG_LAUNCH_CHECK();
   return SIMVG_OK;
 }

@@ -118,3 +118,14 @@ def test_reduced_loss_refuses_before_launching():
     for bad in (dict(M=-1), dict(M=(1 << 22) + 1), dict(loss=None), dict(target=None), dict(total=None), dict(count=None)):
         a = dict(loss=256, target=512, ignore_index=-100, M=4, mean=1, total=768, count=1024) | bad
         assert fn(*a.values(), None) < 0 and b"vocab_ce_reduce" in _lib.load().simvg_last_error(), bad
+
+
+@NO_DEVICE
+def test_strides_that_are_never_walked_are_not_looked_at():
+    lib, names = _lib.load(), ("q", "k", "v", "o", "do", "dq", "dk", "dv")
+    for ok in ({"T": 1} | {n + "_ts": (1 << 30) + 3 for n in names}, {"Hq": 1, "Hkv": 1} | {n + "_hs": 1 for n in names}):
+        for fn in (lib.simvg_packed_attn_fwd, lib.simvg_packed_attn_bwd):
+            assert not refused(fn, attn_args(**ok), "packed_attn"), ok
+    for bad, words in (({n + "_ts": 3 for n in names}, "16 bytes"), ({n + "_hs": 3 for n in names}, "16 bytes"), (dict(q_ts=1 << 24), "2^24")):
+        assert refused(lib.simvg_packed_attn_fwd, attn_args(**bad), words), bad
+    assert lib.simvg_packed_attn_fwd(None, None) < 0 and lib.simvg_packed_attn_bwd(None, None) < 0

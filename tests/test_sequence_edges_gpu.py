@@ -268,3 +268,24 @@ def test_reduced_loss_and_its_gradients(M):
         each = torch.full((M,), 512.0 if reduction == "sum" else 512.0 / n, device=DEV)
         for a, c in zip(got, ops.vocab_ce_bwd(x, w, t, lse, each, b)):
             assert torch.equal(a, c)
+
+
+@pytest.mark.parametrize("T,Hkv", [(1, 1), (1, 2), (70, 1)])
+def test_strides_of_dimensions_of_one_mean_nothing(T, Hkv):
+    """a token stride of a single token, a head stride of a single head: whatever they are, the same results"""
+    Hq, D = 4 * Hkv, 64
+    q, k, v, do, cu = (t if t.dim() == 1 else t.clone() for t in attn_case([T], Hq, Hkv, D, F16))
+
+    def odd(t):
+        ts, hs, _ = t.stride()
+        room = torch.zeros(t.numel() + 64, dtype=t.dtype, device=DEV)
+        room[:t.numel()] = t.flatten()
+        return room.as_strided(t.shape, (ts if T > 1 else (1 << 24) + 3, hs if t.shape[1] > 1 else 1, 1))
+    plan = ops.packed_plan(cu, T)
+    want = ops.packed_attn_fwd(q, k, v, plan)
+    want += ops.packed_attn_bwd(q, k, v, *want, do, plan)
+    a, b, c, d = (odd(t) for t in (q, k, v, do))
+    got = ops.packed_attn_fwd(a, b, c, plan, out=odd(torch.zeros_like(q)))
+    got += ops.packed_attn_bwd(a, b, c, odd(got[0]), got[1], d, plan, dq=odd(torch.zeros_like(q)), dk=odd(torch.zeros_like(k)),
+                               dv=odd(torch.zeros_like(v)))
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
