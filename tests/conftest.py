@@ -1,3 +1,4 @@
+import gc
 import os
 import sys
 
@@ -25,3 +26,11 @@ def golden():
     def load(name):
         return torch.load(os.path.join(GOLDEN, name + ".pt"), weights_only=False)
     return load
+
+
+@pytest.fixture(scope="module", autouse=True)
+def leave_nothing_behind():
+    """Models and captured graphs are cycles: a module's are destroyed here, and not, at some later time, by the collector of a process that
+    another module's test has forked."""
+    yield
+    gc.collect()
