@@ -455,7 +455,8 @@ int simvg_philox4x32(const unsigned* ctr, const unsigned* key, unsigned* out);
  * x: [T][H][D], D even and <= 256, fp32 / fp16 / bf16; pos: [T][n_axes] int32 or (pos_is_64) int64; gq, gk: fp32 [D], both or
  * neither (rotation alone).  Forward writes q_out / k_out.  Backward reads q, k and the gradients
  * dq, dk of the outputs, writes the inputs' gradients to q_out / k_out and the weights' to dgq / dgk (sums over rows and heads,
- * written, not added).  q_out / k_out may be q / k themselves (backward: dq / dk too) and may not overlap anything else; ws: simvg_qk_norm_rope_ws_floats(T, D) floats. */
+ * written, not added).  q_out / k_out may be q / k themselves (backward: dq / dk too) and may not overlap anything else.
+ * ws: simvg_qk_norm_rope_ws_floats(T, D) floats. */
 typedef struct simvg_qk_norm_rope_args {
   int dtype, T, Hq, Hkv, D, n_axes, sections[4], interleaved, pos_is_64;
   float eps;
@@ -503,7 +504,7 @@ int simvg_packed_attn_bwd(const simvg_packed_attn_args* args, simvg_stream_t str
  *   neither a word in [0, V) nor ignore_index.
  * x: [M][K], w: [V][K], fp16 / bf16, K a multiple of 8; bias: fp32 [V] or NULL; target: int64 [M].
  * Backward, for the gradients dloss [M] of the rows' losses: dx [M][K], dw [V][K] in the operands' type, dbias fp32 [V] (NULL: not
- * wanted); all are written, not added.  Ignored rows, and rows whose target is no word, have no part in any of them.
+ * wanted); all are written, not added, and may not overlap the operands.  Ignored rows, and rows whose target is no word, have no part in any of them.
  * ws: simvg_vocab_ce_ws_bytes(M, V, K, bias wanted, backward) bytes, aligned to 256. */
 typedef struct simvg_vocab_ce_args {
   int dtype, M, V, K;

@@ -1160,10 +1160,11 @@ int attn_check(const simvg_packed_attn_args* a, bool bwd) {
     SIMVG_CHECK_ARG(a->ws && (uintptr_t)a->ws % 16 == 0, "packed_attn: the backward pass needs a workspace, aligned to 16 bytes");
   }
   // the operands are read by many workgroups until the last one is done: results have memory of their own
-  const Rows in[] = {{a->q, a->q_ts, a->q_hs, a->Hq}, {a->k, a->k_ts, a->k_hs, a->Hkv}, {a->v, a->v_ts, a->v_hs, a->Hkv},
-                     {a->o, a->o_ts, a->o_hs, a->Hq}, {a->d_o, a->do_ts, a->do_hs, a->Hq}};
-  const Rows out[] = {{a->dq, a->dq_ts, a->dq_hs, a->Hq}, {a->dk, a->dk_ts, a->dk_hs, a->Hkv}, {a->dv, a->dv_ts, a->dv_hs, a->Hkv}};
-  const auto apart = [&](const Rows& x, const Rows& y) { return rows_apart(x, y, a->T, a->D, 2); };
+  const int T = a->T, Hq = a->Hq, Hkv = a->Hkv;
+  const Rows in[] = {{a->q, a->q_ts, a->q_hs, T, Hq}, {a->k, a->k_ts, a->k_hs, T, Hkv}, {a->v, a->v_ts, a->v_hs, T, Hkv},
+                     {a->o, a->o_ts, a->o_hs, T, Hq}, {a->d_o, a->do_ts, a->do_hs, T, Hq}};
+  const Rows out[] = {{a->dq, a->dq_ts, a->dq_hs, T, Hq}, {a->dk, a->dk_ts, a->dk_hs, T, Hkv}, {a->dv, a->dv_ts, a->dv_hs, T, Hkv}};
+  const auto apart = [&](const Rows& x, const Rows& y) { return rows_apart(x, y, T, a->D, 2); };
   for (int i = 0; i < 5; ++i)
     for (int j = 0; j < 3; ++j)
       SIMVG_CHECK_ARG(bwd ? apart(in[i], out[j]) : i || apart(in[j], in[3]), "packed_attn: a result overlaps an operand or another result");

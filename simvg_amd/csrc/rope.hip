@@ -367,8 +367,8 @@ int rope_check(const simvg_qk_norm_rope_args* a, bool bwd, int& P) {
   SIMVG_CHECK_ARG(!bwd || !a->gq || (a->dgq && a->dgk && a->ws), "qk_norm_rope: the weights' gradients need outputs and a workspace");
   SIMVG_CHECK_ARG(a->pos_ld >= a->n_axes || a->T <= 1, "qk_norm_rope: rows of positions are shorter than the axes");
   // a row is read whole before it is written: results may lie where their own operands do, row on row, and nowhere else on an operand
-  const Rows q = {a->q, a->q_ts, a->q_hs, a->Hq}, k = {a->k, a->k_ts, a->k_hs, a->Hkv}, dq = {a->dq, a->dq_ts, a->dq_hs, a->Hq},
-             dk = {a->dk, a->dk_ts, a->dk_hs, a->Hkv}, qo = {a->q_out, a->qo_ts, a->qo_hs, a->Hq}, ko = {a->k_out, a->ko_ts, a->ko_hs, a->Hkv};
+  const Rows q(a->q, a->q_ts, a->q_hs, a->T, a->Hq), k(a->k, a->k_ts, a->k_hs, a->T, a->Hkv), dq(a->dq, a->dq_ts, a->dq_hs, a->T, a->Hq),
+      dk(a->dk, a->dk_ts, a->dk_hs, a->T, a->Hkv), qo(a->q_out, a->qo_ts, a->qo_hs, a->T, a->Hq), ko(a->k_out, a->ko_ts, a->ko_hs, a->T, a->Hkv);
   const auto apart = [&](const Rows& x, const Rows& y) { return rows_apart(x, y, a->T, a->D, a->dtype == SEQ_F32 ? 4 : 2); };
   const auto over = [&](const Rows& out, const Rows& in) { return out.same(in) || apart(out, in); };
   SIMVG_CHECK_ARG(apart(qo, ko) && over(qo, q) && over(ko, k) && apart(qo, k) && apart(ko, q),

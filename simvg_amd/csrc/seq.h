@@ -8,7 +8,6 @@
 #include <algorithm>
 #include <atomic>
 #include <cstdlib>
-#include <initializer_list>
 #include <numeric>
 
 #include "common.h"
@@ -86,18 +85,15 @@ __device__ __forceinline__ void wave_barrier_only() { asm volatile("s_waitcnt lg
 // ---- where an operand [T][H][D] lies, for the host's checks that results have memory of their own
 struct Rows {
   const void* p; long ts, hs; int H;
+  Rows(const void* p, long ts, long hs, int T, int H) : p(p), ts(T > 1 ? ts : 0), hs(H > 1 ? hs : 0), H(H) {}       // (strides that are never walked)
   bool same(const Rows& o) const { return p == o.p && ts == o.ts && hs == o.hs && H == o.H; }
 };
 // Whether two operands of the same T, D and size of a value have no value in common.  Slices of one buffer lie in each other's range and
 // are told apart by their rows: the distance of two heads' rows is d + i ts for tokens i apart.  Exact where the token strides are the
 // same; where they are not, rows that could meet in an endless tensor (a multiple of the strides' common divisor apart) count as meeting.
-inline bool rows_apart(Rows a, Rows b, int T, int D, int size) {
-  if (T <= 0 || a.H <= 0 || b.H <= 0 || !a.p || !b.p) return true;
-  for (Rows* r : {&a, &b}) {                                 // strides that are never walked
-    if (T == 1) r->ts = 0;
-    if (r->H == 1) r->hs = 0;
-  }
-  const long start = ((intptr_t)b.p - (intptr_t)a.p), row = (long)D * size;
+inline bool rows_apart(const Rows& a, const Rows& b, int T, int D, int size) {
+  if (T <= 0 || !a.p || !b.p) return true;
+  const long start = (intptr_t)b.p - (intptr_t)a.p, row = (long)D * size;
   const auto low = [&](const Rows& r) { return std::min(0L, (T - 1) * r.ts * size) + std::min(0L, (r.H - 1) * r.hs * size); };
   const auto high = [&](const Rows& r) { return std::max(0L, (T - 1) * r.ts * size) + std::max(0L, (r.H - 1) * r.hs * size) + row; };
   if (start + low(b) >= high(a) || low(a) >= start + high(b)) return true;

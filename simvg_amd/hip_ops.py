@@ -1417,8 +1417,9 @@ def _packed_args(q, k, v, plan, causal, scale, fill_tail):
 def packed_attn_fwd(q, k, v, plan, causal=True, scale=None, out=None):
     """Attention over packed sequences (csrc/packed_attn.hip): q [T, Hq, D], k, v [T, Hkv, D], fp16 or bf16, `plan` from `packed_plan`.
     Returns (out [T, Hq, D], lse [Hq, T] fp32).  Rows behind the last sequence are zeros; in an `out` of the caller's, which may not
-    overlap the operands, they stay as they were (lse's are zeros; NaN where `cu_seqlens` was no valid list).  A row whose visible scores are all -inf is NaN.  Scores of any finite size are right here;
-    `packed_attn_bwd` takes the probabilities from lse, which holds them to one part in 2^24 of a row's largest |scale q k|."""
+    overlap the operands, they stay as they were (lse's are zeros; NaN where `cu_seqlens` was no valid list).  A row whose visible scores are
+    all -inf is NaN.  Finite scores may be of any size here; `packed_attn_bwd` has the probabilities from lse, whose rounding, 2^-24 of a
+    row's largest score, is their relative error.  scale: positive, None: D ** -0.5."""
     lib = _lib.load()
     fill = out is None
     args, dev = _packed_args(q, k, v, plan, causal, scale, 1 if fill else 2)

@@ -4,6 +4,7 @@ import itertools
 import random
 
 import pytest
+import torch
 
 from simvg_amd import _lib
 
@@ -32,7 +33,7 @@ def rope_args(**over):
                                        inv_freq=1 << 21, gq=1 << 22, gk=1 << 22, dgq=1 << 23, dgk=1 << 24, ws=1 << 25) | at | strides | over))
 
 
-NO_DEVICE = pytest.mark.skipif(__import__("torch").cuda.is_available(), reason="would launch on made-up addresses")
+NO_DEVICE = pytest.mark.skipif(torch.cuda.device_count() > 0, reason="would launch on made-up addresses")
 
 
 def test_rotation_refuses_results_on_other_operands():
@@ -57,6 +58,8 @@ def test_rotation_takes_results_in_place_and_slices_of_one_buffer():
                dict(k=q + 512, q_out=q, k_out=q + 512, **fused)):
         for fn in (lib.simvg_qk_norm_rope_fwd, lib.simvg_qk_norm_rope_bwd):
             assert not refused(fn, rope_args(**ok), "overlaps"), ok
+    for ok in (dict(T=1, q_out=q, qo_ts=8, k_out=k, ko_ts=1 << 24), dict(Hkv=1, k_out=k, ko_hs=8)):       # strides that are never walked
+        assert not refused(lib.simvg_qk_norm_rope_fwd, rope_args(**ok), "overlaps"), ok
     for ok in (dict(q_out=dq, k_out=dk), dict(q_out=q, k_out=dk)):
         assert not refused(lib.simvg_qk_norm_rope_bwd, rope_args(**ok), "overlaps"), ok
 
