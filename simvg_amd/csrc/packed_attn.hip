@@ -50,6 +50,10 @@ using namespace seq;
 
 constexpr int QT = 128;                                      // rows of a plan entry
 constexpr int KT = 64;                                       // rows of a tile in LDS
+// Up to this many tiles of keys to a workgroup's queries (queries to its keys) P and dS go into their products in two parts, as rounded to
+// 16 bits and what that took off: a result of few terms, in a batch of few and short sequences, shows their rounding beside its own
+// (154 sequences of two rows: dQ off by 1.53 of what its last rounding costs, bf16), longer sums keep sqrt(2) of it.
+constexpr int FEW = 2;
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr float NEG_INF = -__builtin_huge_valf();
 constexpr float FAR = 4096.f;                                // exponents beyond it: the reference is subtracted before the scaling, not in its fma
@@ -235,6 +239,18 @@ __device__ __forceinline__ lpx8_t acc_frag(const f32x16& p, int rk) {
                      E::pack(p[8 * rk + 6], p[8 * rk + 7])};
   return __builtin_bit_cast(lpx8_t, u);
 }
+// what that rounding took off them: the registers less what the operand holds
+template <class E>
+__device__ __forceinline__ lpx8_t acc_rest(f32x16& p, int rk) {
+#pragma unroll
+  for (int r = 8 * rk; r < 8 * rk + 8; r += 2) {
+    float a, b;
+    unpack2<E>(E::pack(p[r], p[r + 1]), a, b);
+    p[r] -= a;
+    p[r + 1] -= b;
+  }
+  return acc_frag<E>(p, rk);
+}
 // the other half of the wave's value of v (lane ^ 32), joined with this half's
 __device__ __forceinline__ float max_halves(float v) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -255,6 +271,14 @@ template <class E>
 __device__ __forceinline__ unsigned finite_mask(unsigned u) {          // all bits of each half that holds a finite value
   const int lo = (int)(u & 0x7fffu) - E::kInf, hi = (int)(u >> 16 & 0x7fffu) - E::kInf;
   return ((unsigned)(lo >> 31) & 0xffffu) | ((unsigned)(hi >> 31) << 16);
+}
+// a fragment with zeros where values are not finite
+template <class E>
+__device__ __forceinline__ lpx8_t finite(lpx8_t f) {
+  u32x4_t v = __builtin_bit_cast(u32x4_t, f);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] &= finite_mask<E>(v[j]);
+  return __builtin_bit_cast(lpx8_t, v);
 }
 // The workgroup's 256 threads look through a tile, each its share; the same answer in all of them.  (The barrier inside also waits for
 // the tile that is on its way: this is done for the two or three tiles of a workgroup that a mask crosses, not for the others.)
@@ -381,7 +405,7 @@ __device__ __forceinline__ void store_sums(const f32x16 (&acc)[DP / 32], float m
 // ------------------------------------------------------------------------------------------------------------- forward
 // ws, where the keys are cut into parts: (reference, sum) [parts][T][Hq], a multiple of 16 bytes, then numerators [parts][T][Hq][D]
 __host__ __device__ __forceinline__ long ws_stats(long parts, long T, long Hq) { return (2 * parts * T * Hq + 3) / 4 * 4; }
-template <class E, int DP, bool CAUSAL>
+template <class E, int DP, bool CAUSAL, bool SHORT>
 __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_fwd_kernel(simvg_packed_attn_args a, int parts) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   constexpr int TILE = KT * DP * 2, DB = DP / 32, KS = DP / 16;
@@ -401,6 +425,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_fwd_kernel(
   // the tiles of keys, and this part's of them: [kt0, tiles)
   const int keys = CAUSAL ? min(e.len, (e.t + 1) * QT) : e.len, all_tiles = (keys + KT - 1) / KT;
   const int kt0 = all_tiles * part / parts, tiles = all_tiles * (part + 1) / parts;
+  const bool few = SHORT && all_tiles <= FEW;
   const int wave_first = e.t * QT + wave * 32;               // the wave's first query
   // tiles that no mask touches come first, then those that the diagonal or the sequence's end crosses, then (for the wave) nothing
   const int whole = min(tiles, min(CAUSAL ? (e.t * QT + 1) / KT : tiles, e.len / KT));         // of all four waves
@@ -415,6 +440,10 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_fwd_kernel(
   if (kt0 < tiles) {
     gk.template next<0>();
     gv.template next<0>();
+  }
+  if (few && kt0 + 1 < tiles) {
+    gk.template next<1>();
+    gv.template next<1>();
   }
   lpx8_t qf[KS];
 #pragma unroll
@@ -509,6 +538,74 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_fwd_kernel(
       }
     }
   };
+  auto finish = [&] {
+    l += __shfl_xor(l, 32, 64);
+    const auto z = late_args<simvg_packed_attn_args>();
+    if (parts == 1) {
+      unsigned short* out = (unsigned short*)z->o + (long)(e.first + row) * z->o_ts + (long)h * z->o_hs;
+      store_rows<E, DP>(o, 1.f / l, out, z->D, valid, lane);
+      if (valid && lane < 32) z->lse[(long)h * z->lse_hs + e.first + row] = m * z->scale + __builtin_logf(l);
+    } else {
+      const long n = (long)z->T * z->Hq, at = (long)(e.first + row) * z->Hq + h;
+      store_sums<DP>(o, 1.f, z->ws + ws_stats(parts, z->T, z->Hq) + (part * n + at) * z->D, z->D, valid, lane);
+      if (valid && lane < 32) ((float2*)z->ws)[part * n + at] = make_float2(m, l);
+    }
+  };
+  if (few) {
+    // Both tiles are in LDS, one behind the other: 32 keys at a time, the maximum first, then exponentials and products
+    dma_wait<0>();
+    wave_barrier_only();
+    bool odd = false;
+    for (int kt = 0; kt < tiles - kt0; ++kt) odd |= tile_nonfinite<E, DP>(smem + (2 + kt) * TILE);
+    const int last = (CAUSAL ? min(row, e.len - 1) : e.len - 1) - kt0 * KT;
+    const int wave_last = (CAUSAL ? min(wave_first + 31, e.len - 1) : e.len - 1) - kt0 * KT;
+    const int blocks = live ? min(2 * (tiles - kt0), (wave_last >> 5) + 1) : 0;
+    auto scores = [&](int b) {
+      const int last4 = last - b * 32 - (lane >> 5) * 4;
+      f32x16 s = zero16();
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) s = E::mfma(at.row(b * 32 * DP * 2, 0, ks), qf[ks], s);
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (reg_row(r) > last4) s[r] = NEG_INF;
+      return s;
+    };
+#pragma unroll 1
+    for (int b = 0; b < blocks; ++b) {
+      const f32x16 s = scores(b);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) m = fmaxf(m, s[r]);
+    }
+    m = max_halves(m);
+    if (odd && live)
+      for (int kt = 0; kt < tiles - kt0; ++kt)
+        add_nonfinite<E, DP, false>(o, smem + (2 + kt) * TILE, lane, [&](int j) { return j <= last - kt * KT; });
+    const bool far = fabsf(m * c) > FAR;                     // as in a tile of many
+    const float mc = far ? 0.f : m * c, base = far && m != NEG_INF ? m : 0.f;
+#pragma unroll 1
+    for (int b = 0; b < blocks; ++b) {
+      f32x16 s = scores(b);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[r] = __builtin_amdgcn_exp2f(fmaf(s[r] - base, c, -mc));
+        l += s[r];
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int rk = 0; rk < 2; ++rk) {
+        const lpx8_t p = acc_frag<E>(s, rk), rest = acc_rest<E>(s, rk);
+#pragma unroll
+        for (int cb = 0; cb < DB; ++cb) {
+          lpx8_t v = at.col(2 * TILE + b * 32 * DP * 2, rk, cb);
+          if (odd) v = finite<E>(v);
+          o[cb] = E::mfma(v, p, o[cb]);
+          o[cb] = E::mfma(v, rest, o[cb]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    return finish();
+  }
   int kt = kt0;
   for (; kt + 1 < whole; kt += 2) {
     tile(kt, std::integral_constant<int, 0>{}, std::false_type{});
@@ -518,17 +615,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_fwd_kernel(
     tile(kt, std::integral_constant<int, 0>{}, std::true_type{});
     if (kt + 1 < tiles) tile(kt + 1, std::integral_constant<int, 1>{}, std::true_type{});
   }
-  l += __shfl_xor(l, 32, 64);
-  const auto z = late_args<simvg_packed_attn_args>();
-  if (parts == 1) {
-    unsigned short* out = (unsigned short*)z->o + (long)(e.first + row) * z->o_ts + (long)h * z->o_hs;
-    store_rows<E, DP>(o, 1.f / l, out, z->D, valid, lane);
-    if (valid && lane < 32) z->lse[(long)h * z->lse_hs + e.first + row] = m * z->scale + __builtin_logf(l);
-  } else {
-    const long n = (long)z->T * z->Hq, at = (long)(e.first + row) * z->Hq + h;
-    store_sums<DP>(o, 1.f, z->ws + ws_stats(parts, z->T, z->Hq) + (part * n + at) * z->D, z->D, valid, lane);
-    if (valid && lane < 32) ((float2*)z->ws)[part * n + at] = make_float2(m, l);
-  }
+  finish();
 }
 // the parts of a row joined: out = sum O_p 2^((m_p - m) c) / sum l_p 2^((m_p - m) c), c = scale log2(e); 16 lanes a row
 template <class E>
@@ -685,7 +772,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_dq_kernel(s
   // would show: dS of a row that sees n keys alike is off by its own rounding and by about 1 / sqrt(n) of it for delta's, and the few rows
   // with few keys hold the largest gradients (a sequence of 100 rows: dK 1.62 times as far off as its last rounding alone, and 1.42, what
   // dS's own rounding costs, with this).  Both tiles stay in LDS for the second pass.
-  const bool few = all_tiles <= 2;
+  const bool few = all_tiles <= FEW;
   const int kt0 = few ? (part ? all_tiles : 0) : all_tiles * part / parts, tiles = few ? all_tiles : all_tiles * (part + 1) / parts;
   const int wave_first = e.t * QT + wave * 32;
   const int whole = min(tiles, min(CAUSAL ? (e.t * QT + 1) / KT : tiles, e.len / KT));         // of all four waves
@@ -755,7 +842,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_dq_kernel(s
     constexpr bool MASKED = decltype(crossed)::value;
     dma_wait<0>();
     wave_barrier_only();
-    if (kt + 1 < tiles && !few) {
+    if (kt + 1 < tiles) {
       gk.template next<BUF ^ 1>();
       gv.template next<BUF ^ 1>();
     }
@@ -807,14 +894,49 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void packed_attn_dq_kernel(s
       products(1);
     }
   };
-  int kt = kt0;
-  for (; kt + 1 < whole; kt += 2) {
-    tile(kt, std::integral_constant<int, 0>{}, std::false_type{});
-    tile(kt + 1, std::integral_constant<int, 1>{}, std::false_type{});
-  }
-  for (; kt < tiles; kt += 2) {
-    tile(kt, std::integral_constant<int, 0>{}, std::true_type{});
-    if (kt + 1 < tiles) tile(kt + 1, std::integral_constant<int, 1>{}, std::true_type{});
+  if (few) {                                                 // as in the forward pass
+    bool odd = false;
+    for (int kt = 0; kt < tiles - kt0; ++kt) odd |= tile_nonfinite<E, DP>(smem + kt * TILE);
+    const int last = CAUSAL ? min(row, e.len - 1) : e.len - 1;
+    if (odd && live)
+      for (int kt = 0; kt < tiles - kt0; ++kt)
+        add_nonfinite<E, DP, true>(dq, smem + kt * TILE, lane, [&](int j) { return j <= last - kt * KT; });
+#pragma unroll 1
+    for (int b = 2 * kt0; b < 2 * wave_tiles; ++b) {
+      const int at_b = b * 32 * DP * 2, last4 = last - b * 32 - (lane >> 5) * 4;
+      f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        s = E::mfma(at.row(at_b, 0, ks), qf[ks], s);
+        dp = E::mfma(at.row(2 * TILE + at_b, 0, ks), dof[ks], dp);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float p = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse2));
+        s[r] = reg_row(r) > last4 ? 0.f : E::kScaled ? p * ((dp[r] - delta) * up) : p * (dp[r] - delta);
+      }
+#pragma unroll
+      for (int rk = 0; rk < 2; ++rk) {
+        const lpx8_t ds = acc_frag<E>(s, rk), rest = acc_rest<E>(s, rk);
+#pragma unroll
+        for (int cb = 0; cb < DB; ++cb) {
+          lpx8_t k = at.col(at_b, rk, cb);
+          if (odd) k = finite<E>(k);
+          dq[cb] = E::mfma(k, ds, dq[cb]);
+          dq[cb] = E::mfma(k, rest, dq[cb]);
+        }
+      }
+    }
+  } else {
+    int kt = kt0;
+    for (; kt + 1 < whole; kt += 2) {
+      tile(kt, std::integral_constant<int, 0>{}, std::false_type{});
+      tile(kt + 1, std::integral_constant<int, 1>{}, std::false_type{});
+    }
+    for (; kt < tiles; kt += 2) {
+      tile(kt, std::integral_constant<int, 0>{}, std::true_type{});
+      if (kt + 1 < tiles) tile(kt + 1, std::integral_constant<int, 1>{}, std::true_type{});
+    }
   }
   const auto z = late_args<simvg_packed_attn_args>();
   const float mul = z->scale * __builtin_amdgcn_exp2f(-power - shift);
@@ -1004,6 +1126,37 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void packed_attn_dkv_kernel(
         }
         p[0] = np[0]; p[1] = np[1]; ds[0] = nds[0]; ds[1] = nds[1];
       };
+      if (tiles <= FEW) {                                    // what the rounding of P and dS will take off, first
+        stay_a_branch();
+#pragma unroll 1
+        for (int qb = 0; qb < 2; ++qb) {
+#pragma unroll
+          for (int g = 0; g < N; ++g) rows(g, stage, qb);
+          start(0);
+#pragma unroll
+          for (int g = 0; g < N; ++g) scores(g, 0);
+#pragma unroll
+          for (int g = 0; g < N; ++g) cols(g, stage, qb);
+#pragma unroll
+          for (int r = 0; r < 16; r += 2) {
+            float p0 = __builtin_amdgcn_exp2f(fmaf(s[0][r], c, -ls[0][r / 4][r % 4])), p1 = __builtin_amdgcn_exp2f(fmaf(s[0][r + 1], c, -ls[0][r / 4][r % 4 + 1]));
+            float d0 = E::kScaled ? p0 * (dp[0][r] * up) : p0 * dp[0][r], d1 = E::kScaled ? p1 * (dp[0][r + 1] * up) : p1 * dp[0][r + 1], a0, a1;
+            unpack2<E>(E::pack(p0, p1), a0, a1);
+            np[r / 8][r % 8 / 2] = E::pack(p0 - a0, p1 - a1);
+            unpack2<E>(E::pack(d0, d1), a0, a1);
+            nds[r / 8][r % 8 / 2] = E::pack(d0 - a0, d1 - a1);
+          }
+          rounded(qb);
+#pragma unroll
+          for (int g = 0; g < N; ++g) products(g);
+          stat += 32;
+        }
+        stat -= 64;
+        if constexpr (PIPED) {
+#pragma unroll
+          for (int g = 0; g < N; ++g) rows(g, stage, 0);
+        }
+      }
       if constexpr (PIPED) {
         start(0);
 #pragma unroll
@@ -1129,6 +1282,10 @@ int row_parts(int T, int nseq, int Hq, int causal) {
 int key_parts(int T, int nseq, int Hq, int Hkv, int causal) {
   return parts_of((long)plan_capacity(T, nseq) * Hkv, (long)T / std::max(nseq, 1) / KT * (Hq / Hkv), causal);
 }
+// Whether a forward pass looks for workgroups with few tiles (FEW): where sequences are of 128 rows or less on average, or few rows at
+// all.  The path for them takes registers from the others' (64 x 411 rows, 12 heads of 64: 65.0 us without and 66.6 with it; one sequence of
+// 16384 rows, 16 heads of 128: 1013 and 1022); dQ, dK and dV have it at no cost.
+bool short_rows(int T, int nseq) { return T <= (long)QT * std::max(nseq, 16); }
 // the parts' sums of the backward pass: dQ's and then dK's and dV's use the same room
 long bwd_sums(int T, int nseq, int Hq, int Hkv, int D, int causal) {
   const int r = row_parts(T, nseq, Hq, causal), k = key_parts(T, nseq, Hq, Hkv, causal);
@@ -1184,15 +1341,20 @@ constexpr int dkv_lds(int DP) { return DKV_STAGES * (2 * KT * DP * 2 + 2 * KT * 
 
 template <class E, int DP, bool CAUSAL>
 void attn_launch(const simvg_packed_attn_args& a, bool bwd, hipStream_t s) {
-  static std::atomic<unsigned long> done[3] = {{0}, {0}, {0}};               // the tiles of 128 columns and the kernels' own few bytes pass 64 KiB
-  if (!bwd) allow_lds((const void*)packed_attn_fwd_kernel<E, DP, CAUSAL>, 4 * KT * DP * 2, done[0]);
+  static std::atomic<unsigned long> done[4] = {{0}, {0}, {0}, {0}};               // the tiles of 128 columns and the kernels' own few bytes pass 64 KiB
+  if (!bwd) allow_lds((const void*)packed_attn_fwd_kernel<E, DP, CAUSAL, false>, 4 * KT * DP * 2, done[0]);
   else {
     allow_lds((const void*)packed_attn_dq_kernel<E, DP, CAUSAL>, 4 * KT * DP * 2, done[1]);
     allow_lds((const void*)packed_attn_dkv_kernel<E, DP, CAUSAL>, dkv_lds(DP), done[2]);
   }
   const int entries = plan_capacity(a.T, a.nseq), lds = 4 * KT * DP * 2, rparts = row_parts(a.T, a.nseq, a.Hq, a.causal);
   if (!bwd) {
-    hipLaunchKernelGGL((packed_attn_fwd_kernel<E, DP, CAUSAL>), dim3(entries * a.Hq * rparts), dim3(256), lds, s, a, rparts);
+    if (short_rows(a.T, a.nseq)) {
+      allow_lds((const void*)packed_attn_fwd_kernel<E, DP, CAUSAL, true>, lds, done[3]);
+      hipLaunchKernelGGL((packed_attn_fwd_kernel<E, DP, CAUSAL, true>), dim3(entries * a.Hq * rparts), dim3(256), lds, s, a, rparts);
+    } else {
+      hipLaunchKernelGGL((packed_attn_fwd_kernel<E, DP, CAUSAL, false>), dim3(entries * a.Hq * rparts), dim3(256), lds, s, a, rparts);
+    }
     if (rparts > 1)
       hipLaunchKernelGGL((packed_attn_fwd_join_kernel<E>), dim3((int)min(((long)a.T * a.Hq + 15) / 16, 8192L)), dim3(256), 0, s, a, rparts);
     return;

@@ -289,3 +289,70 @@ def test_strides_of_dimensions_of_one_mean_nothing(T, Hkv):
     got += ops.packed_attn_bwd(a, b, c, odd(got[0]), got[1], d, plan, dq=odd(torch.zeros_like(q)), dk=odd(torch.zeros_like(k)),
                                dv=odd(torch.zeros_like(v)))
     assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+# ------------------------------------------------------------------------------------------------------------- few terms in a result
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("lens,Hq,Hkv,D", [([2] * 154, 2, 2, 32), ([2] * 9, 1, 1, 128), ([1, 20, 5, 128, 127, 0, 65], 4, 2, 64), ([3, 7] * 11, 3, 1, 128),
+                                           ([64] * 7, 6, 2, 80), ([33], 1, 1, 8)], ids=lambda x: "-".join(map(str, x[:3])) if isinstance(x, list) else str(x))
+def test_short_sequences_are_as_exact_as_their_last_rounding(lens, Hq, Hkv, D, dt, causal):
+    """P and dS, where few of them make a result, are not rounded to 16 bits: what is off is the result's own rounding and what 32 bits lose
+    (at most n + 2 D + 64 steps of 2^-24 of the terms' magnitudes: a fourteenth of half a step of fp16 where all of them add up)"""
+    q, k, v, do, cu = attn_case(lens, Hq, Hkv, D, dt)
+    plan = ops.packed_plan(cu, sum(lens))
+    o, lse = ops.packed_attn_fwd(q, k, v, plan, causal)
+    dq, dk, dv = ops.packed_attn_bwd(q, k, v, o, lse, do, plan, causal)
+    ref = R.attention(q, k, v, lens, causal, D ** -0.5, do)
+    for name, got in dict(o=o, dq=dq, dk=dk, dv=dv).items():
+        least = (ref[name].to(dt).double() - ref[name]).norm()
+        assert float((got.double() - ref[name]).norm()) <= 1.1 * float(least) + 1e-6 * float(ref[name].norm()), name
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("lens,D", [([20, 0, 7, 1, 13], 64), ([65, 63, 129, 127, 1], 64), ([421, 401, 0, 413], 128), ([64, 128, 700], 40)],
+                         ids=["few", "tiles", "long", "odd"])
+def test_short_sequences_in_a_long_batch(lens, D, dt, causal):
+    """many rows behind the last sequence: on average a batch of long ones, whose forward pass has no path of its own for short ones"""
+    n, tail = sum(lens), 2100
+    q, k, v, do, cu = attn_case(lens, 4, 2, D, dt, tail=tail)
+    plan = ops.packed_plan(cu, n + tail)
+    o, lse = ops.packed_attn_fwd(q, k, v, plan, causal)
+    dq, dk, dv = ops.packed_attn_bwd(q, k, v, o, lse, do, plan, causal)
+    ref = R.attention(q[:n], k[:n], v[:n], lens, causal, D ** -0.5, do[:n])
+    got = dict(o=o[:n], lse=lse[:, :n], dq=dq[:n], dk=dk[:n], dv=dv[:n])
+    worst = {name: R.off(t, ref[name], ref["tol"][name]) for name, t in got.items()}
+    assert max(worst.values()) <= 1, worst
+    assert not any(t[n:].any() for t in (o, dq, dk, dv)) and not lse[:, n:].any()
+
+
+@pytest.mark.parametrize("tail", [0, 2100])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("lens,at", [([100], 60), ([70, 190], 160), ([128], 0)])
+def test_later_rows_that_are_not_finite(lens, at, value, tail):
+    """under `causal`, in the path for few tiles and in the other one, forward and backward"""
+    q, k, v, do, cu = attn_case(lens, 4, 2, 64, BF16, tail=tail)
+    n = sum(lens)
+    plan = ops.packed_plan(cu, n + tail)
+
+    def run(**x):
+        a = dict(q=q, k=k, v=v, do=do) | x
+        o, lse = ops.packed_attn_fwd(a["q"], a["k"], a["v"], plan)
+        return (o, *ops.packed_attn_bwd(a["q"], a["k"], a["v"], o, lse, a["do"], plan))
+    want = run()
+    for name, t in dict(q=q, k=k, v=v, do=do).items():
+        x = t.clone()
+        x[at] = value
+        got = run(**{name: x})
+        if name in "kv":                                                   # earlier queries do not see the key
+            assert torch.equal(got[0][:at], want[0][:at]) and torch.equal(got[1][:at], want[1][:at]), name
+            if name == "v":
+                assert not bool(torch.isfinite(got[0][at:n]).any())
+                assert value != value or bool((got[0][at:n] == value).all())
+        else:                                                              # later keys are not seen by the query
+            assert torch.equal(got[2][at + 1:], want[2][at + 1:]) and torch.equal(got[3][at + 1:], want[3][at + 1:]), name
+            assert not bool(torch.isfinite(got[2][at]).all()), name
+            rows = torch.arange(n + tail, device=DEV) != at
+            assert torch.equal(got[0][rows], want[0][rows]) and torch.equal(got[1][rows], want[1][rows]), name
