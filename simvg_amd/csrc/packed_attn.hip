@@ -12,12 +12,12 @@
 // lane already has -- the order of the contraction's keys is free, and the transposed reads (ds_read_b64_tr_b16) that fetch V^T use
 // the order in which the accumulator holds them.  P and dS never leave registers.
 //
-// Measured, of 1.46 (fp16) and 1.44 (bf16) PFLOP/s that a library product of 8192^3 reaches: one sequence of 16384 rows, 16 heads of 128
-// on 2, causal, bf16, forward 1.01 ms, 1.09 PFLOP/s; nine of up to 4097 rows, 32 heads on 8: forward 0.49 ms, 0.92; dQ 0.69 ms and dK, dV
-// 1.06 ms, 0.98 and 0.85 of what each computes (6 D and 8 D: both need the scores).  Half of the time the matrix pipes work (the clock
-// falls to 1.7 GHz under them), a third goes to the exponentials and the rest of the vector work, which one or two waves to a SIMD
-// cover in part.  Heads of 64 (64 x 411 rows, 12 heads, no mask, fp16): forward 68 us, dQ 92, dK and dV 132: vector work, as much
-// for half the products.
+// Measured, medians, of 1.46 (fp16) and 1.44 (bf16) PFLOP/s that a library product of 8192^3 reaches: one sequence of 16384 rows, 16 heads
+// of 128 on 2, causal, bf16, forward 1.00 ms (1.05 on a slower card), 1.10 PFLOP/s; nine of up to 4097 rows, 32 heads on 8: forward 0.49 ms,
+// 0.92; dQ 0.69 ms and dK, dV 1.05 ms, 0.99 and 0.86 of what each computes (6 D and 8 D: both need the scores).  Half of the time the matrix
+// pipes work (the clock falls to 1.7 GHz under them), a third goes to the exponentials and the rest of the vector work, which one or two
+// waves to a SIMD cover in part.  Heads of 64 (64 x 411 rows, 12 heads, no mask, fp16): forward 66 us, delta and norms 24, dQ 91, dK and dV
+// 133: vector work, as much for half the products, and for dK and dV start and end of workgroups of seven tiles, about half of their time.
 //
 // Which rows a workgroup takes stands in a plan that the caller has built once for a batch (packed_plan_kernel): one entry for each
 // tile of 128 rows of each sequence, tiles far down a sequence first, because under `causal` they cost most and the last workgroups to

@@ -13,9 +13,10 @@
 // take a head's row each, a lane holding the two chunks of 16 bytes whose values are each other's partners, so that nothing but the
 // sum of squares crosses lanes.
 //
-// Measured (a copy of 4 GiB reaches 4.7 TB/s, one that stays in the 256 MB memory-side cache 7.2): 26944 tokens, 24 heads of 64, fp16,
-// forward: 35 us, 4.7 TB/s; 16384 tokens, 40 heads of 128, bf16: forward 56 us, 6.0 TB/s, backward 110 us with the join of the weights'
-// gradients, 4.6 TB/s; one token: 4 us.
+// Measured, medians (a copy of 4 GiB reaches 4.7 TB/s, one that stays in the 256 MB memory-side cache 7.2): 26944 tokens, 24 heads of 64,
+// fp16, forward: 36 us, 4.6 TB/s; 16384 tokens, 40 heads of 128, bf16: forward 60 us, 5.6 TB/s, backward 116 us and the join of the weights'
+// gradients 5, 4.2 TB/s; one token: 4 us.  Rows that start anywhere, a value at a time: 144 us where chunks take 48 (26944 tokens, fp16,
+// the call included), backward 292 and 87.
 #include "seq.h"
 
 struct simvg_qk_norm_rope_args {
@@ -35,8 +36,9 @@ using namespace seq;
 
 constexpr int ROPE_MAX_D = 256;
 // Workgroups of the backward pass, one partial sum of (dgq | dgk) each: as many as the chip holds at once (three to a compute unit with
-// 16-bit values, four with 32-bit ones), each walking its share of the tokens.  16384 tokens, 40 heads of 128, bf16: 110 us with 768, 134
-// with 1024, 121 with 2048; 4099 tokens, fp32: 17.9, 17.0, 18.8.
+// 16-bit values, four with 32-bit ones), each walking its share of the tokens.  16384 tokens, 40 heads of 128, bf16, in turn on one card: 110
+// us with 768, 134 with 1024, 121 with 2048; 4099 tokens, fp32: 17.9, 17.0, 18.8.  (The kernels for single values would fit six to a
+// compute unit; they were not measured with other numbers.)
 constexpr int ROPE_BWD_BLOCKS = 1024;
 int rope_bwd_blocks(int T, int dtype) { return min(cdiv(T, 4), dtype == SEQ_F32 ? ROPE_BWD_BLOCKS : 768); }
 

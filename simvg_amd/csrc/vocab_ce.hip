@@ -12,9 +12,9 @@
 // are products over the vocabulary and over the rows: their operands lie "the other way round" in memory and are read from LDS with
 // the transposing ds_read_b64_tr_b16, so that nothing is ever laid out twice.
 //
-// Measured at 8191 rows, 64010 words, K = 1024, bf16: forward 0.90 ms (1.19 PFLOP/s; the library's product alone, which writes the logits,
-// 1.05 ms), backward 2.87 ms (1.12) in four pieces of e 260, dx 225 and dw 203 us (the library's products of a piece: 285 and 291 us for
-// the last two).  Half of the time the matrix pipes work, at 1.75 to 1.83 GHz, which they themselves bring down; the rest is the
+// Measured, medians, at 8191 rows, 64010 words, K = 1024, bf16: forward 0.94 ms (1.15 PFLOP/s; the library's product alone, which writes
+// the logits, 1.05 ms), backward 2.96 ms (1.09) in four pieces of e 273, dx 243 and dw 212 us (the library's products of a piece: 285 and
+// 291 us for the last two); the best of several runs were 0.90 and 2.87 ms.  Half of the time the matrix pipes work, at 1.75 to 1.83 GHz, which they themselves bring down; the rest is the
 // start and the epilogue of a tile (28 us, of which 18 are products), which one workgroup to a compute unit cannot cover.  20 rows, 64010
 // words, K = 768: 17 us for 98 MB of w, 5.7 TB/s.
 //
